@@ -1,4 +1,5 @@
-"""ctypes binding of ``libdsa_mi355x.so`` (C ABI: include/dsa_mi355x.h).
+"""ctypes binding of ``libdsa_mi355x.so`` (C ABI: include/dsa_mi355x.h and
+include/dsa_mi355x_cache.h).
 
 The library is required: there is no fallback path.  Loading it touches no
 GPU (the planning entry points are pure host logic), so the binding also works
@@ -46,6 +47,55 @@ class DsaFwdOptions(ctypes.Structure):
     ]
 
 
+class DsaRotaryArgs(ctypes.Structure):
+    """Mirror of ``struct dsa_rotary_args`` (include/dsa_mi355x_cache.h)."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("frequencies", ctypes.c_void_p),
+        ("groups", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64 * 3),
+        ("out_stride", ctypes.c_int64 * 3),
+        ("heads", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("start", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("positions_64", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("transposed", ctypes.c_int32),
+        ("magnitude", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class DsaWriteArgs(ctypes.Structure):
+    """Mirror of ``struct dsa_write_args`` (include/dsa_mi355x_cache.h)."""
+
+    _fields_ = [
+        ("kv", ctypes.c_void_p),
+        ("k_rope", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("frequencies", ctypes.c_void_p),
+        ("cache", ctypes.c_void_p),
+        ("rope_cache", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("cache_rows", ctypes.c_int64),
+        ("kv_stride", ctypes.c_int64),
+        ("rope_stride", ctypes.c_int64),
+        ("kv_format", ctypes.c_int32),
+        ("pow2_scales", ctypes.c_int32),
+        ("positions_64", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("magnitude", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 KV_BF16 = 0  # DSA_KV_BF16
 KV_FP8 = 1   # DSA_KV_FP8: 656-byte rows (512 e4m3, 4 fp32 scales, 64 bf16 rope)
 
@@ -81,6 +131,13 @@ SIGNATURES = {
     "dsa_indexer_topk_ws": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
 }
 
+# Entry points of include/dsa_mi355x_cache.h.
+CACHE_SIGNATURES = {
+    "dsa_extend_block_table": (_i32, [_vp] * 9 + [_i32] * 5 + [_vp]),
+    "dsa_rotary": (_i32, [ctypes.POINTER(DsaRotaryArgs), _vp]),
+    "dsa_write_kv_rows": (_i32, [ctypes.POINTER(DsaWriteArgs), _vp]),
+}
+
 # Entry points of csrc/host_entry.h, called by this package only.
 PRIVATE_SIGNATURES = {
     "dsa_kv_quantize_rows": (_i32, [_vp, _vp, _vp, _i64, _i32, _vp]),
@@ -102,7 +159,7 @@ def load() -> ctypes.CDLL:
                     f"{LIB_PATH} is missing: build it with `python -m dsa_amd.build` "
                     "(dsa_amd has no CPU or fallback path)")
             lib = ctypes.CDLL(str(LIB_PATH))
-            for name, (res, args) in {**SIGNATURES, **PRIVATE_SIGNATURES}.items():
+            for name, (res, args) in {**SIGNATURES, **CACHE_SIGNATURES, **PRIVATE_SIGNATURES}.items():
                 fn = getattr(lib, name)
                 fn.restype = res
                 fn.argtypes = args

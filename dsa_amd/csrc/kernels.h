@@ -6,6 +6,7 @@
 #include <hip/hip_runtime_api.h>
 
 #include "../../include/dsa_mi355x.h"
+#include "../../include/dsa_mi355x_cache.h"
 
 namespace dsa {
 
@@ -161,5 +162,27 @@ int64_t indexer_topk_ws_bytes(int rows, int L);
 // contents on entry).
 int launch_indexer_topk_seg(const float* logits, const int32_t* len, int32_t* indices, void* ws, int rows, int L,
                             int topk, hipStream_t stream);
+
+}  // namespace dsa
+
+namespace dsa {
+
+// One step of a paged cache (dsa_extend_block_table).
+struct TableParams {
+    int32_t* block_table;       // [B, max_blocks], updated in place
+    const int32_t* lengths;     // [B]
+    const int32_t* new_tokens;  // [B]
+    const int32_t* free_blocks; // [num_free]
+    int32_t *slots, *positions; // [max_tokens]
+    int32_t* starts;            // [B + 1]
+    int32_t* totals;            // [B]
+    int32_t* used;              // [1]
+    int B, max_blocks, block_size, num_free, max_tokens;
+};
+int launch_extend_table(const TableParams& p, hipStream_t stream);
+
+int launch_rotary(const dsa_rotary_args& p, hipStream_t stream);
+
+int launch_write_rows(const dsa_write_args& p, hipStream_t stream);
 
 }  // namespace dsa
