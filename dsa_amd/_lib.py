@@ -96,6 +96,17 @@ class DsaWriteArgs(ctypes.Structure):
     ]
 
 
+class DsaSharedArgs(ctypes.Structure):
+    """Mirror of ``struct dsa_shared_args`` (include/dsa_mi355x_cache.h)."""
+
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("q", "kv", "q_rope", "k_rope", "lengths", "block_table", "out",
+                                                      "out_max", "out_sum", "workspace")]
+                + [("workspace_bytes", ctypes.c_int64)]
+                + [(name, ctypes.c_int32) for name in ("B", "SQ", "H", "L", "prefix", "block_size", "max_blocks",
+                                                       "num_blocks", "kv_format", "num_cus")]
+                + [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)])
+
+
 KV_BF16 = 0  # DSA_KV_BF16
 KV_FP8 = 1   # DSA_KV_FP8: 656-byte rows (512 e4m3, 4 fp32 scales, 64 bf16 rope)
 
@@ -135,6 +146,8 @@ SIGNATURES = {
 CACHE_SIGNATURES = {
     "dsa_extend_block_table": (_i32, [_vp] * 9 + [_i32] * 5 + [_vp]),
     "dsa_rotary": (_i32, [ctypes.POINTER(DsaRotaryArgs), _vp]),
+    "dsa_fwd_shared_ws_bytes": (_i64, [ctypes.POINTER(DsaSharedArgs)]),
+    "dsa_fwd_shared": (_i32, [ctypes.POINTER(DsaSharedArgs), _vp]),
     "dsa_write_kv_rows": (_i32, [ctypes.POINTER(DsaWriteArgs), _vp]),
 }
 

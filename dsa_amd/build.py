@@ -22,7 +22,8 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libdsa_mi355x.so"
 OBJ_DIR = PKG / "_build"
 SOURCES = ["sparse_mla_fwd.hip", "merge.hip", "project_uv.hip", "indexer.hip", "fwd_scratch.hip", "bucket_rows.hip",
-           "kv_rows.hip", "rotary.hip", "block_table.hip", "abi.cpp", "abi_cache.cpp"]
+           "kv_rows.hip", "rotary.hip", "block_table.hip", "shared_attn.hip",
+           "abi.cpp", "abi_cache.cpp"]
 ARCH = "gfx950"
 ROCM_INCLUDE = Path(os.environ.get("ROCM_PATH", "/opt/rocm")) / "include"
 

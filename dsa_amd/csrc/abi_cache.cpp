@@ -26,6 +26,56 @@ int finish(int rc, const char* what) {
     return dsa::set_error(0, "%s", "");
 }
 
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Query rows of a sequence from which its own blocks of kSharedRows are at least
+// this full; emptier ones make the prefix worth a pass over stacked rows.
+bool fills_blocks(int64_t rows) {
+    const int64_t blocks = (rows + dsa::kSharedRows - 1) / dsa::kSharedRows;
+    return rows * 8 >= blocks * dsa::kSharedRows * 7;
+}
+
+struct SharedPlan {
+    bool stacked;
+    int prefix_items, seq_blocks, items, workgroups;
+    int64_t tiles_bytes, slots, bytes;
+};
+
+int64_t round_256(int64_t n) { return (n + 255) / 256 * 256; }
+
+int shared_plan(const dsa_shared_args* a, SharedPlan* plan) {
+    if (!a) return fail(-1, "args is NULL");
+    if (a->B <= 0 || a->SQ <= 0 || a->H <= 0 || a->L <= 0)
+        return fail(-1, "B, SQ, H, L must be positive (got %d, %d, %d, %d)", a->B, a->SQ, a->H, a->L);
+    if (a->H % 16) return fail(-1, "H must be a multiple of 16 (got %d)", a->H);
+    if (a->L >= 1 << 25) return fail(-1, "L must be below 33554432 (got %d)", a->L);
+    if (a->prefix < 0 || a->prefix > a->L) return fail(-1, "prefix must be in [0, L = %d] (got %d)", a->L, a->prefix);
+    if (a->num_cus < 0) return fail(-1, "num_cus must not be negative");
+    const int64_t seq_rows = (int64_t)a->SQ * a->H, rows = seq_rows * a->B;
+    if (seq_rows > 1 << 30 || rows > 1 << 30) return fail(-1, "B * SQ * H must be at most 2^30");
+    plan->stacked = a->prefix > 0 && a->B > 1 && !fills_blocks(seq_rows);
+    plan->seq_blocks = (int)((seq_rows + dsa::kSharedRows - 1) / dsa::kSharedRows);
+    plan->prefix_items = plan->stacked ? (int)((rows + dsa::kSharedRows - 1) / dsa::kSharedRows) : 0;
+    const int64_t items = plan->prefix_items + (int64_t)a->B * plan->seq_blocks;
+    if (items * (ceil_div(a->L, dsa::kSharedKeys) + 2) >= (int64_t)1 << 31)
+        return fail(-1, "too many query rows for a context of %d (B * SQ * H * L)", a->L);
+    plan->items = (int)items;
+    plan->workgroups = a->num_cus;
+    if (plan->workgroups == 0) {
+        int device = 0, cus = 0;
+        int rc = (int)hipGetDevice(&device);
+        if (!rc) rc = (int)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
+        if (rc) return fail(rc, "device query: %s", hipGetErrorString((hipError_t)rc));
+        plan->workgroups = cus;
+    }
+    // Pieces: every cut of an item's tiles starts a new one; a stacked call keeps
+    // all of them, another only those of cut items, two at most a workgroup.
+    plan->slots = plan->stacked ? items + plan->workgroups : 2 * (int64_t)plan->workgroups;
+    plan->tiles_bytes = round_256(4 * (items + 1));
+    plan->bytes = plan->tiles_bytes + plan->slots * dsa::kSharedRows * (512 + 2) * 4;
+    return 0;
+}
+
 bool aligned(const void* p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
 }  // namespace
@@ -79,6 +129,70 @@ int dsa_write_kv_rows(const dsa_write_args* a, void* stream) {
                     "rope_stride of 2");
     if (!std::isfinite(a->magnitude)) return fail(-1, "magnitude must be finite");
     return finish(dsa::launch_write_rows(*a, static_cast<hipStream_t>(stream)), "cache row launch");
+}
+
+int64_t dsa_fwd_shared_ws_bytes(const dsa_shared_args* a) {
+    SharedPlan plan;
+    const int rc = shared_plan(a, &plan);
+    if (rc) return rc < 0 ? rc : -rc;
+    dsa::set_error(0, "%s", "");
+    return plan.bytes;
+}
+
+int dsa_fwd_shared(const dsa_shared_args* a, void* stream) {
+    SharedPlan plan;
+    if (const int rc = shared_plan(a, &plan)) return rc;
+    if (a->kv_format != DSA_KV_BF16 && a->kv_format != DSA_KV_FP8) return fail(-1, "unknown kv_format %d", a->kv_format);
+    const bool fp8 = a->kv_format == DSA_KV_FP8;
+    if (!a->q || !a->kv || !a->q_rope || (!fp8 && !a->k_rope) || !a->lengths || !a->out || !a->out_max || !a->out_sum ||
+        !a->workspace)
+        return fail(-1, "NULL pointer argument");
+    if (!aligned(a->q, 16) || !aligned(a->kv, 16) || !aligned(a->q_rope, 16) || (!fp8 && !aligned(a->k_rope, 16)) ||
+        !aligned(a->out, 16) || !aligned(a->lengths, 4) || !aligned(a->block_table, 4) || !aligned(a->out_max, 4) ||
+        !aligned(a->out_sum, 4) || !aligned(a->workspace, 256))
+        return fail(-1, "tensors must be 16-byte (lengths, block_table, max and sum 4-byte, workspace 256-byte) aligned");
+    if (!(a->scale >= 0.f) || !std::isfinite(a->scale)) return fail(-1, "scale must be a positive finite number, or 0");
+    if (a->block_table) {
+        if (a->block_size <= 0 || a->max_blocks <= 0 || a->num_blocks <= 0 ||
+            (int64_t)a->block_size * a->max_blocks != a->L)
+            return fail(-1, "paged kv: block_size, max_blocks and num_blocks must be positive, L = max_blocks * block_size");
+        if ((int64_t)a->num_blocks * a->block_size >= 1 << 25)
+            return fail(-1, "paged kv: num_blocks * block_size must be below 33554432");
+    }
+    if (a->workspace_bytes < plan.bytes)
+        return fail(-1, "workspace of %lld bytes is below the %lld needed", (long long)a->workspace_bytes,
+                    (long long)plan.bytes);
+    dsa::SharedParams p{};
+    p.q = a->q;
+    p.kv = static_cast<const char*>(a->kv);
+    p.q_rope = a->q_rope;
+    p.k_rope = a->k_rope;
+    p.lengths = a->lengths;
+    p.block_table = a->block_table;
+    p.out = a->out;
+    p.out_max = a->out_max;
+    p.out_sum = a->out_sum;
+    char* ws = static_cast<char*>(a->workspace);
+    p.tiles = reinterpret_cast<int32_t*>(ws);
+    p.part_o = reinterpret_cast<float*>(ws + plan.tiles_bytes);
+    p.part_m = p.part_o + plan.slots * dsa::kSharedRows * 512;
+    p.part_l = p.part_m + plan.slots * dsa::kSharedRows;
+    p.B = a->B;
+    p.SQ = a->SQ;
+    p.H = a->H;
+    p.L = a->L;
+    p.prefix = a->prefix;
+    p.block_size = a->block_size;
+    p.max_blocks = a->max_blocks;
+    p.num_blocks = a->num_blocks;
+    p.kv_fp8 = fp8;
+    p.scale_log2 = (a->scale == 0.f ? 1.f / 24.f : a->scale) * 1.4426950408889634f;
+    p.stacked = plan.stacked;
+    p.prefix_items = plan.prefix_items;
+    p.seq_blocks = plan.seq_blocks;
+    p.items = plan.items;
+    p.workgroups = plan.workgroups;
+    return finish(dsa::launch_shared(p, static_cast<hipStream_t>(stream)), "shared attention launch");
 }
 
 }  // extern "C"

@@ -185,4 +185,36 @@ int launch_rotary(const dsa_rotary_args& p, hipStream_t stream);
 
 int launch_write_rows(const dsa_write_args& p, hipStream_t stream);
 
+// Dense attention over a shared prefix and each sequence's own rows
+// (shared_attn.hip).  Query rows (token, head) are cut into blocks of
+// kSharedRows; an item is one block over one range of keys.  Items are listed
+// prefix blocks first (stacked: blocks of rows of any sequences over the
+// prefix), then each sequence's own blocks, over its own rows (stacked) or over
+// prefix and own rows (not stacked: then there are no prefix items).  The tiles
+// of all items in that order are cut evenly over the workgroups, so an item may
+// be cut over several; the merge kernel joins its pieces.
+constexpr int kSharedRows = 64;
+constexpr int kSharedKeys = 32;  // keys a tile
+struct SharedParams {
+    const uint16_t* q;
+    const char* kv;
+    const uint16_t* q_rope;
+    const uint16_t* k_rope;
+    const int32_t* lengths;      // [B, SQ]
+    const int32_t* block_table;  // [B, max_blocks] or NULL
+    uint16_t* out;
+    float *out_max, *out_sum;
+    int32_t* tiles;   // [items + 1]: tiles of the items before
+    float* part_o;    // [slots, kSharedRows, 512] pieces of cut items
+    float* part_m;    // [slots, kSharedRows] (log2 units)
+    float* part_l;    // [slots, kSharedRows]
+    int B, SQ, H, L, prefix;
+    int block_size, max_blocks, num_blocks;
+    int kv_fp8;
+    float scale_log2;
+    int stacked, prefix_items, seq_blocks, items;
+    int workgroups;
+};
+int launch_shared(const SharedParams& p, hipStream_t stream);
+
 }  // namespace dsa

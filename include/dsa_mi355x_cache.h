@@ -104,6 +104,51 @@ typedef struct dsa_write_args {
 } dsa_write_args;
 int dsa_write_kv_rows(const dsa_write_args* args, void* stream);
 
+/*
+ * Dense attention of a batch whose sequences share their first `prefix` rows.
+ * With the rows as dsa_fwd's kv and k_rope (contiguous, paged or fp8, as in
+ * dsa_fwd_options), for query t of sequence b and head h:
+ *
+ *   score_j = (q[b,t,h,:] . kv_j + q_rope[b,t,h,:] . k_rope_j) * scale     j < lengths[b,t]
+ *   max = max_j score_j;  sum = sum_j exp(score_j - max);  out = sum_j exp(score_j - max) kv_j / sum
+ *
+ * where row j is row j of sequence 0 for j < prefix, and of sequence b from
+ * there on: the prefix is read, and its products formed, for the whole batch
+ * at once.  A row whose block entry lies outside [0, num_blocks) is masked.  A
+ * query with no row left gives out 0, max -inf, sum 0.  Rows a query does not
+ * see, whatever their bits, do not touch its result.
+ *
+ *   q [B, SQ, H, 512], q_rope [B, SQ, H, 64] bf16, H a multiple of 16
+ *   lengths [B, SQ] int32: rows each query sees, clamped to [0, L]
+ *   out [B, SQ, H, 512] bf16, out_max / out_sum [B, 1, SQ, H] fp32
+ *   workspace: at least dsa_fwd_shared_ws_bytes bytes, 256-byte aligned, any
+ *   contents; calls that can overlap need one each
+ * Probabilities are rounded to bf16 before the second product, sums and
+ * statistics are fp32; the output is finite for max|kv| < 2^38.
+ */
+typedef struct dsa_shared_args {
+    const uint16_t* q;
+    const void* kv;             /* [B, L, 512] bf16 or [B, L] fp8 rows; a pool when paged */
+    const uint16_t* q_rope;
+    const uint16_t* k_rope;     /* [B, L, 64] bf16 or a pool; unused with fp8 rows */
+    const int32_t* lengths;
+    const int32_t* block_table; /* [B, max_blocks], or NULL */
+    uint16_t* out;
+    float* out_max;
+    float* out_sum;
+    void* workspace;
+    int64_t workspace_bytes;
+    int32_t B, SQ, H, L, prefix;
+    int32_t block_size, max_blocks, num_blocks; /* paged: L = max_blocks * block_size */
+    int32_t kv_format;          /* DSA_KV_BF16, DSA_KV_FP8 */
+    int32_t num_cus;            /* compute units to plan for; 0: the device's */
+    float scale;                /* 0: 1/24 */
+    int32_t reserved;           /* zero */
+} dsa_shared_args;
+/* < 0: the sizes are refused (dsa_last_error).  Reads no pointer of args. */
+int64_t dsa_fwd_shared_ws_bytes(const dsa_shared_args* args);
+int dsa_fwd_shared(const dsa_shared_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

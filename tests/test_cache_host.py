@@ -28,7 +28,8 @@ def test_struct_layouts(tmp_path):
     """Field offsets of the argument structs as a C compiler lays them out."""
     import subprocess
 
-    structs = {"dsa_rotary_args": _lib.DsaRotaryArgs, "dsa_write_args": _lib.DsaWriteArgs}
+    structs = {"dsa_rotary_args": _lib.DsaRotaryArgs, "dsa_write_args": _lib.DsaWriteArgs,
+               "dsa_shared_args": _lib.DsaSharedArgs}
     lines = [f'printf("%s %s %zu\\n", "{n}", "{f[0]}", offsetof({n}, {f[0]}));' for n, s in structs.items()
              for f in s._fields_]
     lines += [f'printf("%s sizeof %zu\\n", "{n}", sizeof({n}));' for n in structs]
