@@ -185,6 +185,12 @@ int dsa_fwd_shared(const dsa_shared_args* a, void* stream) {
     p.block_size = a->block_size;
     p.max_blocks = a->max_blocks;
     p.num_blocks = a->num_blocks;
+    // d in (2^s, 2^(s+1)]: ceil(2^(32+s) / d) d < 2^(32+s) + d, so the quotient is exact for keys below 2^31
+    if (a->block_table && a->block_size > 1) {
+        while ((int64_t)2 << p.block_shift < a->block_size) ++p.block_shift;
+        const uint64_t num = (uint64_t)1 << (32 + p.block_shift), d = (uint64_t)a->block_size;
+        p.block_magic = (uint32_t)((num + d - 1) / d);
+    }
     p.kv_fp8 = fp8;
     p.scale_log2 = (a->scale == 0.f ? 1.f / 24.f : a->scale) * 1.4426950408889634f;
     p.stacked = plan.stacked;

@@ -210,6 +210,8 @@ struct SharedParams {
     float* part_l;    // [slots, kSharedRows]
     int B, SQ, H, L, prefix;
     int block_size, max_blocks, num_blocks;
+    uint32_t block_magic;  // key / block_size = mulhi(key, block_magic) >> block_shift for block_size > 1
+    int block_shift;
     int kv_fp8;
     float scale_log2;
     int stacked, prefix_items, seq_blocks, items;

@@ -16,6 +16,7 @@
 #include <hip/hip_runtime.h>
 #include <float.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "kernels.h"
 #include "mla_tiles.h"
@@ -283,6 +284,503 @@ __global__ __launch_bounds__(kThreads) void shared_main_kernel(SharedParams p) {
     }
 }
 
+// ------------------------------------------------------------------ bf16 rows
+// Eight waves in two groups of four (waves w and w + 4 share a SIMD).  Both
+// groups own the block's 64 rows and take its tiles in turn, half a tile apart,
+// so that on every SIMD one wave's softmax runs beside the other's MFMAs:
+//
+//   half u:  group u % 2: S = K Q^T of tile u, a wave a block of 16 query rows, and
+//            its weights to the group's P buffer;
+//            the other group: gathers of tile u + 2 into the ring, then
+//            O^T += V^T P^T of tile u - 1, a wave 128 of the 512 columns
+//
+// with a workgroup barrier at the start of each half.  The running maximum is
+// taken once, from a row's first tile: P is formed against that reference, and
+// a piece whose maximum grows past it by 2^64 is computed once more against the
+// exact one, so O is never rescaled in the loop.  The groups' sums are brought
+// to a common maximum and added at the end.
+//
+// A query row sees keys [0, seen) only, and rows behind a bad block entry are
+// masked: their scores become -inf, their weights 0 (clear_specials).
+constexpr int kPPThreads = 512;
+constexpr float kRestartLog2 = 64.0f;
+
+struct PPLds {
+    static constexpr int NSTAGE = 4;
+    static constexpr int KV_BYTES = kKeys * 1024, STAGE_BYTES = kKeys * 1152;
+    // P of one group, 64 rows x 32 bf16 in the k order of the PV operand (pp_pchunk)
+    static constexpr int P_OFF = NSTAGE * STAGE_BYTES, P_GROUP = 64 * 64;
+    // per stage: block entries of a later tile (four waves x 8 rows), and which of the tile's rows are in the pool
+    static constexpr int ENTRY_OFF = P_OFF + 2 * P_GROUP;
+    static constexpr int VALID_OFF = ENTRY_OFF + NSTAGE * kKeys * 4;
+    static constexpr int ML_OFF = VALID_OFF + NSTAGE * 4;  // [3][128] floats: l, reference and maximum of each group's rows
+    static constexpr int FLAG_OFF = ML_OFF + 3 * 128 * 4;
+    static constexpr int LDS_BYTES = FLAG_OFF + 16;
+    static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
+    __device__ static uint32_t stage(uint32_t lds, int u) { return lds + (uint32_t)(u % NSTAGE) * STAGE_BYTES; }
+};
+
+// One tile of a piece: where its keys start, and the rows they are looked up in.
+struct Tile {
+    int key0, key_end, seq;
+};
+struct Piece {
+    Item it;
+    int a, nt;      // first tile of the item, and how many
+    int seen_low;   // least number of rows a query row of the block sees
+};
+__device__ __forceinline__ Tile tile_at(const SharedParams& p, const Piece& c, int u) {
+    const int t = c.a + u;
+    const bool shared = t < c.it.first;
+    Tile k;
+    k.key0 = shared ? t * kKeys : p.prefix + (t - c.it.first) * kKeys;
+    k.key_end = shared ? p.prefix : p.L;
+    k.seq = shared ? 0 : c.it.seq;
+    return k;
+}
+
+// key / block_size, without a division (keys are below 2^25).
+__device__ __forceinline__ int block_of(const SharedParams& p, int key) {
+    return p.block_size == 1 ? key : (int)(__umulhi((uint32_t)key, p.block_magic) >> p.block_shift);
+}
+
+// 4 bytes a lane straight into LDS (lane l at m0 + 4 l).
+__device__ __forceinline__ void gather_words(uint32_t lds_base, rsrc_t rsrc, uint32_t voff) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "buffer_load_dword %1, %2, 0 offen lds"
+        :
+        : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(voff), "s"(rsrc)
+        : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
+// Gathers of tile u by wave gw of a group: rows 8 gw .. 8 gw + 7, 1 KiB each in
+// one instruction, and their rotary parts in one.  Paged: the rows' block
+// entries were loaded into LDS when this wave issued tile u - 2 (waited for
+// since) -- for the piece's first tiles, `first`, they are loaded here -- and
+// those of tile u + 2 are issued behind the rows.
+__device__ __forceinline__ void issue_rows(const SharedParams& p, const Piece& c, int u, bool first, uint32_t lds,
+                                           int gw, int lane) {
+    asm volatile("" : "+v"(lane));
+    const Tile k = tile_at(p, c, u);
+    const uint32_t stage = PPLds::stage(lds, u);
+    const int r0 = 8 * gw;
+    const int key_r = min(k.key0 + r0 + (lane & 7), k.key_end - 1);  // the row the wave reads ..
+    const int key_l = min(k.key0 + r0 + (lane >> 3), k.key_end - 1); // .. and the one whose rotary part the lane reads
+    const char* kv = p.kv;
+    const char* kr = reinterpret_cast<const char*>(p.k_rope);
+    int my_row, rope_row;
+    uint32_t pool;
+    if (p.block_table == nullptr) {
+        const int64_t base = (int64_t)k.seq * p.L;
+        kv += base << 10;
+        kr += base << 7;
+        my_row = key_r;
+        rope_row = key_l;
+        pool = (uint32_t)p.L << 7;
+    } else {
+        const uint32_t entries = lds + PPLds::ENTRY_OFF + (uint32_t)(u % PPLds::NSTAGE) * (kKeys * 4) + 4 * r0;
+        const int32_t* table = p.block_table + (int64_t)k.seq * p.max_blocks;
+        const int col_r = block_of(p, key_r), col_l = block_of(p, key_l);
+        int e_r, e_l;
+        if (first) {
+            e_r = table[col_r];
+            e_l = table[col_l];
+        } else {
+            e_r = lds_load<int>(entries + 4 * (lane & 7));
+            e_l = lds_load<int>(entries + 4 * (lane >> 3));
+        }
+        const bool ok_r = (uint32_t)e_r < (uint32_t)p.num_blocks, ok_l = (uint32_t)e_l < (uint32_t)p.num_blocks;
+        const uint64_t valid = __ballot(ok_r) & 0xff;
+        if (lane == 0)
+            lds_store<uint8_t>(lds + PPLds::VALID_OFF + 4 * (u % PPLds::NSTAGE) + gw, (uint8_t)valid);
+        my_row = (ok_r ? e_r : 0) * p.block_size + (key_r - col_r * p.block_size);
+        rope_row = (ok_l ? e_l : 0) * p.block_size + (key_l - col_l * p.block_size);
+        pool = (uint32_t)(p.num_blocks * p.block_size) << 7;
+    }
+    const uint32_t lane16 = (uint32_t)lane << 4;
+#pragma unroll
+    for (int rr = 0; rr < 8; ++rr)
+        gather_row(stage + (r0 + rr) * 1024, row_rsrc(kv, (uint32_t)__builtin_amdgcn_readlane(my_row, rr)), lane16,
+                   (uint32_t)sw_kv(r0 + rr) << 4);
+    const int r = r0 + (lane >> 3);
+    gather_lanes(stage + PPLds::KV_BYTES + r0 * 128, make_rsrc(kr, pool),
+                 ((uint32_t)rope_row << 7) + (((lane & 7) ^ sw_rope(r)) << 4));
+    if (p.block_table != nullptr && u + 2 < c.nt) {
+        const Tile n = tile_at(p, c, u + 2);
+        const int key = min(n.key0 + r0 + lane, n.key_end - 1);
+        if (lane < 8)
+            gather_words(lds + PPLds::ENTRY_OFF + (uint32_t)((u + 2) % PPLds::NSTAGE) * (kKeys * 4) + 4 * r0,
+                         make_rsrc(p.block_table + (int64_t)n.seq * p.max_blocks, 4u * (uint32_t)p.max_blocks),
+                         4u * (uint32_t)block_of(p, key));
+    }
+}
+
+// Which of the 32 keys of a tile a query row that sees `seen` rows has: bit r is tile row r.
+__device__ __forceinline__ uint32_t key_mask(const Tile& k, int seen, uint32_t valid) {
+    const int n = min(max(min(seen, k.key_end) - k.key0, 0), kKeys);
+    return n == kKeys ? valid : valid & ((1u << n) - 1);
+}
+
+// Lane g's rows of a tile -- 4 g + j (j < 4) and 16 + 4 g + j -- from a key mask: bit j, bit 4 + j.
+__device__ __forceinline__ uint32_t lane_rows(uint32_t mask, int g) {
+    return (mask >> (4 * g) & 15u) | (mask >> (16 + 4 * g) & 15u) << 4;
+}
+
+// Infinities and NaN in this wave's 128 columns of a tile become zeros, where
+// some query row does not see all of the tile: a hidden row's weight is 0, which
+// they would turn into NaN.  A query row that does see such a value has a score,
+// a sum and so a whole result that are NaN already, as the key row that it lies
+// in is the value row too.  (The wave's own LDS accesses are in order, and no
+// other wave reads these columns any more.)
+__device__ __forceinline__ void clear_specials(uint32_t stage, int gw, int lane) {
+    asm volatile("" : "+v"(lane));
+    const uint32_t at = stage + (uint32_t)((lane >> 4) * 1024 + gw * 256 + (lane & 15) * 16);
+#pragma unroll 1
+    for (int r = 0; r < kKeys; r += 4) {
+        i32x4 v = lds_load<i32x4>(at + r * 1024);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            if ((v[d] & 0x7f80) == 0x7f80) v[d] &= 0xffff0000;
+            if ((v[d] & 0x7f800000) == 0x7f800000) v[d] &= 0xffff;
+        }
+        lds_store<i32x4>(at + r * 1024, v);
+    }
+}
+
+// One piece of an item with up to 16 NB rows.
+template <int NB>
+__device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece& c, bool whole, int64_t slot,
+                                             uint32_t lds, int wave, int lane) {
+    using X = PPLds;
+    const int grp = wave >> 2, gw = wave & 3;
+    const int g = lane >> 4, n16 = lane & 15;
+    const bool live = 16 * gw < c.it.rows;  // this wave has query rows
+    const int row = c.it.row0 + 16 * gw;
+    const int seen = live ? __builtin_amdgcn_readfirstlane(seen_by(p, row / p.H)) : 0;
+    const uint32_t p_lds = lds + X::P_OFF + grp * X::P_GROUP;
+
+    bf16x8 qf[18];
+    {
+        const int r = live ? row : c.it.row0;
+        const uint16_t* q = p.q + (int64_t)(r + n16) * 512 + 8 * qk_lane_chunk(g);
+#pragma unroll
+        for (int ks = 0; ks < 16; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(q + 32 * ks);
+        const uint16_t* rr = p.q_rope + (int64_t)(r + n16) * 64 + 8 * g;
+        qf[16] = *reinterpret_cast<const bf16x8*>(rr);
+        qf[17] = *reinterpret_cast<const bf16x8*>(rr + 32);
+    }
+
+    f32x4 oacc[NB][8];
+    float m_ref = -FLT_MAX, m_true = -FLT_MAX, l_run = 0.f;
+
+    // This lane's LDS offsets in the loop, packed as in the sparse ping-pong kernel.
+    uint32_t off_kv, off_rope, off_p;
+    {
+        const uint32_t koff = (uint32_t)(n16 * 1024) | ((uint32_t)(qk_lane_chunk(g) ^ sw_kv(n16)) << 4);
+        const int tr_row = 4 * g + (n16 >> 2);
+        const uint32_t voff = (uint32_t)(tr_row * 1024 + (gw << 8)) +
+                              ((uint32_t)((((n16 & 3) >> 1) ^ sw_kv(tr_row)) << 4) + ((n16 & 1) << 3));
+        off_kv = koff | (voff << 16);
+        off_rope = (uint32_t)(X::KV_BYTES + n16 * 128) | ((uint32_t)(g ^ sw_rope(n16)) << 4);
+        off_p = pp_pchunk(n16, g) | (pp_pchunk(16 * gw + n16, g) << 16);
+    }
+
+    auto qk_softmax = [&](int u, bool& overflow) __attribute__((always_inline)) {
+        const uint32_t stage = X::stage(lds, u);
+        asm volatile("" : "+v"(off_kv), "+v"(off_rope), "+v"(off_p));
+        const uint32_t kbase = stage + (off_kv & 0xffffu);
+        const uint32_t rbase = stage + off_rope;
+        const int valid_v = lds_load<int>(lds + X::VALID_OFF + 4 * (u % X::NSTAGE));
+        auto kfrag = [&](int step) -> bf16x8 {
+            const int ks = step >> 1, sub = step & 1;
+            if (ks < 16) return lds_load<bf16x8>((kbase ^ (64u * (ks & 3))) + 256u * (ks >> 2) + sub * 16 * 1024);
+            return lds_load<bf16x8>((rbase ^ (64u * (ks - 16))) + sub * 16 * 128);
+        };
+        constexpr int KD = 7;  // K fragments in flight
+        __builtin_amdgcn_s_setprio(2);
+        f32x4 sacc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+        bf16x8 kf[KD];
+#pragma unroll
+        for (int j = 0; j < KD; ++j) kf[j] = kfrag(j);
+#pragma unroll
+        for (int step = 0; step < 36; ++step) {
+            sacc[step & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[step % KD], qf[step >> 1], sacc[step & 1], 0, 0, 0);
+            if (step + KD < 36) kf[step % KD] = kfrag(step + KD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        float x[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) x[r] = sacc[r >> 2][r & 3];
+        const uint32_t mask = key_mask(tile_at(p, c, u), seen, (uint32_t)__builtin_amdgcn_readfirstlane(valid_v));
+        if (mask != 0xffffffffu) {
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            const uint32_t mine = lane_rows(mask, ln >> 4);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (!(mine >> r & 1)) x[r] = -INFINITY;
+        }
+        float smax = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) smax = fmaxf(smax, x[r]);
+        smax = max_xor32(max_xor16(smax));
+        m_true = fmaxf(m_true, smax * p.scale_log2);
+        if (m_ref == -FLT_MAX) m_ref = m_true;  // the row's first keys: O and l are still zero
+        const bool ovf = m_true > m_ref + kRestartLog2;
+        overflow |= ovf;
+        const float neg_ref = -m_ref;
+        float psum = 0.f;
+        bf16x8 pk;
+        if (__any(ovf)) {  // this pass is to be discarded: the clamp keeps it free of inf
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const float e = fast_exp2(fminf(fmaf(x[r], p.scale_log2, neg_ref), kRestartLog2));
+                psum += e;
+                pk[r] = (__bf16)e;
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const float e = fast_exp2(fmaf(x[r], p.scale_log2, neg_ref));
+                psum += e;
+                pk[r] = (__bf16)e;
+            }
+        }
+        l_run += psum;
+        lds_store<bf16x8>(p_lds + (off_p >> 16), pk);
+    };
+
+    auto pv = [&](int u) __attribute__((always_inline)) {
+        const uint32_t stage = X::stage(lds, u);
+        asm volatile("" : "+v"(off_kv), "+v"(off_p));
+        const uint32_t valid = (uint32_t)__builtin_amdgcn_readfirstlane(
+            lds_load<int>(lds + X::VALID_OFF + 4 * (u % X::NSTAGE)));
+        const Tile k = tile_at(p, c, u);
+        const uint32_t vbase = stage + (off_kv >> 16);
+        auto vfrag = [&](int cb) -> bf16x8 {
+            const uint32_t a = vbase ^ (32u * cb);
+            const bf16x4 v0 = lds_load_tr(a);
+            const bf16x4 v1 = lds_load_tr(a + 16 * 1024);
+            return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        if (__builtin_expect(key_mask(k, c.seen_low, valid) != 0xffffffffu, 0)) clear_specials(stage, gw, lane);
+        bf16x8 pf[NB];
+#pragma unroll
+        for (int hb = 0; hb < NB; ++hb) pf[hb] = lds_load<bf16x8>(p_lds + (off_p & 0xffffu) + 1024 * hb);
+        constexpr int VD = NB == 4 ? 2 : 4;  // V fragments in flight
+        bf16x8 vf[VD];
+#pragma unroll
+        for (int j = 0; j < VD; ++j) vf[j] = vfrag(j);
+#pragma unroll
+        for (int cb = 0; cb < 8; ++cb) {
+#pragma unroll
+            for (int hb = 0; hb < NB; ++hb)
+                oacc[hb][cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[cb % VD], pf[hb], oacc[hb][cb], 0, 0, 0);
+            if (cb + VD < 8) vf[cb % VD] = vfrag(cb + VD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    const int nt = c.nt;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+        for (int hb = 0; hb < NB; ++hb)
+#pragma unroll
+            for (int cb = 0; cb < 8; ++cb) oacc[hb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        l_run = 0.f;
+        if (pass == 1) m_ref = m_true;
+        bool overflow = false;
+        // Half u: group u % 2 scores tile u; the other group issues tile u + 2
+        // (into the stage of tile u - 2, whose last reader ran in half u - 1)
+        // and runs PV of tile u - 1.  A group scores the tile after the one it
+        // issued last, and its full wait behind that covers the tile it issued
+        // and the block entries of the one it issues next.
+        if (grp == 1) issue_rows(p, c, 0, true, lds, gw, lane);
+        wait_vmcnt<0>();
+        if (grp == 0 && nt > 1) issue_rows(p, c, 1, true, lds, gw, lane);
+        if (grp == 0) {
+            for (int u = 0; u < nt; u += 2) {
+                lds_barrier();
+                if (live) qk_softmax(u, overflow);
+                wait_vmcnt<0>();
+                lds_barrier();
+                if (u + 3 < nt) issue_rows(p, c, u + 3, false, lds, gw, lane);
+                pv(u);
+            }
+            if ((nt & 1) == 0) lds_barrier();  // half nt: group 1's last PV
+        } else {
+            lds_barrier();
+            if (2 < nt) issue_rows(p, c, 2, false, lds, gw, lane);
+            for (int u = 1; u < nt; u += 2) {
+                lds_barrier();
+                if (live) qk_softmax(u, overflow);
+                wait_vmcnt<0>();
+                lds_barrier();
+                if (u + 3 < nt) issue_rows(p, c, u + 3, false, lds, gw, lane);
+                pv(u);
+            }
+            if (nt & 1) lds_barrier();  // half nt: group 0's last PV
+        }
+        if (pass == 1) break;
+        // does any row need the second pass?
+        const uint32_t flag = lds + X::FLAG_OFF;
+        lds_barrier();
+        if (threadIdx.x == 0) lds_store<int>(flag, 0);
+        lds_barrier();
+        if (__any(overflow) && lane == 0) lds_store<int>(flag, 1);
+        lds_barrier();
+        if (__builtin_amdgcn_readfirstlane(lds_load<int>(flag)) == 0) break;
+        lds_barrier();  // read by every wave before the second pass ends in another vote's first store
+    }
+
+    // ---- both groups hold O of the same rows over their own tiles: each is
+    // scaled to the common maximum, a wave hands half of its column blocks to
+    // the wave of the other group with the same columns and adds what it gets.
+    lds_barrier();
+    const uint32_t ml = lds + X::ML_OFF;
+    l_run = sum_xor32(sum_xor16(l_run));
+    int eln = lane;
+    asm volatile("" : "+v"(eln));
+    const int eg = eln >> 4, en16 = eln & 15;
+    if (eg == 0) {
+        const int hl = 64 * grp + 16 * gw + en16;
+        lds_store<float>(ml + 4 * hl, l_run);
+        lds_store<float>(ml + 4 * (128 + hl), m_ref);
+        lds_store<float>(ml + 4 * (256 + hl), m_true);
+    }
+    lds_barrier();
+    constexpr int HROW = 1040;       // bytes of a staged bf16 row (16 more: rows spread over the banks)
+    constexpr int kPartRow = 2064;   // of a staged fp32 row
+    constexpr uint32_t kHand = NB * 4 * 1024;  // one wave's half: NB row x 4 column blocks of 64 lanes x 16 bytes
+    static_assert(8 * kHand <= X::P_OFF && 64 * kPartRow <= X::P_OFF, "staging fits the ring");
+    const uint32_t give = lds + (uint32_t)wave * kHand + 16u * (uint32_t)eln;
+    const uint32_t take = lds + (uint32_t)(wave ^ 4) * kHand + 16u * (uint32_t)eln;
+    float scale[NB];
+#pragma unroll
+    for (int hb = 0; hb < NB; ++hb) {
+        const int hl = 16 * hb + en16;
+        float l[2], mr[2], mt[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            l[k] = lds_load<float>(ml + 4 * (64 * k + hl));
+            mr[k] = lds_load<float>(ml + 4 * (128 + 64 * k + hl));
+            mt[k] = lds_load<float>(ml + 4 * (256 + 64 * k + hl));
+        }
+        const float top = fmaxf(mt[0], mt[1]);
+        const float f0 = fast_exp2(mr[0] - top), f1 = fast_exp2(mr[1] - top);
+        const float sum = fmaf(l[0], f0, l[1] * f1);
+        scale[hb] = grp == 0 ? f0 : f1;
+        if (whole) scale[hb] *= sum == 0.f ? 0.f : 1.f / sum;
+        if (wave == 0 && eg == 0 && hl < c.it.rows) {
+            if (whole) {
+                p.out_max[c.it.row0 + hl] = sum == 0.f ? -INFINITY : top * kLn2;
+                p.out_sum[c.it.row0 + hl] = sum;
+            } else {
+                p.part_m[slot * kRows + hl] = top;
+                p.part_l[slot * kRows + hl] = sum;
+            }
+        }
+    }
+    auto finish = [&](auto kept) __attribute__((always_inline)) {  // kept: 0 (blocks 0-3) or 4 (blocks 4-7)
+        constexpr int KEEP = decltype(kept)::value, GIVE = 4 - KEEP;
+#pragma unroll
+        for (int hb = 0; hb < NB; ++hb)
+#pragma unroll
+            for (int cb = 0; cb < 4; ++cb)
+                lds_store<f32x4>(give + 1024u * (4 * hb + cb), oacc[hb][GIVE + cb] * scale[hb]);
+        lds_barrier();
+#pragma unroll
+        for (int hb = 0; hb < NB; ++hb)
+#pragma unroll
+            for (int cb = 0; cb < 4; ++cb)
+                oacc[hb][KEEP + cb] = oacc[hb][KEEP + cb] * scale[hb] + lds_load<f32x4>(take + 1024u * (4 * hb + cb));
+        lds_barrier();  // the halves are read: the ring is free for the staged rows
+        const int col0 = 128 * gw + 16 * KEEP + 4 * eg;
+#pragma unroll
+        for (int hb = 0; hb < NB; ++hb) {
+            const int hl = 16 * hb + en16;
+#pragma unroll
+            for (int cb = 0; cb < 4; ++cb) {
+                const f32x4 o = oacc[hb][KEEP + cb];
+                if (whole) {
+                    bf16x4 v;
+                    v[0] = (__bf16)o[0];
+                    v[1] = (__bf16)o[1];
+                    v[2] = (__bf16)o[2];
+                    v[3] = (__bf16)o[3];
+                    lds_store<bf16x4>(lds + (uint32_t)(hl * HROW + 2 * (col0 + 16 * cb)), v);
+                } else {
+                    lds_store<f32x4>(lds + (uint32_t)(hl * kPartRow + 4 * (col0 + 16 * cb)), o);
+                }
+            }
+        }
+    };
+    if (grp == 0) finish(std::integral_constant<int, 0>{});
+    else finish(std::integral_constant<int, 4>{});
+    lds_barrier();
+    if (whole) {
+        uint16_t* obase = p.out + (int64_t)c.it.row0 * 512 + 8 * eln;
+        for (int hr = wave; hr < c.it.rows; hr += 8)
+            *reinterpret_cast<bf16x8*>(obase + (int64_t)hr * 512) = lds_load<bf16x8>(lds + hr * HROW + 16 * eln);
+    } else {
+        float* base = p.part_o + slot * (kRows * 512) + 4 * eln;
+        for (int i = wave; i < 2 * c.it.rows; i += 8)
+            *reinterpret_cast<f32x4*>(base + (i >> 1) * 512 + 256 * (i & 1)) =
+                lds_load<f32x4>(lds + (uint32_t)((i >> 1) * kPartRow + 1024 * (i & 1) + 16 * eln));
+    }
+    lds_barrier();  // the ring is free for the next piece
+}
+
+__global__ __launch_bounds__(kPPThreads, 1) void shared_pp_kernel(SharedParams p) {
+    __shared__ __attribute__((aligned(1024))) char smem[PPLds::LDS_BYTES];
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int total = p.tiles[p.items], groups = groups_of(p, total);
+    const int w = blockIdx.x;
+    if (w >= groups) return;
+    int t0 = (int)((int64_t)w * total / groups);
+    const int t1 = (int)((int64_t)(w + 1) * total / groups);
+    if (t0 >= t1) return;
+    if (threadIdx.x < PPLds::NSTAGE) lds_store<uint32_t>(lds + PPLds::VALID_OFF + 4 * threadIdx.x, 0xffffffffu);
+    int i = 0, high = p.items;  // the item that holds tile t0: tiles[i] <= t0 < tiles[i + 1]
+    while (high - i > 1) {
+        const int mid = (i + high) >> 1;
+        if (p.tiles[mid] <= t0) i = mid;
+        else high = mid;
+    }
+#pragma unroll 1
+    for (; t0 < t1; ++i) {
+        const int begin = p.tiles[i], end = p.tiles[i + 1];
+        if (end <= t0) continue;
+        Piece c;
+        c.it = item_rows(p, i);
+        int most = 0, least = p.L;
+        for (int t = c.it.row0 / p.H; t <= (c.it.row0 + c.it.rows - 1) / p.H; ++t) {
+            const int n = seen_by(p, t);
+            most = max(most, n);
+            least = min(least, n);
+        }
+        item_tiles(p, i, most, c.it);
+        c.it.first = __builtin_amdgcn_readfirstlane(c.it.first);
+        c.seen_low = __builtin_amdgcn_readfirstlane(least);
+        c.a = __builtin_amdgcn_readfirstlane(t0 - begin);
+        c.nt = __builtin_amdgcn_readfirstlane(min(t1, end) - t0);
+        const bool whole = !p.stacked && c.nt == end - begin;
+        const int64_t slot = slot_of(p, i, w, c.a == 0);
+        if (c.it.rows <= 16) shared_piece<1>(p, c, whole, slot, lds, wave, lane);
+        else if (c.it.rows <= 32) shared_piece<2>(p, c, whole, slot, lds, wave, lane);
+        else shared_piece<4>(p, c, whole, slot, lds, wave, lane);
+        t0 = min(t1, end);
+    }
+}
+
 // ------------------------------------------------------------------ merge
 // One workgroup a row pair; thread t of a row's 128 owns columns 4 t .. 4 t + 3.
 __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams p) {
@@ -326,7 +824,10 @@ int launch_shared(const SharedParams& p, hipStream_t stream) {
     hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
     int rc = (int)hipGetLastError();
     if (rc) return rc;
-    hipLaunchKernelGGL(shared_main_kernel, dim3(p.workgroups), dim3(kThreads), 0, stream, p);
+    if (p.kv_fp8)
+        hipLaunchKernelGGL(shared_main_kernel, dim3(p.workgroups), dim3(kThreads), 0, stream, p);
+    else
+        hipLaunchKernelGGL(shared_pp_kernel, dim3(p.workgroups), dim3(kPPThreads), 0, stream, p);
     rc = (int)hipGetLastError();
     if (rc) return rc;
     const int rows = p.B * p.SQ * p.H;
