@@ -27,6 +27,7 @@ namespace {
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr int kRows = kSharedRows, kKeys = kSharedKeys;
 constexpr int kFp8Row = 656, kFp8ScaleOff = 512, kFp8RopeOff = 528;
+constexpr int kThreads = 256;
 // Fewest tiles a workgroup is given.
 constexpr int kMinTiles = 2;
 
@@ -121,170 +122,6 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
 }
 
 // ------------------------------------------------------------------ main
-constexpr int kThreads = 256;
-
-// Row of the cache behind key `key` of sequence `seq`, or -1 (masked).
-__device__ __forceinline__ int64_t cache_row(const SharedParams& p, int seq, int key) {
-    if (p.block_table == nullptr) return (int64_t)seq * p.L + key;
-    const int blk = p.block_table[(int64_t)seq * p.max_blocks + key / p.block_size];
-    if ((uint32_t)blk >= (uint32_t)p.num_blocks) return -1;
-    return (int64_t)blk * p.block_size + key % p.block_size;
-}
-
-__global__ __launch_bounds__(kThreads) void shared_main_kernel(SharedParams p) {
-    __shared__ __attribute__((aligned(1024))) char smem[kKeys * 1152];
-    __shared__ uint32_t valid_rows;
-    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
-    const int lane = threadIdx.x & 63, g = lane >> 4, n16 = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-
-    const int total = p.tiles[p.items], groups = groups_of(p, total);
-    const int w = blockIdx.x;
-    if (w >= groups) return;
-    int t0 = (int)((int64_t)w * total / groups);
-    const int t1 = (int)((int64_t)(w + 1) * total / groups);
-    if (t0 >= t1) return;
-    int low = 0, high = p.items;  // the item that holds tile t0: tiles[low] <= t0 < tiles[low + 1]
-    while (high - low > 1) {
-        const int mid = (low + high) >> 1;
-        if (p.tiles[mid] <= t0) low = mid;
-        else high = mid;
-    }
-    for (int i = low; t0 < t1; ++i) {
-        const int begin = p.tiles[i], end = p.tiles[i + 1];
-        if (end <= t0) continue;
-        Item it = item_rows(p, i);
-        item_tiles(p, i, most_seen(p, it), it);
-        const int a = t0 - begin, b = min(t1, end) - begin;  // the item's tiles [a, b)
-        const bool live = 16 * wave < it.rows;
-        const int row = it.row0 + 16 * wave;
-        const int seen = live ? seen_by(p, row / p.H) : 0;
-        bf16x8 qf[18];
-        if (live) {
-            const uint16_t* q = p.q + (int64_t)(row + n16) * 512 + 8 * qk_lane_chunk(g);
-            for (int ks = 0; ks < 16; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(q + 32 * ks);
-            const uint16_t* r = p.q_rope + (int64_t)(row + n16) * 64 + 8 * g;
-            qf[16] = *reinterpret_cast<const bf16x8*>(r);
-            qf[17] = *reinterpret_cast<const bf16x8*>(r + 32);
-        }
-        f32x4 o[32];
-        for (int cb = 0; cb < 32; ++cb) o[cb] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float m = -FLT_MAX, l = 0.f;
-        for (int t = a; t < b; ++t) {
-            const bool shared = t < it.first;
-            const int key0 = shared ? t * kKeys : p.prefix + (t - it.first) * kKeys;
-            const int limit = shared ? min(seen, p.prefix) : seen;
-            const int key_end = shared ? p.prefix : p.L;
-            __syncthreads();
-            if (threadIdx.x < kKeys) {
-                const int key = key0 + (int)threadIdx.x;
-                const bool ok = key < key_end && cache_row(p, shared ? 0 : it.seq, key) >= 0;
-                const uint64_t v = __ballot(ok);
-                if (threadIdx.x == 0) valid_rows = (uint32_t)v;
-            }
-            for (int c = threadIdx.x; c < kKeys * 72; c += kThreads) {
-                const int r = c / 72, ch = c % 72, key = key0 + r;
-                const int64_t src = key < key_end ? cache_row(p, shared ? 0 : it.seq, key) : -1;
-                bf16x8 v = {};
-                if (src >= 0 && p.kv_fp8) {
-                    const char* raw = p.kv + src * kFp8Row;
-                    if (ch >= 64) {
-                        v = *reinterpret_cast<const bf16x8*>(raw + kFp8RopeOff + 16 * (ch - 64));
-                    } else {
-                        const float sc = *reinterpret_cast<const float*>(raw + kFp8ScaleOff + 4 * (ch >> 4));
-                        const int2 codes = *reinterpret_cast<const int2*>(raw + 8 * ch);
-                        for (int d = 0; d < 2; ++d) {
-                            const int code = d ? codes.y : codes.x;
-                            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(code, false);
-                            const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(code, true);
-                            v[4 * d + 0] = (__bf16)(lo[0] * sc);
-                            v[4 * d + 1] = (__bf16)(lo[1] * sc);
-                            v[4 * d + 2] = (__bf16)(hi[0] * sc);
-                            v[4 * d + 3] = (__bf16)(hi[1] * sc);
-                        }
-                    }
-                } else if (src >= 0) {
-                    v = ch < 64 ? *reinterpret_cast<const bf16x8*>(p.kv + src * 1024 + 16 * ch)
-                                : *reinterpret_cast<const bf16x8*>(p.k_rope + src * 64 + 8 * (ch - 64));
-                }
-                const uint32_t dst = ch < 64 ? r * 1024 + ((ch ^ sw_kv(r)) << 4)
-                                             : kKeys * 1024 + r * 128 + (((ch - 64) ^ sw_rope(r)) << 4);
-                lds_store<bf16x8>(lds + dst, v);
-            }
-            __syncthreads();
-            if (!live) continue;
-            // rows this wave's query sees: bit r is tile row r
-            const int n = min(max(limit - key0, 0), kKeys);
-            const uint32_t mask = valid_rows & (n == kKeys ? 0xffffffffu : (1u << n) - 1);
-            if (mask == 0) continue;
-            f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-            for (int ks = 0; ks < 18; ++ks)
-                for (int sub = 0; sub < 2; ++sub) {
-                    const int r = 16 * sub + n16;
-                    const uint32_t at = ks < 16 ? r * 1024 + (((4 * ks + qk_lane_chunk(g)) ^ sw_kv(r)) << 4)
-                                                : kKeys * 1024 + r * 128 + (((4 * (ks - 16) + g) ^ sw_rope(r)) << 4);
-                    s[sub] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lds_load<bf16x8>(lds + at), qf[ks], s[sub], 0, 0, 0);
-                }
-            // lane: rows 4 g + r (j < 4) and 16 + 4 g + r of head n16
-            float x[8], top = m;
-            uint32_t keep[4] = {0, 0, 0, 0};
-            for (int j = 0; j < 8; ++j) {
-                const bool on = mask >> (4 * g + (j & 3) + 16 * (j >> 2)) & 1;
-                x[j] = on ? s[j >> 2][j & 3] * p.scale_log2 : -INFINITY;
-                top = fmaxf(top, x[j]);
-                keep[j >> 1] |= on ? 0xffffu << (16 * (j & 1)) : 0u;
-            }
-            top = max_xor32(max_xor16(top));
-            const float alpha = fast_exp2(m - top);
-            m = top;
-            float sum = 0.f;
-            bf16x8 pk;
-            for (int j = 0; j < 8; ++j) {
-                const float e = fast_exp2(x[j] - top);
-                sum += e;
-                pk[j] = (__bf16)e;
-            }
-            l = l * alpha + sum;
-            const int vr = 4 * g + (n16 >> 2);
-            for (int cb = 0; cb < 32; ++cb) {
-                const uint32_t at = lds + vr * 1024 + (((2 * cb + ((n16 & 3) >> 1)) ^ sw_kv(vr)) << 4) + 8 * (n16 & 1);
-                const bf16x4 v0 = lds_load_tr(at), v1 = lds_load_tr(at + 16 * 1024);
-                // masked rows have weight 0, and are cleared so that no NaN or infinity in them counts
-                i32x4 v = __builtin_bit_cast(i32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-                for (int d = 0; d < 4; ++d) v[d] &= (int)keep[d];
-                o[cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), pk, o[cb] * alpha, 0, 0, 0);
-            }
-        }
-        l = sum_xor32(sum_xor16(l));
-        if (live) {
-            const bool whole = !p.stacked && a == 0 && b == end - begin;
-            if (whole) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                uint16_t* out = p.out + (int64_t)(row + n16) * 512 + 4 * g;
-                for (int cb = 0; cb < 32; ++cb) {
-                    bf16x4 v;
-                    for (int r = 0; r < 4; ++r) v[r] = (__bf16)(o[cb][r] * inv);
-                    *reinterpret_cast<bf16x4*>(out + 16 * cb) = v;
-                }
-                if (g == 0) {
-                    p.out_max[row + n16] = l == 0.f ? -INFINITY : m * kLn2;
-                    p.out_sum[row + n16] = l;
-                }
-            } else {
-                const int64_t prow = slot_of(p, i, w, a == 0) * kRows + 16 * wave + n16;
-                for (int cb = 0; cb < 32; ++cb)
-                    *reinterpret_cast<f32x4*>(p.part_o + prow * 512 + 16 * cb + 4 * g) = o[cb];
-                if (g == 0) {
-                    p.part_m[prow] = m;
-                    p.part_l[prow] = l;
-                }
-            }
-        }
-        t0 = min(t1, end);
-    }
-}
-
-// ------------------------------------------------------------------ bf16 rows
 // Eight waves in two groups of four (waves w and w + 4 share a SIMD).  Both
 // groups own the block's 64 rows and take its tiles in turn, half a tile apart,
 // so that on every SIMD one wave's softmax runs beside the other's MFMAs:
@@ -305,19 +142,36 @@ __global__ __launch_bounds__(kThreads) void shared_main_kernel(SharedParams p) {
 constexpr int kPPThreads = 512;
 constexpr float kRestartLog2 = 64.0f;
 
+// With fp8 rows the gathers land as stored (656 bytes) in a raw buffer of the
+// group that issues them, and that group expands the tile it issued last while
+// the other one scores:
+//
+//   half u:  the other group: tile u + 1 from raw to the ring, gathers of tile
+//            u + 3, PV of tile u - 1
+//
+// so the ring holds three tiles (scored, expanded, read by PV).
+template <bool FP8>
 struct PPLds {
-    static constexpr int NSTAGE = 4;
+    static constexpr int NSTAGE = FP8 ? 3 : 4;
     static constexpr int KV_BYTES = kKeys * 1024, STAGE_BYTES = kKeys * 1152;
+    static constexpr int RAW_OFF = NSTAGE * STAGE_BYTES, RAW_BYTES = FP8 ? kKeys * kFp8Row : 0;  // one a group
     // P of one group, 64 rows x 32 bf16 in the k order of the PV operand (pp_pchunk)
-    static constexpr int P_OFF = NSTAGE * STAGE_BYTES, P_GROUP = 64 * 64;
-    // per stage: block entries of a later tile (four waves x 8 rows), and which of the tile's rows are in the pool
+    static constexpr int P_OFF = RAW_OFF + 2 * RAW_BYTES, P_GROUP = 64 * 64;
+    // tiles whose block entries and pool bits are held: entries (four waves x 8
+    // rows) from when the tile two before it is issued, the bits of the rows
+    // that are in the pool from when it is issued until PV
+    static constexpr int NTILE = 8;
     static constexpr int ENTRY_OFF = P_OFF + 2 * P_GROUP;
-    static constexpr int VALID_OFF = ENTRY_OFF + NSTAGE * kKeys * 4;
-    static constexpr int ML_OFF = VALID_OFF + NSTAGE * 4;  // [3][128] floats: l, reference and maximum of each group's rows
-    static constexpr int FLAG_OFF = ML_OFF + 3 * 128 * 4;
+    static constexpr int VALID_OFF = ENTRY_OFF + NTILE * kKeys * 4;
+    static constexpr int FLAG_OFF = VALID_OFF + NTILE * 4;
     static constexpr int LDS_BYTES = FLAG_OFF + 16;
+    static constexpr int ML_OFF = P_OFF;  // [3][128] floats, at the end: l, reference and maximum of each group's rows
     static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
     __device__ static uint32_t stage(uint32_t lds, int u) { return lds + (uint32_t)(u % NSTAGE) * STAGE_BYTES; }
+    __device__ static uint32_t entries(uint32_t lds, int u, int row) {
+        return lds + ENTRY_OFF + (uint32_t)(u % NTILE) * (kKeys * 4) + 4 * row;
+    }
+    __device__ static uint32_t valid(uint32_t lds, int u) { return lds + VALID_OFF + 4 * (u % NTILE); }
 };
 
 // One tile of a piece: where its keys start, and the rows they are looked up in.
@@ -344,6 +198,17 @@ __device__ __forceinline__ int block_of(const SharedParams& p, int key) {
     return p.block_size == 1 ? key : (int)(__umulhi((uint32_t)key, p.block_magic) >> p.block_shift);
 }
 
+// One fp8 row: lanes 0..40 load 16 bytes each of its 656.
+__device__ __forceinline__ rsrc_t fp8_rsrc(const char* base, uint32_t row) {
+    const uint64_t a = reinterpret_cast<uint64_t>(base) + (uint64_t)row * kFp8Row;
+    rsrc_t r;
+    r[0] = (int)(uint32_t)a;
+    r[1] = (int)((a >> 32) & 0xffff);
+    r[2] = kFp8Row;
+    r[3] = 0x00020000;
+    return r;
+}
+
 // 4 bytes a lane straight into LDS (lane l at m0 + 4 l).
 __device__ __forceinline__ void gather_words(uint32_t lds_base, rsrc_t rsrc, uint32_t voff) {
 #pragma clang diagnostic push
@@ -357,66 +222,140 @@ __device__ __forceinline__ void gather_words(uint32_t lds_base, rsrc_t rsrc, uin
 #pragma clang diagnostic pop
 }
 
-// Gathers of tile u by wave gw of a group: rows 8 gw .. 8 gw + 7, 1 KiB each in
-// one instruction, and their rotary parts in one.  Paged: the rows' block
+// Gathers of tile u by wave gw of group grp: rows 8 gw .. 8 gw + 7, one
+// instruction each, and (bf16) their rotary parts in one.  Paged: the rows' block
 // entries were loaded into LDS when this wave issued tile u - 2 (waited for
 // since) -- for the piece's first tiles, `first`, they are loaded here -- and
 // those of tile u + 2 are issued behind the rows.
+template <bool FP8>
 __device__ __forceinline__ void issue_rows(const SharedParams& p, const Piece& c, int u, bool first, uint32_t lds,
-                                           int gw, int lane) {
+                                           int grp, int gw, int lane) {
+    using X = PPLds<FP8>;
     asm volatile("" : "+v"(lane));
     const Tile k = tile_at(p, c, u);
-    const uint32_t stage = PPLds::stage(lds, u);
     const int r0 = 8 * gw;
     const int key_r = min(k.key0 + r0 + (lane & 7), k.key_end - 1);  // the row the wave reads ..
     const int key_l = min(k.key0 + r0 + (lane >> 3), k.key_end - 1); // .. and the one whose rotary part the lane reads
     const char* kv = p.kv;
     const char* kr = reinterpret_cast<const char*>(p.k_rope);
-    int my_row, rope_row;
+    int my_row, rope_row = 0;
     uint32_t pool;
     if (p.block_table == nullptr) {
         const int64_t base = (int64_t)k.seq * p.L;
-        kv += base << 10;
+        kv += base * (FP8 ? kFp8Row : 1024);
         kr += base << 7;
         my_row = key_r;
         rope_row = key_l;
         pool = (uint32_t)p.L << 7;
     } else {
-        const uint32_t entries = lds + PPLds::ENTRY_OFF + (uint32_t)(u % PPLds::NSTAGE) * (kKeys * 4) + 4 * r0;
         const int32_t* table = p.block_table + (int64_t)k.seq * p.max_blocks;
         const int col_r = block_of(p, key_r), col_l = block_of(p, key_l);
-        int e_r, e_l;
+        int e_r, e_l = 0;
         if (first) {
             e_r = table[col_r];
-            e_l = table[col_l];
+            if (!FP8) e_l = table[col_l];
         } else {
-            e_r = lds_load<int>(entries + 4 * (lane & 7));
-            e_l = lds_load<int>(entries + 4 * (lane >> 3));
+            e_r = lds_load<int>(X::entries(lds, u, r0 + (lane & 7)));
+            if (!FP8) e_l = lds_load<int>(X::entries(lds, u, r0 + (lane >> 3)));
         }
-        const bool ok_r = (uint32_t)e_r < (uint32_t)p.num_blocks, ok_l = (uint32_t)e_l < (uint32_t)p.num_blocks;
+        const bool ok_r = (uint32_t)e_r < (uint32_t)p.num_blocks;
         const uint64_t valid = __ballot(ok_r) & 0xff;
-        if (lane == 0)
-            lds_store<uint8_t>(lds + PPLds::VALID_OFF + 4 * (u % PPLds::NSTAGE) + gw, (uint8_t)valid);
+        if (lane == 0) lds_store<uint8_t>(X::valid(lds, u) + gw, (uint8_t)valid);
         my_row = (ok_r ? e_r : 0) * p.block_size + (key_r - col_r * p.block_size);
-        rope_row = (ok_l ? e_l : 0) * p.block_size + (key_l - col_l * p.block_size);
+        if (!FP8) {
+            const bool ok_l = (uint32_t)e_l < (uint32_t)p.num_blocks;
+            rope_row = (ok_l ? e_l : 0) * p.block_size + (key_l - col_l * p.block_size);
+        }
         pool = (uint32_t)(p.num_blocks * p.block_size) << 7;
     }
     const uint32_t lane16 = (uint32_t)lane << 4;
+    if constexpr (FP8) {
+        const uint32_t raw = lds + X::RAW_OFF + grp * X::RAW_BYTES + r0 * kFp8Row;
+        if (lane < kFp8Row / 16) {
 #pragma unroll
-    for (int rr = 0; rr < 8; ++rr)
-        gather_row(stage + (r0 + rr) * 1024, row_rsrc(kv, (uint32_t)__builtin_amdgcn_readlane(my_row, rr)), lane16,
-                   (uint32_t)sw_kv(r0 + rr) << 4);
-    const int r = r0 + (lane >> 3);
-    gather_lanes(stage + PPLds::KV_BYTES + r0 * 128, make_rsrc(kr, pool),
-                 ((uint32_t)rope_row << 7) + (((lane & 7) ^ sw_rope(r)) << 4));
+            for (int rr = 0; rr < 8; ++rr)
+                gather_lanes(raw + rr * kFp8Row, fp8_rsrc(kv, (uint32_t)__builtin_amdgcn_readlane(my_row, rr)), lane16);
+        }
+    } else {
+        const uint32_t stage = X::stage(lds, u);
+#pragma unroll
+        for (int rr = 0; rr < 8; ++rr)
+            gather_row(stage + (r0 + rr) * 1024, row_rsrc(kv, (uint32_t)__builtin_amdgcn_readlane(my_row, rr)), lane16,
+                       (uint32_t)sw_kv(r0 + rr) << 4);
+        const int r = r0 + (lane >> 3);
+        gather_lanes(stage + X::KV_BYTES + r0 * 128, make_rsrc(kr, pool),
+                     ((uint32_t)rope_row << 7) + (((lane & 7) ^ sw_rope(r)) << 4));
+    }
     if (p.block_table != nullptr && u + 2 < c.nt) {
         const Tile n = tile_at(p, c, u + 2);
         const int key = min(n.key0 + r0 + lane, n.key_end - 1);
         if (lane < 8)
-            gather_words(lds + PPLds::ENTRY_OFF + (uint32_t)((u + 2) % PPLds::NSTAGE) * (kKeys * 4) + 4 * r0,
+            gather_words(X::entries(lds, u + 2, r0),
                          make_rsrc(p.block_table + (int64_t)n.seq * p.max_blocks, 4u * (uint32_t)p.max_blocks),
                          4u * (uint32_t)block_of(p, key));
     }
+}
+
+// The rows that this wave gathered last, from the group's raw buffer to tile u
+// of the ring: lane l takes 64 latent values of row l % 8, from 64 (l / 8) on,
+// and 16 bytes of the rotary part of row l / 8.  kv[d] = bf16(fp32(e4m3) *
+// scale), both roundings to nearest even; where all scales are powers of two
+// (2^-100 .. 2^100), one conversion a pair gives the same bits.
+__device__ __forceinline__ void expand_rows(uint32_t lds, int u, int grp, int gw, int lane) {
+    using X = PPLds<true>;
+    asm volatile("" : "+v"(lane));
+    const uint32_t raw = lds + X::RAW_OFF + grp * X::RAW_BYTES + 8 * gw * kFp8Row;
+    const uint32_t stage = X::stage(lds, u);
+    const int r = lane & 7, part = lane >> 3, row = 8 * gw + r;
+    const uint32_t src = raw + r * kFp8Row;
+    const float sc = lds_load<float>(src + kFp8ScaleOff + 4 * (part >> 1));
+    i32x4 v[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) v[m] = lds_load<i32x4>(src + 64 * part + 16 * m);
+    const int rope = 8 * gw + part;
+    const i32x4 turned = lds_load<i32x4>(raw + part * kFp8Row + kFp8RopeOff + 16 * r);
+    const uint32_t sb = __float_as_uint(sc), sexp = sb >> 23 & 0xffu;
+    const bool pow2 = (sb & 0x807fffffu) == 0 && sexp >= 27u && sexp <= 227u;
+    const uint32_t dst = stage + row * 1024, sw = (uint32_t)sw_kv(row);
+    auto put = [&](int m, int h, const bf16x8& o) {
+        lds_store<bf16x8>(dst + (((uint32_t)(8 * part + 2 * m + h) ^ sw) << 4), o);
+    };
+    if (__all(pow2)) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                bf16x8 o;
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[m][2 * h + d], sc, false);
+                    const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[m][2 * h + d], sc, true);
+                    o[4 * d + 0] = lo[0];
+                    o[4 * d + 1] = lo[1];
+                    o[4 * d + 2] = hi[0];
+                    o[4 * d + 3] = hi[1];
+                }
+                put(m, h, o);
+            }
+    } else {
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                bf16x8 o;
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(v[m][2 * h + d], false);
+                    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(v[m][2 * h + d], true);
+                    o[4 * d + 0] = (__bf16)(lo[0] * sc);
+                    o[4 * d + 1] = (__bf16)(lo[1] * sc);
+                    o[4 * d + 2] = (__bf16)(hi[0] * sc);
+                    o[4 * d + 3] = (__bf16)(hi[1] * sc);
+                }
+                put(m, h, o);
+            }
+    }
+    lds_store<i32x4>(stage + X::KV_BYTES + rope * 128 + ((r ^ sw_rope(rope)) << 4), turned);
 }
 
 // Which of the 32 keys of a tile a query row that sees `seen` rows has: bit r is tile row r.
@@ -452,10 +391,10 @@ __device__ __forceinline__ void clear_specials(uint32_t stage, int gw, int lane)
 }
 
 // One piece of an item with up to 16 NB rows.
-template <int NB>
+template <bool FP8, int NB>
 __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece& c, bool whole, int64_t slot,
                                              uint32_t lds, int wave, int lane) {
-    using X = PPLds;
+    using X = PPLds<FP8>;
     const int grp = wave >> 2, gw = wave & 3;
     const int g = lane >> 4, n16 = lane & 15;
     const bool live = 16 * gw < c.it.rows;  // this wave has query rows
@@ -494,7 +433,7 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         asm volatile("" : "+v"(off_kv), "+v"(off_rope), "+v"(off_p));
         const uint32_t kbase = stage + (off_kv & 0xffffu);
         const uint32_t rbase = stage + off_rope;
-        const int valid_v = lds_load<int>(lds + X::VALID_OFF + 4 * (u % X::NSTAGE));
+        const int valid_v = lds_load<int>(X::valid(lds, u));
         auto kfrag = [&](int step) -> bf16x8 {
             const int ks = step >> 1, sub = step & 1;
             if (ks < 16) return lds_load<bf16x8>((kbase ^ (64u * (ks & 3))) + 256u * (ks >> 2) + sub * 16 * 1024);
@@ -559,7 +498,7 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         const uint32_t stage = X::stage(lds, u);
         asm volatile("" : "+v"(off_kv), "+v"(off_p));
         const uint32_t valid = (uint32_t)__builtin_amdgcn_readfirstlane(
-            lds_load<int>(lds + X::VALID_OFF + 4 * (u % X::NSTAGE)));
+            lds_load<int>(X::valid(lds, u)));
         const Tile k = tile_at(p, c, u);
         const uint32_t vbase = stage + (off_kv >> 16);
         auto vfrag = [&](int cb) -> bf16x8 {
@@ -596,33 +535,60 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         l_run = 0.f;
         if (pass == 1) m_ref = m_true;
         bool overflow = false;
-        // Half u: group u % 2 scores tile u; the other group issues tile u + 2
-        // (into the stage of tile u - 2, whose last reader ran in half u - 1)
-        // and runs PV of tile u - 1.  A group scores the tile after the one it
-        // issued last, and its full wait behind that covers the tile it issued
-        // and the block entries of the one it issues next.
-        if (grp == 1) issue_rows(p, c, 0, true, lds, gw, lane);
-        wait_vmcnt<0>();
-        if (grp == 0 && nt > 1) issue_rows(p, c, 1, true, lds, gw, lane);
+        // Half u: group u % 2 scores tile u.  The other group, bf16: issues tile
+        // u + 2 (into the stage of tile u - 2, whose last reader ran in half
+        // u - 1) and runs PV of tile u - 1; a group scores the tile after the
+        // one it issued last, and its full wait behind that covers the tile it
+        // issued and the block entries of the one it issues next.  fp8: waits
+        // for tile u + 1, which it issued in half u - 2, expands it (into the
+        // stage of tile u - 2), issues tile u + 3 and runs PV of tile u - 1.
+        auto scored = [&]() __attribute__((always_inline)) {
+            if constexpr (!FP8) wait_vmcnt<0>();
+        };
+        auto between = [&](int u) __attribute__((always_inline)) {  // in half u, ahead of PV
+            if constexpr (FP8) {
+                if (u + 1 < nt) {
+                    wait_vmcnt<0>();
+                    expand_rows(lds, u + 1, grp, gw, lane);
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // raw is read before it is written again
+                    if (u + 3 < nt) issue_rows<FP8>(p, c, u + 3, false, lds, grp, gw, lane);
+                }
+            } else {
+                if (u + 2 < nt) issue_rows<FP8>(p, c, u + 2, false, lds, grp, gw, lane);
+            }
+        };
+        if constexpr (FP8) {
+            if (grp == 0 || nt > 1) issue_rows<FP8>(p, c, grp, true, lds, grp, gw, lane);
+            wait_vmcnt<0>();
+            if (grp == 0) {
+                expand_rows(lds, 0, grp, gw, lane);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (nt > 2) issue_rows<FP8>(p, c, 2, false, lds, grp, gw, lane);
+            }
+        } else {
+            if (grp == 1) issue_rows<FP8>(p, c, 0, true, lds, grp, gw, lane);
+            wait_vmcnt<0>();
+            if (grp == 0 && nt > 1) issue_rows<FP8>(p, c, 1, true, lds, grp, gw, lane);
+        }
         if (grp == 0) {
             for (int u = 0; u < nt; u += 2) {
                 lds_barrier();
                 if (live) qk_softmax(u, overflow);
-                wait_vmcnt<0>();
+                scored();
                 lds_barrier();
-                if (u + 3 < nt) issue_rows(p, c, u + 3, false, lds, gw, lane);
+                between(u + 1);
                 pv(u);
             }
             if ((nt & 1) == 0) lds_barrier();  // half nt: group 1's last PV
         } else {
             lds_barrier();
-            if (2 < nt) issue_rows(p, c, 2, false, lds, gw, lane);
+            between(0);
             for (int u = 1; u < nt; u += 2) {
                 lds_barrier();
                 if (live) qk_softmax(u, overflow);
-                wait_vmcnt<0>();
+                scored();
                 lds_barrier();
-                if (u + 3 < nt) issue_rows(p, c, u + 3, false, lds, gw, lane);
+                between(u + 1);
                 pv(u);
             }
             if (nt & 1) lds_barrier();  // half nt: group 0's last PV
@@ -658,7 +624,8 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
     constexpr int HROW = 1040;       // bytes of a staged bf16 row (16 more: rows spread over the banks)
     constexpr int kPartRow = 2064;   // of a staged fp32 row
     constexpr uint32_t kHand = NB * 4 * 1024;  // one wave's half: NB row x 4 column blocks of 64 lanes x 16 bytes
-    static_assert(8 * kHand <= X::P_OFF && 64 * kPartRow <= X::P_OFF, "staging fits the ring");
+    static_assert(8 * kHand <= X::P_OFF && 64 * kPartRow <= X::P_OFF, "staging fits the ring and raw buffers");
+    static_assert(3 * 128 * 4 <= 2 * X::P_GROUP, "statistics fit the P buffers");
     const uint32_t give = lds + (uint32_t)wave * kHand + 16u * (uint32_t)eln;
     const uint32_t take = lds + (uint32_t)(wave ^ 4) * kHand + 16u * (uint32_t)eln;
     float scale[NB];
@@ -737,8 +704,10 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
     lds_barrier();  // the ring is free for the next piece
 }
 
-__global__ __launch_bounds__(kPPThreads, 1) void shared_pp_kernel(SharedParams p) {
-    __shared__ __attribute__((aligned(1024))) char smem[PPLds::LDS_BYTES];
+template <bool FP8>
+__global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams p) {
+    using X = PPLds<FP8>;
+    __shared__ __attribute__((aligned(1024))) char smem[X::LDS_BYTES];
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -748,7 +717,7 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_pp_kernel(SharedParams p
     int t0 = (int)((int64_t)w * total / groups);
     const int t1 = (int)((int64_t)(w + 1) * total / groups);
     if (t0 >= t1) return;
-    if (threadIdx.x < PPLds::NSTAGE) lds_store<uint32_t>(lds + PPLds::VALID_OFF + 4 * threadIdx.x, 0xffffffffu);
+    if (threadIdx.x < X::NTILE) lds_store<uint32_t>(X::valid(lds, threadIdx.x), 0xffffffffu);
     int i = 0, high = p.items;  // the item that holds tile t0: tiles[i] <= t0 < tiles[i + 1]
     while (high - i > 1) {
         const int mid = (i + high) >> 1;
@@ -774,9 +743,9 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_pp_kernel(SharedParams p
         c.nt = __builtin_amdgcn_readfirstlane(min(t1, end) - t0);
         const bool whole = !p.stacked && c.nt == end - begin;
         const int64_t slot = slot_of(p, i, w, c.a == 0);
-        if (c.it.rows <= 16) shared_piece<1>(p, c, whole, slot, lds, wave, lane);
-        else if (c.it.rows <= 32) shared_piece<2>(p, c, whole, slot, lds, wave, lane);
-        else shared_piece<4>(p, c, whole, slot, lds, wave, lane);
+        if (c.it.rows <= 16) shared_piece<FP8, 1>(p, c, whole, slot, lds, wave, lane);
+        else if (c.it.rows <= 32) shared_piece<FP8, 2>(p, c, whole, slot, lds, wave, lane);
+        else shared_piece<FP8, 4>(p, c, whole, slot, lds, wave, lane);
         t0 = min(t1, end);
     }
 }
@@ -824,10 +793,8 @@ int launch_shared(const SharedParams& p, hipStream_t stream) {
     hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
     int rc = (int)hipGetLastError();
     if (rc) return rc;
-    if (p.kv_fp8)
-        hipLaunchKernelGGL(shared_main_kernel, dim3(p.workgroups), dim3(kThreads), 0, stream, p);
-    else
-        hipLaunchKernelGGL(shared_pp_kernel, dim3(p.workgroups), dim3(kPPThreads), 0, stream, p);
+    hipLaunchKernelGGL(p.kv_fp8 ? shared_main_kernel<true> : shared_main_kernel<false>, dim3(p.workgroups),
+                       dim3(kPPThreads), 0, stream, p);
     rc = (int)hipGetLastError();
     if (rc) return rc;
     const int rows = p.B * p.SQ * p.H;
