@@ -222,79 +222,101 @@ __device__ __forceinline__ void gather_words(uint32_t lds_base, rsrc_t rsrc, uin
 #pragma clang diagnostic pop
 }
 
-// Gathers of tile u by wave gw of group grp: rows 8 gw .. 8 gw + 7, one
-// instruction each, and (bf16) their rotary parts in one.  Paged: the rows' block
-// entries were loaded into LDS when this wave issued tile u - 2 (waited for
-// since) -- for the piece's first tiles, `first`, they are loaded here -- and
-// those of tile u + 2 are issued behind the rows.
-template <bool FP8>
-__device__ __forceinline__ void issue_rows(const SharedParams& p, const Piece& c, int u, bool first, uint32_t lds,
-                                           int grp, int gw, int lane) {
-    using X = PPLds<FP8>;
-    asm volatile("" : "+v"(lane));
-    const Tile k = tile_at(p, c, u);
-    const int r0 = 8 * gw;
-    const int key_r = min(k.key0 + r0 + (lane & 7), k.key_end - 1);  // the row the wave reads ..
-    const int key_l = min(k.key0 + r0 + (lane >> 3), k.key_end - 1); // .. and the one whose rotary part the lane reads
-    const char* kv = p.kv;
-    const char* kr = reinterpret_cast<const char*>(p.k_rope);
-    int my_row, rope_row = 0;
-    uint32_t pool;
-    if (p.block_table == nullptr) {
-        const int64_t base = (int64_t)k.seq * p.L;
-        kv += base * (FP8 ? kFp8Row : 1024);
-        kr += base << 7;
-        my_row = key_r;
-        rope_row = key_l;
-        pool = (uint32_t)p.L << 7;
-    } else {
-        const int32_t* table = p.block_table + (int64_t)k.seq * p.max_blocks;
-        const int col_r = block_of(p, key_r), col_l = block_of(p, key_l);
-        int e_r, e_l = 0;
-        if (first) {
-            e_r = table[col_r];
-            if (!FP8) e_l = table[col_l];
+// Gathers of one tile by wave gw of a group: rows 8 gw .. 8 gw + 7, one
+// instruction each (row), and (bf16) their rotary parts in one (rest).  They are
+// issued one at a time between the steps of PV: the texture path takes 64 bytes
+// a clock, and issued together they would hold the wave up.  Paged: the rows'
+// block entries were loaded into LDS when this wave issued the tile two before
+// (waited for since) -- for the piece's first tiles, `first`, they are loaded
+// here -- and those of the tile two further on are issued last.
+template <bool FP8, bool PAGED>
+struct Gathers {
+    const char* kv;
+    rsrc_t kr;
+    int my_row;        // lane l: row 8 gw + l % 8
+    uint32_t rope_off; // lane l: its 16 bytes of the rotary part of row 8 gw + l / 8
+    uint32_t dst, rope_dst;
+
+    __device__ __forceinline__ void prepare(const SharedParams& p, const Piece& c, int u, bool first, uint32_t lds,
+                                            int grp, int gw, int lane) {
+        using X = PPLds<FP8>;
+        asm volatile("" : "+v"(lane));
+        const Tile k = tile_at(p, c, u);
+        const int r0 = 8 * gw;
+        const int key_r = min(k.key0 + r0 + (lane & 7), k.key_end - 1);
+        const int key_l = min(k.key0 + r0 + (lane >> 3), k.key_end - 1);
+        int rope_row = 0;
+        kv = p.kv;
+        const char* rope = reinterpret_cast<const char*>(p.k_rope);
+        uint32_t pool;
+        if constexpr (!PAGED) {
+            const int64_t base = (int64_t)k.seq * p.L;
+            kv += base * (FP8 ? kFp8Row : 1024);
+            rope += base << 7;
+            my_row = key_r;
+            rope_row = key_l;
+            pool = (uint32_t)p.L << 7;
         } else {
-            e_r = lds_load<int>(X::entries(lds, u, r0 + (lane & 7)));
-            if (!FP8) e_l = lds_load<int>(X::entries(lds, u, r0 + (lane >> 3)));
+            const int32_t* table = p.block_table + (int64_t)k.seq * p.max_blocks;
+            const int col_r = block_of(p, key_r), col_l = block_of(p, key_l);
+            int e_r, e_l = 0;
+            if (first) {
+                e_r = table[col_r];
+                if (!FP8) e_l = table[col_l];
+            } else {
+                e_r = lds_load<int>(X::entries(lds, u, r0 + (lane & 7)));
+                if (!FP8) e_l = lds_load<int>(X::entries(lds, u, r0 + (lane >> 3)));
+            }
+            const bool ok_r = (uint32_t)e_r < (uint32_t)p.num_blocks;
+            const uint64_t valid = __ballot(ok_r) & 0xff;
+            if (lane == 0) lds_store<uint8_t>(X::valid(lds, u) + gw, (uint8_t)valid);
+            my_row = (ok_r ? e_r : 0) * p.block_size + (key_r - col_r * p.block_size);
+            if (!FP8) {
+                const bool ok_l = (uint32_t)e_l < (uint32_t)p.num_blocks;
+                rope_row = (ok_l ? e_l : 0) * p.block_size + (key_l - col_l * p.block_size);
+            }
+            pool = (uint32_t)(p.num_blocks * p.block_size) << 7;
         }
-        const bool ok_r = (uint32_t)e_r < (uint32_t)p.num_blocks;
-        const uint64_t valid = __ballot(ok_r) & 0xff;
-        if (lane == 0) lds_store<uint8_t>(X::valid(lds, u) + gw, (uint8_t)valid);
-        my_row = (ok_r ? e_r : 0) * p.block_size + (key_r - col_r * p.block_size);
-        if (!FP8) {
-            const bool ok_l = (uint32_t)e_l < (uint32_t)p.num_blocks;
-            rope_row = (ok_l ? e_l : 0) * p.block_size + (key_l - col_l * p.block_size);
+        if constexpr (FP8) {
+            dst = lds + X::RAW_OFF + grp * X::RAW_BYTES + r0 * kFp8Row;
+        } else {
+            dst = X::stage(lds, u) + r0 * 1024;
+            rope_dst = X::stage(lds, u) + X::KV_BYTES + r0 * 128;
+            kr = make_rsrc(rope, pool);
+            rope_off = ((uint32_t)rope_row << 7) + (((lane & 7) ^ sw_rope(r0 + (lane >> 3))) << 4);
         }
-        pool = (uint32_t)(p.num_blocks * p.block_size) << 7;
     }
-    const uint32_t lane16 = (uint32_t)lane << 4;
-    if constexpr (FP8) {
-        const uint32_t raw = lds + X::RAW_OFF + grp * X::RAW_BYTES + r0 * kFp8Row;
-        if (lane < kFp8Row / 16) {
+    __device__ __forceinline__ void row(int rr, int gw, int lane) const {
+        const uint32_t lane16 = (uint32_t)lane << 4;
+        const uint32_t r = (uint32_t)__builtin_amdgcn_readlane(my_row, rr);
+        if constexpr (FP8) {
+            if (lane < kFp8Row / 16) gather_lanes(dst + rr * kFp8Row, fp8_rsrc(kv, r), lane16);
+        } else {
+            gather_row(dst + rr * 1024, row_rsrc(kv, r), lane16, (uint32_t)sw_kv(8 * gw + rr) << 4);
+        }
+    }
+    __device__ __forceinline__ void rest(const SharedParams& p, const Piece& c, int u, uint32_t lds, int gw,
+                                         int lane) const {
+        using X = PPLds<FP8>;
+        if constexpr (!FP8) gather_lanes(rope_dst, kr, rope_off);
+        if constexpr (PAGED)
+            if (u + 2 < c.nt) {
+                const Tile n = tile_at(p, c, u + 2);
+                const int key = min(n.key0 + 8 * gw + lane, n.key_end - 1);
+                if (lane < 8)
+                    gather_words(X::entries(lds, u + 2, 8 * gw),
+                                 make_rsrc(p.block_table + (int64_t)n.seq * p.max_blocks, 4u * (uint32_t)p.max_blocks),
+                                 4u * (uint32_t)block_of(p, key));
+            }
+    }
+    __device__ __forceinline__ void all(const SharedParams& p, const Piece& c, int u, bool first, uint32_t lds, int grp,
+                                        int gw, int lane) {
+        prepare(p, c, u, first, lds, grp, gw, lane);
 #pragma unroll
-            for (int rr = 0; rr < 8; ++rr)
-                gather_lanes(raw + rr * kFp8Row, fp8_rsrc(kv, (uint32_t)__builtin_amdgcn_readlane(my_row, rr)), lane16);
-        }
-    } else {
-        const uint32_t stage = X::stage(lds, u);
-#pragma unroll
-        for (int rr = 0; rr < 8; ++rr)
-            gather_row(stage + (r0 + rr) * 1024, row_rsrc(kv, (uint32_t)__builtin_amdgcn_readlane(my_row, rr)), lane16,
-                       (uint32_t)sw_kv(r0 + rr) << 4);
-        const int r = r0 + (lane >> 3);
-        gather_lanes(stage + X::KV_BYTES + r0 * 128, make_rsrc(kr, pool),
-                     ((uint32_t)rope_row << 7) + (((lane & 7) ^ sw_rope(r)) << 4));
+        for (int rr = 0; rr < 8; ++rr) row(rr, gw, lane);
+        rest(p, c, u, lds, gw, lane);
     }
-    if (p.block_table != nullptr && u + 2 < c.nt) {
-        const Tile n = tile_at(p, c, u + 2);
-        const int key = min(n.key0 + r0 + lane, n.key_end - 1);
-        if (lane < 8)
-            gather_words(X::entries(lds, u + 2, r0),
-                         make_rsrc(p.block_table + (int64_t)n.seq * p.max_blocks, 4u * (uint32_t)p.max_blocks),
-                         4u * (uint32_t)block_of(p, key));
-    }
-}
+};
 
 // The rows that this wave gathered last, from the group's raw buffer to tile u
 // of the ring: lane l takes 64 latent values of row l % 8, from 64 (l / 8) on,
@@ -391,7 +413,7 @@ __device__ __forceinline__ void clear_specials(uint32_t stage, int gw, int lane)
 }
 
 // One piece of an item with up to 16 NB rows.
-template <bool FP8, int NB>
+template <bool FP8, bool PAGED, int NB>
 __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece& c, bool whole, int64_t slot,
                                              uint32_t lds, int wave, int lane) {
     using X = PPLds<FP8>;
@@ -399,6 +421,7 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
     const int g = lane >> 4, n16 = lane & 15;
     const bool live = 16 * gw < c.it.rows;  // this wave has query rows
     const int row = c.it.row0 + 16 * gw;
+    const int nt = c.nt;
     const int seen = live ? __builtin_amdgcn_readfirstlane(seen_by(p, row / p.H)) : 0;
     const uint32_t p_lds = lds + X::P_OFF + grp * X::P_GROUP;
 
@@ -494,7 +517,8 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         lds_store<bf16x8>(p_lds + (off_p >> 16), pk);
     };
 
-    auto pv = [&](int u) __attribute__((always_inline)) {
+    // PV of tile u, with the gathers of tile `next` (if any) between its steps.
+    auto pv = [&](int u, int next) __attribute__((always_inline)) {
         const uint32_t stage = X::stage(lds, u);
         asm volatile("" : "+v"(off_kv), "+v"(off_p));
         const uint32_t valid = (uint32_t)__builtin_amdgcn_readfirstlane(
@@ -508,6 +532,9 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
             return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
         };
         if (__builtin_expect(key_mask(k, c.seen_low, valid) != 0xffffffffu, 0)) clear_specials(stage, gw, lane);
+        const bool more = next < nt;
+        Gathers<FP8, PAGED> gather;
+        if (more) gather.prepare(p, c, next, false, lds, grp, gw, lane);
         bf16x8 pf[NB];
 #pragma unroll
         for (int hb = 0; hb < NB; ++hb) pf[hb] = lds_load<bf16x8>(p_lds + (off_p & 0xffffu) + 1024 * hb);
@@ -521,11 +548,12 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
             for (int hb = 0; hb < NB; ++hb)
                 oacc[hb][cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[cb % VD], pf[hb], oacc[hb][cb], 0, 0, 0);
             if (cb + VD < 8) vf[cb % VD] = vfrag(cb + VD);
+            if (more) gather.row(cb, gw, lane);
             __builtin_amdgcn_sched_barrier(0);
         }
+        if (more) gather.rest(p, c, next, lds, gw, lane);
     };
 
-    const int nt = c.nt;
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
@@ -545,54 +573,43 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         auto scored = [&]() __attribute__((always_inline)) {
             if constexpr (!FP8) wait_vmcnt<0>();
         };
-        auto between = [&](int u) __attribute__((always_inline)) {  // in half u, ahead of PV
-            if constexpr (FP8) {
-                if (u + 1 < nt) {
+        auto expand = [&](int u) __attribute__((always_inline)) {
+            if constexpr (FP8)
+                if (u < nt) {
                     wait_vmcnt<0>();
-                    expand_rows(lds, u + 1, grp, gw, lane);
+                    expand_rows(lds, u, grp, gw, lane);
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // raw is read before it is written again
-                    if (u + 3 < nt) issue_rows<FP8>(p, c, u + 3, false, lds, grp, gw, lane);
                 }
-            } else {
-                if (u + 2 < nt) issue_rows<FP8>(p, c, u + 2, false, lds, grp, gw, lane);
-            }
         };
+        Gathers<FP8, PAGED> gather;
+        constexpr int AHEAD = FP8 ? 3 : 2;  // the tile issued in half u is u + AHEAD
         if constexpr (FP8) {
-            if (grp == 0 || nt > 1) issue_rows<FP8>(p, c, grp, true, lds, grp, gw, lane);
+            if (grp == 0 || nt > 1) gather.all(p, c, grp, true, lds, grp, gw, lane);
             wait_vmcnt<0>();
             if (grp == 0) {
-                expand_rows(lds, 0, grp, gw, lane);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (nt > 2) issue_rows<FP8>(p, c, 2, false, lds, grp, gw, lane);
+                expand(0);
+                if (nt > 2) gather.all(p, c, 2, false, lds, grp, gw, lane);
             }
         } else {
-            if (grp == 1) issue_rows<FP8>(p, c, 0, true, lds, grp, gw, lane);
+            if (grp == 1) gather.all(p, c, 0, true, lds, grp, gw, lane);
             wait_vmcnt<0>();
-            if (grp == 0 && nt > 1) issue_rows<FP8>(p, c, 1, true, lds, grp, gw, lane);
+            if (grp == 0 && nt > 1) gather.all(p, c, 1, true, lds, grp, gw, lane);
         }
-        if (grp == 0) {
-            for (int u = 0; u < nt; u += 2) {
-                lds_barrier();
-                if (live) qk_softmax(u, overflow);
-                scored();
-                lds_barrier();
-                between(u + 1);
-                pv(u);
-            }
-            if ((nt & 1) == 0) lds_barrier();  // half nt: group 1's last PV
-        } else {
+        if (grp == 1) {  // half 0, without PV
             lds_barrier();
-            between(0);
-            for (int u = 1; u < nt; u += 2) {
-                lds_barrier();
-                if (live) qk_softmax(u, overflow);
-                scored();
-                lds_barrier();
-                between(u + 1);
-                pv(u);
-            }
-            if (nt & 1) lds_barrier();  // half nt: group 0's last PV
+            expand(1);
+            if (AHEAD < nt) gather.all(p, c, AHEAD, false, lds, grp, gw, lane);
         }
+#pragma unroll 1
+        for (int u = grp; u < nt; u += 2) {
+            lds_barrier();
+            if (live) qk_softmax(u, overflow);
+            scored();
+            lds_barrier();
+            expand(u + 2);
+            pv(u, u + 1 + AHEAD);
+        }
+        if (((nt ^ grp) & 1) == 0) lds_barrier();  // half nt: the other group's last PV
         if (pass == 1) break;
         // does any row need the second pass?
         const uint32_t flag = lds + X::FLAG_OFF;
@@ -704,7 +721,7 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
     lds_barrier();  // the ring is free for the next piece
 }
 
-template <bool FP8>
+template <bool FP8, bool PAGED>
 __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams p) {
     using X = PPLds<FP8>;
     __shared__ __attribute__((aligned(1024))) char smem[X::LDS_BYTES];
@@ -743,9 +760,9 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
         c.nt = __builtin_amdgcn_readfirstlane(min(t1, end) - t0);
         const bool whole = !p.stacked && c.nt == end - begin;
         const int64_t slot = slot_of(p, i, w, c.a == 0);
-        if (c.it.rows <= 16) shared_piece<FP8, 1>(p, c, whole, slot, lds, wave, lane);
-        else if (c.it.rows <= 32) shared_piece<FP8, 2>(p, c, whole, slot, lds, wave, lane);
-        else shared_piece<FP8, 4>(p, c, whole, slot, lds, wave, lane);
+        if (c.it.rows <= 16) shared_piece<FP8, PAGED, 1>(p, c, whole, slot, lds, wave, lane);
+        else if (c.it.rows <= 32) shared_piece<FP8, PAGED, 2>(p, c, whole, slot, lds, wave, lane);
+        else shared_piece<FP8, PAGED, 4>(p, c, whole, slot, lds, wave, lane);
         t0 = min(t1, end);
     }
 }
@@ -793,8 +810,9 @@ int launch_shared(const SharedParams& p, hipStream_t stream) {
     hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
     int rc = (int)hipGetLastError();
     if (rc) return rc;
-    hipLaunchKernelGGL(p.kv_fp8 ? shared_main_kernel<true> : shared_main_kernel<false>, dim3(p.workgroups),
-                       dim3(kPPThreads), 0, stream, p);
+    auto* kernel = p.kv_fp8 ? (p.block_table ? shared_main_kernel<true, true> : shared_main_kernel<true, false>)
+                            : (p.block_table ? shared_main_kernel<false, true> : shared_main_kernel<false, false>);
+    hipLaunchKernelGGL(kernel, dim3(p.workgroups), dim3(kPPThreads), 0, stream, p);
     rc = (int)hipGetLastError();
     if (rc) return rc;
     const int rows = p.B * p.SQ * p.H;
