@@ -38,7 +38,7 @@ bool fills_blocks(int64_t rows) {
 struct SharedPlan {
     bool stacked;
     int prefix_items, seq_blocks, items, workgroups;
-    int64_t tiles_bytes, slots, bytes;
+    int64_t costs_bytes, slots, bytes;
 };
 
 int64_t round_256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -57,7 +57,7 @@ int shared_plan(const dsa_shared_args* a, SharedPlan* plan) {
     plan->seq_blocks = (int)((seq_rows + dsa::kSharedRows - 1) / dsa::kSharedRows);
     plan->prefix_items = plan->stacked ? (int)((rows + dsa::kSharedRows - 1) / dsa::kSharedRows) : 0;
     const int64_t items = plan->prefix_items + (int64_t)a->B * plan->seq_blocks;
-    if (items * (ceil_div(a->L, dsa::kSharedKeys) + 2) >= (int64_t)1 << 31)
+    if (items * (ceil_div(a->L, dsa::kSharedKeys) + 2) * dsa::kSharedMaxCost >= (int64_t)1 << 31)
         return fail(-1, "too many query rows for a context of %d (B * SQ * H * L)", a->L);
     plan->items = (int)items;
     plan->workgroups = a->num_cus;
@@ -71,8 +71,8 @@ int shared_plan(const dsa_shared_args* a, SharedPlan* plan) {
     // Pieces: every cut of an item's tiles starts a new one; a stacked call keeps
     // all of them, another only those of cut items, two at most a workgroup.
     plan->slots = plan->stacked ? items + plan->workgroups : 2 * (int64_t)plan->workgroups;
-    plan->tiles_bytes = round_256(4 * (items + 1));
-    plan->bytes = plan->tiles_bytes + plan->slots * dsa::kSharedRows * (512 + 2) * 4;
+    plan->costs_bytes = round_256(4 * (items + 1));
+    plan->bytes = plan->costs_bytes + plan->slots * dsa::kSharedRows * (512 + 2) * 4;
     return 0;
 }
 
@@ -173,8 +173,8 @@ int dsa_fwd_shared(const dsa_shared_args* a, void* stream) {
     p.out_max = a->out_max;
     p.out_sum = a->out_sum;
     char* ws = static_cast<char*>(a->workspace);
-    p.tiles = reinterpret_cast<int32_t*>(ws);
-    p.part_o = reinterpret_cast<float*>(ws + plan.tiles_bytes);
+    p.costs = reinterpret_cast<int32_t*>(ws);
+    p.part_o = reinterpret_cast<float*>(ws + plan.costs_bytes);
     p.part_m = p.part_o + plan.slots * dsa::kSharedRows * 512;
     p.part_l = p.part_m + plan.slots * dsa::kSharedRows;
     p.B = a->B;

@@ -191,10 +191,11 @@ int launch_write_rows(const dsa_write_args& p, hipStream_t stream);
 // prefix blocks first (stacked: blocks of rows of any sequences over the
 // prefix), then each sequence's own blocks, over its own rows (stacked) or over
 // prefix and own rows (not stacked: then there are no prefix items).  The tiles
-// of all items in that order are cut evenly over the workgroups, so an item may
-// be cut over several; the merge kernel joins its pieces.
-constexpr int kSharedRows = 64;
-constexpr int kSharedKeys = 32;  // keys a tile
+// of all items in that order, by cost, are cut evenly over the workgroups, so an
+// item may be cut over several; the merge kernel joins its pieces.
+constexpr int kSharedRows = 128;
+constexpr int kSharedKeys = 32;      // keys a tile
+constexpr int kSharedMaxCost = 3;    // most a tile costs
 struct SharedParams {
     const uint16_t* q;
     const char* kv;
@@ -204,7 +205,7 @@ struct SharedParams {
     const int32_t* block_table;  // [B, max_blocks] or NULL
     uint16_t* out;
     float *out_max, *out_sum;
-    int32_t* tiles;   // [items + 1]: tiles of the items before
+    int32_t* costs;   // [items + 1]: cost of the items before
     float* part_o;    // [slots, kSharedRows, 512] pieces of cut items
     float* part_m;    // [slots, kSharedRows] (log2 units)
     float* part_l;    // [slots, kSharedRows]

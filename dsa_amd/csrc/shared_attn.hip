@@ -4,12 +4,12 @@
 //
 // Every head of every sequence reads the same key rows in the prefix, so the
 // (token, head) pairs of the whole batch are rows of one product there: a block
-// of 64 such rows takes each tile of 32 key rows once from memory, whatever
-// sequences the rows belong to.  Three launches:
+// of up to 128 such rows takes each tile of 32 key rows once from memory,
+// whatever sequences the rows belong to.  Three launches:
 //
-//   plan   tiles of every item (kernels.h: SharedParams) from the lengths, summed
+//   plan   cost of every item (kernels.h: SharedParams) from the lengths, summed
 //   main   the tiles of all items, cut evenly over the workgroups: one pass over
-//          a piece's keys with the running maximum and sum of the softmax
+//          a piece's keys with the sum of the softmax
 //   merge  rows of cut items joined (FP32), rows without keys filled in
 //
 // Tiles are laid out and swizzled in LDS as in the sparse kernels (mla_tiles.h).
@@ -25,11 +25,9 @@ namespace dsa {
 namespace {
 
 constexpr float kLn2 = 0.69314718055994531f;
-constexpr int kRows = kSharedRows, kKeys = kSharedKeys;
+constexpr int kKeys = kSharedKeys;
 constexpr int kFp8Row = 656, kFp8ScaleOff = 512, kFp8RopeOff = 528;
 constexpr int kThreads = 256;
-// Fewest tiles a workgroup is given.
-constexpr int kMinTiles = 2;
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
@@ -49,14 +47,14 @@ __device__ __forceinline__ int seen_by(const SharedParams& p, int token) {
 __device__ __forceinline__ Item item_rows(const SharedParams& p, int i) {
     Item it;
     if (i < p.prefix_items) {
-        it.row0 = i * kRows;
-        it.rows = min(kRows, p.B * p.SQ * p.H - it.row0);
+        it.row0 = i * kSharedRows;
+        it.rows = min(kSharedRows, p.B * p.SQ * p.H - it.row0);
         it.seq = 0;
     } else {
         const int j = i - p.prefix_items, b = j / p.seq_blocks, k = j - b * p.seq_blocks;
         const int seq_rows = p.SQ * p.H;
-        it.row0 = b * seq_rows + k * kRows;
-        it.rows = min(kRows, seq_rows - k * kRows);
+        it.row0 = b * seq_rows + k * kSharedRows;
+        it.rows = min(kSharedRows, seq_rows - k * kSharedRows);
         it.seq = b;
     }
     return it;
@@ -68,19 +66,19 @@ __device__ __forceinline__ void item_tiles(const SharedParams& p, int i, int mos
     it.second = i < p.prefix_items ? 0 : ceil_div(max(most - p.prefix, 0), kKeys);
 }
 
-__device__ __forceinline__ int most_seen(const SharedParams& p, const Item& it) {
-    int most = 0;
-    for (int t = it.row0 / p.H; t <= (it.row0 + it.rows - 1) / p.H; ++t) most = max(most, seen_by(p, t));
-    return most;
-}
+// What one tile of an item costs: see the kernel's two forms below.
+__device__ __forceinline__ int tile_cost(const Item& it) { return it.rows > 64 ? 3 : 2; }
+constexpr int kMinCost = 6;  // least cost a workgroup is given (no less than one tile's)
 
 __device__ __forceinline__ int groups_of(const SharedParams& p, int total) {
-    return max(1, min(p.workgroups, total / kMinTiles));
+    return max(1, min(p.workgroups, total / kMinCost));
 }
 
-// The workgroup whose share [w * total / groups, (w + 1) * total / groups) holds tile t.
-__device__ __forceinline__ int group_at(int t, int total, int groups) {
-    return (int)(((int64_t)(t + 1) * groups + total - 1) / total) - 1;
+// Workgroup w computes the tiles that start in its share [w * total / groups,
+// (w + 1) * total / groups) of the summed costs.
+__device__ __forceinline__ int share_of(int w, int total, int groups) { return (int)((int64_t)w * total / groups); }
+__device__ __forceinline__ int group_at(int cost, int total, int groups) {
+    return (int)(((int64_t)(cost + 1) * groups + total - 1) / total) - 1;
 }
 
 // Slot of the piece of item i that workgroup w computes; `head`: it starts at the item's first tile.
@@ -99,8 +97,10 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
         int n = 0;
         if (i < p.items) {
             Item it = item_rows(p, i);
-            item_tiles(p, i, most_seen(p, it), it);
-            n = it.first + it.second;
+            int most = 0;
+            for (int t = it.row0 / p.H; t <= (it.row0 + it.rows - 1) / p.H; ++t) most = max(most, seen_by(p, t));
+            item_tiles(p, i, most, it);
+            n = (it.first + it.second) * tile_cost(it);
         }
         int scan = n;
         for (int d = 1; d < 64; d <<= 1) {
@@ -114,67 +114,69 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
             if (w < wave) before += sums[w];
             all += sums[w];
         }
-        if (i < p.items) p.tiles[i] = base + before + scan - n;
+        if (i < p.items) p.costs[i] = base + before + scan - n;
         base += all;
         __syncthreads();
     }
-    if (tid == 0) p.tiles[p.items] = base;
+    if (tid == 0) p.costs[p.items] = base;
 }
 
 // ------------------------------------------------------------------ main
-// Eight waves in two groups of four (waves w and w + 4 share a SIMD).  Both
-// groups own the block's 64 rows and take its tiles in turn, half a tile apart,
-// so that on every SIMD one wave's softmax runs beside the other's MFMAs:
+// Eight waves in two groups of four (waves w and w + 4 share a SIMD), half a
+// tile apart, so that on every SIMD one wave's softmax (VALU) runs beside the
+// other's MFMAs.  A group's turn at a tile is
 //
-//   half u:  group u % 2: S = K Q^T of tile u, a wave a block of 16 query rows, and
-//            its weights to the group's P buffer;
-//            the other group: gathers of tile u + 2 into the ring, then
-//            O^T += V^T P^T of tile u - 1, a wave 128 of the 512 columns
+//   QK  S^T = K Q^T and its weights: a wave one block of 16 query rows (Q in
+//       registers) and all 32 keys; P (bf16) to the group's LDS buffer
+//   PV  O^T += V^T P^T: a wave 128 of the 512 columns (O in registers) and
+//       four blocks of 16 rows
 //
-// with a workgroup barrier at the start of each half.  The running maximum is
-// taken once, from a row's first tile: P is formed against that reference, and
-// a piece whose maximum grows past it by 2^64 is computed once more against the
-// exact one, so O is never rescaled in the loop.  The groups' sums are brought
-// to a common maximum and added at the end.
+// with a workgroup barrier at the start of each half.
+//
+//   up to 64 rows (narrow): both groups own the same rows and take the tiles in
+//       turn; their sums are joined at the end.
+//       half u:       group u % 2 QK (u)    the other PV (u - 1)
+//   up to 128 rows (wide): group k owns rows 64 k ..; both take every tile.
+//       half 2 t:     group 0 QK (t)        group 1 PV (t - 1)
+//       half 2 t + 1: group 0 PV (t)        group 1 QK (t)
+//
+// P is formed against a reference maximum, a row's from its first tile, and a
+// piece whose scores pass it by 64 (log2 units) is computed once more against
+// the exact one, so O is never rescaled in the loop.
 //
 // A query row sees keys [0, seen) only, and rows behind a bad block entry are
-// masked: their scores become -inf, their weights 0 (clear_specials).
+// masked: their scores become -inf, their weights 0 (see clear_specials).
 constexpr int kPPThreads = 512;
 constexpr float kRestartLog2 = 64.0f;
 
-// With fp8 rows the gathers land as stored (656 bytes) in a raw buffer of the
-// group that issues them, and that group expands the tile it issued last while
-// the other one scores:
-//
-//   half u:  the other group: tile u + 1 from raw to the ring, gathers of tile
-//            u + 3, PV of tile u - 1
-//
-// so the ring holds three tiles (scored, expanded, read by PV).
+// Each wave brings in four rows of every tile.  bf16 rows are gathered straight
+// into a ring of four tiles; fp8 rows land as stored (656 bytes) in one of two
+// raw tiles, and the wave expands them into a ring of three.
 template <bool FP8>
 struct PPLds {
     static constexpr int NSTAGE = FP8 ? 3 : 4;
     static constexpr int KV_BYTES = kKeys * 1024, STAGE_BYTES = kKeys * 1152;
-    static constexpr int RAW_OFF = NSTAGE * STAGE_BYTES, RAW_BYTES = FP8 ? kKeys * kFp8Row : 0;  // one a group
+    static constexpr int RAW_OFF = NSTAGE * STAGE_BYTES, RAW_BYTES = FP8 ? kKeys * kFp8Row : 0;
     // P of one group, 64 rows x 32 bf16 in the k order of the PV operand (pp_pchunk)
     static constexpr int P_OFF = RAW_OFF + 2 * RAW_BYTES, P_GROUP = 64 * 64;
-    // tiles whose block entries and pool bits are held: entries (four waves x 8
-    // rows) from when the tile two before it is issued, the bits of the rows
-    // that are in the pool from when it is issued until PV
+    // of the last eight tiles: the rows' block entries (from when the tile three
+    // before it is issued), and four bits a wave, which of its rows are in the pool
     static constexpr int NTILE = 8;
     static constexpr int ENTRY_OFF = P_OFF + 2 * P_GROUP;
     static constexpr int VALID_OFF = ENTRY_OFF + NTILE * kKeys * 4;
-    static constexpr int FLAG_OFF = VALID_OFF + NTILE * 4;
+    static constexpr int FLAG_OFF = VALID_OFF + NTILE * 8;
     static constexpr int LDS_BYTES = FLAG_OFF + 16;
-    static constexpr int ML_OFF = P_OFF;  // [3][128] floats, at the end: l, reference and maximum of each group's rows
+    static constexpr int ML_OFF = P_OFF;  // [3][128] floats, at the end: l, reference and maximum
     static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
     __device__ static uint32_t stage(uint32_t lds, int u) { return lds + (uint32_t)(u % NSTAGE) * STAGE_BYTES; }
+    __device__ static uint32_t raw(uint32_t lds, int u) { return lds + RAW_OFF + (uint32_t)(u % 2) * RAW_BYTES; }
     __device__ static uint32_t entries(uint32_t lds, int u, int row) {
         return lds + ENTRY_OFF + (uint32_t)(u % NTILE) * (kKeys * 4) + 4 * row;
     }
-    __device__ static uint32_t valid(uint32_t lds, int u) { return lds + VALID_OFF + 4 * (u % NTILE); }
+    __device__ static uint32_t valid(uint32_t lds, int u) { return lds + VALID_OFF + 8 * (u % NTILE); }
 };
 
-// One tile of a piece: where its keys start, and the rows they are looked up in.
+// One tile of a piece: where its keys start and end, and the sequence they are looked up in.
 struct Tile {
     int key0, key_end, seq;
 };
@@ -222,30 +224,34 @@ __device__ __forceinline__ void gather_words(uint32_t lds_base, rsrc_t rsrc, uin
 #pragma clang diagnostic pop
 }
 
-// Gathers of one tile by wave gw of a group: rows 8 gw .. 8 gw + 7, one
-// instruction each (row), and (bf16) their rotary parts in one (rest).  They are
-// issued one at a time between the steps of PV: the texture path takes 64 bytes
-// a clock, and issued together they would hold the wave up.  Paged: the rows'
-// block entries were loaded into LDS when this wave issued the tile two before
-// (waited for since) -- for the piece's first tiles, `first`, they are loaded
-// here -- and those of the tile two further on are issued last.
+// Gathers of one tile by one wave: its rows 4 wave .. 4 wave + 3, an instruction
+// each (row), and (rest) the bf16 rows' rotary parts in one.  PV issues them one
+// at a time between its steps: the texture path takes about 50 bytes a clock,
+// and issued together they hold the wave up.  Paged: the rows' block entries
+// were loaded into LDS when the wave issued the tile three before (a piece's
+// first three before the loop), waited for since; those of the tile three
+// further on are issued last.
 template <bool FP8, bool PAGED>
 struct Gathers {
+    static constexpr int LOADS = (FP8 ? 4 : 5) + (PAGED ? 1 : 0);  // VMEM instructions
+    static constexpr int ENTRIES_AHEAD = 3;
     const char* kv;
     rsrc_t kr;
-    int my_row;        // lane l: row 8 gw + l % 8
-    uint32_t rope_off; // lane l: its 16 bytes of the rotary part of row 8 gw + l / 8
+    int my_row;        // lane l: row 4 wave + l % 4
+    uint32_t rope_off; // lane l < 32: its 16 bytes of the rotary part of row 4 wave + l / 8
     uint32_t dst, rope_dst;
+    uint32_t lane16;   // 16 times the lane, computed here: kept across the loop it would be spilled
 
-    __device__ __forceinline__ void prepare(const SharedParams& p, const Piece& c, int u, bool first, uint32_t lds,
-                                            int grp, int gw, int lane) {
+    __device__ __forceinline__ void prepare(const SharedParams& p, const Piece& c, int u, uint32_t lds, int wave,
+                                            int lane) {
         using X = PPLds<FP8>;
         asm volatile("" : "+v"(lane));
         const Tile k = tile_at(p, c, u);
-        const int r0 = 8 * gw;
-        const int key_r = min(k.key0 + r0 + (lane & 7), k.key_end - 1);
-        const int key_l = min(k.key0 + r0 + (lane >> 3), k.key_end - 1);
+        const int r0 = 4 * wave;
+        const int key_r = min(k.key0 + r0 + (lane & 3), k.key_end - 1);
+        const int in4 = (lane >> 3) & 3, key_l = min(k.key0 + r0 + in4, k.key_end - 1);
         int rope_row = 0;
+        lane16 = (uint32_t)lane << 4;
         kv = p.kv;
         const char* rope = reinterpret_cast<const char*>(p.k_rope);
         uint32_t pool;
@@ -257,19 +263,12 @@ struct Gathers {
             rope_row = key_l;
             pool = (uint32_t)p.L << 7;
         } else {
-            const int32_t* table = p.block_table + (int64_t)k.seq * p.max_blocks;
             const int col_r = block_of(p, key_r), col_l = block_of(p, key_l);
-            int e_r, e_l = 0;
-            if (first) {
-                e_r = table[col_r];
-                if (!FP8) e_l = table[col_l];
-            } else {
-                e_r = lds_load<int>(X::entries(lds, u, r0 + (lane & 7)));
-                if (!FP8) e_l = lds_load<int>(X::entries(lds, u, r0 + (lane >> 3)));
-            }
+            const int e_r = lds_load<int>(X::entries(lds, u, r0 + (lane & 3)));
+            const int e_l = FP8 ? 0 : lds_load<int>(X::entries(lds, u, r0 + in4));
             const bool ok_r = (uint32_t)e_r < (uint32_t)p.num_blocks;
-            const uint64_t valid = __ballot(ok_r) & 0xff;
-            if (lane == 0) lds_store<uint8_t>(X::valid(lds, u) + gw, (uint8_t)valid);
+            const uint64_t valid = __ballot(ok_r) & 0xf;
+            if (lane == 0) lds_store<uint8_t>(X::valid(lds, u) + wave, (uint8_t)valid);
             my_row = (ok_r ? e_r : 0) * p.block_size + (key_r - col_r * p.block_size);
             if (!FP8) {
                 const bool ok_l = (uint32_t)e_l < (uint32_t)p.num_blocks;
@@ -278,73 +277,75 @@ struct Gathers {
             pool = (uint32_t)(p.num_blocks * p.block_size) << 7;
         }
         if constexpr (FP8) {
-            dst = lds + X::RAW_OFF + grp * X::RAW_BYTES + r0 * kFp8Row;
+            dst = X::raw(lds, u) + r0 * kFp8Row;
         } else {
             dst = X::stage(lds, u) + r0 * 1024;
             rope_dst = X::stage(lds, u) + X::KV_BYTES + r0 * 128;
             kr = make_rsrc(rope, pool);
-            rope_off = ((uint32_t)rope_row << 7) + (((lane & 7) ^ sw_rope(r0 + (lane >> 3))) << 4);
+            rope_off = ((uint32_t)rope_row << 7) + (((lane & 7) ^ sw_rope(r0 + in4)) << 4);
         }
     }
-    __device__ __forceinline__ void row(int rr, int gw, int lane) const {
-        const uint32_t lane16 = (uint32_t)lane << 4;
+    __device__ __forceinline__ void row(int rr, int wave) const {
         const uint32_t r = (uint32_t)__builtin_amdgcn_readlane(my_row, rr);
         if constexpr (FP8) {
-            if (lane < kFp8Row / 16) gather_lanes(dst + rr * kFp8Row, fp8_rsrc(kv, r), lane16);
+            if (lane16 < kFp8Row) gather_lanes(dst + rr * kFp8Row, fp8_rsrc(kv, r), lane16);
         } else {
-            gather_row(dst + rr * 1024, row_rsrc(kv, r), lane16, (uint32_t)sw_kv(8 * gw + rr) << 4);
+            gather_row(dst + rr * 1024, row_rsrc(kv, r), lane16, (uint32_t)sw_kv(4 * wave + rr) << 4);
         }
     }
-    __device__ __forceinline__ void rest(const SharedParams& p, const Piece& c, int u, uint32_t lds, int gw,
-                                         int lane) const {
+    __device__ __forceinline__ void rest(const SharedParams& p, const Piece& c, int u, uint32_t lds, int wave) const {
         using X = PPLds<FP8>;
-        if constexpr (!FP8) gather_lanes(rope_dst, kr, rope_off);
-        if constexpr (PAGED)
-            if (u + 2 < c.nt) {
-                const Tile n = tile_at(p, c, u + 2);
-                const int key = min(n.key0 + 8 * gw + lane, n.key_end - 1);
-                if (lane < 8)
-                    gather_words(X::entries(lds, u + 2, 8 * gw),
-                                 make_rsrc(p.block_table + (int64_t)n.seq * p.max_blocks, 4u * (uint32_t)p.max_blocks),
-                                 4u * (uint32_t)block_of(p, key));
-            }
+        if constexpr (!FP8)
+            if (lane16 < 512) gather_lanes(rope_dst, kr, rope_off);
+        entries(p, c, u + ENTRIES_AHEAD, lds, wave, (int)(lane16 >> 4));
     }
-    __device__ __forceinline__ void all(const SharedParams& p, const Piece& c, int u, bool first, uint32_t lds, int grp,
-                                        int gw, int lane) {
-        prepare(p, c, u, first, lds, grp, gw, lane);
+    // Block entries of the wave's rows of tile u into LDS (past the item: some entry, not used).
+    static __device__ __forceinline__ void entries(const SharedParams& p, const Piece& c, int u, uint32_t lds, int wave,
+                                                   int lane) {
+        if constexpr (PAGED) {
+            const Tile n = tile_at(p, c, u);
+            const int key = min(n.key0 + 4 * wave + lane, n.key_end - 1);
+            if (lane < 4)
+                gather_words(PPLds<FP8>::entries(lds, u, 4 * wave),
+                             make_rsrc(p.block_table + (int64_t)n.seq * p.max_blocks, 4u * (uint32_t)p.max_blocks),
+                             4u * (uint32_t)block_of(p, key));
+        }
+    }
+    __device__ __forceinline__ void all(const SharedParams& p, const Piece& c, int u, uint32_t lds, int wave, int lane) {
+        prepare(p, c, u, lds, wave, lane);
 #pragma unroll
-        for (int rr = 0; rr < 8; ++rr) row(rr, gw, lane);
-        rest(p, c, u, lds, gw, lane);
+        for (int rr = 0; rr < 4; ++rr) row(rr, wave);
+        rest(p, c, u, lds, wave);
     }
 };
 
-// The rows that this wave gathered last, from the group's raw buffer to tile u
-// of the ring: lane l takes 64 latent values of row l % 8, from 64 (l / 8) on,
-// and 16 bytes of the rotary part of row l / 8.  kv[d] = bf16(fp32(e4m3) *
-// scale), both roundings to nearest even; where all scales are powers of two
-// (2^-100 .. 2^100), one conversion a pair gives the same bits.
-__device__ __forceinline__ void expand_rows(uint32_t lds, int u, int grp, int gw, int lane) {
+// The wave's four rows of tile u, from raw to the ring: lane l takes 32 latent
+// values of row l % 4, from 32 (l / 4) on, and lane l < 32 16 bytes of the
+// rotary part of row l / 8.  kv[d] = bf16(fp32(e4m3) * scale), both roundings to
+// nearest even; where all scales are powers of two (2^-100 .. 2^100), one
+// conversion a pair gives the same bits.
+__device__ __forceinline__ void expand_rows(uint32_t lds, int u, int wave, int lane) {
     using X = PPLds<true>;
     asm volatile("" : "+v"(lane));
-    const uint32_t raw = lds + X::RAW_OFF + grp * X::RAW_BYTES + 8 * gw * kFp8Row;
+    const uint32_t raw = X::raw(lds, u) + 4 * wave * kFp8Row;
     const uint32_t stage = X::stage(lds, u);
-    const int r = lane & 7, part = lane >> 3, row = 8 * gw + r;
+    const int r = lane & 3, part = lane >> 2, row = 4 * wave + r;
     const uint32_t src = raw + r * kFp8Row;
-    const float sc = lds_load<float>(src + kFp8ScaleOff + 4 * (part >> 1));
-    i32x4 v[4];
+    const float sc = lds_load<float>(src + kFp8ScaleOff + 4 * (part >> 2));
+    i32x4 v[2];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) v[m] = lds_load<i32x4>(src + 64 * part + 16 * m);
-    const int rope = 8 * gw + part;
-    const i32x4 turned = lds_load<i32x4>(raw + part * kFp8Row + kFp8RopeOff + 16 * r);
+    for (int m = 0; m < 2; ++m) v[m] = lds_load<i32x4>(src + 32 * part + 16 * m);
+    const int in4 = (lane >> 3) & 3, rope = 4 * wave + in4;
+    const i32x4 turned = lds_load<i32x4>(raw + in4 * kFp8Row + kFp8RopeOff + 16 * (lane & 7));
     const uint32_t sb = __float_as_uint(sc), sexp = sb >> 23 & 0xffu;
     const bool pow2 = (sb & 0x807fffffu) == 0 && sexp >= 27u && sexp <= 227u;
     const uint32_t dst = stage + row * 1024, sw = (uint32_t)sw_kv(row);
     auto put = [&](int m, int h, const bf16x8& o) {
-        lds_store<bf16x8>(dst + (((uint32_t)(8 * part + 2 * m + h) ^ sw) << 4), o);
+        lds_store<bf16x8>(dst + (((uint32_t)(4 * part + 2 * m + h) ^ sw) << 4), o);
     };
     if (__all(pow2)) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 bf16x8 o;
@@ -361,7 +362,7 @@ __device__ __forceinline__ void expand_rows(uint32_t lds, int u, int grp, int gw
             }
     } else {
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 bf16x8 o;
@@ -377,7 +378,19 @@ __device__ __forceinline__ void expand_rows(uint32_t lds, int u, int grp, int gw
                 put(m, h, o);
             }
     }
-    lds_store<i32x4>(stage + X::KV_BYTES + rope * 128 + ((r ^ sw_rope(rope)) << 4), turned);
+    if (lane < 32) lds_store<i32x4>(stage + X::KV_BYTES + rope * 128 + (((lane & 7) ^ sw_rope(rope)) << 4), turned);
+}
+
+// Rows of a tile that are in the pool, bit r for row r, from the waves' four bits each.
+template <bool FP8, bool PAGED>
+__device__ __forceinline__ uint32_t pool_rows(uint32_t lds, int u) {
+    if constexpr (!PAGED) return 0xffffffffu;
+    const uint64_t v = lds_load<uint64_t>(PPLds<FP8>::valid(lds, u));
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+    if (__builtin_expect((lo & hi) == 0x0f0f0f0fu, 1)) return 0xffffffffu;
+    auto squeeze = [](uint32_t b) { return (b & 0xfu) | (b >> 4 & 0xf0u) | (b >> 8 & 0xf00u) | (b >> 12 & 0xf000u); };
+    return squeeze(lo) | squeeze(hi) << 16;
 }
 
 // Which of the 32 keys of a tile a query row that sees `seen` rows has: bit r is tile row r.
@@ -386,17 +399,17 @@ __device__ __forceinline__ uint32_t key_mask(const Tile& k, int seen, uint32_t v
     return n == kKeys ? valid : valid & ((1u << n) - 1);
 }
 
-// Lane g's rows of a tile -- 4 g + j (j < 4) and 16 + 4 g + j -- from a key mask: bit j, bit 4 + j.
+// Lane group g's rows of a tile -- 4 g + j (j < 4) and 16 + 4 g + j -- from a key mask: bit j, bit 4 + j.
 __device__ __forceinline__ uint32_t lane_rows(uint32_t mask, int g) {
     return (mask >> (4 * g) & 15u) | (mask >> (16 + 4 * g) & 15u) << 4;
 }
 
-// Infinities and NaN in this wave's 128 columns of a tile become zeros, where
-// some query row does not see all of the tile: a hidden row's weight is 0, which
-// they would turn into NaN.  A query row that does see such a value has a score,
-// a sum and so a whole result that are NaN already, as the key row that it lies
-// in is the value row too.  (The wave's own LDS accesses are in order, and no
-// other wave reads these columns any more.)
+// Infinities and NaN in a wave's 128 columns of a tile become zeros, where some
+// query row does not see all of the tile: a hidden row's weight is 0, which they
+// would turn into NaN.  A query row that does see such a value has a score, a
+// sum and so a whole result that are NaN already, as the key row that it lies in
+// is the value row too.  Both groups are past QK of the tile; the wave's own LDS
+// accesses are in order, and no other wave of its group reads these columns.
 __device__ __forceinline__ void clear_specials(uint32_t stage, int gw, int lane) {
     asm volatile("" : "+v"(lane));
     const uint32_t at = stage + (uint32_t)((lane >> 4) * 1024 + gw * 256 + (lane & 15) * 16);
@@ -412,32 +425,35 @@ __device__ __forceinline__ void clear_specials(uint32_t stage, int gw, int lane)
     }
 }
 
-// One piece of an item with up to 16 NB rows.
-template <bool FP8, bool PAGED, int NB>
+// One piece of an item, WIDE: up to 128 rows, else up to 16 NB (NB = 4 if WIDE).
+template <bool FP8, bool PAGED, bool WIDE, int NB>
 __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece& c, bool whole, int64_t slot,
                                              uint32_t lds, int wave, int lane) {
+    static_assert(!WIDE || NB == 4, "a group's four row blocks");
     using X = PPLds<FP8>;
+    using G = Gathers<FP8, PAGED>;
     const int grp = wave >> 2, gw = wave & 3;
     const int g = lane >> 4, n16 = lane & 15;
-    const bool live = 16 * gw < c.it.rows;  // this wave has query rows
-    const int row = c.it.row0 + 16 * gw;
+    const int block = (WIDE ? 64 * grp : 0) + 16 * gw;  // this wave's query rows in QK
+    const bool live = block < c.it.rows;
+    const int row = c.it.row0 + (live ? block : 0);
     const int nt = c.nt;
     const int seen = live ? __builtin_amdgcn_readfirstlane(seen_by(p, row / p.H)) : 0;
     const uint32_t p_lds = lds + X::P_OFF + grp * X::P_GROUP;
 
     bf16x8 qf[18];
     {
-        const int r = live ? row : c.it.row0;
-        const uint16_t* q = p.q + (int64_t)(r + n16) * 512 + 8 * qk_lane_chunk(g);
+        const uint16_t* q = p.q + (int64_t)(row + n16) * 512 + 8 * qk_lane_chunk(g);
 #pragma unroll
         for (int ks = 0; ks < 16; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(q + 32 * ks);
-        const uint16_t* rr = p.q_rope + (int64_t)(r + n16) * 64 + 8 * g;
+        const uint16_t* rr = p.q_rope + (int64_t)(row + n16) * 64 + 8 * g;
         qf[16] = *reinterpret_cast<const bf16x8*>(rr);
         qf[17] = *reinterpret_cast<const bf16x8*>(rr + 32);
     }
 
     f32x4 oacc[NB][8];
-    float m_ref = -FLT_MAX, m_true = -FLT_MAX, l_run = 0.f;
+    // log2 units; the maximum of this lane's own scores
+    float m_ref = -FLT_MAX, m_lane = -FLT_MAX, l_run = 0.f;
 
     // This lane's LDS offsets in the loop, packed as in the sparse ping-pong kernel.
     uint32_t off_kv, off_rope, off_p;
@@ -456,7 +472,6 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         asm volatile("" : "+v"(off_kv), "+v"(off_rope), "+v"(off_p));
         const uint32_t kbase = stage + (off_kv & 0xffffu);
         const uint32_t rbase = stage + off_rope;
-        const int valid_v = lds_load<int>(X::valid(lds, u));
         auto kfrag = [&](int step) -> bf16x8 {
             const int ks = step >> 1, sub = step & 1;
             if (ks < 16) return lds_load<bf16x8>((kbase ^ (64u * (ks & 3))) + 256u * (ks >> 2) + sub * 16 * 1024);
@@ -478,8 +493,8 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         float x[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) x[r] = sacc[r >> 2][r & 3];
-        const uint32_t mask = key_mask(tile_at(p, c, u), seen, (uint32_t)__builtin_amdgcn_readfirstlane(valid_v));
-        if (mask != 0xffffffffu) {
+        const uint32_t mask = key_mask(tile_at(p, c, u), seen, pool_rows<FP8, PAGED>(lds, u));
+        if (__builtin_expect(mask != 0xffffffffu, 0)) {
             int ln = lane;
             asm volatile("" : "+v"(ln));
             const uint32_t mine = lane_rows(mask, ln >> 4);
@@ -487,43 +502,45 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
             for (int r = 0; r < 8; ++r)
                 if (!(mine >> r & 1)) x[r] = -INFINITY;
         }
-        float smax = -INFINITY;
+        float top = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) smax = fmaxf(smax, x[r]);
-        smax = max_xor32(max_xor16(smax));
-        m_true = fmaxf(m_true, smax * p.scale_log2);
-        if (m_ref == -FLT_MAX) m_ref = m_true;  // the row's first keys: O and l are still zero
-        const bool ovf = m_true > m_ref + kRestartLog2;
+        for (int r = 0; r < 8; ++r) top = fmaxf(top, x[r]);
+        m_lane = fmaxf(m_lane, top * p.scale_log2);
+        if (__builtin_expect(__any(m_ref == -FLT_MAX), 0)) {  // a row's first keys: O and l are still zero
+            const float m = max_xor32(max_xor16(m_lane));
+            m_ref = m_ref == -FLT_MAX ? m : m_ref;
+        }
+        const bool ovf = m_lane > m_ref + kRestartLog2;
         overflow |= ovf;
         const float neg_ref = -m_ref;
         float psum = 0.f;
         bf16x8 pk;
-        if (__any(ovf)) {  // this pass is to be discarded: the clamp keeps it free of inf
+        if (__builtin_expect(__any(ovf), 0)) {  // this pass is to be discarded: the clamp keeps it free of inf
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const float e = fast_exp2(fminf(fmaf(x[r], p.scale_log2, neg_ref), kRestartLog2));
-                psum += e;
-                pk[r] = (__bf16)e;
-            }
+            for (int r = 0; r < 8; ++r) x[r] = fminf(fmaf(x[r], p.scale_log2, neg_ref), kRestartLog2);
         } else {
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const float e = fast_exp2(fmaf(x[r], p.scale_log2, neg_ref));
-                psum += e;
-                pk[r] = (__bf16)e;
-            }
+            for (int r = 0; r < 8; ++r) x[r] = fmaf(x[r], p.scale_log2, neg_ref);
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const float e = fast_exp2(x[r]);
+            psum += e;
+            pk[r] = (__bf16)e;
         }
         l_run += psum;
         lds_store<bf16x8>(p_lds + (off_p >> 16), pk);
     };
 
-    // PV of tile u, with the gathers of tile `next` (if any) between its steps.
+    // Whether some query row of the block does not see all keys of tile u (every wave agrees).
+    auto partial = [&](int u) __attribute__((always_inline)) -> bool {
+        return key_mask(tile_at(p, c, u), c.seen_low, pool_rows<FP8, PAGED>(lds, u)) != 0xffffffffu;
+    };
+
+    // PV of tile u, with the gathers of tile `next` (bf16; if there is one) between its steps.
     auto pv = [&](int u, int next) __attribute__((always_inline)) {
         const uint32_t stage = X::stage(lds, u);
         asm volatile("" : "+v"(off_kv), "+v"(off_p));
-        const uint32_t valid = (uint32_t)__builtin_amdgcn_readfirstlane(
-            lds_load<int>(X::valid(lds, u)));
-        const Tile k = tile_at(p, c, u);
         const uint32_t vbase = stage + (off_kv >> 16);
         auto vfrag = [&](int cb) -> bf16x8 {
             const uint32_t a = vbase ^ (32u * cb);
@@ -531,14 +548,14 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
             const bf16x4 v1 = lds_load_tr(a + 16 * 1024);
             return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
         };
-        if (__builtin_expect(key_mask(k, c.seen_low, valid) != 0xffffffffu, 0)) clear_specials(stage, gw, lane);
-        const bool more = next < nt;
-        Gathers<FP8, PAGED> gather;
-        if (more) gather.prepare(p, c, next, false, lds, grp, gw, lane);
+        if (__builtin_expect(partial(u), 0)) clear_specials(stage, gw, lane);
+        const bool more = !FP8 && next < nt;
+        G gather;
+        if (more) gather.prepare(p, c, next, lds, wave, lane);
         bf16x8 pf[NB];
 #pragma unroll
         for (int hb = 0; hb < NB; ++hb) pf[hb] = lds_load<bf16x8>(p_lds + (off_p & 0xffffu) + 1024 * hb);
-        constexpr int VD = NB == 4 ? 2 : 4;  // V fragments in flight
+        constexpr int VD = NB == 4 ? 3 : 4;  // V fragments in flight
         bf16x8 vf[VD];
 #pragma unroll
         for (int j = 0; j < VD; ++j) vf[j] = vfrag(j);
@@ -548,10 +565,29 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
             for (int hb = 0; hb < NB; ++hb)
                 oacc[hb][cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[cb % VD], pf[hb], oacc[hb][cb], 0, 0, 0);
             if (cb + VD < 8) vf[cb % VD] = vfrag(cb + VD);
-            if (more) gather.row(cb, gw, lane);
+            if (more && cb < 4) gather.row(cb, wave);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (more) gather.rest(p, c, next, lds, gw, lane);
+        if (more) gather.rest(p, c, next, lds, wave);
+    };
+
+    // fp8: the wave's rows of tile u into the ring, and the gathers of tile u + 2 into their place.
+    auto advance = [&](int u) __attribute__((always_inline)) {
+        if constexpr (FP8)
+            if (u < nt) {
+                if (u + 1 < nt) wait_vmcnt<G::LOADS>();
+                else wait_vmcnt<0>();
+                expand_rows(lds, u, wave, lane);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // raw is read before it is written again
+                G gather;
+                if (u + 2 < nt) gather.all(p, c, u + 2, lds, wave, lane);
+            }
+    };
+    // Waits until the gathers that this wave issued before its last n tiles' have landed.
+    auto landed = [&](int n) __attribute__((always_inline)) {
+        if (n >= 2) wait_vmcnt<2 * G::LOADS>();
+        else if (n == 1) wait_vmcnt<G::LOADS>();
+        else wait_vmcnt<0>();
     };
 
 #pragma unroll 1
@@ -561,55 +597,90 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
 #pragma unroll
             for (int cb = 0; cb < 8; ++cb) oacc[hb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
         l_run = 0.f;
-        if (pass == 1) m_ref = m_true;
+        if (pass == 1) m_ref = max_xor32(max_xor16(m_lane));
         bool overflow = false;
-        // Half u: group u % 2 scores tile u.  The other group, bf16: issues tile
-        // u + 2 (into the stage of tile u - 2, whose last reader ran in half
-        // u - 1) and runs PV of tile u - 1; a group scores the tile after the
-        // one it issued last, and its full wait behind that covers the tile it
-        // issued and the block entries of the one it issues next.  fp8: waits
-        // for tile u + 1, which it issued in half u - 2, expands it (into the
-        // stage of tile u - 2), issues tile u + 3 and runs PV of tile u - 1.
-        auto scored = [&]() __attribute__((always_inline)) {
-            if constexpr (!FP8) wait_vmcnt<0>();
-        };
-        auto expand = [&](int u) __attribute__((always_inline)) {
-            if constexpr (FP8)
-                if (u < nt) {
-                    wait_vmcnt<0>();
-                    expand_rows(lds, u, grp, gw, lane);
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // raw is read before it is written again
-                }
-        };
-        Gathers<FP8, PAGED> gather;
-        constexpr int AHEAD = FP8 ? 3 : 2;  // the tile issued in half u is u + AHEAD
+        // The first tile's rows, and Q: a full wait, as the compiler does not
+        // count the gathers (it would wait for Q in the loop).
+        G gather;
+        if constexpr (PAGED) {
+            for (int u = 0; u < G::ENTRIES_AHEAD; ++u) G::entries(p, c, u, lds, wave, lane);
+            wait_vmcnt<0>();
+        }
+        gather.all(p, c, 0, lds, wave, lane);
+        wait_vmcnt<0>();
         if constexpr (FP8) {
-            if (grp == 0 || nt > 1) gather.all(p, c, grp, true, lds, grp, gw, lane);
-            wait_vmcnt<0>();
-            if (grp == 0) {
-                expand(0);
-                if (nt > 2) gather.all(p, c, 2, false, lds, grp, gw, lane);
+            // Every wave, once a tile: waits for its rows of the next tile (issued
+            // two tiles ago), expands them, issues two tiles ahead into their place.
+            if (nt > 1) gather.all(p, c, 1, lds, wave, lane);
+            advance(0);
+        } else if (nt > 1) {
+            gather.all(p, c, 1, lds, wave, lane);
+        }
+        if constexpr (!WIDE) {
+            // In half u every wave issues (bf16) its rows of tile u + 2 into the
+            // stage of tile u - 2, whose last reader ran in half u - 1: after QK,
+            // where it would otherwise wait, or between the steps of PV.  The
+            // half ends with its rows of tile u + 1 landed.
+            if (grp == 1) {  // half 0, without PV
+                lds_barrier();
+                if constexpr (FP8) {
+                    advance(1);
+                } else {
+                    wait_vmcnt<0>();
+                    if (2 < nt) gather.all(p, c, 2, lds, wave, lane);
+                }
             }
-        } else {
-            if (grp == 1) gather.all(p, c, 0, true, lds, grp, gw, lane);
-            wait_vmcnt<0>();
-            if (grp == 0 && nt > 1) gather.all(p, c, 1, true, lds, grp, gw, lane);
-        }
-        if (grp == 1) {  // half 0, without PV
-            lds_barrier();
-            expand(1);
-            if (AHEAD < nt) gather.all(p, c, AHEAD, false, lds, grp, gw, lane);
-        }
 #pragma unroll 1
-        for (int u = grp; u < nt; u += 2) {
-            lds_barrier();
-            if (live) qk_softmax(u, overflow);
-            scored();
-            lds_barrier();
-            expand(u + 2);
-            pv(u, u + 1 + AHEAD);
+            for (int u = grp; u < nt; u += 2) {
+                lds_barrier();
+                if (live) qk_softmax(u, overflow);
+                if constexpr (FP8) {
+                    advance(u + 1);
+                } else {
+                    wait_vmcnt<0>();
+                    if (u + 2 < nt) gather.all(p, c, u + 2, lds, wave, lane);
+                }
+                lds_barrier();
+                if constexpr (FP8) advance(u + 2);
+                pv(u, u + 3);
+                if constexpr (!FP8) landed(u + 3 < nt ? 1 : 0);
+            }
+            if (((nt ^ grp) & 1) == 0) lds_barrier();  // half nt: the other group's last PV
+        } else {
+            // In PV of tile t a group issues (bf16) its rows of tile t + 3, into
+            // the stage of tile t - 1, which both groups are past.  A tile in
+            // which some row sees less than all has one barrier more, between
+            // group 1's QK and group 0's clear_specials of it.
+            if constexpr (!FP8)
+                if (grp == 0 && nt > 2) gather.all(p, c, 2, lds, wave, lane);
+            if (grp == 0) {
+#pragma unroll 1
+                for (int t = 0; t < nt; ++t) {
+                    lds_barrier();
+                    if (live) qk_softmax(t, overflow);
+                    lds_barrier();
+                    if (__builtin_expect(partial(t), 0)) lds_barrier();
+                    if constexpr (FP8) advance(t + 1);
+                    pv(t, t + 3);
+                    if constexpr (!FP8) landed(min(2, nt - 2 - t));
+                }
+                lds_barrier();  // half 2 nt: group 1's last PV
+            } else {
+                lds_barrier();
+                if constexpr (FP8) advance(1);
+                else if (2 < nt) gather.all(p, c, 2, lds, wave, lane);
+#pragma unroll 1
+                for (int t = 0; t < nt; ++t) {
+                    lds_barrier();
+                    if (live) qk_softmax(t, overflow);
+                    if (__builtin_expect(partial(t), 0)) lds_barrier();
+                    if constexpr (!FP8) landed(min(1, nt - 2 - t));
+                    lds_barrier();
+                    if constexpr (FP8) advance(t + 2);
+                    pv(t, t + 3);
+                }
+            }
         }
-        if (((nt ^ grp) & 1) == 0) lds_barrier();  // half nt: the other group's last PV
         if (pass == 1) break;
         // does any row need the second pass?
         const uint32_t flag = lds + X::FLAG_OFF;
@@ -619,15 +690,13 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         if (__any(overflow) && lane == 0) lds_store<int>(flag, 1);
         lds_barrier();
         if (__builtin_amdgcn_readfirstlane(lds_load<int>(flag)) == 0) break;
-        lds_barrier();  // read by every wave before the second pass ends in another vote's first store
     }
 
-    // ---- both groups hold O of the same rows over their own tiles: each is
-    // scaled to the common maximum, a wave hands half of its column blocks to
-    // the wave of the other group with the same columns and adds what it gets.
+    // ---- the QK waves publish (l, reference, maximum) of their rows; the PV waves scale their blocks
     lds_barrier();
     const uint32_t ml = lds + X::ML_OFF;
     l_run = sum_xor32(sum_xor16(l_run));
+    const float m_true = max_xor32(max_xor16(m_lane));
     int eln = lane;
     asm volatile("" : "+v"(eln));
     const int eg = eln >> 4, en16 = eln & 15;
@@ -638,87 +707,130 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         lds_store<float>(ml + 4 * (256 + hl), m_true);
     }
     lds_barrier();
-    constexpr int HROW = 1040;       // bytes of a staged bf16 row (16 more: rows spread over the banks)
-    constexpr int kPartRow = 2064;   // of a staged fp32 row
-    constexpr uint32_t kHand = NB * 4 * 1024;  // one wave's half: NB row x 4 column blocks of 64 lanes x 16 bytes
-    static_assert(8 * kHand <= X::P_OFF && 64 * kPartRow <= X::P_OFF, "staging fits the ring and raw buffers");
+    constexpr int HROW = 1040;      // bytes of a staged bf16 row (16 more: rows spread over the banks)
+    constexpr int kPartRow = 2064;  // of a staged fp32 row
+    static_assert(128 * HROW <= X::P_OFF && 64 * kPartRow <= X::P_OFF, "staging fits the ring and raw tiles");
     static_assert(3 * 128 * 4 <= 2 * X::P_GROUP, "statistics fit the P buffers");
-    const uint32_t give = lds + (uint32_t)wave * kHand + 16u * (uint32_t)eln;
-    const uint32_t take = lds + (uint32_t)(wave ^ 4) * kHand + 16u * (uint32_t)eln;
-    float scale[NB];
-#pragma unroll
-    for (int hb = 0; hb < NB; ++hb) {
-        const int hl = 16 * hb + en16;
-        float l[2], mr[2], mt[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            l[k] = lds_load<float>(ml + 4 * (64 * k + hl));
-            mr[k] = lds_load<float>(ml + 4 * (128 + 64 * k + hl));
-            mt[k] = lds_load<float>(ml + 4 * (256 + 64 * k + hl));
+    auto put_stats = [&](int hl, float top, float sum) __attribute__((always_inline)) {
+        if (hl >= c.it.rows) return;
+        if (whole) {
+            p.out_max[c.it.row0 + hl] = sum == 0.f ? -INFINITY : top * kLn2;
+            p.out_sum[c.it.row0 + hl] = sum;
+        } else {
+            p.part_m[slot * kSharedRows + hl] = top;
+            p.part_l[slot * kSharedRows + hl] = sum;
         }
-        const float top = fmaxf(mt[0], mt[1]);
-        const float f0 = fast_exp2(mr[0] - top), f1 = fast_exp2(mr[1] - top);
-        const float sum = fmaf(l[0], f0, l[1] * f1);
-        scale[hb] = grp == 0 ? f0 : f1;
-        if (whole) scale[hb] *= sum == 0.f ? 0.f : 1.f / sum;
-        if (wave == 0 && eg == 0 && hl < c.it.rows) {
-            if (whole) {
-                p.out_max[c.it.row0 + hl] = sum == 0.f ? -INFINITY : top * kLn2;
-                p.out_sum[c.it.row0 + hl] = sum;
-            } else {
-                p.part_m[slot * kRows + hl] = top;
-                p.part_l[slot * kRows + hl] = sum;
-            }
+    };
+    // Staged rows [first, first + n) of the block, row r at HROW (bf16) or kPartRow (fp32) * (r - first), stored whole.
+    auto store_rows = [&](int first, int n) __attribute__((always_inline)) {
+        const int end = min(first + n, c.it.rows);
+        if (whole) {
+            uint16_t* base = p.out + (int64_t)c.it.row0 * 512 + 8 * eln;
+            for (int r = first + wave; r < end; r += 8)
+                *reinterpret_cast<bf16x8*>(base + (int64_t)r * 512) = lds_load<bf16x8>(lds + (r - first) * HROW + 16 * eln);
+        } else {
+            float* base = p.part_o + slot * (kSharedRows * 512) + 4 * eln;
+            for (int i = 2 * first + wave; i < 2 * end; i += 8)
+                *reinterpret_cast<f32x4*>(base + (i >> 1) * 512 + 256 * (i & 1)) =
+                    lds_load<f32x4>(lds + (uint32_t)(((i >> 1) - first) * kPartRow + 1024 * (i & 1) + 16 * eln));
         }
-    }
-    auto finish = [&](auto kept) __attribute__((always_inline)) {  // kept: 0 (blocks 0-3) or 4 (blocks 4-7)
-        constexpr int KEEP = decltype(kept)::value, GIVE = 4 - KEEP;
+    };
+    auto stage_block = [&](int r, int col, const f32x4& o) __attribute__((always_inline)) {  // r: row within the staged ones
+        if (whole) {
+            bf16x4 v;
+            v[0] = (__bf16)o[0];
+            v[1] = (__bf16)o[1];
+            v[2] = (__bf16)o[2];
+            v[3] = (__bf16)o[3];
+            lds_store<bf16x4>(lds + (uint32_t)(r * HROW + 2 * col), v);
+        } else {
+            lds_store<f32x4>(lds + (uint32_t)(r * kPartRow + 4 * col), o);
+        }
+    };
+    if constexpr (WIDE) {
+        float scale[NB];
 #pragma unroll
-        for (int hb = 0; hb < NB; ++hb)
+        for (int hb = 0; hb < NB; ++hb) {
+            const int hl = 64 * grp + 16 * hb + en16;
+            const float l = lds_load<float>(ml + 4 * hl), mr = lds_load<float>(ml + 4 * (128 + hl));
+            const float top = lds_load<float>(ml + 4 * (256 + hl));
+            const float to_true = fast_exp2(mr - top), sum = l * to_true;
+            scale[hb] = to_true;
+            if (whole) scale[hb] *= sum == 0.f ? 0.f : 1.f / sum;
+            if (gw == 0 && eg == 0) put_stats(hl, top, sum);
+        }
+        auto stage = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
-            for (int cb = 0; cb < 4; ++cb)
-                lds_store<f32x4>(give + 1024u * (4 * hb + cb), oacc[hb][GIVE + cb] * scale[hb]);
-        lds_barrier();
+            for (int hb = 0; hb < NB; ++hb)
 #pragma unroll
-        for (int hb = 0; hb < NB; ++hb)
-#pragma unroll
-            for (int cb = 0; cb < 4; ++cb)
-                oacc[hb][KEEP + cb] = oacc[hb][KEEP + cb] * scale[hb] + lds_load<f32x4>(take + 1024u * (4 * hb + cb));
-        lds_barrier();  // the halves are read: the ring is free for the staged rows
-        const int col0 = 128 * gw + 16 * KEEP + 4 * eg;
+                for (int cb = 0; cb < 8; ++cb)
+                    stage_block(at + 16 * hb + en16, 128 * gw + 16 * cb + 4 * eg, oacc[hb][cb] * scale[hb]);
+        };
+        if (whole) {
+            stage(64 * grp);
+            lds_barrier();
+            store_rows(0, 128);
+        } else {  // fp32 rows: one group's at a time
+            if (grp == 0) stage(0);
+            lds_barrier();
+            store_rows(0, 64);
+            lds_barrier();
+            if (grp == 1) stage(0);
+            lds_barrier();
+            store_rows(64, 64);
+        }
+    } else {
+        // Both groups hold O of the same rows over their own tiles: each is scaled
+        // to the common maximum, a wave hands half of its column blocks to the wave
+        // of the other group with the same columns and adds what it gets.
+        constexpr uint32_t kHand = NB * 4 * 1024;  // one wave's half: NB row x 4 column blocks of 64 lanes x 16 bytes
+        static_assert(8 * kHand <= X::P_OFF, "handed halves fit");
+        const uint32_t give = lds + (uint32_t)wave * kHand + 16u * (uint32_t)eln;
+        const uint32_t take = lds + (uint32_t)(wave ^ 4) * kHand + 16u * (uint32_t)eln;
+        float scale[NB];
 #pragma unroll
         for (int hb = 0; hb < NB; ++hb) {
             const int hl = 16 * hb + en16;
+            float l[2], mr[2], mt[2];
 #pragma unroll
-            for (int cb = 0; cb < 4; ++cb) {
-                const f32x4 o = oacc[hb][KEEP + cb];
-                if (whole) {
-                    bf16x4 v;
-                    v[0] = (__bf16)o[0];
-                    v[1] = (__bf16)o[1];
-                    v[2] = (__bf16)o[2];
-                    v[3] = (__bf16)o[3];
-                    lds_store<bf16x4>(lds + (uint32_t)(hl * HROW + 2 * (col0 + 16 * cb)), v);
-                } else {
-                    lds_store<f32x4>(lds + (uint32_t)(hl * kPartRow + 4 * (col0 + 16 * cb)), o);
-                }
+            for (int k = 0; k < 2; ++k) {
+                l[k] = lds_load<float>(ml + 4 * (64 * k + hl));
+                mr[k] = lds_load<float>(ml + 4 * (128 + 64 * k + hl));
+                mt[k] = lds_load<float>(ml + 4 * (256 + 64 * k + hl));
             }
+            const float top = fmaxf(mt[0], mt[1]);
+            const float f0 = fast_exp2(mr[0] - top), f1 = fast_exp2(mr[1] - top);
+            const float sum = fmaf(l[0], f0, l[1] * f1);
+            scale[hb] = grp == 0 ? f0 : f1;
+            if (whole) scale[hb] *= sum == 0.f ? 0.f : 1.f / sum;
+            if (wave == 0 && eg == 0) put_stats(hl, top, sum);
         }
-    };
-    if (grp == 0) finish(std::integral_constant<int, 0>{});
-    else finish(std::integral_constant<int, 4>{});
-    lds_barrier();
-    if (whole) {
-        uint16_t* obase = p.out + (int64_t)c.it.row0 * 512 + 8 * eln;
-        for (int hr = wave; hr < c.it.rows; hr += 8)
-            *reinterpret_cast<bf16x8*>(obase + (int64_t)hr * 512) = lds_load<bf16x8>(lds + hr * HROW + 16 * eln);
-    } else {
-        float* base = p.part_o + slot * (kRows * 512) + 4 * eln;
-        for (int i = wave; i < 2 * c.it.rows; i += 8)
-            *reinterpret_cast<f32x4*>(base + (i >> 1) * 512 + 256 * (i & 1)) =
-                lds_load<f32x4>(lds + (uint32_t)((i >> 1) * kPartRow + 1024 * (i & 1) + 16 * eln));
+        auto finish = [&](auto kept) __attribute__((always_inline)) {  // kept: 0 (blocks 0-3) or 4 (blocks 4-7)
+            constexpr int KEEP = decltype(kept)::value, GIVE = 4 - KEEP;
+#pragma unroll
+            for (int hb = 0; hb < NB; ++hb)
+#pragma unroll
+                for (int cb = 0; cb < 4; ++cb)
+                    lds_store<f32x4>(give + 1024u * (4 * hb + cb), oacc[hb][GIVE + cb] * scale[hb]);
+            lds_barrier();
+#pragma unroll
+            for (int hb = 0; hb < NB; ++hb)
+#pragma unroll
+                for (int cb = 0; cb < 4; ++cb)
+                    oacc[hb][KEEP + cb] = oacc[hb][KEEP + cb] * scale[hb] + lds_load<f32x4>(take + 1024u * (4 * hb + cb));
+            lds_barrier();  // the halves are read: the ring is free for the staged rows
+#pragma unroll
+            for (int hb = 0; hb < NB; ++hb)
+#pragma unroll
+                for (int cb = 0; cb < 4; ++cb)
+                    stage_block(16 * hb + en16, 128 * gw + 16 * (KEEP + cb) + 4 * eg, oacc[hb][KEEP + cb]);
+        };
+        if (grp == 0) finish(std::integral_constant<int, 0>{});
+        else finish(std::integral_constant<int, 4>{});
+        lds_barrier();
+        store_rows(0, 16 * NB);
     }
-    lds_barrier();  // the ring is free for the next piece
+    lds_barrier();  // LDS is free for the next piece
 }
 
 template <bool FP8, bool PAGED>
@@ -728,25 +840,26 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int total = p.tiles[p.items], groups = groups_of(p, total);
+    const int total = p.costs[p.items], groups = groups_of(p, total);
     const int w = blockIdx.x;
     if (w >= groups) return;
-    int t0 = (int)((int64_t)w * total / groups);
-    const int t1 = (int)((int64_t)(w + 1) * total / groups);
-    if (t0 >= t1) return;
-    if (threadIdx.x < X::NTILE) lds_store<uint32_t>(X::valid(lds, threadIdx.x), 0xffffffffu);
-    int i = 0, high = p.items;  // the item that holds tile t0: tiles[i] <= t0 < tiles[i + 1]
+    const int c0 = share_of(w, total, groups), c1 = share_of(w + 1, total, groups);
+    if (c0 >= c1) return;
+    int i = 0, high = p.items;  // the item that holds cost c0: costs[i] <= c0 < costs[i + 1]
     while (high - i > 1) {
         const int mid = (i + high) >> 1;
-        if (p.tiles[mid] <= t0) i = mid;
+        if (p.costs[mid] <= c0) i = mid;
         else high = mid;
     }
 #pragma unroll 1
-    for (; t0 < t1; ++i) {
-        const int begin = p.tiles[i], end = p.tiles[i + 1];
-        if (end <= t0) continue;
+    for (; i < p.items; ++i) {
+        const int begin = p.costs[i], end = p.costs[i + 1];
+        if (begin >= c1) break;
         Piece c;
         c.it = item_rows(p, i);
+        const int cost = tile_cost(c.it);
+        const int a = max(0, ceil_div(c0 - begin, cost)), b = min(ceil_div(c1 - begin, cost), (end - begin) / cost);
+        if (a >= b) continue;
         int most = 0, least = p.L;
         for (int t = c.it.row0 / p.H; t <= (c.it.row0 + c.it.rows - 1) / p.H; ++t) {
             const int n = seen_by(p, t);
@@ -756,14 +869,14 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
         item_tiles(p, i, most, c.it);
         c.it.first = __builtin_amdgcn_readfirstlane(c.it.first);
         c.seen_low = __builtin_amdgcn_readfirstlane(least);
-        c.a = __builtin_amdgcn_readfirstlane(t0 - begin);
-        c.nt = __builtin_amdgcn_readfirstlane(min(t1, end) - t0);
-        const bool whole = !p.stacked && c.nt == end - begin;
+        c.a = __builtin_amdgcn_readfirstlane(a);
+        c.nt = __builtin_amdgcn_readfirstlane(b - a);
+        const bool whole = !p.stacked && c.nt * cost == end - begin;
         const int64_t slot = slot_of(p, i, w, c.a == 0);
-        if (c.it.rows <= 16) shared_piece<FP8, PAGED, 1>(p, c, whole, slot, lds, wave, lane);
-        else if (c.it.rows <= 32) shared_piece<FP8, PAGED, 2>(p, c, whole, slot, lds, wave, lane);
-        else shared_piece<FP8, PAGED, 4>(p, c, whole, slot, lds, wave, lane);
-        t0 = min(t1, end);
+        if (c.it.rows > 64) shared_piece<FP8, PAGED, true, 4>(p, c, whole, slot, lds, wave, lane);
+        else if (c.it.rows > 32) shared_piece<FP8, PAGED, false, 4>(p, c, whole, slot, lds, wave, lane);
+        else if (c.it.rows > 16) shared_piece<FP8, PAGED, false, 2>(p, c, whole, slot, lds, wave, lane);
+        else shared_piece<FP8, PAGED, false, 1>(p, c, whole, slot, lds, wave, lane);
     }
 }
 
@@ -773,19 +886,19 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams p) 
     const int rows = p.B * p.SQ * p.H;
     const int row = blockIdx.x * 2 + (threadIdx.x >> 7), col = (threadIdx.x & 127) * 4;
     if (row >= rows) return;
-    const int total = p.tiles[p.items], groups = groups_of(p, total);
+    const int total = p.costs[p.items], groups = groups_of(p, total);
     const int seq_rows = p.SQ * p.H, b = row / seq_rows, in_seq = row - b * seq_rows;
     float m = -FLT_MAX, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int part = p.stacked ? 0 : 1; part < 2; ++part) {
-        const int i = part == 0 ? row / kRows : p.prefix_items + b * p.seq_blocks + in_seq / kRows;
-        const int hl = part == 0 ? row % kRows : in_seq % kRows;
-        const int begin = p.tiles[i], end = p.tiles[i + 1];
+        const int i = part == 0 ? row / kSharedRows : p.prefix_items + b * p.seq_blocks + in_seq / kSharedRows;
+        const int hl = part == 0 ? row % kSharedRows : in_seq % kSharedRows;
+        const int begin = p.costs[i], end = p.costs[i + 1];
         if (begin == end) continue;
-        const int w0 = group_at(begin, total, groups), w1 = group_at(end - 1, total, groups);
+        const int w0 = group_at(begin, total, groups), w1 = group_at(end - tile_cost(item_rows(p, i)), total, groups);
         if (!p.stacked && w0 == w1) return;  // a whole item: written by the main kernel
         for (int w = w0; w <= w1; ++w) {
-            const int64_t prow = slot_of(p, i, w, w == w0) * kRows + hl;
+            const int64_t prow = slot_of(p, i, w, w == w0) * kSharedRows + hl;
             const float ms = p.part_m[prow], ls = p.part_l[prow];
             const f32x4 u = *reinterpret_cast<const f32x4*>(p.part_o + prow * 512 + col);
             const float top = fmaxf(m, ms), keep = fast_exp2(m - top), add = fast_exp2(ms - top);
