@@ -31,6 +31,18 @@ constexpr int kThreads = 256;
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
+// The kernel's arguments, read from memory here and now.  As ordinary arguments
+// the compiler holds all of them in scalar registers from the start, spills
+// those into vector registers, and these, in the loop, into memory -- where the
+// wait for a reload is a full wait for the gathers too.  What the loop needs
+// (Hot) is passed along, the rest is read where it is used.
+typedef const __attribute__((address_space(4))) SharedParams* ArgsPtr;
+__device__ __forceinline__ ArgsPtr args_now() {
+    uint64_t a = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    return (ArgsPtr)a;
+}
+
 // One block of query rows and its keys: tiles of the prefix (sequence 0) and
 // then of the own rows.
 struct Item {
@@ -39,20 +51,20 @@ struct Item {
     int first, second;  // tiles over the prefix, over the own rows
 };
 
-__device__ __forceinline__ int seen_by(const SharedParams& p, int token) {
-    return min(max(p.lengths[token], 0), p.L);
+__device__ __forceinline__ int seen_by(ArgsPtr p, int token) {
+    return min(max(p->lengths[token], 0), p->L);
 }
 
 // Rows and sequence of item i, without its tiles.
-__device__ __forceinline__ Item item_rows(const SharedParams& p, int i) {
+__device__ __forceinline__ Item item_rows(ArgsPtr p, int i) {
     Item it;
-    if (i < p.prefix_items) {
+    if (i < p->prefix_items) {
         it.row0 = i * kSharedRows;
-        it.rows = min(kSharedRows, p.B * p.SQ * p.H - it.row0);
+        it.rows = min(kSharedRows, p->B * p->SQ * p->H - it.row0);
         it.seq = 0;
     } else {
-        const int j = i - p.prefix_items, b = j / p.seq_blocks, k = j - b * p.seq_blocks;
-        const int seq_rows = p.SQ * p.H;
+        const int j = i - p->prefix_items, b = j / p->seq_blocks, k = j - b * p->seq_blocks;
+        const int seq_rows = p->SQ * p->H;
         it.row0 = b * seq_rows + k * kSharedRows;
         it.rows = min(kSharedRows, seq_rows - k * kSharedRows);
         it.seq = b;
@@ -60,18 +72,19 @@ __device__ __forceinline__ Item item_rows(const SharedParams& p, int i) {
     return it;
 }
 
-// Tiles of an item whose longest query sees `most` rows.
-__device__ __forceinline__ void item_tiles(const SharedParams& p, int i, int most, Item& it) {
-    it.first = p.stacked && i >= p.prefix_items ? 0 : ceil_div(min(most, p.prefix), kKeys);
-    it.second = i < p.prefix_items ? 0 : ceil_div(max(most - p.prefix, 0), kKeys);
+// Tiles of an item whose longest query sees `most` rows.  Tiles start at
+// multiples of 32 keys: one that the prefix ends in is there twice, for either side.
+__device__ __forceinline__ void item_tiles(ArgsPtr p, int i, int most, Item& it) {
+    it.first = p->stacked && i >= p->prefix_items ? 0 : ceil_div(min(most, p->prefix), kKeys);
+    it.second = i < p->prefix_items || most <= p->prefix ? 0 : ceil_div(most, kKeys) - p->prefix / kKeys;
 }
 
 // What one tile of an item costs: see the kernel's two forms below.
 __device__ __forceinline__ int tile_cost(const Item& it) { return it.rows > 64 ? 3 : 2; }
 constexpr int kMinCost = 6;  // least cost a workgroup is given (no less than one tile's)
 
-__device__ __forceinline__ int groups_of(const SharedParams& p, int total) {
-    return max(1, min(p.workgroups, total / kMinCost));
+__device__ __forceinline__ int groups_of(ArgsPtr p, int total) {
+    return max(1, min(p->workgroups, total / kMinCost));
 }
 
 // Workgroup w computes the tiles that start in its share [w * total / groups,
@@ -82,23 +95,24 @@ __device__ __forceinline__ int group_at(int cost, int total, int groups) {
 }
 
 // Slot of the piece of item i that workgroup w computes; `head`: it starts at the item's first tile.
-__device__ __forceinline__ int64_t slot_of(const SharedParams& p, int i, int w, bool head) {
-    return p.stacked ? (int64_t)i + w : 2 * (int64_t)w + (head ? 1 : 0);
+__device__ __forceinline__ int64_t slot_of(ArgsPtr p, int i, int w, bool head) {
+    return p->stacked ? (int64_t)i + w : 2 * (int64_t)w + (head ? 1 : 0);
 }
 
 // ------------------------------------------------------------------ plan
 constexpr int kPlanThreads = 1024;
-__global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams p) {
+__global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams) {
+    const ArgsPtr p = args_now();
     __shared__ int sums[kPlanThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int base = 0;
-    for (int i0 = 0; i0 < p.items; i0 += kPlanThreads) {
+    for (int i0 = 0; i0 < p->items; i0 += kPlanThreads) {
         const int i = i0 + tid;
         int n = 0;
-        if (i < p.items) {
+        if (i < p->items) {
             Item it = item_rows(p, i);
             int most = 0;
-            for (int t = it.row0 / p.H; t <= (it.row0 + it.rows - 1) / p.H; ++t) most = max(most, seen_by(p, t));
+            for (int t = it.row0 / p->H; t <= (it.row0 + it.rows - 1) / p->H; ++t) most = max(most, seen_by(p, t));
             item_tiles(p, i, most, it);
             n = (it.first + it.second) * tile_cost(it);
         }
@@ -114,11 +128,11 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
             if (w < wave) before += sums[w];
             all += sums[w];
         }
-        if (i < p.items) p.costs[i] = base + before + scan - n;
+        if (i < p->items) p->costs[i] = base + before + scan - n;
         base += all;
         __syncthreads();
     }
-    if (tid == 0) p.costs[p.items] = base;
+    if (tid == 0) p->costs[p->items] = base;
 }
 
 // ------------------------------------------------------------------ main
@@ -176,39 +190,41 @@ struct PPLds {
     __device__ static uint32_t valid(uint32_t lds, int u) { return lds + VALID_OFF + 8 * (u % NTILE); }
 };
 
-// One tile of a piece: where its keys start and end, and the sequence they are looked up in.
+// What the main kernel's loop needs of them.
+struct Hot {
+    const char* kv;
+    const char* k_rope;
+    const int32_t* block_table;
+    int L, prefix, max_blocks, block_size, num_blocks;
+    uint32_t block_magic;
+    int block_shift;
+    float scale_log2;
+};
+
+// One tile of a piece: its first key (a multiple of 32), the keys [low, high)
+// of it that count, and the sequence they are looked up in.
 struct Tile {
-    int key0, key_end, seq;
+    int key0, low, high, seq;
 };
 struct Piece {
     Item it;
     int a, nt;      // first tile of the item, and how many
     int seen_low;   // least number of rows a query row of the block sees
 };
-__device__ __forceinline__ Tile tile_at(const SharedParams& p, const Piece& c, int u) {
+__device__ __forceinline__ Tile tile_at(const Hot& p, const Piece& c, int u) {
     const int t = c.a + u;
     const bool shared = t < c.it.first;
     Tile k;
-    k.key0 = shared ? t * kKeys : p.prefix + (t - c.it.first) * kKeys;
-    k.key_end = shared ? p.prefix : p.L;
+    k.key0 = (shared ? t : p.prefix / kKeys + (t - c.it.first)) * kKeys;
+    k.low = shared ? 0 : p.prefix;
+    k.high = shared ? p.prefix : p.L;
     k.seq = shared ? 0 : c.it.seq;
     return k;
 }
 
 // key / block_size, without a division (keys are below 2^25).
-__device__ __forceinline__ int block_of(const SharedParams& p, int key) {
+__device__ __forceinline__ int block_of(const Hot& p, int key) {
     return p.block_size == 1 ? key : (int)(__umulhi((uint32_t)key, p.block_magic) >> p.block_shift);
-}
-
-// One fp8 row: lanes 0..40 load 16 bytes each of its 656.
-__device__ __forceinline__ rsrc_t fp8_rsrc(const char* base, uint32_t row) {
-    const uint64_t a = reinterpret_cast<uint64_t>(base) + (uint64_t)row * kFp8Row;
-    rsrc_t r;
-    r[0] = (int)(uint32_t)a;
-    r[1] = (int)((a >> 32) & 0xffff);
-    r[2] = kFp8Row;
-    r[3] = 0x00020000;
-    return r;
 }
 
 // 4 bytes a lane straight into LDS (lane l at m0 + 4 l).
@@ -224,98 +240,138 @@ __device__ __forceinline__ void gather_words(uint32_t lds_base, rsrc_t rsrc, uin
 #pragma clang diagnostic pop
 }
 
-// Gathers of one tile by one wave: its rows 4 wave .. 4 wave + 3, an instruction
-// each (row), and (rest) the bf16 rows' rotary parts in one.  PV issues them one
-// at a time between its steps: the texture path takes about 50 bytes a clock,
-// and issued together they hold the wave up.  Paged: the rows' block entries
-// were loaded into LDS when the wave issued the tile three before (a piece's
-// first three before the loop), waited for since; those of the tile three
-// further on are issued last.
-template <bool FP8, bool PAGED>
-struct Gathers {
-    static constexpr int LOADS = (FP8 ? 4 : 5) + (PAGED ? 1 : 0);  // VMEM instructions
-    static constexpr int ENTRIES_AHEAD = 3;
-    const char* kv;
-    rsrc_t kr;
-    int my_row;        // lane l: row 4 wave + l % 4
-    uint32_t rope_off; // lane l < 32: its 16 bytes of the rotary part of row 4 wave + l / 8
-    uint32_t dst, rope_dst;
-    uint32_t lane16;   // 16 times the lane, computed here: kept across the loop it would be spilled
+// 16 bytes a lane, OFFSET + off on, straight into LDS: lane l at m0 + OFFSET + 16 l.
+template <int OFFSET>
+__device__ __forceinline__ void gather_at(uint32_t lds_base, rsrc_t rsrc, uint32_t off) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen offset:%3 lds"
+        :
+        : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(off), "s"(rsrc), "n"(OFFSET)
+        : "memory", "m0");
+#pragma clang diagnostic pop
+}
 
-    __device__ __forceinline__ void prepare(const SharedParams& p, const Piece& c, int u, uint32_t lds, int wave,
-                                            int lane) {
+// How a tile's rows lie: in one sequence (rows), in blocks of a multiple of
+// four rows (blocks), in any blocks (pages).
+enum { kRows = 0, kBlocks = 1, kPages = 2 };
+
+// Gathers of one tile by one wave: its rows 4 wave .. 4 wave + 3.  bf16: an
+// instruction a row (1 KiB), and one for their rotary parts; fp8: three
+// instructions, or one a row.  The four rows follow each other unless LAYOUT is
+// kPages, so that they have one descriptor (rows past a sequence's end are out of
+// its range and read as zeros); of a tile behind the piece (u >= nt) nothing is
+// read, but the instructions are the same, so that they can be counted on.
+//
+// They are issued together, behind the first LDS reads of QK or PV: the queue in
+// front of the texture path holds that many, and in the chain of MFMAs each
+// would cost about 60 clocks (a chain of 36 with its LDS reads: 764 clocks,
+// 772 with four gathers in front, 1000 with the four between its steps).
+//
+// Blocks and pages: the block entries come into LDS by a gather of their own,
+// issued with the tile AHEAD before.
+template <bool FP8, int LAYOUT>
+struct Gathers {
+    static constexpr int ENTRIES = LAYOUT == kPages ? 4 : 1;
+    static constexpr int AHEAD = FP8 ? 2 : 3;
+    static constexpr int LOADS = (FP8 ? (LAYOUT == kPages ? 4 : 3) : 5) + (LAYOUT != kRows ? 1 : 0);
+    int64_t first;  // row that the four start with, from the cache's start
+    int rows;       // how many of them can be read
+    int my_row;     // kPages: lane l: row 4 wave + l % 4
+    int tile;
+
+    __device__ __forceinline__ void prepare(const Hot& p, const Piece& c, int u, uint32_t lds, int wave, int lane) {
         using X = PPLds<FP8>;
-        asm volatile("" : "+v"(lane));
         const Tile k = tile_at(p, c, u);
         const int r0 = 4 * wave;
-        const int key_r = min(k.key0 + r0 + (lane & 3), k.key_end - 1);
-        const int in4 = (lane >> 3) & 3, key_l = min(k.key0 + r0 + in4, k.key_end - 1);
-        int rope_row = 0;
-        lane16 = (uint32_t)lane << 4;
-        kv = p.kv;
-        const char* rope = reinterpret_cast<const char*>(p.k_rope);
-        uint32_t pool;
-        if constexpr (!PAGED) {
-            const int64_t base = (int64_t)k.seq * p.L;
-            kv += base * (FP8 ? kFp8Row : 1024);
-            rope += base << 7;
-            my_row = key_r;
-            rope_row = key_l;
-            pool = (uint32_t)p.L << 7;
+        const bool on = u < c.nt;
+        tile = u;
+        if constexpr (LAYOUT == kRows) {
+            const int key = k.key0 + r0;
+            first = (int64_t)k.seq * p.L + key;
+            rows = on ? min(max(k.high - key, 0), 4) : 0;
+        } else if constexpr (LAYOUT == kBlocks) {
+            const int key = min(k.key0 + r0, p.L - 4);
+            const int entry = __builtin_amdgcn_readfirstlane(lds_load<int>(X::entries(lds, u, wave)));
+            const bool ok = (uint32_t)entry < (uint32_t)p.num_blocks;
+            first = (ok ? entry : 0) * p.block_size + (key - block_of(p, key) * p.block_size);
+            rows = on && ok ? 4 : 0;
+            if (lane == 0) lds_store<uint8_t>(X::valid(lds, u) + wave, ok ? 0xf : 0);
         } else {
-            const int col_r = block_of(p, key_r), col_l = block_of(p, key_l);
-            const int e_r = lds_load<int>(X::entries(lds, u, r0 + (lane & 3)));
-            const int e_l = FP8 ? 0 : lds_load<int>(X::entries(lds, u, r0 + in4));
-            const bool ok_r = (uint32_t)e_r < (uint32_t)p.num_blocks;
-            const uint64_t valid = __ballot(ok_r) & 0xf;
+            asm volatile("" : "+v"(lane));
+            const int key = min(k.key0 + r0 + (lane & 3), p.L - 1);
+            const int entry = lds_load<int>(X::entries(lds, u, r0 + (lane & 3)));
+            const bool ok = (uint32_t)entry < (uint32_t)p.num_blocks;
+            const uint64_t valid = __ballot(ok) & 0xf;
             if (lane == 0) lds_store<uint8_t>(X::valid(lds, u) + wave, (uint8_t)valid);
-            my_row = (ok_r ? e_r : 0) * p.block_size + (key_r - col_r * p.block_size);
-            if (!FP8) {
-                const bool ok_l = (uint32_t)e_l < (uint32_t)p.num_blocks;
-                rope_row = (ok_l ? e_l : 0) * p.block_size + (key_l - col_l * p.block_size);
-            }
-            pool = (uint32_t)(p.num_blocks * p.block_size) << 7;
-        }
-        if constexpr (FP8) {
-            dst = X::raw(lds, u) + r0 * kFp8Row;
-        } else {
-            dst = X::stage(lds, u) + r0 * 1024;
-            rope_dst = X::stage(lds, u) + X::KV_BYTES + r0 * 128;
-            kr = make_rsrc(rope, pool);
-            rope_off = ((uint32_t)rope_row << 7) + (((lane & 7) ^ sw_rope(r0 + in4)) << 4);
+            my_row = (ok ? entry : 0) * p.block_size + (key - block_of(p, key) * p.block_size);
+            rows = on ? 4 : 0;
         }
     }
-    __device__ __forceinline__ void row(int rr, int wave) const {
-        const uint32_t r = (uint32_t)__builtin_amdgcn_readlane(my_row, rr);
-        if constexpr (FP8) {
-            if (lane16 < kFp8Row) gather_lanes(dst + rr * kFp8Row, fp8_rsrc(kv, r), lane16);
-        } else {
-            gather_row(dst + rr * 1024, row_rsrc(kv, r), lane16, (uint32_t)sw_kv(4 * wave + rr) << 4);
-        }
-    }
-    __device__ __forceinline__ void rest(const SharedParams& p, const Piece& c, int u, uint32_t lds, int wave) const {
+    __device__ __forceinline__ void issue(const Hot& p, const Piece& c, uint32_t lds, int wave, int lane) const {
         using X = PPLds<FP8>;
-        if constexpr (!FP8)
-            if (lane16 < 512) gather_lanes(rope_dst, kr, rope_off);
-        entries(p, c, u + ENTRIES_AHEAD, lds, wave, (int)(lane16 >> 4));
+        asm volatile("" : "+v"(lane));  // lane offsets kept across the loop would be spilled
+        if constexpr (FP8) {
+            const uint32_t dst = X::raw(lds, tile) + 4 * wave * kFp8Row, off = (uint32_t)lane << 4;
+            if constexpr (LAYOUT == kPages) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t r = __builtin_amdgcn_readlane(my_row, i);
+                    if (lane < kFp8Row / 16)
+                        gather_at<0>(dst + i * kFp8Row, make_rsrc(p.kv + r * kFp8Row, rows ? kFp8Row : 0), off);
+                }
+            } else {
+                const rsrc_t rs = make_rsrc(p.kv + first * kFp8Row, (uint32_t)rows * kFp8Row);
+                gather_at<0>(dst, rs, off);
+                gather_at<1024>(dst, rs, off);
+                if (lane < (4 * kFp8Row - 2048) / 16) gather_at<2048>(dst, rs, off);
+            }
+        } else {
+            const uint32_t dst = X::stage(lds, tile) + 4 * wave * 1024;
+            const uint32_t rope_dst = X::stage(lds, tile) + X::KV_BYTES + 4 * wave * 128;
+            const int in4 = (lane >> 3) & 3;
+            const uint32_t chunk = (uint32_t)((lane & 7) ^ sw_rope(4 * wave + in4)) << 4;
+            // sw_kv(4 wave + i) = sw_kv(4 wave) ^ 4 i
+            const uint32_t off = (uint32_t)(lane ^ sw_kv(4 * wave)) << 4;
+            if constexpr (LAYOUT == kPages) {
+                const int row = __shfl(my_row, in4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t r = __builtin_amdgcn_readlane(my_row, i);
+                    gather_at<0>(dst + i * 1024, make_rsrc(p.kv + (r << 10), rows ? 1024 : 0), off ^ (64u * i));
+                }
+                if (lane < 32)
+                    gather_at<0>(rope_dst, make_rsrc(p.k_rope, rows ? (uint32_t)(p.num_blocks * p.block_size) << 7 : 0),
+                                 ((uint32_t)row << 7) + chunk);
+            } else {
+                const rsrc_t rs = make_rsrc(p.kv + (first << 10), (uint32_t)rows << 10);
+                gather_at<0>(dst, rs, off);
+                gather_at<1024>(dst, rs, off ^ 64u);
+                gather_at<2048>(dst, rs, off ^ 128u);
+                gather_at<3072>(dst, rs, off ^ 192u);
+                if (lane < 32)
+                    gather_at<0>(rope_dst, make_rsrc(p.k_rope + (first << 7), (uint32_t)rows << 7),
+                                 (uint32_t)(in4 << 7) + chunk);
+            }
+        }
+        entries(p, c, tile + AHEAD, lds, wave, lane);
     }
-    // Block entries of the wave's rows of tile u into LDS (past the item: some entry, not used).
-    static __device__ __forceinline__ void entries(const SharedParams& p, const Piece& c, int u, uint32_t lds, int wave,
-                                                   int lane) {
-        if constexpr (PAGED) {
+    // Block entries of the wave's rows of tile u into LDS (behind the cache: some entry, not used).
+    static __device__ __forceinline__ void entries(const Hot& p, const Piece& c, int u, uint32_t lds, int wave, int lane) {
+        if constexpr (LAYOUT != kRows) {
             const Tile n = tile_at(p, c, u);
-            const int key = min(n.key0 + 4 * wave + lane, n.key_end - 1);
-            if (lane < 4)
-                gather_words(PPLds<FP8>::entries(lds, u, 4 * wave),
+            const int key = min(n.key0 + 4 * wave + lane, p.L - 1);
+            if (lane < ENTRIES)
+                gather_words(PPLds<FP8>::entries(lds, u, LAYOUT == kPages ? 4 * wave : wave),
                              make_rsrc(p.block_table + (int64_t)n.seq * p.max_blocks, 4u * (uint32_t)p.max_blocks),
                              4u * (uint32_t)block_of(p, key));
         }
     }
-    __device__ __forceinline__ void all(const SharedParams& p, const Piece& c, int u, uint32_t lds, int wave, int lane) {
+    __device__ __forceinline__ void all(const Hot& p, const Piece& c, int u, uint32_t lds, int wave, int lane) {
         prepare(p, c, u, lds, wave, lane);
-#pragma unroll
-        for (int rr = 0; rr < 4; ++rr) row(rr, wave);
-        rest(p, c, u, lds, wave);
+        issue(p, c, lds, wave, lane);
     }
 };
 
@@ -382,9 +438,9 @@ __device__ __forceinline__ void expand_rows(uint32_t lds, int u, int wave, int l
 }
 
 // Rows of a tile that are in the pool, bit r for row r, from the waves' four bits each.
-template <bool FP8, bool PAGED>
+template <bool FP8, int LAYOUT>
 __device__ __forceinline__ uint32_t pool_rows(uint32_t lds, int u) {
-    if constexpr (!PAGED) return 0xffffffffu;
+    if constexpr (LAYOUT == kRows) return 0xffffffffu;
     const uint64_t v = lds_load<uint64_t>(PPLds<FP8>::valid(lds, u));
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
     const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
@@ -395,8 +451,8 @@ __device__ __forceinline__ uint32_t pool_rows(uint32_t lds, int u) {
 
 // Which of the 32 keys of a tile a query row that sees `seen` rows has: bit r is tile row r.
 __device__ __forceinline__ uint32_t key_mask(const Tile& k, int seen, uint32_t valid) {
-    const int n = min(max(min(seen, k.key_end) - k.key0, 0), kKeys);
-    return n == kKeys ? valid : valid & ((1u << n) - 1);
+    const int n = min(max(min(seen, k.high) - k.key0, 0), kKeys), skip = max(k.low - k.key0, 0);  // skip < 32
+    return valid & (n == kKeys ? 0xffffffffu : (1u << n) - 1) & (0xffffffffu << skip);
 }
 
 // Lane group g's rows of a tile -- 4 g + j (j < 4) and 16 + 4 g + j -- from a key mask: bit j, bit 4 + j.
@@ -426,27 +482,28 @@ __device__ __forceinline__ void clear_specials(uint32_t stage, int gw, int lane)
 }
 
 // One piece of an item, WIDE: up to 128 rows, else up to 16 NB (NB = 4 if WIDE).
-template <bool FP8, bool PAGED, bool WIDE, int NB>
-__device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece& c, bool whole, int64_t slot,
+template <bool FP8, int LAYOUT, bool WIDE, int NB>
+__device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool whole, int64_t slot,
                                              uint32_t lds, int wave, int lane) {
     static_assert(!WIDE || NB == 4, "a group's four row blocks");
     using X = PPLds<FP8>;
-    using G = Gathers<FP8, PAGED>;
+    using G = Gathers<FP8, LAYOUT>;
     const int grp = wave >> 2, gw = wave & 3;
     const int g = lane >> 4, n16 = lane & 15;
     const int block = (WIDE ? 64 * grp : 0) + 16 * gw;  // this wave's query rows in QK
     const bool live = block < c.it.rows;
     const int row = c.it.row0 + (live ? block : 0);
     const int nt = c.nt;
-    const int seen = live ? __builtin_amdgcn_readfirstlane(seen_by(p, row / p.H)) : 0;
+    const ArgsPtr args = args_now();
+    const int seen = live ? __builtin_amdgcn_readfirstlane(seen_by(args, row / args->H)) : 0;
     const uint32_t p_lds = lds + X::P_OFF + grp * X::P_GROUP;
 
     bf16x8 qf[18];
     {
-        const uint16_t* q = p.q + (int64_t)(row + n16) * 512 + 8 * qk_lane_chunk(g);
+        const uint16_t* q = args->q + (int64_t)(row + n16) * 512 + 8 * qk_lane_chunk(g);
 #pragma unroll
         for (int ks = 0; ks < 16; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(q + 32 * ks);
-        const uint16_t* rr = p.q_rope + (int64_t)(row + n16) * 64 + 8 * g;
+        const uint16_t* rr = args->q_rope + (int64_t)(row + n16) * 64 + 8 * g;
         qf[16] = *reinterpret_cast<const bf16x8*>(rr);
         qf[17] = *reinterpret_cast<const bf16x8*>(rr + 32);
     }
@@ -467,6 +524,9 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         off_p = pp_pchunk(n16, g) | (pp_pchunk(16 * gw + n16, g) << 16);
     }
 
+    // bf16: gathers are prepared behind QK, where the wave would otherwise wait
+    // (behind: narrow, those of the QK after the PV in between).
+    G gather, behind;
     auto qk_softmax = [&](int u, bool& overflow) __attribute__((always_inline)) {
         const uint32_t stage = X::stage(lds, u);
         asm volatile("" : "+v"(off_kv), "+v"(off_rope), "+v"(off_p));
@@ -477,12 +537,13 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
             if (ks < 16) return lds_load<bf16x8>((kbase ^ (64u * (ks & 3))) + 256u * (ks >> 2) + sub * 16 * 1024);
             return lds_load<bf16x8>((rbase ^ (64u * (ks - 16))) + sub * 16 * 128);
         };
-        constexpr int KD = 7;  // K fragments in flight
+        constexpr int KD = 6;  // K fragments in flight
         __builtin_amdgcn_s_setprio(2);
         f32x4 sacc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
         bf16x8 kf[KD];
 #pragma unroll
         for (int j = 0; j < KD; ++j) kf[j] = kfrag(j);
+        if constexpr (!FP8) gather.issue(p, c, lds, wave, lane);
 #pragma unroll
         for (int step = 0; step < 36; ++step) {
             sacc[step & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[step % KD], qf[step >> 1], sacc[step & 1], 0, 0, 0);
@@ -493,7 +554,7 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         float x[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) x[r] = sacc[r >> 2][r & 3];
-        const uint32_t mask = key_mask(tile_at(p, c, u), seen, pool_rows<FP8, PAGED>(lds, u));
+        const uint32_t mask = key_mask(tile_at(p, c, u), seen, pool_rows<FP8, LAYOUT>(lds, u));
         if (__builtin_expect(mask != 0xffffffffu, 0)) {
             int ln = lane;
             asm volatile("" : "+v"(ln));
@@ -534,11 +595,10 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
 
     // Whether some query row of the block does not see all keys of tile u (every wave agrees).
     auto partial = [&](int u) __attribute__((always_inline)) -> bool {
-        return key_mask(tile_at(p, c, u), c.seen_low, pool_rows<FP8, PAGED>(lds, u)) != 0xffffffffu;
+        return key_mask(tile_at(p, c, u), c.seen_low, pool_rows<FP8, LAYOUT>(lds, u)) != 0xffffffffu;
     };
 
-    // PV of tile u, with the gathers of tile `next` (bf16; if there is one) between its steps.
-    auto pv = [&](int u, int next) __attribute__((always_inline)) {
+    auto pv = [&](int u) __attribute__((always_inline)) {
         const uint32_t stage = X::stage(lds, u);
         asm volatile("" : "+v"(off_kv), "+v"(off_p));
         const uint32_t vbase = stage + (off_kv >> 16);
@@ -549,9 +609,6 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
             return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
         };
         if (__builtin_expect(partial(u), 0)) clear_specials(stage, gw, lane);
-        const bool more = !FP8 && next < nt;
-        G gather;
-        if (more) gather.prepare(p, c, next, lds, wave, lane);
         bf16x8 pf[NB];
 #pragma unroll
         for (int hb = 0; hb < NB; ++hb) pf[hb] = lds_load<bf16x8>(p_lds + (off_p & 0xffffu) + 1024 * hb);
@@ -559,35 +616,26 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         bf16x8 vf[VD];
 #pragma unroll
         for (int j = 0; j < VD; ++j) vf[j] = vfrag(j);
+        if constexpr (!FP8 && !WIDE) gather.issue(p, c, lds, wave, lane);
 #pragma unroll
         for (int cb = 0; cb < 8; ++cb) {
 #pragma unroll
             for (int hb = 0; hb < NB; ++hb)
                 oacc[hb][cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[cb % VD], pf[hb], oacc[hb][cb], 0, 0, 0);
             if (cb + VD < 8) vf[cb % VD] = vfrag(cb + VD);
-            if (more && cb < 4) gather.row(cb, wave);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (more) gather.rest(p, c, next, lds, wave);
     };
 
-    // fp8: the wave's rows of tile u into the ring, and the gathers of tile u + 2 into their place.
+    // fp8, every wave once a tile: its rows of tile u (issued two tiles ago) into
+    // the ring, and the gathers of tile u + 2 into their place.
     auto advance = [&](int u) __attribute__((always_inline)) {
-        if constexpr (FP8)
-            if (u < nt) {
-                if (u + 1 < nt) wait_vmcnt<G::LOADS>();
-                else wait_vmcnt<0>();
-                expand_rows(lds, u, wave, lane);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // raw is read before it is written again
-                G gather;
-                if (u + 2 < nt) gather.all(p, c, u + 2, lds, wave, lane);
-            }
-    };
-    // Waits until the gathers that this wave issued before its last n tiles' have landed.
-    auto landed = [&](int n) __attribute__((always_inline)) {
-        if (n >= 2) wait_vmcnt<2 * G::LOADS>();
-        else if (n == 1) wait_vmcnt<G::LOADS>();
-        else wait_vmcnt<0>();
+        if constexpr (FP8) {
+            wait_vmcnt<G::LOADS>();
+            if (u < nt) expand_rows(lds, u, wave, lane);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // raw is read before it is written again
+            gather.all(p, c, u + 2, lds, wave, lane);
+        }
     };
 
 #pragma unroll 1
@@ -599,88 +647,82 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
         l_run = 0.f;
         if (pass == 1) m_ref = max_xor32(max_xor16(m_lane));
         bool overflow = false;
-        // The first tile's rows, and Q: a full wait, as the compiler does not
-        // count the gathers (it would wait for Q in the loop).
-        G gather;
-        if constexpr (PAGED) {
-            for (int u = 0; u < G::ENTRIES_AHEAD; ++u) G::entries(p, c, u, lds, wave, lane);
+        if constexpr (LAYOUT != kRows) {
+            for (int u = 0; u < G::AHEAD; ++u) G::entries(p, c, u, lds, wave, lane);
             wait_vmcnt<0>();
         }
+        // The first tile's rows, and Q: a full wait, as the compiler does not
+        // count the gathers (it would wait for Q in the loop).
         gather.all(p, c, 0, lds, wave, lane);
         wait_vmcnt<0>();
-        if constexpr (FP8) {
-            // Every wave, once a tile: waits for its rows of the next tile (issued
-            // two tiles ago), expands them, issues two tiles ahead into their place.
-            if (nt > 1) gather.all(p, c, 1, lds, wave, lane);
-            advance(0);
-        } else if (nt > 1) {
-            gather.all(p, c, 1, lds, wave, lane);
-        }
+        gather.all(p, c, 1, lds, wave, lane);
+        if constexpr (FP8) advance(0);
+        else gather.prepare(p, c, 2, lds, wave, lane);
         if constexpr (!WIDE) {
-            // In half u every wave issues (bf16) its rows of tile u + 2 into the
-            // stage of tile u - 2, whose last reader ran in half u - 1: after QK,
-            // where it would otherwise wait, or between the steps of PV.  The
-            // half ends with its rows of tile u + 1 landed.
+            // bf16: in half u every wave issues its rows of tile u + 2, into the
+            // stage of tile u - 2, which was last read in half u - 1; the half
+            // ends with its rows of tile u + 1 landed.
             if (grp == 1) {  // half 0, without PV
                 lds_barrier();
                 if constexpr (FP8) {
                     advance(1);
                 } else {
-                    wait_vmcnt<0>();
-                    if (2 < nt) gather.all(p, c, 2, lds, wave, lane);
+                    gather.issue(p, c, lds, wave, lane);
+                    wait_vmcnt<G::LOADS>();
+                    gather.prepare(p, c, 3, lds, wave, lane);
                 }
             }
 #pragma unroll 1
             for (int u = grp; u < nt; u += 2) {
                 lds_barrier();
                 if (live) qk_softmax(u, overflow);
+                else if constexpr (!FP8) gather.issue(p, c, lds, wave, lane);
                 if constexpr (FP8) {
                     advance(u + 1);
                 } else {
-                    wait_vmcnt<0>();
-                    if (u + 2 < nt) gather.all(p, c, u + 2, lds, wave, lane);
+                    wait_vmcnt<G::LOADS>();
+                    gather.prepare(p, c, u + 3, lds, wave, lane);
+                    behind.prepare(p, c, u + 4, lds, wave, lane);
                 }
                 lds_barrier();
                 if constexpr (FP8) advance(u + 2);
-                pv(u, u + 3);
-                if constexpr (!FP8) landed(u + 3 < nt ? 1 : 0);
+                pv(u);
+                if constexpr (!FP8) {
+                    wait_vmcnt<G::LOADS>();
+                    gather = behind;
+                }
             }
             if (((nt ^ grp) & 1) == 0) lds_barrier();  // half nt: the other group's last PV
         } else {
-            // In PV of tile t a group issues (bf16) its rows of tile t + 3, into
-            // the stage of tile t - 1, which both groups are past.  A tile in
-            // which some row sees less than all has one barrier more, between
-            // group 1's QK and group 0's clear_specials of it.
-            if constexpr (!FP8)
-                if (grp == 0 && nt > 2) gather.all(p, c, 2, lds, wave, lane);
-            if (grp == 0) {
-#pragma unroll 1
-                for (int t = 0; t < nt; ++t) {
-                    lds_barrier();
-                    if (live) qk_softmax(t, overflow);
-                    lds_barrier();
-                    if (__builtin_expect(partial(t), 0)) lds_barrier();
-                    if constexpr (FP8) advance(t + 1);
-                    pv(t, t + 3);
-                    if constexpr (!FP8) landed(min(2, nt - 2 - t));
-                }
-                lds_barrier();  // half 2 nt: group 1's last PV
-            } else {
+            // bf16: tile t + 2 is issued in QK of tile t, into the stage of tile
+            // t - 2, which both groups are past.  A tile in which some row sees
+            // less than all has one barrier more, between group 1's QK and group
+            // 0's clear_specials of it.
+            if (grp == 1) {
                 lds_barrier();
-                if constexpr (FP8) advance(1);
-                else if (2 < nt) gather.all(p, c, 2, lds, wave, lane);
-#pragma unroll 1
-                for (int t = 0; t < nt; ++t) {
-                    lds_barrier();
-                    if (live) qk_softmax(t, overflow);
-                    if (__builtin_expect(partial(t), 0)) lds_barrier();
-                    if constexpr (!FP8) landed(min(1, nt - 2 - t));
-                    lds_barrier();
-                    if constexpr (FP8) advance(t + 2);
-                    pv(t, t + 3);
-                }
+                advance(1);
             }
+#pragma unroll 1
+            for (int t = 0; t < nt; ++t) {
+                lds_barrier();
+                if (live) qk_softmax(t, overflow);
+                else if constexpr (!FP8) gather.issue(p, c, lds, wave, lane);
+                const bool clears = partial(t);
+                if (grp == 1) {
+                    if (__builtin_expect(clears, 0)) lds_barrier();
+                    if constexpr (!FP8) wait_vmcnt<G::LOADS>();
+                }
+                if constexpr (!FP8) gather.prepare(p, c, t + 3, lds, wave, lane);
+                lds_barrier();
+                if (grp == 0 && __builtin_expect(clears, 0)) lds_barrier();
+                advance(t + 1 + grp);
+                pv(t);
+                if constexpr (!FP8)
+                    if (grp == 0) wait_vmcnt<G::LOADS>();
+            }
+            if (grp == 0) lds_barrier();  // half 2 nt: group 1's last PV
         }
+        wait_vmcnt<0>();  // gathers behind the piece write zeros into LDS
         if (pass == 1) break;
         // does any row need the second pass?
         const uint32_t flag = lds + X::FLAG_OFF;
@@ -694,6 +736,7 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
 
     // ---- the QK waves publish (l, reference, maximum) of their rows; the PV waves scale their blocks
     lds_barrier();
+    const ArgsPtr out = args_now();
     const uint32_t ml = lds + X::ML_OFF;
     l_run = sum_xor32(sum_xor16(l_run));
     const float m_true = max_xor32(max_xor16(m_lane));
@@ -714,22 +757,22 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
     auto put_stats = [&](int hl, float top, float sum) __attribute__((always_inline)) {
         if (hl >= c.it.rows) return;
         if (whole) {
-            p.out_max[c.it.row0 + hl] = sum == 0.f ? -INFINITY : top * kLn2;
-            p.out_sum[c.it.row0 + hl] = sum;
+            out->out_max[c.it.row0 + hl] = sum == 0.f ? -INFINITY : top * kLn2;
+            out->out_sum[c.it.row0 + hl] = sum;
         } else {
-            p.part_m[slot * kSharedRows + hl] = top;
-            p.part_l[slot * kSharedRows + hl] = sum;
+            out->part_m[slot * kSharedRows + hl] = top;
+            out->part_l[slot * kSharedRows + hl] = sum;
         }
     };
     // Staged rows [first, first + n) of the block, row r at HROW (bf16) or kPartRow (fp32) * (r - first), stored whole.
     auto store_rows = [&](int first, int n) __attribute__((always_inline)) {
         const int end = min(first + n, c.it.rows);
         if (whole) {
-            uint16_t* base = p.out + (int64_t)c.it.row0 * 512 + 8 * eln;
+            uint16_t* base = out->out + (int64_t)c.it.row0 * 512 + 8 * eln;
             for (int r = first + wave; r < end; r += 8)
                 *reinterpret_cast<bf16x8*>(base + (int64_t)r * 512) = lds_load<bf16x8>(lds + (r - first) * HROW + 16 * eln);
         } else {
-            float* base = p.part_o + slot * (kSharedRows * 512) + 4 * eln;
+            float* base = out->part_o + slot * (kSharedRows * 512) + 4 * eln;
             for (int i = 2 * first + wave; i < 2 * end; i += 8)
                 *reinterpret_cast<f32x4*>(base + (i >> 1) * 512 + 256 * (i & 1)) =
                     lds_load<f32x4>(lds + (uint32_t)(((i >> 1) - first) * kPartRow + 1024 * (i & 1) + 16 * eln));
@@ -833,35 +876,41 @@ __device__ __forceinline__ void shared_piece(const SharedParams& p, const Piece&
     lds_barrier();  // LDS is free for the next piece
 }
 
-template <bool FP8, bool PAGED>
-__global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams p) {
+template <bool FP8, int LAYOUT>
+__global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams arguments) {
     using X = PPLds<FP8>;
     __shared__ __attribute__((aligned(1024))) char smem[X::LDS_BYTES];
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int total = p.costs[p.items], groups = groups_of(p, total);
+    const Hot hot{arguments.kv,          reinterpret_cast<const char*>(arguments.k_rope), arguments.block_table,
+                  arguments.L,           arguments.prefix,      arguments.max_blocks,   arguments.block_size,
+                  arguments.num_blocks,  arguments.block_magic, arguments.block_shift,  arguments.scale_log2};
+    ArgsPtr p = args_now();
+    const int total = p->costs[p->items], groups = groups_of(p, total);
     const int w = blockIdx.x;
     if (w >= groups) return;
     const int c0 = share_of(w, total, groups), c1 = share_of(w + 1, total, groups);
     if (c0 >= c1) return;
-    int i = 0, high = p.items;  // the item that holds cost c0: costs[i] <= c0 < costs[i + 1]
+    int i = 0, high = p->items;  // the item that holds cost c0: costs[i] <= c0 < costs[i + 1]
     while (high - i > 1) {
         const int mid = (i + high) >> 1;
-        if (p.costs[mid] <= c0) i = mid;
+        if (p->costs[mid] <= c0) i = mid;
         else high = mid;
     }
 #pragma unroll 1
-    for (; i < p.items; ++i) {
-        const int begin = p.costs[i], end = p.costs[i + 1];
+    for (;; ++i) {
+        p = args_now();
+        if (i >= p->items) break;
+        const int begin = p->costs[i], end = p->costs[i + 1];
         if (begin >= c1) break;
         Piece c;
         c.it = item_rows(p, i);
         const int cost = tile_cost(c.it);
         const int a = max(0, ceil_div(c0 - begin, cost)), b = min(ceil_div(c1 - begin, cost), (end - begin) / cost);
         if (a >= b) continue;
-        int most = 0, least = p.L;
-        for (int t = c.it.row0 / p.H; t <= (c.it.row0 + c.it.rows - 1) / p.H; ++t) {
+        int most = 0, least = p->L;
+        for (int t = c.it.row0 / p->H; t <= (c.it.row0 + c.it.rows - 1) / p->H; ++t) {
             const int n = seen_by(p, t);
             most = max(most, n);
             least = min(least, n);
@@ -871,36 +920,37 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
         c.seen_low = __builtin_amdgcn_readfirstlane(least);
         c.a = __builtin_amdgcn_readfirstlane(a);
         c.nt = __builtin_amdgcn_readfirstlane(b - a);
-        const bool whole = !p.stacked && c.nt * cost == end - begin;
+        const bool whole = !p->stacked && c.nt * cost == end - begin;
         const int64_t slot = slot_of(p, i, w, c.a == 0);
-        if (c.it.rows > 64) shared_piece<FP8, PAGED, true, 4>(p, c, whole, slot, lds, wave, lane);
-        else if (c.it.rows > 32) shared_piece<FP8, PAGED, false, 4>(p, c, whole, slot, lds, wave, lane);
-        else if (c.it.rows > 16) shared_piece<FP8, PAGED, false, 2>(p, c, whole, slot, lds, wave, lane);
-        else shared_piece<FP8, PAGED, false, 1>(p, c, whole, slot, lds, wave, lane);
+        if (c.it.rows > 64) shared_piece<FP8, LAYOUT, true, 4>(hot, c, whole, slot, lds, wave, lane);
+        else if (c.it.rows > 32) shared_piece<FP8, LAYOUT, false, 4>(hot, c, whole, slot, lds, wave, lane);
+        else if (c.it.rows > 16) shared_piece<FP8, LAYOUT, false, 2>(hot, c, whole, slot, lds, wave, lane);
+        else shared_piece<FP8, LAYOUT, false, 1>(hot, c, whole, slot, lds, wave, lane);
     }
 }
 
 // ------------------------------------------------------------------ merge
 // One workgroup a row pair; thread t of a row's 128 owns columns 4 t .. 4 t + 3.
-__global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams p) {
-    const int rows = p.B * p.SQ * p.H;
+__global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams) {
+    const ArgsPtr p = args_now();
+    const int rows = p->B * p->SQ * p->H;
     const int row = blockIdx.x * 2 + (threadIdx.x >> 7), col = (threadIdx.x & 127) * 4;
     if (row >= rows) return;
-    const int total = p.costs[p.items], groups = groups_of(p, total);
-    const int seq_rows = p.SQ * p.H, b = row / seq_rows, in_seq = row - b * seq_rows;
+    const int total = p->costs[p->items], groups = groups_of(p, total);
+    const int seq_rows = p->SQ * p->H, b = row / seq_rows, in_seq = row - b * seq_rows;
     float m = -FLT_MAX, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int part = p.stacked ? 0 : 1; part < 2; ++part) {
-        const int i = part == 0 ? row / kSharedRows : p.prefix_items + b * p.seq_blocks + in_seq / kSharedRows;
+    for (int part = p->stacked ? 0 : 1; part < 2; ++part) {
+        const int i = part == 0 ? row / kSharedRows : p->prefix_items + b * p->seq_blocks + in_seq / kSharedRows;
         const int hl = part == 0 ? row % kSharedRows : in_seq % kSharedRows;
-        const int begin = p.costs[i], end = p.costs[i + 1];
+        const int begin = p->costs[i], end = p->costs[i + 1];
         if (begin == end) continue;
         const int w0 = group_at(begin, total, groups), w1 = group_at(end - tile_cost(item_rows(p, i)), total, groups);
-        if (!p.stacked && w0 == w1) return;  // a whole item: written by the main kernel
+        if (!p->stacked && w0 == w1) return;  // a whole item: written by the main kernel
         for (int w = w0; w <= w1; ++w) {
             const int64_t prow = slot_of(p, i, w, w == w0) * kSharedRows + hl;
-            const float ms = p.part_m[prow], ls = p.part_l[prow];
-            const f32x4 u = *reinterpret_cast<const f32x4*>(p.part_o + prow * 512 + col);
+            const float ms = p->part_m[prow], ls = p->part_l[prow];
+            const f32x4 u = *reinterpret_cast<const f32x4*>(p->part_o + prow * 512 + col);
             const float top = fmaxf(m, ms), keep = fast_exp2(m - top), add = fast_exp2(ms - top);
             l = l * keep + ls * add;
             acc = acc * keep + u * add;
@@ -910,10 +960,10 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams p) 
     const float inv = l == 0.f ? 0.f : 1.f / l;
     bf16x4 v;
     for (int r = 0; r < 4; ++r) v[r] = (__bf16)(acc[r] * inv);
-    *reinterpret_cast<bf16x4*>(p.out + (int64_t)row * 512 + col) = v;
+    *reinterpret_cast<bf16x4*>(p->out + (int64_t)row * 512 + col) = v;
     if (col == 0) {
-        p.out_max[row] = l == 0.f ? -INFINITY : m * kLn2;
-        p.out_sum[row] = l;
+        p->out_max[row] = l == 0.f ? -INFINITY : m * kLn2;
+        p->out_sum[row] = l;
     }
 }
 
@@ -923,8 +973,13 @@ int launch_shared(const SharedParams& p, hipStream_t stream) {
     hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
     int rc = (int)hipGetLastError();
     if (rc) return rc;
-    auto* kernel = p.kv_fp8 ? (p.block_table ? shared_main_kernel<true, true> : shared_main_kernel<true, false>)
-                            : (p.block_table ? shared_main_kernel<false, true> : shared_main_kernel<false, false>);
+    const int layout = !p.block_table ? kRows : p.block_size % 4 == 0 ? kBlocks : kPages;
+    auto* kernel = p.kv_fp8 ? (layout == kRows     ? shared_main_kernel<true, kRows>
+                               : layout == kBlocks ? shared_main_kernel<true, kBlocks>
+                                                   : shared_main_kernel<true, kPages>)
+                            : (layout == kRows     ? shared_main_kernel<false, kRows>
+                               : layout == kBlocks ? shared_main_kernel<false, kBlocks>
+                                                   : shared_main_kernel<false, kPages>);
     hipLaunchKernelGGL(kernel, dim3(p.workgroups), dim3(kPPThreads), 0, stream, p);
     rc = (int)hipGetLastError();
     if (rc) return rc;
