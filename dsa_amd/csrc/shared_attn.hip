@@ -524,9 +524,11 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         off_p = pp_pchunk(n16, g) | (pp_pchunk(16 * gw + n16, g) << 16);
     }
 
-    // bf16: gathers are prepared behind QK, where the wave would otherwise wait
-    // (behind: narrow, those of the QK after the PV in between).
+    // What the wave's next turn takes is made ready behind PV, the shorter of the
+    // two: the gathers (behind: narrow, those of PV), and the rows of its tile
+    // that are in the pool.
     G gather, behind;
+    uint32_t valid = 0;
     auto qk_softmax = [&](int u, bool& overflow) __attribute__((always_inline)) {
         const uint32_t stage = X::stage(lds, u);
         asm volatile("" : "+v"(off_kv), "+v"(off_rope), "+v"(off_p));
@@ -543,7 +545,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         bf16x8 kf[KD];
 #pragma unroll
         for (int j = 0; j < KD; ++j) kf[j] = kfrag(j);
-        if constexpr (!FP8) gather.issue(p, c, lds, wave, lane);
+        if constexpr (!FP8 && !WIDE) gather.issue(p, c, lds, wave, lane);
 #pragma unroll
         for (int step = 0; step < 36; ++step) {
             sacc[step & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[step % KD], qf[step >> 1], sacc[step & 1], 0, 0, 0);
@@ -554,7 +556,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         float x[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) x[r] = sacc[r >> 2][r & 3];
-        const uint32_t mask = key_mask(tile_at(p, c, u), seen, pool_rows<FP8, LAYOUT>(lds, u));
+        const uint32_t mask = key_mask(tile_at(p, c, u), seen, valid);
         if (__builtin_expect(mask != 0xffffffffu, 0)) {
             int ln = lane;
             asm volatile("" : "+v"(ln));
@@ -593,9 +595,9 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         lds_store<bf16x8>(p_lds + (off_p >> 16), pk);
     };
 
-    // Whether some query row of the block does not see all keys of tile u (every wave agrees).
+    // Whether some query row of the block does not see all keys of tile u, the wave's last scored (every wave agrees).
     auto partial = [&](int u) __attribute__((always_inline)) -> bool {
-        return key_mask(tile_at(p, c, u), c.seen_low, pool_rows<FP8, LAYOUT>(lds, u)) != 0xffffffffu;
+        return key_mask(tile_at(p, c, u), c.seen_low, valid) != 0xffffffffu;
     };
 
     auto pv = [&](int u) __attribute__((always_inline)) {
@@ -616,7 +618,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         bf16x8 vf[VD];
 #pragma unroll
         for (int j = 0; j < VD; ++j) vf[j] = vfrag(j);
-        if constexpr (!FP8 && !WIDE) gather.issue(p, c, lds, wave, lane);
+        if constexpr (!FP8) gather.issue(p, c, lds, wave, lane);
 #pragma unroll
         for (int cb = 0; cb < 8; ++cb) {
 #pragma unroll
@@ -657,13 +659,15 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         wait_vmcnt<0>();
         gather.all(p, c, 1, lds, wave, lane);
         if constexpr (FP8) advance(0);
-        else gather.prepare(p, c, 2, lds, wave, lane);
+        auto in_pool = [&](int u) __attribute__((always_inline)) { valid = pool_rows<FP8, LAYOUT>(lds, u); };
         if constexpr (!WIDE) {
             // bf16: in half u every wave issues its rows of tile u + 2, into the
             // stage of tile u - 2, which was last read in half u - 1; the half
             // ends with its rows of tile u + 1 landed.
+            if constexpr (!FP8) gather.prepare(p, c, 2, lds, wave, lane);
+            lds_barrier();
+            in_pool(grp);
             if (grp == 1) {  // half 0, without PV
-                lds_barrier();
                 if constexpr (FP8) {
                     advance(1);
                 } else {
@@ -671,54 +675,72 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                     wait_vmcnt<G::LOADS>();
                     gather.prepare(p, c, 3, lds, wave, lane);
                 }
+                lds_barrier();
             }
+            if constexpr (!FP8) behind.prepare(p, c, 3 + grp, lds, wave, lane);
 #pragma unroll 1
             for (int u = grp; u < nt; u += 2) {
-                lds_barrier();
                 if (live) qk_softmax(u, overflow);
                 else if constexpr (!FP8) gather.issue(p, c, lds, wave, lane);
                 if constexpr (FP8) {
                     advance(u + 1);
                 } else {
                     wait_vmcnt<G::LOADS>();
-                    gather.prepare(p, c, u + 3, lds, wave, lane);
-                    behind.prepare(p, c, u + 4, lds, wave, lane);
+                    gather = behind;
                 }
                 lds_barrier();
                 if constexpr (FP8) advance(u + 2);
                 pv(u);
                 if constexpr (!FP8) {
                     wait_vmcnt<G::LOADS>();
-                    gather = behind;
+                    gather.prepare(p, c, u + 4, lds, wave, lane);
+                    behind.prepare(p, c, u + 5, lds, wave, lane);
                 }
+                in_pool(u + 2);
+                lds_barrier();
             }
             if (((nt ^ grp) & 1) == 0) lds_barrier();  // half nt: the other group's last PV
         } else {
-            // bf16: tile t + 2 is issued in QK of tile t, into the stage of tile
-            // t - 2, which both groups are past.  A tile in which some row sees
+            // bf16: tile t + 3 is issued in PV of tile t, into the stage of tile
+            // t - 1, which both groups are past.  A tile in which some row sees
             // less than all has one barrier more, between group 1's QK and group
             // 0's clear_specials of it.
-            if (grp == 1) {
+            if constexpr (!FP8) {
+                gather.prepare(p, c, 2, lds, wave, lane);
+                if (grp == 0) {
+                    gather.issue(p, c, lds, wave, lane);
+                    gather.prepare(p, c, 3, lds, wave, lane);
+                }
+            }
+            lds_barrier();
+            in_pool(0);
+            if (grp == 1) {  // half 0, without PV
+                if constexpr (FP8) {
+                    advance(1);
+                } else {
+                    gather.issue(p, c, lds, wave, lane);
+                    gather.prepare(p, c, 3, lds, wave, lane);
+                }
                 lds_barrier();
-                advance(1);
             }
 #pragma unroll 1
             for (int t = 0; t < nt; ++t) {
-                lds_barrier();
                 if (live) qk_softmax(t, overflow);
-                else if constexpr (!FP8) gather.issue(p, c, lds, wave, lane);
                 const bool clears = partial(t);
                 if (grp == 1) {
                     if (__builtin_expect(clears, 0)) lds_barrier();
                     if constexpr (!FP8) wait_vmcnt<G::LOADS>();
                 }
-                if constexpr (!FP8) gather.prepare(p, c, t + 3, lds, wave, lane);
                 lds_barrier();
                 if (grp == 0 && __builtin_expect(clears, 0)) lds_barrier();
                 advance(t + 1 + grp);
                 pv(t);
-                if constexpr (!FP8)
-                    if (grp == 0) wait_vmcnt<G::LOADS>();
+                if constexpr (!FP8) {
+                    if (grp == 0) wait_vmcnt<2 * G::LOADS>();
+                    gather.prepare(p, c, t + 4, lds, wave, lane);
+                }
+                in_pool(t + 1);
+                lds_barrier();
             }
             if (grp == 0) lds_barrier();  // half 2 nt: group 1's last PV
         }
