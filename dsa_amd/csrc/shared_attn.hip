@@ -24,6 +24,8 @@
 namespace dsa {
 namespace {
 
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr int kKeys = kSharedKeys;
 constexpr int kFp8Row = 656, kFp8ScaleOff = 512, kFp8RopeOff = 528;
@@ -275,13 +277,19 @@ enum { kRows = 0, kBlocks = 1, kPages = 2 };
 template <bool FP8, int LAYOUT>
 struct Gathers {
     static constexpr int ENTRIES = LAYOUT == kPages ? 4 : 1;
-    static constexpr int AHEAD = FP8 ? 2 : 3;
+    static constexpr int AHEAD = 4;
     static constexpr int LOADS = (FP8 ? (LAYOUT == kPages ? 4 : 3) : 5) + (LAYOUT != kRows ? 1 : 0);
     int64_t first;  // row that the four start with, from the cache's start
     int rows;       // how many of them can be read
     int my_row;     // kPages: lane l: row 4 wave + l % 4
     int tile;
+    int entry;      // of the tile prepared next, read ahead so that nothing waits for it
 
+    // Reads the block entries of tile u, which have landed.
+    __device__ __forceinline__ void fetch(int u, uint32_t lds, int wave, int lane) {
+        if constexpr (LAYOUT == kBlocks) entry = lds_load<int>(PPLds<FP8>::entries(lds, u, wave));
+        if constexpr (LAYOUT == kPages) entry = lds_load<int>(PPLds<FP8>::entries(lds, u, 4 * wave + (lane & 3)));
+    }
     __device__ __forceinline__ void prepare(const Hot& p, const Piece& c, int u, uint32_t lds, int wave, int lane) {
         using X = PPLds<FP8>;
         const Tile k = tile_at(p, c, u);
@@ -294,15 +302,14 @@ struct Gathers {
             rows = on ? min(max(k.high - key, 0), 4) : 0;
         } else if constexpr (LAYOUT == kBlocks) {
             const int key = min(k.key0 + r0, p.L - 4);
-            const int entry = __builtin_amdgcn_readfirstlane(lds_load<int>(X::entries(lds, u, wave)));
-            const bool ok = (uint32_t)entry < (uint32_t)p.num_blocks;
-            first = (ok ? entry : 0) * p.block_size + (key - block_of(p, key) * p.block_size);
+            const int blk = __builtin_amdgcn_readfirstlane(entry);
+            const bool ok = (uint32_t)blk < (uint32_t)p.num_blocks;
+            first = (ok ? blk : 0) * p.block_size + (key - block_of(p, key) * p.block_size);
             rows = on && ok ? 4 : 0;
             if (lane == 0) lds_store<uint8_t>(X::valid(lds, u) + wave, ok ? 0xf : 0);
         } else {
             asm volatile("" : "+v"(lane));
             const int key = min(k.key0 + r0 + (lane & 3), p.L - 1);
-            const int entry = lds_load<int>(X::entries(lds, u, r0 + (lane & 3)));
             const bool ok = (uint32_t)entry < (uint32_t)p.num_blocks;
             const uint64_t valid = __ballot(ok) & 0xf;
             if (lane == 0) lds_store<uint8_t>(X::valid(lds, u) + wave, (uint8_t)valid);
@@ -370,80 +377,76 @@ struct Gathers {
         }
     }
     __device__ __forceinline__ void all(const Hot& p, const Piece& c, int u, uint32_t lds, int wave, int lane) {
+        fetch(u, lds, wave, lane);
         prepare(p, c, u, lds, wave, lane);
         issue(p, c, lds, wave, lane);
     }
 };
 
-// The wave's four rows of tile u, from raw to the ring: lane l takes 32 latent
-// values of row l % 4, from 32 (l / 4) on, and lane l < 32 16 bytes of the
-// rotary part of row l / 8.  kv[d] = bf16(fp32(e4m3) * scale), both roundings to
-// nearest even; where all scales are powers of two (2^-100 .. 2^100), one
-// conversion a pair gives the same bits.
+// The wave's four rows of tile u, from raw to the ring: lane l takes the latent
+// values 8 l .. 8 l + 7 of each (no bank is met twice), and lane l < 32 16 bytes
+// of the rotary part of row l / 8.  kv[d] = bf16(fp32(e4m3) * scale), both
+// roundings to nearest even; where all scales are powers of two (2^-100 ..
+// 2^100), one conversion a pair gives the same bits.
 __device__ __forceinline__ void expand_rows(uint32_t lds, int u, int wave, int lane) {
     using X = PPLds<true>;
     asm volatile("" : "+v"(lane));
     const uint32_t raw = X::raw(lds, u) + 4 * wave * kFp8Row;
     const uint32_t stage = X::stage(lds, u);
-    const int r = lane & 3, part = lane >> 2, row = 4 * wave + r;
-    const uint32_t src = raw + r * kFp8Row;
-    const float sc = lds_load<float>(src + kFp8ScaleOff + 4 * (part >> 2));
-    i32x4 v[2];
+    float sc[4];
+    u32x2 v[4];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) v[m] = lds_load<i32x4>(src + 32 * part + 16 * m);
+    for (int r = 0; r < 4; ++r) {
+        v[r] = lds_load<u32x2>(raw + r * kFp8Row + 8 * lane);
+        sc[r] = lds_load<float>(raw + r * kFp8Row + kFp8ScaleOff + 4 * (lane >> 4));
+    }
     const int in4 = (lane >> 3) & 3, rope = 4 * wave + in4;
     const i32x4 turned = lds_load<i32x4>(raw + in4 * kFp8Row + kFp8RopeOff + 16 * (lane & 7));
-    const uint32_t sb = __float_as_uint(sc), sexp = sb >> 23 & 0xffu;
-    const bool pow2 = (sb & 0x807fffffu) == 0 && sexp >= 27u && sexp <= 227u;
-    const uint32_t dst = stage + row * 1024, sw = (uint32_t)sw_kv(row);
-    auto put = [&](int m, int h, const bf16x8& o) {
-        lds_store<bf16x8>(dst + (((uint32_t)(4 * part + 2 * m + h) ^ sw) << 4), o);
-    };
+    bool pow2 = true;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const uint32_t sb = __float_as_uint(sc[r]);
+        pow2 &= (sb & 0x807fffffu) == 0 && sb - (27u << 23) <= 200u << 23;
+    }
+    const uint32_t dst = stage + 4 * wave * 1024, chunk = (uint32_t)(lane ^ sw_kv(4 * wave)) << 4;
     if (__all(pow2)) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int r = 0; r < 4; ++r) {
+            bf16x8 o;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                bf16x8 o;
-#pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[m][2 * h + d], sc, false);
-                    const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[m][2 * h + d], sc, true);
-                    o[4 * d + 0] = lo[0];
-                    o[4 * d + 1] = lo[1];
-                    o[4 * d + 2] = hi[0];
-                    o[4 * d + 3] = hi[1];
-                }
-                put(m, h, o);
+            for (int d = 0; d < 2; ++d) {
+                const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)v[r][d], sc[r], false);
+                const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)v[r][d], sc[r], true);
+                o[4 * d + 0] = lo[0];
+                o[4 * d + 1] = lo[1];
+                o[4 * d + 2] = hi[0];
+                o[4 * d + 3] = hi[1];
             }
+            lds_store<bf16x8>(dst + r * 1024 + (chunk ^ (64u * r)), o);  // sw_kv(4 wave + r) = sw_kv(4 wave) ^ 4 r
+        }
     } else {
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int r = 0; r < 4; ++r) {
+            bf16x8 o;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                bf16x8 o;
-#pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(v[m][2 * h + d], false);
-                    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(v[m][2 * h + d], true);
-                    o[4 * d + 0] = (__bf16)(lo[0] * sc);
-                    o[4 * d + 1] = (__bf16)(lo[1] * sc);
-                    o[4 * d + 2] = (__bf16)(hi[0] * sc);
-                    o[4 * d + 3] = (__bf16)(hi[1] * sc);
-                }
-                put(m, h, o);
+            for (int d = 0; d < 2; ++d) {
+                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[r][d], false);
+                const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[r][d], true);
+                o[4 * d + 0] = (__bf16)(lo[0] * sc[r]);
+                o[4 * d + 1] = (__bf16)(lo[1] * sc[r]);
+                o[4 * d + 2] = (__bf16)(hi[0] * sc[r]);
+                o[4 * d + 3] = (__bf16)(hi[1] * sc[r]);
             }
+            lds_store<bf16x8>(dst + r * 1024 + (chunk ^ (64u * r)), o);
+        }
     }
     if (lane < 32) lds_store<i32x4>(stage + X::KV_BYTES + rope * 128 + (((lane & 7) ^ sw_rope(rope)) << 4), turned);
 }
 
 // Rows of a tile that are in the pool, bit r for row r, from the waves' four bits each.
-template <bool FP8, int LAYOUT>
-__device__ __forceinline__ uint32_t pool_rows(uint32_t lds, int u) {
-    if constexpr (LAYOUT == kRows) return 0xffffffffu;
-    const uint64_t v = lds_load<uint64_t>(PPLds<FP8>::valid(lds, u));
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+__device__ __forceinline__ uint32_t pool_rows(u32x2 v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)v[0]);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)v[1]);
     if (__builtin_expect((lo & hi) == 0x0f0f0f0fu, 1)) return 0xffffffffu;
     auto squeeze = [](uint32_t b) { return (b & 0xfu) | (b >> 4 & 0xf0u) | (b >> 8 & 0xf00u) | (b >> 12 & 0xf000u); };
     return squeeze(lo) | squeeze(hi) << 16;
@@ -636,7 +639,9 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             wait_vmcnt<G::LOADS>();
             if (u < nt) expand_rows(lds, u, wave, lane);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // raw is read before it is written again
-            gather.all(p, c, u + 2, lds, wave, lane);
+            gather.prepare(p, c, u + 2, lds, wave, lane);
+            gather.issue(p, c, lds, wave, lane);
+            gather.fetch(u + 3, lds, wave, lane);
         }
     };
 
@@ -658,26 +663,42 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         gather.all(p, c, 0, lds, wave, lane);
         wait_vmcnt<0>();
         gather.all(p, c, 1, lds, wave, lane);
+        gather.fetch(2, lds, wave, lane);
         if constexpr (FP8) advance(0);
-        auto in_pool = [&](int u) __attribute__((always_inline)) { valid = pool_rows<FP8, LAYOUT>(lds, u); };
+        // The rows of tile u in the pool, and between reading and using them the next gathers.
+        auto turn_to = [&](int u, auto&& prepare) __attribute__((always_inline)) {
+            if constexpr (LAYOUT == kRows) {
+                prepare();
+                valid = 0xffffffffu;
+            } else {
+                const u32x2 v = lds_load<u32x2>(X::valid(lds, u));
+                prepare();
+                valid = pool_rows(v);
+            }
+        };
+        auto nothing = [] {};
         if constexpr (!WIDE) {
             // bf16: in half u every wave issues its rows of tile u + 2, into the
             // stage of tile u - 2, which was last read in half u - 1; the half
             // ends with its rows of tile u + 1 landed.
             if constexpr (!FP8) gather.prepare(p, c, 2, lds, wave, lane);
             lds_barrier();
-            in_pool(grp);
+            turn_to(grp, nothing);
             if (grp == 1) {  // half 0, without PV
                 if constexpr (FP8) {
                     advance(1);
                 } else {
                     gather.issue(p, c, lds, wave, lane);
                     wait_vmcnt<G::LOADS>();
+                    gather.fetch(3, lds, wave, lane);
                     gather.prepare(p, c, 3, lds, wave, lane);
                 }
                 lds_barrier();
             }
-            if constexpr (!FP8) behind.prepare(p, c, 3 + grp, lds, wave, lane);
+            if constexpr (!FP8) {
+                behind.fetch(3 + grp, lds, wave, lane);
+                behind.prepare(p, c, 3 + grp, lds, wave, lane);
+            }
 #pragma unroll 1
             for (int u = grp; u < nt; u += 2) {
                 if (live) qk_softmax(u, overflow);
@@ -687,16 +708,19 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                 } else {
                     wait_vmcnt<G::LOADS>();
                     gather = behind;
+                    gather.fetch(u + 4, lds, wave, lane);
+                    behind.fetch(u + 5, lds, wave, lane);
                 }
                 lds_barrier();
                 if constexpr (FP8) advance(u + 2);
                 pv(u);
-                if constexpr (!FP8) {
-                    wait_vmcnt<G::LOADS>();
-                    gather.prepare(p, c, u + 4, lds, wave, lane);
-                    behind.prepare(p, c, u + 5, lds, wave, lane);
-                }
-                in_pool(u + 2);
+                turn_to(u + 2, [&]() __attribute__((always_inline)) {
+                    if constexpr (!FP8) {
+                        wait_vmcnt<G::LOADS>();
+                        gather.prepare(p, c, u + 4, lds, wave, lane);
+                        behind.prepare(p, c, u + 5, lds, wave, lane);
+                    }
+                });
                 lds_barrier();
             }
             if (((nt ^ grp) & 1) == 0) lds_barrier();  // half nt: the other group's last PV
@@ -709,20 +733,23 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                 gather.prepare(p, c, 2, lds, wave, lane);
                 if (grp == 0) {
                     gather.issue(p, c, lds, wave, lane);
+                    gather.fetch(3, lds, wave, lane);
                     gather.prepare(p, c, 3, lds, wave, lane);
                 }
             }
             lds_barrier();
-            in_pool(0);
+            turn_to(0, nothing);
             if (grp == 1) {  // half 0, without PV
                 if constexpr (FP8) {
                     advance(1);
                 } else {
                     gather.issue(p, c, lds, wave, lane);
+                    gather.fetch(3, lds, wave, lane);
                     gather.prepare(p, c, 3, lds, wave, lane);
                 }
                 lds_barrier();
             }
+            if constexpr (!FP8) gather.fetch(4, lds, wave, lane);
 #pragma unroll 1
             for (int t = 0; t < nt; ++t) {
                 if (live) qk_softmax(t, overflow);
@@ -735,11 +762,13 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                 if (grp == 0 && __builtin_expect(clears, 0)) lds_barrier();
                 advance(t + 1 + grp);
                 pv(t);
-                if constexpr (!FP8) {
-                    if (grp == 0) wait_vmcnt<2 * G::LOADS>();
-                    gather.prepare(p, c, t + 4, lds, wave, lane);
-                }
-                in_pool(t + 1);
+                turn_to(t + 1, [&]() __attribute__((always_inline)) {
+                    if constexpr (!FP8) {
+                        if (grp == 0) wait_vmcnt<2 * G::LOADS>();
+                        gather.prepare(p, c, t + 4, lds, wave, lane);
+                        gather.fetch(t + 5, lds, wave, lane);
+                    }
+                });
                 lds_barrier();
             }
             if (grp == 0) lds_barrier();  // half 2 nt: group 1's last PV
