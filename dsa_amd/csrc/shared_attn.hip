@@ -527,9 +527,9 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         off_p = pp_pchunk(n16, g) | (pp_pchunk(16 * gw + n16, g) << 16);
     }
 
-    // What the wave's next turn takes is made ready behind PV, the shorter of the
-    // two: the gathers (behind: narrow, those of PV), and the rows of its tile
-    // that are in the pool.
+    // Made ready behind QK, the shorter turn of the two: the gathers (behind:
+    // narrow, those of the next QK), and the rows of its next tile that are in
+    // the pool.
     G gather, behind;
     uint32_t valid = 0;
     auto qk_softmax = [&](int u, bool& overflow) __attribute__((always_inline)) {
@@ -548,7 +548,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         bf16x8 kf[KD];
 #pragma unroll
         for (int j = 0; j < KD; ++j) kf[j] = kfrag(j);
-        if constexpr (!FP8 && !WIDE) gather.issue(p, c, lds, wave, lane);
+        if constexpr (!FP8 && !WIDE) behind.issue(p, c, lds, wave, lane);
 #pragma unroll
         for (int step = 0; step < 36; ++step) {
             sacc[step & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[step % KD], qf[step >> 1], sacc[step & 1], 0, 0, 0);
@@ -603,7 +603,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         return key_mask(tile_at(p, c, u), c.seen_low, valid) != 0xffffffffu;
     };
 
-    auto pv = [&](int u) __attribute__((always_inline)) {
+    auto pv = [&](int u, bool clears) __attribute__((always_inline)) {
         const uint32_t stage = X::stage(lds, u);
         asm volatile("" : "+v"(off_kv), "+v"(off_p));
         const uint32_t vbase = stage + (off_kv >> 16);
@@ -613,7 +613,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             const bf16x4 v1 = lds_load_tr(a + 16 * 1024);
             return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
         };
-        if (__builtin_expect(partial(u), 0)) clear_specials(stage, gw, lane);
+        if (__builtin_expect(clears, 0)) clear_specials(stage, gw, lane);
         bf16x8 pf[NB];
 #pragma unroll
         for (int hb = 0; hb < NB; ++hb) pf[hb] = lds_load<bf16x8>(p_lds + (off_p & 0xffffu) + 1024 * hb);
@@ -665,6 +665,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         gather.all(p, c, 1, lds, wave, lane);
         gather.fetch(2, lds, wave, lane);
         if constexpr (FP8) advance(0);
+        else gather.prepare(p, c, 2, lds, wave, lane);
         // The rows of tile u in the pool, and between reading and using them the next gathers.
         auto turn_to = [&](int u, auto&& prepare) __attribute__((always_inline)) {
             if constexpr (LAYOUT == kRows) {
@@ -681,7 +682,6 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             // bf16: in half u every wave issues its rows of tile u + 2, into the
             // stage of tile u - 2, which was last read in half u - 1; the half
             // ends with its rows of tile u + 1 landed.
-            if constexpr (!FP8) gather.prepare(p, c, 2, lds, wave, lane);
             lds_barrier();
             turn_to(grp, nothing);
             if (grp == 1) {  // half 0, without PV
@@ -695,32 +695,38 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                 }
                 lds_barrier();
             }
+            int entry = 0;  // of the tile behind the one that gather.entry is of
             if constexpr (!FP8) {
-                behind.fetch(3 + grp, lds, wave, lane);
-                behind.prepare(p, c, 3 + grp, lds, wave, lane);
+                behind = gather;
+                gather.fetch(4 + grp, lds, wave, lane);
+                entry = gather.entry;
+                gather.fetch(3 + grp, lds, wave, lane);
             }
 #pragma unroll 1
             for (int u = grp; u < nt; u += 2) {
                 if (live) qk_softmax(u, overflow);
-                else if constexpr (!FP8) gather.issue(p, c, lds, wave, lane);
-                if constexpr (FP8) {
-                    advance(u + 1);
-                } else {
-                    wait_vmcnt<G::LOADS>();
-                    gather = behind;
-                    gather.fetch(u + 4, lds, wave, lane);
-                    behind.fetch(u + 5, lds, wave, lane);
-                }
-                lds_barrier();
-                if constexpr (FP8) advance(u + 2);
-                pv(u);
+                else if constexpr (!FP8) behind.issue(p, c, lds, wave, lane);
+                const bool clears = partial(u);
                 turn_to(u + 2, [&]() __attribute__((always_inline)) {
-                    if constexpr (!FP8) {
+                    if constexpr (FP8) {
+                        advance(u + 1);
+                    } else {
                         wait_vmcnt<G::LOADS>();
-                        gather.prepare(p, c, u + 4, lds, wave, lane);
-                        behind.prepare(p, c, u + 5, lds, wave, lane);
+                        gather.prepare(p, c, u + 3, lds, wave, lane);
+                        behind.entry = entry;
+                        behind.prepare(p, c, u + 4, lds, wave, lane);
                     }
                 });
+                lds_barrier();
+                pv(u, clears);
+                if constexpr (FP8) {
+                    advance(u + 2);
+                } else {
+                    wait_vmcnt<G::LOADS>();
+                    gather.fetch(u + 6, lds, wave, lane);
+                    entry = gather.entry;
+                    gather.fetch(u + 5, lds, wave, lane);
+                }
                 lds_barrier();
             }
             if (((nt ^ grp) & 1) == 0) lds_barrier();  // half nt: the other group's last PV
@@ -729,27 +735,16 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             // t - 1, which both groups are past.  A tile in which some row sees
             // less than all has one barrier more, between group 1's QK and group
             // 0's clear_specials of it.
-            if constexpr (!FP8) {
-                gather.prepare(p, c, 2, lds, wave, lane);
-                if (grp == 0) {
-                    gather.issue(p, c, lds, wave, lane);
-                    gather.fetch(3, lds, wave, lane);
-                    gather.prepare(p, c, 3, lds, wave, lane);
-                }
-            }
+            if constexpr (!FP8)
+                if (grp == 0) gather.issue(p, c, lds, wave, lane);
             lds_barrier();
             turn_to(0, nothing);
             if (grp == 1) {  // half 0, without PV
-                if constexpr (FP8) {
-                    advance(1);
-                } else {
-                    gather.issue(p, c, lds, wave, lane);
-                    gather.fetch(3, lds, wave, lane);
-                    gather.prepare(p, c, 3, lds, wave, lane);
-                }
+                if constexpr (FP8) advance(1);
+                else gather.issue(p, c, lds, wave, lane);
                 lds_barrier();
             }
-            if constexpr (!FP8) gather.fetch(4, lds, wave, lane);
+            if constexpr (!FP8) gather.fetch(3, lds, wave, lane);
 #pragma unroll 1
             for (int t = 0; t < nt; ++t) {
                 if (live) qk_softmax(t, overflow);
@@ -758,17 +753,18 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                     if (__builtin_expect(clears, 0)) lds_barrier();
                     if constexpr (!FP8) wait_vmcnt<G::LOADS>();
                 }
-                lds_barrier();
-                if (grp == 0 && __builtin_expect(clears, 0)) lds_barrier();
-                advance(t + 1 + grp);
-                pv(t);
                 turn_to(t + 1, [&]() __attribute__((always_inline)) {
                     if constexpr (!FP8) {
-                        if (grp == 0) wait_vmcnt<2 * G::LOADS>();
-                        gather.prepare(p, c, t + 4, lds, wave, lane);
-                        gather.fetch(t + 5, lds, wave, lane);
+                        gather.prepare(p, c, t + 3, lds, wave, lane);
+                        gather.fetch(t + 4, lds, wave, lane);
                     }
                 });
+                lds_barrier();
+                if (grp == 0 && __builtin_expect(clears, 0)) lds_barrier();
+                pv(t, clears);
+                advance(t + 1 + grp);  // fp8: behind PV, when the other group's QK has left the LDS
+                if constexpr (!FP8)
+                    if (grp == 0) wait_vmcnt<2 * G::LOADS>();
                 lds_barrier();
             }
             if (grp == 0) lds_barrier();  // half 2 nt: group 1's last PV
