@@ -175,21 +175,13 @@ struct PPLds {
     static constexpr int RAW_OFF = NSTAGE * STAGE_BYTES, RAW_BYTES = FP8 ? kKeys * kFp8Row : 0;
     // P of one group, 64 rows x 32 bf16 in the k order of the PV operand (pp_pchunk)
     static constexpr int P_OFF = RAW_OFF + 2 * RAW_BYTES, P_GROUP = 64 * 64;
-    // of the last eight tiles: the rows' block entries (from when the tile three
-    // before it is issued), and four bits a wave, which of its rows are in the pool
-    static constexpr int NTILE = 8;
-    static constexpr int ENTRY_OFF = P_OFF + 2 * P_GROUP;
-    static constexpr int VALID_OFF = ENTRY_OFF + NTILE * kKeys * 4;
-    static constexpr int FLAG_OFF = VALID_OFF + NTILE * 8;
+    static constexpr int FLAG_OFF = P_OFF + 2 * P_GROUP;  // a second pass is needed
+    static constexpr int BAD_OFF = FLAG_OFF + 4;          // some block entry of the piece lies outside the pool
     static constexpr int LDS_BYTES = FLAG_OFF + 16;
     static constexpr int ML_OFF = P_OFF;  // [3][128] floats, at the end: l, reference and maximum
     static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
     __device__ static uint32_t stage(uint32_t lds, int u) { return lds + (uint32_t)(u % NSTAGE) * STAGE_BYTES; }
     __device__ static uint32_t raw(uint32_t lds, int u) { return lds + RAW_OFF + (uint32_t)(u % 2) * RAW_BYTES; }
-    __device__ static uint32_t entries(uint32_t lds, int u, int row) {
-        return lds + ENTRY_OFF + (uint32_t)(u % NTILE) * (kKeys * 4) + 4 * row;
-    }
-    __device__ static uint32_t valid(uint32_t lds, int u) { return lds + VALID_OFF + 8 * (u % NTILE); }
 };
 
 // What the main kernel's loop needs of them.
@@ -211,7 +203,7 @@ struct Tile {
 struct Piece {
     Item it;
     int a, nt;      // first tile of the item, and how many
-    int seen_low;   // least number of rows a query row of the block sees
+    int seen_low, seen_high;  // least and greatest number of rows a query row of the block sees
 };
 __device__ __forceinline__ Tile tile_at(const Hot& p, const Piece& c, int u) {
     const int t = c.a + u;
@@ -227,19 +219,6 @@ __device__ __forceinline__ Tile tile_at(const Hot& p, const Piece& c, int u) {
 // key / block_size, without a division (keys are below 2^25).
 __device__ __forceinline__ int block_of(const Hot& p, int key) {
     return p.block_size == 1 ? key : (int)(__umulhi((uint32_t)key, p.block_magic) >> p.block_shift);
-}
-
-// 4 bytes a lane straight into LDS (lane l at m0 + 4 l).
-__device__ __forceinline__ void gather_words(uint32_t lds_base, rsrc_t rsrc, uint32_t voff) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-    asm volatile(
-        "s_mov_b32 m0, %0\n\t"
-        "buffer_load_dword %1, %2, 0 offen lds"
-        :
-        : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(voff), "s"(rsrc)
-        : "memory", "m0");
-#pragma clang diagnostic pop
 }
 
 // 16 bytes a lane, OFFSET + off on, straight into LDS: lane l at m0 + OFFSET + 16 l.
@@ -260,75 +239,83 @@ __device__ __forceinline__ void gather_at(uint32_t lds_base, rsrc_t rsrc, uint32
 // four rows (blocks), in any blocks (pages).
 enum { kRows = 0, kBlocks = 1, kPages = 2 };
 
+// The block table's entry of a key of sequence seq: a scalar load.
+__device__ __forceinline__ int table_entry(const Hot& p, int seq, int key) {
+    const auto* t = (const __attribute__((address_space(4))) int32_t*)(uint64_t)p.block_table;
+    return t[(int64_t)seq * p.max_blocks + block_of(p, key)];
+}
+
 // Gathers of one tile by one wave: its rows 4 wave .. 4 wave + 3.  bf16: an
-// instruction a row (1 KiB), and one for their rotary parts; fp8: three
-// instructions, or one a row.  The four rows follow each other unless LAYOUT is
-// kPages, so that they have one descriptor (rows past a sequence's end are out of
-// its range and read as zeros); of a tile behind the piece (u >= nt) nothing is
-// read, but the instructions are the same, so that they can be counted on.
+// instruction a row (1 KiB), and one for their rotary parts (kPages: one a row);
+// fp8: three instructions, or one a row.  The four rows follow each other unless
+// LAYOUT is kPages, so that they have one descriptor (rows past a sequence's end
+// are out of its range and read as zeros); of a tile behind the piece (u >= nt)
+// nothing is read, but the instructions are the same, so that they can be counted
+// on.
 //
 // They are issued together, behind the first LDS reads of QK or PV: the queue in
 // front of the texture path holds that many, and in the chain of MFMAs each
 // would cost about 60 clocks (a chain of 36 with its LDS reads: 764 clocks,
 // 772 with four gathers in front, 1000 with the four between its steps).
 //
-// Blocks and pages: the block entries come into LDS by a gather of their own,
-// issued with the tile AHEAD before.
+// Blocks and pages: all the wave needs of the block table it reads by scalar
+// loads, a tile ahead (fetch).
 template <bool FP8, int LAYOUT>
 struct Gathers {
-    static constexpr int ENTRIES = LAYOUT == kPages ? 4 : 1;
-    static constexpr int AHEAD = 4;
-    static constexpr int LOADS = (FP8 ? (LAYOUT == kPages ? 4 : 3) : 5) + (LAYOUT != kRows ? 1 : 0);
-    int64_t first;  // row that the four start with, from the cache's start
-    int rows;       // how many of them can be read
-    int my_row;     // kPages: lane l: row 4 wave + l % 4
+    static constexpr int N = LAYOUT == kRows ? 0 : LAYOUT == kBlocks ? 1 : 4;  // entries of the four rows
+    static constexpr int LOADS = FP8 ? (LAYOUT == kPages ? 4 : 3) : (LAYOUT == kPages ? 8 : 5);
+    int64_t first;               // row that the four start with, from the cache's start
+    int rows;                    // how many of them can be read
+    int row[N == 4 ? 4 : 1];     // kPages: each row, from the cache's start, or -1
     int tile;
-    int entry;      // of the tile prepared next, read ahead so that nothing waits for it
+    int entry[N == 0 ? 1 : N];   // of the tile prepared next
 
-    // Reads the block entries of tile u, which have landed.
-    __device__ __forceinline__ void fetch(int u, uint32_t lds, int wave, int lane) {
-        if constexpr (LAYOUT == kBlocks) entry = lds_load<int>(PPLds<FP8>::entries(lds, u, wave));
-        if constexpr (LAYOUT == kPages) entry = lds_load<int>(PPLds<FP8>::entries(lds, u, 4 * wave + (lane & 3)));
+    __device__ __forceinline__ void fetch(const Hot& p, const Piece& c, int u, int wave) {
+        if constexpr (N > 0) {
+            const Tile k = tile_at(p, c, u);
+#pragma unroll
+            for (int i = 0; i < N; ++i) entry[i] = table_entry(p, k.seq, min(k.key0 + 4 * wave + i, p.L - 1));
+        }
     }
-    __device__ __forceinline__ void prepare(const Hot& p, const Piece& c, int u, uint32_t lds, int wave, int lane) {
-        using X = PPLds<FP8>;
+    // Tile u's gathers, from its entries.  A wave that meets an entry outside the
+    // pool, of rows that some query sees, says so at `bad`.
+    __device__ __forceinline__ void prepare(const Hot& p, const Piece& c, int u, uint32_t bad, int wave) {
         const Tile k = tile_at(p, c, u);
-        const int r0 = 4 * wave;
+        const int key = k.key0 + 4 * wave;
         const bool on = u < c.nt;
         tile = u;
         if constexpr (LAYOUT == kRows) {
-            const int key = k.key0 + r0;
             first = (int64_t)k.seq * p.L + key;
             rows = on ? min(max(k.high - key, 0), 4) : 0;
         } else if constexpr (LAYOUT == kBlocks) {
-            const int key = min(k.key0 + r0, p.L - 4);
-            const int blk = __builtin_amdgcn_readfirstlane(entry);
-            const bool ok = (uint32_t)blk < (uint32_t)p.num_blocks;
-            first = (ok ? blk : 0) * p.block_size + (key - block_of(p, key) * p.block_size);
+            const bool ok = (uint32_t)entry[0] < (uint32_t)p.num_blocks;
+            const int at = min(key, p.L - 4);
+            first = entry[0] * p.block_size + (at - block_of(p, at) * p.block_size);
             rows = on && ok ? 4 : 0;
-            if (lane == 0) lds_store<uint8_t>(X::valid(lds, u) + wave, ok ? 0xf : 0);
+            if (__builtin_expect(on && !ok && key < min(c.seen_high, k.high), 0)) lds_store<int>(bad, 1);
         } else {
-            asm volatile("" : "+v"(lane));
-            const int key = min(k.key0 + r0 + (lane & 3), p.L - 1);
-            const bool ok = (uint32_t)entry < (uint32_t)p.num_blocks;
-            const uint64_t valid = __ballot(ok) & 0xf;
-            if (lane == 0) lds_store<uint8_t>(X::valid(lds, u) + wave, (uint8_t)valid);
-            my_row = (ok ? entry : 0) * p.block_size + (key - block_of(p, key) * p.block_size);
-            rows = on ? 4 : 0;
+            bool ok = true;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = min(key + i, p.L - 1);
+                const bool in = (uint32_t)entry[i] < (uint32_t)p.num_blocks;
+                row[i] = on && in ? entry[i] * p.block_size + (at - block_of(p, at) * p.block_size) : -1;
+                ok &= in || key + i >= min(c.seen_high, k.high);
+            }
+            if (__builtin_expect(on && !ok, 0)) lds_store<int>(bad, 1);
         }
     }
-    __device__ __forceinline__ void issue(const Hot& p, const Piece& c, uint32_t lds, int wave, int lane) const {
+    __device__ __forceinline__ void issue(const Hot& p, uint32_t lds, int wave, int lane) const {
         using X = PPLds<FP8>;
         asm volatile("" : "+v"(lane));  // lane offsets kept across the loop would be spilled
         if constexpr (FP8) {
             const uint32_t dst = X::raw(lds, tile) + 4 * wave * kFp8Row, off = (uint32_t)lane << 4;
             if constexpr (LAYOUT == kPages) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t r = __builtin_amdgcn_readlane(my_row, i);
+                for (int i = 0; i < 4; ++i)
                     if (lane < kFp8Row / 16)
-                        gather_at<0>(dst + i * kFp8Row, make_rsrc(p.kv + r * kFp8Row, rows ? kFp8Row : 0), off);
-                }
+                        gather_at<0>(dst + i * kFp8Row,
+                                     make_rsrc(p.kv + (int64_t)max(row[i], 0) * kFp8Row, row[i] < 0 ? 0 : kFp8Row), off);
             } else {
                 const rsrc_t rs = make_rsrc(p.kv + first * kFp8Row, (uint32_t)rows * kFp8Row);
                 gather_at<0>(dst, rs, off);
@@ -338,48 +325,37 @@ struct Gathers {
         } else {
             const uint32_t dst = X::stage(lds, tile) + 4 * wave * 1024;
             const uint32_t rope_dst = X::stage(lds, tile) + X::KV_BYTES + 4 * wave * 128;
-            const int in4 = (lane >> 3) & 3;
-            const uint32_t chunk = (uint32_t)((lane & 7) ^ sw_rope(4 * wave + in4)) << 4;
             // sw_kv(4 wave + i) = sw_kv(4 wave) ^ 4 i
             const uint32_t off = (uint32_t)(lane ^ sw_kv(4 * wave)) << 4;
             if constexpr (LAYOUT == kPages) {
-                const int row = __shfl(my_row, in4);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t r = __builtin_amdgcn_readlane(my_row, i);
-                    gather_at<0>(dst + i * 1024, make_rsrc(p.kv + (r << 10), rows ? 1024 : 0), off ^ (64u * i));
-                }
-                if (lane < 32)
-                    gather_at<0>(rope_dst, make_rsrc(p.k_rope, rows ? (uint32_t)(p.num_blocks * p.block_size) << 7 : 0),
-                                 ((uint32_t)row << 7) + chunk);
+                for (int i = 0; i < 4; ++i)
+                    gather_at<0>(dst + i * 1024,
+                                 make_rsrc(p.kv + ((int64_t)max(row[i], 0) << 10), row[i] < 0 ? 0 : 1024), off ^ (64u * i));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (lane < 8)
+                        gather_at<0>(rope_dst + i * 128,
+                                     make_rsrc(p.k_rope + ((int64_t)max(row[i], 0) << 7), row[i] < 0 ? 0 : 128),
+                                     (uint32_t)(lane ^ sw_rope(4 * wave + i)) << 4);
             } else {
                 const rsrc_t rs = make_rsrc(p.kv + (first << 10), (uint32_t)rows << 10);
                 gather_at<0>(dst, rs, off);
                 gather_at<1024>(dst, rs, off ^ 64u);
                 gather_at<2048>(dst, rs, off ^ 128u);
                 gather_at<3072>(dst, rs, off ^ 192u);
+                const int in4 = lane >> 3;
                 if (lane < 32)
                     gather_at<0>(rope_dst, make_rsrc(p.k_rope + (first << 7), (uint32_t)rows << 7),
-                                 (uint32_t)(in4 << 7) + chunk);
+                                 (uint32_t)(in4 << 7) + ((uint32_t)((lane & 7) ^ sw_rope(4 * wave + in4)) << 4));
             }
         }
-        entries(p, c, tile + AHEAD, lds, wave, lane);
     }
-    // Block entries of the wave's rows of tile u into LDS (behind the cache: some entry, not used).
-    static __device__ __forceinline__ void entries(const Hot& p, const Piece& c, int u, uint32_t lds, int wave, int lane) {
-        if constexpr (LAYOUT != kRows) {
-            const Tile n = tile_at(p, c, u);
-            const int key = min(n.key0 + 4 * wave + lane, p.L - 1);
-            if (lane < ENTRIES)
-                gather_words(PPLds<FP8>::entries(lds, u, LAYOUT == kPages ? 4 * wave : wave),
-                             make_rsrc(p.block_table + (int64_t)n.seq * p.max_blocks, 4u * (uint32_t)p.max_blocks),
-                             4u * (uint32_t)block_of(p, key));
-        }
-    }
-    __device__ __forceinline__ void all(const Hot& p, const Piece& c, int u, uint32_t lds, int wave, int lane) {
-        fetch(u, lds, wave, lane);
-        prepare(p, c, u, lds, wave, lane);
-        issue(p, c, lds, wave, lane);
+    __device__ __forceinline__ void all(const Hot& p, const Piece& c, int u, uint32_t lds, uint32_t bad, int wave,
+                                        int lane) {
+        fetch(p, c, u, wave);
+        prepare(p, c, u, bad, wave);
+        issue(p, lds, wave, lane);
     }
 };
 
@@ -402,12 +378,10 @@ __device__ __forceinline__ void expand_rows(uint32_t lds, int u, int wave, int l
     }
     const int in4 = (lane >> 3) & 3, rope = 4 * wave + in4;
     const i32x4 turned = lds_load<i32x4>(raw + in4 * kFp8Row + kFp8RopeOff + 16 * (lane & 7));
-    bool pow2 = true;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const uint32_t sb = __float_as_uint(sc[r]);
-        pow2 &= (sb & 0x807fffffu) == 0 && sb - (27u << 23) <= 200u << 23;
-    }
+    const uint32_t s0 = __float_as_uint(sc[0]), s1 = __float_as_uint(sc[1]), s2 = __float_as_uint(sc[2]);
+    const uint32_t s3 = __float_as_uint(sc[3]);
+    const bool pow2 = ((s0 | s1 | s2 | s3) & 0x807fffffu) == 0 && min(min(s0, s1), min(s2, s3)) >= 27u << 23 &&
+                      max(max(s0, s1), max(s2, s3)) <= 227u << 23;
     const uint32_t dst = stage + 4 * wave * 1024, chunk = (uint32_t)(lane ^ sw_kv(4 * wave)) << 4;
     if (__all(pow2)) {
 #pragma unroll
@@ -443,13 +417,13 @@ __device__ __forceinline__ void expand_rows(uint32_t lds, int u, int wave, int l
     if (lane < 32) lds_store<i32x4>(stage + X::KV_BYTES + rope * 128 + (((lane & 7) ^ sw_rope(rope)) << 4), turned);
 }
 
-// Rows of a tile that are in the pool, bit r for row r, from the waves' four bits each.
-__device__ __forceinline__ uint32_t pool_rows(u32x2 v) {
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)v[0]);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)v[1]);
-    if (__builtin_expect((lo & hi) == 0x0f0f0f0fu, 1)) return 0xffffffffu;
-    auto squeeze = [](uint32_t b) { return (b & 0xfu) | (b >> 4 & 0xf0u) | (b >> 8 & 0xf00u) | (b >> 12 & 0xf000u); };
-    return squeeze(lo) | squeeze(hi) << 16;
+// Rows of a tile that are in the pool, bit r for row r, from the block table (of pieces with an entry outside it).
+__device__ __forceinline__ uint32_t pool_rows(const Hot& p, const Piece& c, int u, int lane) {
+    asm volatile("" : "+v"(lane));
+    const Tile k = tile_at(p, c, u);
+    const int key = min(k.key0 + (lane & 31), p.L - 1);
+    const int entry = p.block_table[(int64_t)k.seq * p.max_blocks + block_of(p, key)];
+    return (uint32_t)__ballot((uint32_t)entry < (uint32_t)p.num_blocks);
 }
 
 // Which of the 32 keys of a tile a query row that sees `seen` rows has: bit r is tile row r.
@@ -499,7 +473,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
     const int nt = c.nt;
     const ArgsPtr args = args_now();
     const int seen = live ? __builtin_amdgcn_readfirstlane(seen_by(args, row / args->H)) : 0;
-    const uint32_t p_lds = lds + X::P_OFF + grp * X::P_GROUP;
+    const uint32_t p_lds = lds + X::P_OFF + grp * X::P_GROUP, bad = lds + X::BAD_OFF;
 
     bf16x8 qf[18];
     {
@@ -548,7 +522,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         bf16x8 kf[KD];
 #pragma unroll
         for (int j = 0; j < KD; ++j) kf[j] = kfrag(j);
-        if constexpr (!FP8 && !WIDE) behind.issue(p, c, lds, wave, lane);
+        if constexpr (!FP8 && !WIDE) behind.issue(p, lds, wave, lane);
 #pragma unroll
         for (int step = 0; step < 36; ++step) {
             sacc[step & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[step % KD], qf[step >> 1], sacc[step & 1], 0, 0, 0);
@@ -621,7 +595,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         bf16x8 vf[VD];
 #pragma unroll
         for (int j = 0; j < VD; ++j) vf[j] = vfrag(j);
-        if constexpr (!FP8) gather.issue(p, c, lds, wave, lane);
+        if constexpr (!FP8) gather.issue(p, lds, wave, lane);
 #pragma unroll
         for (int cb = 0; cb < 8; ++cb) {
 #pragma unroll
@@ -639,9 +613,9 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             wait_vmcnt<G::LOADS>();
             if (u < nt) expand_rows(lds, u, wave, lane);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // raw is read before it is written again
-            gather.prepare(p, c, u + 2, lds, wave, lane);
-            gather.issue(p, c, lds, wave, lane);
-            gather.fetch(u + 3, lds, wave, lane);
+            gather.prepare(p, c, u + 2, bad, wave);
+            gather.issue(p, lds, wave, lane);
+            gather.fetch(p, c, u + 3, wave);
         }
     };
 
@@ -654,27 +628,26 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         l_run = 0.f;
         if (pass == 1) m_ref = max_xor32(max_xor16(m_lane));
         bool overflow = false;
-        if constexpr (LAYOUT != kRows) {
-            for (int u = 0; u < G::AHEAD; ++u) G::entries(p, c, u, lds, wave, lane);
-            wait_vmcnt<0>();
-        }
         // The first tile's rows, and Q: a full wait, as the compiler does not
         // count the gathers (it would wait for Q in the loop).
-        gather.all(p, c, 0, lds, wave, lane);
+        if (threadIdx.x == 0) lds_store<int>(bad, 0);
+        lds_barrier();
+        gather.all(p, c, 0, lds, bad, wave, lane);
         wait_vmcnt<0>();
-        gather.all(p, c, 1, lds, wave, lane);
-        gather.fetch(2, lds, wave, lane);
+        gather.all(p, c, 1, lds, bad, wave, lane);
+        gather.fetch(p, c, 2, wave);
         if constexpr (FP8) advance(0);
-        else gather.prepare(p, c, 2, lds, wave, lane);
-        // The rows of tile u in the pool, and between reading and using them the next gathers.
+        else gather.prepare(p, c, 2, bad, wave);
+        // Rows of tile u in the pool: all, unless the piece has met a bad entry (every wave is past preparing tile u).
         auto turn_to = [&](int u, auto&& prepare) __attribute__((always_inline)) {
             if constexpr (LAYOUT == kRows) {
                 prepare();
                 valid = 0xffffffffu;
             } else {
-                const u32x2 v = lds_load<u32x2>(X::valid(lds, u));
+                const int met = lds_load<int>(bad);
                 prepare();
-                valid = pool_rows(v);
+                valid = 0xffffffffu;
+                if (__builtin_expect(__builtin_amdgcn_readfirstlane(met), 0)) valid = pool_rows(p, c, u, lane);
             }
         };
         auto nothing = [] {};
@@ -688,33 +661,32 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                 if constexpr (FP8) {
                     advance(1);
                 } else {
-                    gather.issue(p, c, lds, wave, lane);
+                    gather.issue(p, lds, wave, lane);
                     wait_vmcnt<G::LOADS>();
-                    gather.fetch(3, lds, wave, lane);
-                    gather.prepare(p, c, 3, lds, wave, lane);
+                    gather.fetch(p, c, 3, wave);
+                    gather.prepare(p, c, 3, bad, wave);
                 }
                 lds_barrier();
             }
-            int entry = 0;  // of the tile behind the one that gather.entry is of
             if constexpr (!FP8) {
                 behind = gather;
-                gather.fetch(4 + grp, lds, wave, lane);
-                entry = gather.entry;
-                gather.fetch(3 + grp, lds, wave, lane);
+                gather.fetch(p, c, 3 + grp, wave);
+                behind.fetch(p, c, 4 + grp, wave);
             }
 #pragma unroll 1
             for (int u = grp; u < nt; u += 2) {
                 if (live) qk_softmax(u, overflow);
-                else if constexpr (!FP8) behind.issue(p, c, lds, wave, lane);
+                else if constexpr (!FP8) behind.issue(p, lds, wave, lane);
                 const bool clears = partial(u);
                 turn_to(u + 2, [&]() __attribute__((always_inline)) {
                     if constexpr (FP8) {
                         advance(u + 1);
                     } else {
                         wait_vmcnt<G::LOADS>();
-                        gather.prepare(p, c, u + 3, lds, wave, lane);
-                        behind.entry = entry;
-                        behind.prepare(p, c, u + 4, lds, wave, lane);
+                        gather.prepare(p, c, u + 3, bad, wave);
+                        behind.prepare(p, c, u + 4, bad, wave);
+                        gather.fetch(p, c, u + 5, wave);
+                        behind.fetch(p, c, u + 6, wave);
                     }
                 });
                 lds_barrier();
@@ -723,9 +695,6 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                     advance(u + 2);
                 } else {
                     wait_vmcnt<G::LOADS>();
-                    gather.fetch(u + 6, lds, wave, lane);
-                    entry = gather.entry;
-                    gather.fetch(u + 5, lds, wave, lane);
                 }
                 lds_barrier();
             }
@@ -736,15 +705,15 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             // less than all has one barrier more, between group 1's QK and group
             // 0's clear_specials of it.
             if constexpr (!FP8)
-                if (grp == 0) gather.issue(p, c, lds, wave, lane);
+                if (grp == 0) gather.issue(p, lds, wave, lane);
             lds_barrier();
             turn_to(0, nothing);
             if (grp == 1) {  // half 0, without PV
                 if constexpr (FP8) advance(1);
-                else gather.issue(p, c, lds, wave, lane);
+                else gather.issue(p, lds, wave, lane);
                 lds_barrier();
             }
-            if constexpr (!FP8) gather.fetch(3, lds, wave, lane);
+            if constexpr (!FP8) gather.fetch(p, c, 3, wave);
 #pragma unroll 1
             for (int t = 0; t < nt; ++t) {
                 if (live) qk_softmax(t, overflow);
@@ -755,8 +724,8 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                 }
                 turn_to(t + 1, [&]() __attribute__((always_inline)) {
                     if constexpr (!FP8) {
-                        gather.prepare(p, c, t + 3, lds, wave, lane);
-                        gather.fetch(t + 4, lds, wave, lane);
+                        gather.prepare(p, c, t + 3, bad, wave);
+                        gather.fetch(p, c, t + 4, wave);
                     }
                 });
                 lds_barrier();
@@ -965,6 +934,7 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
         item_tiles(p, i, most, c.it);
         c.it.first = __builtin_amdgcn_readfirstlane(c.it.first);
         c.seen_low = __builtin_amdgcn_readfirstlane(least);
+        c.seen_high = __builtin_amdgcn_readfirstlane(most);
         c.a = __builtin_amdgcn_readfirstlane(a);
         c.nt = __builtin_amdgcn_readfirstlane(b - a);
         const bool whole = !p->stacked && c.nt * cost == end - begin;

@@ -120,10 +120,10 @@ SHAPES = [
     (64, 1, 16, 300, 20), (2, 1, 16, 4000, 3), (9, 1, 80, 50, 200)]
 
 
-@pytest.mark.parametrize("layout", ["rows", "paged16", "paged48", "fp8", "fp8_paged64"])
+@pytest.mark.parametrize("layout", ["rows", "paged16", "paged48", "paged7", "fp8", "fp8_paged64", "fp8_paged5"])
 @pytest.mark.parametrize("B, SQ, H, P, S", SHAPES)
 def test_against_64_bits(B, SQ, H, P, S, layout):
-    block = {"paged16": 16, "paged48": 48, "fp8_paged64": 64}.get(layout, 0)
+    block = {"paged16": 16, "paged48": 48, "paged7": 7, "fp8_paged64": 64, "fp8_paged5": 5}.get(layout, 0)
     s = make(B, SQ, H, P, S, block, layout.startswith("fp8"), seed=B + P, spare=3)
     g = torch.Generator().manual_seed(S)
     ends = P + S - torch.randint(0, max(1, S - SQ + 1), (B,), generator=g)
@@ -191,19 +191,21 @@ def test_unseen_rows_may_hold_anything(B, SQ, H, block, poison):
             assert torch.equal(a[0, :-1], w[0, :-1]) and torch.equal(a[1:], w[1:])
 
 
+@pytest.mark.parametrize("H", [16, 64, 128])
+@pytest.mark.parametrize("block", [16, 64, 3])
 @pytest.mark.parametrize("fp8", [False, True])
-def test_bad_block_entries_are_masked(fp8):
+def test_bad_block_entries_are_masked(fp8, block, H):
     """Entries outside the pool, in the prefix and behind it, hide their rows."""
-    s = make(4, 2, 16, 96, 64, 16, fp8, seed=5, spare=2)
-    n = s["kv"].shape[0]
+    s = make(4, 2, H, 96, 64, block, fp8, seed=5, spare=2)
+    n, prefix = s["kv"].shape[0], torch.arange(s["L"], device="cuda") < 96
     live = torch.ones(4, s["L"], dtype=torch.bool, device="cuda")
-    for b, entry, value in [(0, 1, -1), (0, 4, n), (1, 6, (1 << 31) - 1), (2, 7, -(1 << 31)), (3, 9, n + 5)]:
+    for b, key, value in [(0, 16, -1), (0, 64, n), (1, 96, (1 << 31) - 1), (2, 112, -(1 << 31)), (3, 144, n + 5)]:
+        entry = key // block
         s["table"][b, entry] = value
-        rows = slice(16 * entry, 16 * entry + 16)
-        if entry < 6:
-            live[:, rows] = False
-        else:
-            live[b, rows] = False
+        rows = torch.arange(s["L"], device="cuda") // block == entry
+        live[b, rows & ~prefix] = False
+        if b == 0:
+            live[:, rows & prefix] = False
     lengths = causal(4, 2, torch.tensor([160, 160, 130, 98]))
     check(call(s, lengths), s, lengths, live=live)
     s["table"].fill_(-1)
