@@ -38,7 +38,7 @@ bool fills_blocks(int64_t rows) {
 struct SharedPlan {
     bool stacked;
     int prefix_items, seq_blocks, items, workgroups;
-    int64_t costs_bytes, slots, bytes;
+    int64_t costs_bytes, spans_bytes, starts_bytes, slots, bytes;
 };
 
 int64_t round_256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -50,15 +50,13 @@ int shared_plan(const dsa_shared_args* a, SharedPlan* plan) {
     if (a->H % 16) return fail(-1, "H must be a multiple of 16 (got %d)", a->H);
     if (a->L >= 1 << 25) return fail(-1, "L must be below 33554432 (got %d)", a->L);
     if (a->prefix < 0 || a->prefix > a->L) return fail(-1, "prefix must be in [0, L = %d] (got %d)", a->L, a->prefix);
-    if (a->num_cus < 0) return fail(-1, "num_cus must not be negative");
+    if (a->num_cus < 0 || a->num_cus > 1 << 12) return fail(-1, "num_cus must be 0 .. 4096");
     const int64_t seq_rows = (int64_t)a->SQ * a->H, rows = seq_rows * a->B;
     if (seq_rows > 1 << 30 || rows > 1 << 30) return fail(-1, "B * SQ * H must be at most 2^30");
     plan->stacked = a->prefix > 0 && a->B > 1 && !fills_blocks(seq_rows);
     plan->seq_blocks = (int)((seq_rows + dsa::kSharedRows - 1) / dsa::kSharedRows);
     plan->prefix_items = plan->stacked ? (int)((rows + dsa::kSharedRows - 1) / dsa::kSharedRows) : 0;
     const int64_t items = plan->prefix_items + (int64_t)a->B * plan->seq_blocks;
-    if (items * (ceil_div(a->L, dsa::kSharedKeys) + 2) * dsa::kSharedMaxCost >= (int64_t)1 << 31)
-        return fail(-1, "too many query rows for a context of %d (B * SQ * H * L)", a->L);
     plan->items = (int)items;
     plan->workgroups = a->num_cus;
     if (plan->workgroups == 0) {
@@ -71,8 +69,13 @@ int shared_plan(const dsa_shared_args* a, SharedPlan* plan) {
     // Pieces: every cut of an item's tiles starts a new one; a stacked call keeps
     // all of them, another only those of cut items, two at most a workgroup.
     plan->slots = plan->stacked ? items + plan->workgroups : 2 * (int64_t)plan->workgroups;
-    plan->costs_bytes = round_256(4 * (items + 1));
-    plan->bytes = plan->costs_bytes + plan->slots * dsa::kSharedRows * (512 + 2) * 4;
+    // The summed costs times a workgroup's number stay in 64 bits: at most 2^26
+    // items of 2^20 tiles, and 2^12 workgroups.
+    static_assert(dsa::kSharedMaxCost + dsa::kSharedPieceCost < 1 << 8, "costs fit");
+    plan->costs_bytes = round_256(8 * (items + 1));
+    plan->spans_bytes = round_256(8 * items);
+    plan->starts_bytes = round_256(4 * ((int64_t)plan->workgroups + 1));
+    plan->bytes = plan->costs_bytes + 2 * plan->spans_bytes + plan->starts_bytes + plan->slots * dsa::kSharedRows * (512 + 2) * 4;
     return 0;
 }
 
@@ -173,8 +176,11 @@ int dsa_fwd_shared(const dsa_shared_args* a, void* stream) {
     p.out_max = a->out_max;
     p.out_sum = a->out_sum;
     char* ws = static_cast<char*>(a->workspace);
-    p.costs = reinterpret_cast<int32_t*>(ws);
-    p.part_o = reinterpret_cast<float*>(ws + plan.costs_bytes);
+    p.costs = reinterpret_cast<int64_t*>(ws);
+    p.spans = reinterpret_cast<int2*>(ws + plan.costs_bytes);
+    p.ends = p.spans + plan.spans_bytes / 8;
+    p.starts = reinterpret_cast<int32_t*>(ws + plan.costs_bytes + 2 * plan.spans_bytes);
+    p.part_o = reinterpret_cast<float*>(ws + plan.costs_bytes + 2 * plan.spans_bytes + plan.starts_bytes);
     p.part_m = p.part_o + plan.slots * dsa::kSharedRows * 512;
     p.part_l = p.part_m + plan.slots * dsa::kSharedRows;
     p.B = a->B;

@@ -81,20 +81,26 @@ __device__ __forceinline__ void item_tiles(ArgsPtr p, int i, int most, Item& it)
     it.second = i < p->prefix_items || most <= p->prefix ? 0 : ceil_div(most, kKeys) - p->prefix / kKeys;
 }
 
-// What one tile of an item costs: see the kernel's two forms below.
-__device__ __forceinline__ int tile_cost(const Item& it) { return it.rows > 64 ? 3 : 2; }
-constexpr int kMinCost = 6;  // least cost a workgroup is given (no less than one tile's)
-
-__device__ __forceinline__ int groups_of(ArgsPtr p, int total) {
-    return max(1, min(p->workgroups, total / kMinCost));
+// What an item costs, in tenths of a microsecond on a full chip: each tile, and
+// once the start and end of a piece (Q, the first tile's latency, the stores).
+// Measured on 64 to 256 sequences of their own rows, paged: up to 32 rows 1.5 us
+// a tile of bf16 rows (HBM, 6.4 TB/s) and 1.35 of fp8, up to 64 2.0 and 1.65,
+// up to 128 2.1 and 2.7; a piece 7.5, 10.5 and 12 us beside its tiles.
+struct Cost {
+    int tile, piece;
+};
+__device__ __forceinline__ Cost cost_of(int rows, int fp8) {
+    if (rows > 64) return Cost{fp8 ? 27 : 21, 120};
+    if (rows > 32) return Cost{fp8 ? 16 : 20, 105};
+    return Cost{fp8 ? 13 : 15, 75};
 }
+static_assert(kSharedMaxCost >= 27 + 1 && kSharedPieceCost >= 120, "the host's bound on the summed costs");
+constexpr int kMinShare = 40;  // least cost a workgroup is given: some tiles, and no less than one
 
 // Workgroup w computes the tiles that start in its share [w * total / groups,
-// (w + 1) * total / groups) of the summed costs.
-__device__ __forceinline__ int share_of(int w, int total, int groups) { return (int)((int64_t)w * total / groups); }
-__device__ __forceinline__ int group_at(int cost, int total, int groups) {
-    return (int)(((int64_t)(cost + 1) * groups + total - 1) / total) - 1;
-}
+// (w + 1) * total / groups) of the summed costs; an item that starts at cost
+// `begin` has its tile t at begin + piece + t * tile.
+__device__ __forceinline__ int64_t share_of(int w, int64_t total, int groups) { return (int64_t)w * total / groups; }
 
 // Slot of the piece of item i that workgroup w computes; `head`: it starts at the item's first tile.
 __device__ __forceinline__ int64_t slot_of(ArgsPtr p, int i, int w, bool head) {
@@ -102,39 +108,76 @@ __device__ __forceinline__ int64_t slot_of(ArgsPtr p, int i, int w, bool head) {
 }
 
 // ------------------------------------------------------------------ plan
-constexpr int kPlanThreads = 1024;
+// One workgroup: per item the rows its queries see (spans) and its cost, summed
+// (costs); per workgroup of the main kernel the item its share starts in
+// (starts).  Items of a call that is in a hurry fit LDS.
+constexpr int kPlanThreads = 1024, kPlanItems = 4096;
 __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams) {
     const ArgsPtr p = args_now();
-    __shared__ int sums[kPlanThreads / 64];
+    __shared__ int64_t sums[kPlanThreads / 64];
+    __shared__ int64_t begins[kPlanItems];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int base = 0;
-    for (int i0 = 0; i0 < p->items; i0 += kPlanThreads) {
+    const int items = p->items;
+    int64_t base = 0;
+    for (int i0 = 0; i0 < items; i0 += kPlanThreads) {
         const int i = i0 + tid;
-        int n = 0;
-        if (i < p->items) {
+        int64_t n = 0;
+        if (i < items) {
             Item it = item_rows(p, i);
-            int most = 0;
-            for (int t = it.row0 / p->H; t <= (it.row0 + it.rows - 1) / p->H; ++t) most = max(most, seen_by(p, t));
+            int most = 0, least = p->L;
+            // a block has eight times 16 rows at most, each of one token: as many lengths, read together
+            const int first = it.row0 / p->H, last = (it.row0 + it.rows - 1) / p->H;
+            int seen[kSharedRows / 16];
+#pragma unroll
+            for (int k = 0; k < kSharedRows / 16; ++k) seen[k] = p->lengths[min(first + k, last)];
+#pragma unroll
+            for (int k = 0; k < kSharedRows / 16; ++k) {
+                const int s = min(max(seen[k], 0), p->L);
+                most = max(most, s);
+                least = min(least, s);
+            }
             item_tiles(p, i, most, it);
-            n = (it.first + it.second) * tile_cost(it);
+            p->spans[i] = int2{least, most};
+            const Cost c = cost_of(it.rows, p->kv_fp8);
+            const int tiles = it.first + it.second;
+            n = tiles == 0 ? 0 : c.piece + (int64_t)tiles * c.tile;
         }
-        int scan = n;
+        int64_t scan = n;
         for (int d = 1; d < 64; d <<= 1) {
-            const int u = __shfl_up(scan, d);
+            const int64_t u = __shfl_up(scan, d);
             if (lane >= d) scan += u;
         }
         if (lane == 63) sums[wave] = scan;
         __syncthreads();
-        int before = 0, all = 0;
+        int64_t before = 0, all = 0;
         for (int w = 0; w < kPlanThreads / 64; ++w) {
             if (w < wave) before += sums[w];
             all += sums[w];
         }
-        if (i < p->items) p->costs[i] = base + before + scan - n;
+        if (i < items) {
+            p->costs[i] = base + before + scan - n;
+            if (i < kPlanItems) begins[i] = base + before + scan - n;
+        }
         base += all;
         __syncthreads();
     }
-    if (tid == 0) p->costs[p->items] = base;
+    const int groups = (int)max((int64_t)1, min((int64_t)p->workgroups, base / kMinShare));
+    if (tid == 0) {
+        p->costs[items] = base;
+        p->starts[p->workgroups] = groups;
+    }
+    __threadfence_block();
+    __syncthreads();
+    for (int w = tid; w < p->workgroups; w += kPlanThreads) {
+        const int64_t c0 = share_of(w, base, groups);
+        int low = 0, high = items;  // begin of low <= c0, of high (if an item) > c0
+        while (high - low > 1) {
+            const int mid = (low + high) >> 1;
+            if ((items <= kPlanItems ? begins[mid] : p->costs[mid]) <= c0) low = mid;
+            else high = mid;
+        }
+        p->starts[w] = low;
+    }
 }
 
 // ------------------------------------------------------------------ main
@@ -903,41 +946,38 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
                   arguments.L,           arguments.prefix,      arguments.max_blocks,   arguments.block_size,
                   arguments.num_blocks,  arguments.block_magic, arguments.block_shift,  arguments.scale_log2};
     ArgsPtr p = args_now();
-    const int total = p->costs[p->items], groups = groups_of(p, total);
-    const int w = blockIdx.x;
+    const int w = blockIdx.x, groups = p->starts[p->workgroups];
     if (w >= groups) return;
-    const int c0 = share_of(w, total, groups), c1 = share_of(w + 1, total, groups);
+    int i = p->starts[w];
+    const int64_t total = p->costs[p->items];
+    const int64_t c0 = share_of(w, total, groups), c1 = share_of(w + 1, total, groups);
     if (c0 >= c1) return;
-    int i = 0, high = p->items;  // the item that holds cost c0: costs[i] <= c0 < costs[i + 1]
-    while (high - i > 1) {
-        const int mid = (i + high) >> 1;
-        if (p->costs[mid] <= c0) i = mid;
-        else high = mid;
-    }
 #pragma unroll 1
     for (;; ++i) {
         p = args_now();
         if (i >= p->items) break;
-        const int begin = p->costs[i], end = p->costs[i + 1];
+        const int64_t begin = p->costs[i], end = p->costs[i + 1];
+        const int2 span = p->spans[i];
         if (begin >= c1) break;
+        if (begin == end) continue;
         Piece c;
         c.it = item_rows(p, i);
-        const int cost = tile_cost(c.it);
-        const int a = max(0, ceil_div(c0 - begin, cost)), b = min(ceil_div(c1 - begin, cost), (end - begin) / cost);
+        item_tiles(p, i, span.y, c.it);
+        const Cost cost = cost_of(c.it.rows, FP8);
+        // the first tile that starts at c0 or behind, and at c1
+        const int64_t tile0 = begin + cost.piece;
+        const int tiles = c.it.first + c.it.second;
+        const int a = c0 <= tile0 ? 0 : (int)min((c0 - tile0 + cost.tile - 1) / cost.tile, (int64_t)tiles);
+        const int b = c1 <= tile0 ? 0 : (int)min((c1 - tile0 + cost.tile - 1) / cost.tile, (int64_t)tiles);
         if (a >= b) continue;
-        int most = 0, least = p->L;
-        for (int t = c.it.row0 / p->H; t <= (c.it.row0 + c.it.rows - 1) / p->H; ++t) {
-            const int n = seen_by(p, t);
-            most = max(most, n);
-            least = min(least, n);
-        }
-        item_tiles(p, i, most, c.it);
         c.it.first = __builtin_amdgcn_readfirstlane(c.it.first);
-        c.seen_low = __builtin_amdgcn_readfirstlane(least);
-        c.seen_high = __builtin_amdgcn_readfirstlane(most);
+        c.seen_low = __builtin_amdgcn_readfirstlane(span.x);
+        c.seen_high = __builtin_amdgcn_readfirstlane(span.y);
         c.a = __builtin_amdgcn_readfirstlane(a);
         c.nt = __builtin_amdgcn_readfirstlane(b - a);
-        const bool whole = !p->stacked && c.nt * cost == end - begin;
+        const bool whole = !p->stacked && c.nt == tiles;
+        if (threadIdx.x == 0 && a == 0) p->ends[i].x = w;
+        if (threadIdx.x == 0 && b == tiles) p->ends[i].y = w;
         const int64_t slot = slot_of(p, i, w, c.a == 0);
         if (c.it.rows > 64) shared_piece<FP8, LAYOUT, true, 4>(hot, c, whole, slot, lds, wave, lane);
         else if (c.it.rows > 32) shared_piece<FP8, LAYOUT, false, 4>(hot, c, whole, slot, lds, wave, lane);
@@ -947,40 +987,67 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
 }
 
 // ------------------------------------------------------------------ merge
-// One workgroup a row pair; thread t of a row's 128 owns columns 4 t .. 4 t + 3.
-__global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams) {
+// Rows of cut items joined, and rows without keys filled in; rows of whole items
+// are there already.  A workgroup owns 2 * turns rows of an item (stacked: of all
+// rows), two at a time; thread t of a row's 128 owns columns 4 t .. 4 t + 3.  Four
+// pieces are read at a time.
+constexpr int kMergeBatch = 4;
+template <bool STACKED>
+__global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams, int turns) {
     const ArgsPtr p = args_now();
-    const int rows = p->B * p->SQ * p->H;
-    const int row = blockIdx.x * 2 + (threadIdx.x >> 7), col = (threadIdx.x & 127) * 4;
-    if (row >= rows) return;
-    const int total = p->costs[p->items], groups = groups_of(p, total);
-    const int seq_rows = p->SQ * p->H, b = row / seq_rows, in_seq = row - b * seq_rows;
-    float m = -FLT_MAX, l = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int part = p->stacked ? 0 : 1; part < 2; ++part) {
-        const int i = part == 0 ? row / kSharedRows : p->prefix_items + b * p->seq_blocks + in_seq / kSharedRows;
-        const int hl = part == 0 ? row % kSharedRows : in_seq % kSharedRows;
-        const int begin = p->costs[i], end = p->costs[i + 1];
-        if (begin == end) continue;
-        const int w0 = group_at(begin, total, groups), w1 = group_at(end - tile_cost(item_rows(p, i)), total, groups);
-        if (!p->stacked && w0 == w1) return;  // a whole item: written by the main kernel
-        for (int w = w0; w <= w1; ++w) {
-            const int64_t prow = slot_of(p, i, w, w == w0) * kSharedRows + hl;
-            const float ms = p->part_m[prow], ls = p->part_l[prow];
-            const f32x4 u = *reinterpret_cast<const f32x4*>(p->part_o + prow * 512 + col);
-            const float top = fmaxf(m, ms), keep = fast_exp2(m - top), add = fast_exp2(ms - top);
-            l = l * keep + ls * add;
-            acc = acc * keep + u * add;
-            m = top;
-        }
+    const int rows = p->B * p->SQ * p->H, col = (threadIdx.x & 127) * 4;
+    const int seq_rows = p->SQ * p->H, half = threadIdx.x >> 7;
+    Item it;
+    int first, count;  // the workgroup's rows
+    if constexpr (STACKED) {
+        first = (int)blockIdx.x * 2 * turns;
+        count = min(2 * turns, rows - first);
+    } else {
+        const int chunks = kSharedRows / (2 * turns), i = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x % chunks;
+        const int2 ends = p->ends[i];
+        if (p->costs[i] != p->costs[i + 1] && ends.x == ends.y) return;  // a whole item
+        it = item_rows(p, i);
+        first = it.row0 + chunk * 2 * turns;
+        count = min(2 * turns, it.row0 + it.rows - first);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    bf16x4 v;
-    for (int r = 0; r < 4; ++r) v[r] = (__bf16)(acc[r] * inv);
-    *reinterpret_cast<bf16x4*>(p->out + (int64_t)row * 512 + col) = v;
-    if (col == 0) {
-        p->out_max[row] = l == 0.f ? -INFINITY : m * kLn2;
-        p->out_sum[row] = l;
+    for (int k = half; k < count; k += 2) {
+        const int row = first + k, b = row / seq_rows, in_seq = row - b * seq_rows;
+        float m = -FLT_MAX, l = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int part = STACKED ? 0 : 1; part < 2; ++part) {
+            const int i = part == 0 ? row / kSharedRows : p->prefix_items + b * p->seq_blocks + in_seq / kSharedRows;
+            const int hl = part == 0 ? row % kSharedRows : in_seq % kSharedRows;
+            if (p->costs[i] == p->costs[i + 1]) continue;  // none of its keys is seen
+            const int2 ends = p->ends[i];
+            for (int w = ends.x; w <= ends.y; w += kMergeBatch) {
+                float ms[kMergeBatch], ls[kMergeBatch];
+                f32x4 u[kMergeBatch];
+#pragma unroll
+                for (int n = 0; n < kMergeBatch; ++n) {
+                    const int64_t prow = slot_of(p, i, min(w + n, ends.y), w + n == ends.x) * kSharedRows + hl;
+                    ms[n] = p->part_m[prow];
+                    ls[n] = p->part_l[prow];
+                    u[n] = *reinterpret_cast<const f32x4*>(p->part_o + prow * 512 + col);
+                }
+#pragma unroll
+                for (int n = 0; n < kMergeBatch; ++n) {
+                    if (w + n > ends.y) break;
+                    const float top = fmaxf(m, ms[n]), keep = fast_exp2(m - top), add = fast_exp2(ms[n] - top);
+                    l = l * keep + ls[n] * add;
+                    acc = acc * keep + u[n] * add;
+                    m = top;
+                }
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        bf16x4 v;
+        for (int r = 0; r < 4; ++r) v[r] = (__bf16)(acc[r] * inv);
+        *reinterpret_cast<bf16x4*>(p->out + (int64_t)row * 512 + col) = v;
+        if (col == 0) {
+            p->out_max[row] = l == 0.f ? -INFINITY : m * kLn2;
+            p->out_sum[row] = l;
+        }
     }
 }
 
@@ -1000,8 +1067,12 @@ int launch_shared(const SharedParams& p, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3(p.workgroups), dim3(kPPThreads), 0, stream, p);
     rc = (int)hipGetLastError();
     if (rc) return rc;
-    const int rows = p.B * p.SQ * p.H;
-    hipLaunchKernelGGL(shared_merge_kernel, dim3((rows + 1) / 2), dim3(kThreads), 0, stream, p);
+    // many rows are a prefill's, most of them there already: sixteen a workgroup
+    const int rows = p.B * p.SQ * p.H, turns = rows >= 32768 ? 8 : 1;
+    if (p.stacked)
+        hipLaunchKernelGGL(shared_merge_kernel<true>, dim3((rows + 2 * turns - 1) / (2 * turns)), dim3(kThreads), 0, stream, p, turns);
+    else
+        hipLaunchKernelGGL(shared_merge_kernel<false>, dim3(p.items * (kSharedRows / (2 * turns))), dim3(kThreads), 0, stream, p, turns);
     return (int)hipGetLastError();
 }
 
