@@ -110,6 +110,7 @@ int dsa_rotary(const dsa_rotary_args* a, void* stream) {
     if (a->dim < 2 || a->dim % 2 || a->dim > DSA_ROTARY_MAX_DIM || a->start < 0 || a->start > a->width - a->dim)
         return fail(-1, "dim must be even, in [2, %d], and start .. start + dim lie inside the head (got dim %d, start %d, "
                     "width %d)", DSA_ROTARY_MAX_DIM, a->dim, a->start, a->width);
+    if ((int64_t)a->heads * a->width > (int64_t)1 << 31) return fail(-1, "heads * width must be at most 2^31");
     if (!std::isfinite(a->magnitude)) return fail(-1, "magnitude must be finite");
     const unsigned size = a->dtype == DSA_F32 ? 4 : 2;
     if (!aligned(a->x, size) || !aligned(a->out, size) || !aligned(a->frequencies, 8) ||

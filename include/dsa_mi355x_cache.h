@@ -55,6 +55,7 @@ int dsa_extend_block_table(int32_t* block_table, const int32_t* lengths, const i
  * The angle is formed in 64 bits and reduced to a turn before the 32-bit sine
  * and cosine; the products are 32-bit, rounded once to x's type.  The rest of
  * each head is copied (out == x, with the same strides: left as it is).
+ * heads * width <= 2^31.
  */
 #define DSA_BF16 0
 #define DSA_F16 1
