@@ -653,26 +653,44 @@ _fast_lock = threading.Lock()
 _fast_state = []  # [module or None] once loaded
 
 
+def _load_fast(name, entries):
+    """The extension module ``name`` with the library's ``entries`` set, or None (not built)."""
+    from . import build as _build
+
+    path = _build.fast_path_module(name)
+    if not path.exists():
+        return None
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location(f"dsa_amd.{name}", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    lib = _lib.load()
+    module.set_entry(*(ctypes.cast(getattr(lib, e), ctypes.c_void_p).value for e in entries))
+    return module
+
+
 def _fast_path():
     if _fast_state:
         return _fast_state[0]
     with _fast_lock:
         if not _fast_state:
-            module = None
-            from . import build as _build
-
-            path = _build.fast_path_module()
-            if path.exists():
-                import importlib.util
-
-                spec = importlib.util.spec_from_file_location("dsa_amd._fast", path)
-                module = importlib.util.module_from_spec(spec)
-                spec.loader.exec_module(module)
-                lib = _lib.load()
-                module.set_entry(*(ctypes.cast(f, ctypes.c_void_p).value
-                                   for f in (lib.dsa_fwd, lib.dsa_fwd_main, lib.dsa_merge)))
-            _fast_state.append(module)
+            _fast_state.append(_load_fast("_fast", ("dsa_fwd", "dsa_fwd_main", "dsa_merge")))
     return _fast_state[0]
+
+
+# The same for the paged cache's operators (csrc/fast_cache.cpp), whose shapes need no plan.
+_fast_cache_state = []
+
+
+def _fast_cache():
+    if _fast_cache_state:
+        return _fast_cache_state[0]
+    with _fast_lock:
+        if not _fast_cache_state:
+            _fast_cache_state.append(_load_fast("_fast_cache", ("dsa_extend_block_table", "dsa_rotary",
+                                                                "dsa_write_kv_rows")))
+    return _fast_cache_state[0]
 
 
 def _register_fast(device, shape, plan, partials):

@@ -2,9 +2,10 @@
 
 Usage: ``python -m dsa_amd.build`` (or ``__graft_entry__.build()``).  Compiles
 the kernel sources in ``dsa_amd/csrc`` with ``hipcc --offload-arch=gfx950`` and
-links one shared library exporting the C ABI of ``include/dsa_mi355x.h``, and
-builds ``dsa_amd/_fast*.so``, the host fast path of ``forward`` (g++ against
-the installed PyTorch-ROCm; no device code).
+links one shared library exporting the C ABI of ``include/dsa_mi355x.h`` and
+``include/dsa_mi355x_cache.h``, and builds ``dsa_amd/_fast*.so``, the host fast
+paths of ``forward`` and of the paged cache's operators (g++ against the
+installed PyTorch-ROCm; no device code).
 """
 from __future__ import annotations
 
@@ -58,45 +59,49 @@ def _compile(src: str, verbose: bool) -> Path:
     return obj
 
 
-def fast_path_module() -> Path:
-    """Path of the host fast-path extension module (csrc/fast_forward.cpp)."""
-    return PKG / ("_fast" + sysconfig.get_config_var("EXT_SUFFIX"))
+FAST_SOURCES = {"_fast": "fast_forward.cpp", "_fast_cache": "fast_cache.cpp"}
 
 
-def _compile_fast(verbose: bool) -> Path:
-    """The host fast path of forward() as a CPython extension against the
-    installed PyTorch-ROCm (host code only: g++ with torch's headers and
-    libraries, the HIP headers for the stream type)."""
+def fast_path_module(name: str = "_fast") -> Path:
+    """Path of a host fast-path extension module (csrc/fast_*.cpp)."""
+    return PKG / (name + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def _compile_fast(name: str, verbose: bool) -> Path:
+    """A host fast path as a CPython extension against the installed
+    PyTorch-ROCm (host code only: g++ with torch's headers and libraries, the
+    HIP headers for the stream type)."""
     import torch
     import torch.utils.cpp_extension as ce
 
     torch_dir = Path(torch.__file__).resolve().parent
-    out = fast_path_module()
+    out = fast_path_module(name)
     tmp = out.with_suffix(".tmp")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_fast", "-D__HIP_PLATFORM_AMD__=1",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-DTORCH_EXTENSION_NAME={name}", "-D__HIP_PLATFORM_AMD__=1",
            "-DUSE_ROCM=1", *[f"-I{d}" for d in ce.include_paths()], f"-I{sysconfig.get_paths()['include']}",
-           f"-I{ROCM_INCLUDE}", str(CSRC / "fast_forward.cpp"), "-o", str(tmp), f"-L{torch_dir / 'lib'}",
+           f"-I{ROCM_INCLUDE}", f"-I{ROOT / 'include'}", str(CSRC / FAST_SOURCES[name]), "-o", str(tmp), f"-L{torch_dir / 'lib'}",
            "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",
            f"-Wl,-rpath,{torch_dir / 'lib'}"]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"g++ failed for fast_forward.cpp:\n{res.stdout}{res.stderr}")
+        raise RuntimeError(f"g++ failed for {FAST_SOURCES[name]}:\n{res.stdout}{res.stderr}")
     os.replace(tmp, out)
     return out
 
 
 def build(verbose: bool = False) -> Path:
     """Compile all kernels for gfx950 and link the shared library, and build
-    the host fast-path module (always rebuilds)."""
+    the host fast-path modules (always rebuilds)."""
     OBJ_DIR.mkdir(exist_ok=True)
-    with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
-        fast = ex.submit(_compile_fast, verbose)
+    with ThreadPoolExecutor(max_workers=len(SOURCES) + len(FAST_SOURCES)) as ex:
+        fast = [ex.submit(_compile_fast, name, verbose) for name in FAST_SOURCES]
         objs = list(ex.map(lambda s: _compile(s, verbose), SOURCES))
-        fast.result()
+        for module in fast:
+            module.result()
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [hipcc(), *DEVICE, "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
     if verbose:

@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .api import FP8_ROW, HEAD_DIM, ROPE_DIM, _on_device
+from .api import FP8_ROW, HEAD_DIM, ROPE_DIM, _fast_cache, _on_device
 from .rotary import check_frequencies, check_magnitude, check_positions
 
 MAX_SEQUENCES = 4096
@@ -54,6 +54,13 @@ def extend_block_table(block_table, lengths, new_tokens, free_blocks, block_size
     * ``used [1]``: blocks taken; above ``len(free_blocks)`` the list was short.
 
     One launch, nothing synchronised, B up to 4096."""
+    fast = _fast_cache()
+    if fast is not None:  # checked and launched in C++ (None: not taken)
+        taken = fast.extend_block_table(block_table, lengths, new_tokens, free_blocks, block_size, max_tokens)
+        if taken is not None:
+            if type(taken) is int:
+                _lib.check(taken, "dsa_extend_block_table")
+            return taken
     if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2 or min(block_table.shape) <= 0:
         raise ValueError("block_table must be [B, max_blocks]")
     if type(block_size) is not int or not 0 < block_size < 2 ** 31:
@@ -100,6 +107,14 @@ def write_kv_rows(kv, k_rope, slots, kv_cache, rope_cache=None, *, positions=Non
 
     ``frequencies`` (float64 ``[32]``) with ``positions`` (int32 or int64
     ``[tokens]``) turns ``k_rope`` on its way as :func:`dsa_amd.rotary` does."""
+    fast = _fast_cache()
+    if fast is not None:  # checked and launched in C++ (None: not taken)
+        rc = fast.write_kv_rows(kv, k_rope, slots, kv_cache, rope_cache, positions, frequencies, interleaved, magnitude,
+                                pow2_scales)
+        if rc is not None:
+            if rc:
+                _lib.check(rc, "dsa_write_kv_rows")
+            return
     if (not isinstance(kv, torch.Tensor) or not isinstance(k_rope, torch.Tensor) or kv.dim() != 2 or k_rope.dim() != 2
             or kv.shape[1] != HEAD_DIM or k_rope.shape != (kv.shape[0], ROPE_DIM)):
         raise ValueError("expected kv[tokens, 512] and k_rope[tokens, 64]")

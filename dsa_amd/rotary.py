@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import _lib
-from .api import _on_device
+from .api import _fast_cache, _on_device
 
 ROTARY_MAX_DIM = 512
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -136,6 +136,13 @@ def rotary(x, positions, frequencies, *, interleaved=True, start=0, transposed=F
     untouched), else a new contiguous tensor.  ``transposed`` turns the other
     way, which is the gradient for ``x``; where ``x`` requires a gradient the
     call records that itself (not with ``out``)."""
+    fast = _fast_cache()
+    if fast is not None:  # checked and launched in C++ (None: not taken)
+        taken = fast.rotary(x, positions, frequencies, interleaved, start, transposed, magnitude, out)
+        if taken is not None:
+            if type(taken) is int:
+                _lib.check(taken, "dsa_rotary")
+            return taken
     if not isinstance(x, torch.Tensor) or x.dim() not in (3, 4):
         raise ValueError("x must be [tokens, H, D] or [B, SQ, H, D]")
     device = x.device

@@ -1,0 +1,122 @@
+"""The host fast path of the paged cache's operators (dsa_amd/_fast_cache*.so,
+built from csrc/fast_cache.cpp): the same results as the Python path, and None
+for whatever that refuses or does besides."""
+import sys
+
+import pytest
+import torch
+
+import dsa_amd
+from dsa_amd import api, paging
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def fast():
+    if not torch.cuda.is_available():
+        pytest.skip("no ROCm GPU")
+    module = api._fast_cache()
+    assert module is not None, "the fast path module is built by dsa_amd.build"
+    return module
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32).cuda()
+
+
+def table_args():
+    return [i32(*range(12)).view(3, 4), i32(5, 0, 16), i32(3, 9, 0), i32(40, 41, 42, 43), 4, 14]
+
+
+def rotary_args(dim=3, out=False):
+    x = torch.randn((2, 5, 4, 96)[4 - dim:]).bfloat16().cuda()
+    positions = torch.arange(x.shape[:-2].numel()).view(x.shape[:-2]).cuda()
+    return [x, positions, dsa_amd.rotary_frequencies(64).cuda(), True, 32, False, 1.5, torch.empty_like(x) if out else None]
+
+
+def write_args(fp8=False, turned=True):
+    kv = torch.randn(5, 576).bfloat16().cuda()
+    where = [torch.arange(5).cuda(), dsa_amd.rotary_frequencies(64).cuda()] if turned else [None, None]
+    cache = ([torch.zeros(3, 4, 656, dtype=torch.uint8).cuda(), None] if fp8 else
+             [torch.zeros(3, 4, 512).bfloat16().cuda(), torch.zeros(3, 4, 64).bfloat16().cuda()])
+    return [kv[:, :512], kv[:, 512:], i32(3, -1, 11, 12, 0), *cache, *where, False, 1.0, True]
+
+
+def test_taken_and_equal(fast, monkeypatch):
+    module = sys.modules["dsa_amd.rotary"]
+    for args in (rotary_args(), rotary_args(4), rotary_args(4, out=True)):
+        taken = fast.rotary(*args)
+        assert taken is not None and (args[7] is None or taken is args[7])
+        taken = taken.clone()
+        monkeypatch.setattr(module, "_fast_cache", lambda: None)
+        kw = dict(interleaved=args[3], start=args[4], transposed=args[5], magnitude=args[6], out=args[7])
+        assert torch.equal(dsa_amd.rotary(*args[:3], **kw), taken)
+        monkeypatch.undo()
+        assert torch.equal(dsa_amd.rotary(*args[:3], **kw), taken)
+    one, two = table_args(), table_args()
+    taken = fast.extend_block_table(*one)
+    monkeypatch.setattr(paging, "_fast_cache", lambda: None)
+    for a, b in zip(taken, dsa_amd.extend_block_table(*two)):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+    assert torch.equal(one[0], two[0])
+    for args in (write_args(), write_args(True), write_args(turned=False)):
+        assert fast.write_kv_rows(*args) == 0
+        again = [a.clone() if i in (3, 4) and a is not None else a for i, a in enumerate(args)]
+        for i in (3, 4):
+            if again[i] is not None:
+                again[i].zero_()
+        dsa_amd.write_kv_rows(*again[:5], positions=again[5], frequencies=again[6], interleaved=again[7],
+                              magnitude=again[8], pow2_scales=again[9])
+        assert torch.equal(args[3], again[3]) and (args[4] is None or torch.equal(args[4], again[4]))
+
+
+@pytest.mark.parametrize("call, make, bad", [
+    ("extend_block_table", table_args, {
+        0: [None, torch.zeros(12).int(), "cpu", "long", "apart", torch.zeros(4, 0).int()], 1: ["cpu", "long", "short"],
+        2: ["cpu", "long", "short"], 3: ["cpu", "long", "apart"], 4: [0, -1, 2 ** 31, 4.0, True, None],
+        5: [-1, 2 ** 31, 2.0, False]}),
+    ("rotary", rotary_args, {
+        0: [None, 3, "cpu", "long", "last", "grad", "empty", torch.zeros(2, 2)], 1: [None, "cpu", "float", "short", "apart"],
+        2: [None, "cpu", "float", "apart", torch.zeros(0).double()], 3: [None, 1], 4: [-1, 33, 1.0, True], 5: [None, 0],
+        6: [float("nan"), float("inf"), 1e39, None, 1], 7: [3, "cpu", "short", "over"]}),
+    ("write_kv_rows", write_args, {
+        0: [None, "cpu", "float", "short", "last", "empty", "odd"], 1: [None, "cpu", "float", "short", "last"],
+        2: [None, "cpu", "long", "short", "apart"], 3: [None, "cpu", "float", "last", "bytes"],
+        4: [None, "cpu", "float", "short"], 5: [None, "cpu", "float", "short"], 6: [None, "cpu", "float", "short"],
+        7: [None, 1], 8: [float("nan"), None, 1, 1e39], 9: [None, 0]})])
+def test_declines(fast, call, make, bad):
+    """Declined before anything is allocated or written."""
+    how = {"cpu": lambda t: t.cpu(), "long": lambda t: t.long(), "float": lambda t: t.float(), "short": lambda t: t[:-1],
+           "apart": lambda t: torch.stack([t, t], -1)[..., 0], "last": lambda t: t.transpose(-1, -2),
+           "grad": lambda t: t.clone().requires_grad_(), "empty": lambda t: t[:0], "bytes": lambda t: t.byte(),
+           "odd": lambda t: torch.zeros(5, 577).bfloat16().cuda()[:, :512]}
+    for at, values in bad.items():
+        for value in values:
+            args = make()
+            if isinstance(value, str) and value == "over":
+                args[7] = torch.zeros(args[0].numel() + 8).bfloat16().cuda()
+                args[0], args[7] = args[7][:-8].view(make()[0].shape), args[7][8:].view(make()[0].shape)
+            elif isinstance(value, str):
+                args[at] = how[value](args[at] if args[at] is not None else torch.empty_like(args[0]))
+            else:
+                args[at] = value
+            kept = [a.clone() if isinstance(a, torch.Tensor) else a for a in args]
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            print(call, at, value, flush=True)
+            assert getattr(fast, call)(*args) is None, (at, value)
+            torch.cuda.synchronize()
+            assert torch.cuda.memory_allocated() == before
+            for a, k in zip(args, kept):
+                assert not isinstance(a, torch.Tensor) or torch.equal(a, k)
+
+
+def test_a_gradient_is_recorded_all_the_same(fast):
+    x, positions, freq = rotary_args()[:3]
+    x.requires_grad_()
+    y = dsa_amd.rotary(x, positions, freq)
+    y.sum().backward()
+    assert x.grad is not None
+    with torch.no_grad():
+        assert torch.equal(dsa_amd.rotary(x, positions, freq), y)

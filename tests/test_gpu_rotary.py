@@ -74,6 +74,31 @@ def test_against_64_bits(tokens, heads, width, start, dim, interleaved, dtype):
     assert torch.equal(x, kept)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("tokens, heads, width, start, dim", [
+    (2003, 40, 96, 32, 64),   # a few tokens a workgroup's run of units and a part of one
+    (4999, 1, 64, 0, 64),     # many tokens a workgroup
+    (61, 190, 576, 0, 512),   # several workgroups a token
+    (1201, 33, 67, 3, 64)])   # nothing aligned
+def test_many_units(tokens, heads, width, start, dim, interleaved, dtype):
+    x = make((tokens, heads, width), dtype)
+    positions = (torch.arange(tokens) * 7 + 1).cuda()
+    freq = FREQ[dim].cuda()
+    kw = dict(interleaved=interleaved, start=start)
+    y = dsa_amd.rotary(x, positions, freq, **kw)
+    check(y, x, positions, freq, **kw)
+    keep = torch.ones(width, dtype=torch.bool)
+    keep[start:start + dim] = False
+    assert torch.equal(y[..., keep.cuda()], x[..., keep.cuda()])
+    # the same by groups, in place
+    if tokens % 2 == 0 or tokens == 2003:
+        tokens -= tokens % 2
+        z = x[:tokens].reshape(2, tokens // 2, heads, width).clone()
+        dsa_amd.rotary(z, positions[:tokens].view(2, -1), freq, out=z, **kw)
+        assert torch.equal(z.view(tokens, heads, width), y[:tokens])
+
+
 @pytest.mark.parametrize("interleaved", [True, False])
 def test_far_and_negative_positions(interleaved):
     """Positions to 2^31 - 1 in 32 bits and beyond in 64: angles of 10^9 radians."""
