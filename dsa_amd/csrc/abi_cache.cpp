@@ -38,7 +38,7 @@ bool fills_blocks(int64_t rows) {
 struct SharedPlan {
     bool stacked;
     int prefix_items, seq_blocks, items, workgroups;
-    int64_t costs_bytes, spans_bytes, starts_bytes, slots, bytes;
+    int64_t ends_bytes, slots, bytes;
 };
 
 int64_t round_256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -69,13 +69,11 @@ int shared_plan(const dsa_shared_args* a, SharedPlan* plan) {
     // Pieces: every cut of an item's tiles starts a new one; a stacked call keeps
     // all of them, another only those of cut items, two at most a workgroup.
     plan->slots = plan->stacked ? items + plan->workgroups : 2 * (int64_t)plan->workgroups;
-    // The summed costs times a workgroup's number stay in 64 bits: at most 2^26
-    // items of 2^20 tiles, and 2^12 workgroups.
-    static_assert(dsa::kSharedMaxCost + dsa::kSharedPieceCost < 1 << 8, "costs fit");
-    plan->costs_bytes = round_256(8 * (items + 1));
-    plan->spans_bytes = round_256(8 * items);
-    plan->starts_bytes = round_256(4 * ((int64_t)plan->workgroups + 1));
-    plan->bytes = plan->costs_bytes + 2 * plan->spans_bytes + plan->starts_bytes + plan->slots * dsa::kSharedRows * (512 + 2) * 4;
+    // The kernel's sums: an item of at most 2^20 + 2 tiles costs less than 2^26, at
+    // most 2^26 items times 2^12 workgroups stay in 64 bits.
+    static_assert(dsa::kSharedMaxCost + (dsa::kSharedPieceCost >> 20) < 1 << 6, "an item's cost");
+    plan->ends_bytes = round_256(8 * items);
+    plan->bytes = plan->ends_bytes + plan->slots * dsa::kSharedRows * (512 + 2) * 4;
     return 0;
 }
 
@@ -177,11 +175,8 @@ int dsa_fwd_shared(const dsa_shared_args* a, void* stream) {
     p.out_max = a->out_max;
     p.out_sum = a->out_sum;
     char* ws = static_cast<char*>(a->workspace);
-    p.costs = reinterpret_cast<int64_t*>(ws);
-    p.spans = reinterpret_cast<int2*>(ws + plan.costs_bytes);
-    p.ends = p.spans + plan.spans_bytes / 8;
-    p.starts = reinterpret_cast<int32_t*>(ws + plan.costs_bytes + 2 * plan.spans_bytes);
-    p.part_o = reinterpret_cast<float*>(ws + plan.costs_bytes + 2 * plan.spans_bytes + plan.starts_bytes);
+    p.ends = reinterpret_cast<int2*>(ws);
+    p.part_o = reinterpret_cast<float*>(ws + plan.ends_bytes);
     p.part_m = p.part_o + plan.slots * dsa::kSharedRows * 512;
     p.part_l = p.part_m + plan.slots * dsa::kSharedRows;
     p.B = a->B;

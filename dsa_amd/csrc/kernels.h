@@ -195,7 +195,7 @@ int launch_write_rows(const dsa_write_args& p, hipStream_t stream);
 // item may be cut over several; the merge kernel joins its pieces.
 constexpr int kSharedRows = 128;
 constexpr int kSharedKeys = 32;      // keys a tile
-constexpr int kSharedMaxCost = 32, kSharedPieceCost = 128;  // bounds on a tile's cost and on a piece's own
+constexpr int kSharedMaxCost = 32, kSharedPieceCost = 192;  // bounds: an item of t * 32 keys costs t of one and once the other
 struct SharedParams {
     const uint16_t* q;
     const char* kv;
@@ -205,10 +205,7 @@ struct SharedParams {
     const int32_t* block_table;  // [B, max_blocks] or NULL
     uint16_t* out;
     float *out_max, *out_sum;
-    int64_t* costs;   // [items + 1]: cost of the items before
-    int2* spans;      // [items]: least and greatest number of rows a query of the item sees
     int2* ends;       // [items]: workgroups that compute an item's first and last tile
-    int32_t* starts;  // [workgroups + 1]: item each one's share starts in; how many have a share
     float* part_o;    // [slots, kSharedRows, 512] pieces of cut items
     float* part_m;    // [slots, kSharedRows] (log2 units)
     float* part_l;    // [slots, kSharedRows]

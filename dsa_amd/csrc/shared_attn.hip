@@ -94,7 +94,7 @@ __device__ __forceinline__ Cost cost_of(int rows, int fp8) {
     if (rows > 32) return Cost{fp8 ? 16 : 20, 105};
     return Cost{fp8 ? 13 : 15, 75};
 }
-static_assert(kSharedMaxCost >= 27 + 1 && kSharedPieceCost >= 120, "the host's bound on the summed costs");
+static_assert(kSharedMaxCost >= 27 && kSharedPieceCost >= 2 * 27 + 120, "the host's bound on an item's cost");
 constexpr int kMinShare = 40;  // least cost a workgroup is given: some tiles, and no less than one
 
 // Workgroup w computes the tiles that start in its share [w * total / groups,
@@ -102,82 +102,40 @@ constexpr int kMinShare = 40;  // least cost a workgroup is given: some tiles, a
 // `begin` has its tile t at begin + piece + t * tile.
 __device__ __forceinline__ int64_t share_of(int w, int64_t total, int groups) { return (int64_t)w * total / groups; }
 
+// What an item's queries see (least and most), and with that its tiles and cost.
+struct Look {
+    Item it;
+    int low, high, cost;
+    Cost each;
+};
+__device__ __forceinline__ void look_at(ArgsPtr p, int i, int low, int high, Look& k) {
+    k.it = item_rows(p, i);
+    item_tiles(p, i, high, k.it);
+    k.low = low;
+    k.high = high;
+    k.each = cost_of(k.it.rows, p->kv_fp8);
+    const int tiles = k.it.first + k.it.second;
+    k.cost = tiles == 0 ? 0 : k.each.piece + tiles * k.each.tile;
+}
+__device__ __forceinline__ void look_at(ArgsPtr p, int i, Look& k) {
+    const Item it = item_rows(p, i);
+    // a block has eight times 16 rows at most, each of one token: as many lengths, read together
+    const int first = it.row0 / p->H, last = (it.row0 + it.rows - 1) / p->H;
+    int seen[kSharedRows / 16], most = 0, least = p->L;
+#pragma unroll
+    for (int n = 0; n < kSharedRows / 16; ++n) seen[n] = p->lengths[min(first + n, last)];
+#pragma unroll
+    for (int n = 0; n < kSharedRows / 16; ++n) {
+        const int v = min(max(seen[n], 0), p->L);
+        most = max(most, v);
+        least = min(least, v);
+    }
+    look_at(p, i, least, most, k);
+}
+
 // Slot of the piece of item i that workgroup w computes; `head`: it starts at the item's first tile.
 __device__ __forceinline__ int64_t slot_of(ArgsPtr p, int i, int w, bool head) {
     return p->stacked ? (int64_t)i + w : 2 * (int64_t)w + (head ? 1 : 0);
-}
-
-// ------------------------------------------------------------------ plan
-// One workgroup: per item the rows its queries see (spans) and its cost, summed
-// (costs); per workgroup of the main kernel the item its share starts in
-// (starts).  Items of a call that is in a hurry fit LDS.
-constexpr int kPlanThreads = 1024, kPlanItems = 4096;
-__global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams) {
-    const ArgsPtr p = args_now();
-    __shared__ int64_t sums[kPlanThreads / 64];
-    __shared__ int64_t begins[kPlanItems];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int items = p->items;
-    int64_t base = 0;
-    for (int i0 = 0; i0 < items; i0 += kPlanThreads) {
-        const int i = i0 + tid;
-        int64_t n = 0;
-        if (i < items) {
-            Item it = item_rows(p, i);
-            int most = 0, least = p->L;
-            // a block has eight times 16 rows at most, each of one token: as many lengths, read together
-            const int first = it.row0 / p->H, last = (it.row0 + it.rows - 1) / p->H;
-            int seen[kSharedRows / 16];
-#pragma unroll
-            for (int k = 0; k < kSharedRows / 16; ++k) seen[k] = p->lengths[min(first + k, last)];
-#pragma unroll
-            for (int k = 0; k < kSharedRows / 16; ++k) {
-                const int s = min(max(seen[k], 0), p->L);
-                most = max(most, s);
-                least = min(least, s);
-            }
-            item_tiles(p, i, most, it);
-            p->spans[i] = int2{least, most};
-            const Cost c = cost_of(it.rows, p->kv_fp8);
-            const int tiles = it.first + it.second;
-            n = tiles == 0 ? 0 : c.piece + (int64_t)tiles * c.tile;
-        }
-        int64_t scan = n;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t u = __shfl_up(scan, d);
-            if (lane >= d) scan += u;
-        }
-        if (lane == 63) sums[wave] = scan;
-        __syncthreads();
-        int64_t before = 0, all = 0;
-        for (int w = 0; w < kPlanThreads / 64; ++w) {
-            if (w < wave) before += sums[w];
-            all += sums[w];
-        }
-        if (i < items) {
-            p->costs[i] = base + before + scan - n;
-            if (i < kPlanItems) begins[i] = base + before + scan - n;
-        }
-        base += all;
-        __syncthreads();
-    }
-    const int groups = (int)max((int64_t)1, min((int64_t)p->workgroups, base / kMinShare));
-    if (tid == 0) {
-        p->costs[items] = base;
-        p->starts[p->workgroups] = groups;
-    }
-    __threadfence_block();
-    __syncthreads();
-    for (int w = tid; w < p->workgroups; w += kPlanThreads) {
-        const int64_t c0 = share_of(w, base, groups);
-        int low = 0, high = items;  // begin of low <= c0, of high (if an item) > c0
-        while (high - low > 1) {
-            const int mid = (low + high) >> 1;
-            if ((items <= kPlanItems ? begins[mid] : p->costs[mid]) <= c0) low = mid;
-            else high = mid;
-        }
-        p->starts[w] = low;
-    }
 }
 
 // ------------------------------------------------------------------ main
@@ -220,7 +178,8 @@ struct PPLds {
     static constexpr int P_OFF = RAW_OFF + 2 * RAW_BYTES, P_GROUP = 64 * 64;
     static constexpr int FLAG_OFF = P_OFF + 2 * P_GROUP;  // a second pass is needed
     static constexpr int BAD_OFF = FLAG_OFF + 4;          // some block entry of the piece lies outside the pool
-    static constexpr int LDS_BYTES = FLAG_OFF + 16;
+    static constexpr int PLAN_OFF = FLAG_OFF + 16;        // the workgroup's first item: number, begin, low, high
+    static constexpr int LDS_BYTES = PLAN_OFF + 32;
     static constexpr int ML_OFF = P_OFF;  // [3][128] floats, at the end: l, reference and maximum
     static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
     __device__ static uint32_t stage(uint32_t lds, int u) { return lds + (uint32_t)(u % NSTAGE) * STAGE_BYTES; }
@@ -394,12 +353,6 @@ struct Gathers {
             }
         }
     }
-    __device__ __forceinline__ void all(const Hot& p, const Piece& c, int u, uint32_t lds, uint32_t bad, int wave,
-                                        int lane) {
-        fetch(p, c, u, wave);
-        prepare(p, c, u, bad, wave);
-        issue(p, lds, wave, lane);
-    }
 };
 
 // The wave's four rows of tile u, from raw to the ring: lane l takes the latent
@@ -515,7 +468,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
     const int row = c.it.row0 + (live ? block : 0);
     const int nt = c.nt;
     const ArgsPtr args = args_now();
-    const int seen = live ? __builtin_amdgcn_readfirstlane(seen_by(args, row / args->H)) : 0;
+    int seen = seen_by(args, row / args->H);  // in a scalar register from the first wait on
     const uint32_t p_lds = lds + X::P_OFF + grp * X::P_GROUP, bad = lds + X::BAD_OFF;
 
     bf16x8 qf[18];
@@ -671,14 +624,19 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         l_run = 0.f;
         if (pass == 1) m_ref = max_xor32(max_xor16(m_lane));
         bool overflow = false;
-        // The first tile's rows, and Q: a full wait, as the compiler does not
+        // The first two tiles' rows, and Q: a full wait, as the compiler does not
         // count the gathers (it would wait for Q in the loop).
+        gather.fetch(p, c, 0, wave);
+        behind.fetch(p, c, 1, wave);
         if (threadIdx.x == 0) lds_store<int>(bad, 0);
         lds_barrier();
-        gather.all(p, c, 0, lds, bad, wave, lane);
-        wait_vmcnt<0>();
-        gather.all(p, c, 1, lds, bad, wave, lane);
+        gather.prepare(p, c, 0, bad, wave);
+        gather.issue(p, lds, wave, lane);
+        behind.prepare(p, c, 1, bad, wave);
+        behind.issue(p, lds, wave, lane);
         gather.fetch(p, c, 2, wave);
+        wait_vmcnt<0>();
+        seen = live ? __builtin_amdgcn_readfirstlane(seen) : 0;
         if constexpr (FP8) advance(0);
         else gather.prepare(p, c, 2, bad, wave);
         // Rows of tile u in the pool: all, unless the piece has met a bad entry (every wave is past preparing tile u).
@@ -946,33 +904,83 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
                   arguments.L,           arguments.prefix,      arguments.max_blocks,   arguments.block_size,
                   arguments.num_blocks,  arguments.block_magic, arguments.block_shift,  arguments.scale_log2};
     ArgsPtr p = args_now();
-    const int w = blockIdx.x, groups = p->starts[p->workgroups];
-    if (w >= groups) return;
-    int i = p->starts[w];
-    const int64_t total = p->costs[p->items];
-    const int64_t c0 = share_of(w, total, groups), c1 = share_of(w + 1, total, groups);
-    if (c0 >= c1) return;
+    // The share: every workgroup sums the costs itself (a launch before this one
+    // would take 5 us more), a thread those of a run of items, and finds the item
+    // that its share starts in.
+    const int w = blockIdx.x;
+    int64_t c0, c1;
+    {
+        const int items = p->items, run = (items + kPPThreads - 1) / kPPThreads;
+        const int i0 = min((int)threadIdx.x * run, items), i1 = min(i0 + run, items);
+        int64_t sum = 0;
+        for (int i = i0; i < i1; ++i) {
+            Look k;
+            look_at(p, i, k);
+            sum += k.cost;
+            if (w == 0 && k.cost == 0) p->ends[i] = int2{0, -1};  // nobody's: for the merge
+        }
+        int64_t scan = sum;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t u = __shfl_up(scan, d);
+            if (lane >= d) scan += u;
+        }
+        int64_t* sums = reinterpret_cast<int64_t*>(smem);
+        if (lane == 63) sums[wave] = scan;
+        __syncthreads();
+        int64_t begin = scan - sum, total = 0;
+        for (int v = 0; v < kPPThreads / 64; ++v) {
+            if (v < wave) begin += sums[v];
+            total += sums[v];
+        }
+        total = (int64_t)__builtin_amdgcn_readfirstlane((int)(total >> 32)) << 32 |
+                (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
+        const int groups = (int)max((int64_t)1, min((int64_t)p->workgroups, total / kMinShare));
+        if (total == 0 || w >= groups) return;
+        c0 = share_of(w, total, groups);
+        c1 = share_of(w + 1, total, groups);
+        if (begin <= c0 && c0 < begin + sum) {
+            for (int i = i0; i < i1; ++i) {
+                Look k;
+                look_at(p, i, k);
+                if (c0 < begin + k.cost) {
+                    int* plan = reinterpret_cast<int*>(smem + X::PLAN_OFF);
+                    plan[0] = i;
+                    plan[1] = k.low;
+                    plan[2] = k.high;
+                    *reinterpret_cast<int64_t*>(plan + 4) = begin;
+                    break;
+                }
+                begin += k.cost;
+            }
+        }
+        __syncthreads();
+    }
+    const int* plan = reinterpret_cast<const int*>(smem + X::PLAN_OFF);
+    int i = __builtin_amdgcn_readfirstlane(plan[0]);
+    int low = __builtin_amdgcn_readfirstlane(plan[1]), high = __builtin_amdgcn_readfirstlane(plan[2]);
+    // costs from here on: from the first item's begin
+    int64_t begin;
+    {
+        const int64_t first = *reinterpret_cast<const int64_t*>(plan + 4);
+        begin = (int64_t)__builtin_amdgcn_readfirstlane((int)(first >> 32)) << 32 |
+                (uint32_t)__builtin_amdgcn_readfirstlane((int)first);
+    }
 #pragma unroll 1
-    for (;; ++i) {
+    for (;;) {
         p = args_now();
-        if (i >= p->items) break;
-        const int64_t begin = p->costs[i], end = p->costs[i + 1];
-        const int2 span = p->spans[i];
-        if (begin >= c1) break;
-        if (begin == end) continue;
+        Look k;
+        look_at(p, i, low, high, k);
+        // its first tile that starts at c0 or behind, and at c1
+        const int64_t tile0 = begin + k.each.piece, end = begin + k.cost;
+        const int tiles = k.it.first + k.it.second;
+        const int a = c0 <= tile0 ? 0 : ((int)(c0 - tile0) + k.each.tile - 1) / k.each.tile;
+        const int b = c1 <= tile0 ? 0 : ((int)(min(c1, end) - tile0) + k.each.tile - 1) / k.each.tile;
+        if (a < b) {
         Piece c;
-        c.it = item_rows(p, i);
-        item_tiles(p, i, span.y, c.it);
-        const Cost cost = cost_of(c.it.rows, FP8);
-        // the first tile that starts at c0 or behind, and at c1
-        const int64_t tile0 = begin + cost.piece;
-        const int tiles = c.it.first + c.it.second;
-        const int a = c0 <= tile0 ? 0 : (int)min((c0 - tile0 + cost.tile - 1) / cost.tile, (int64_t)tiles);
-        const int b = c1 <= tile0 ? 0 : (int)min((c1 - tile0 + cost.tile - 1) / cost.tile, (int64_t)tiles);
-        if (a >= b) continue;
+        c.it = k.it;
         c.it.first = __builtin_amdgcn_readfirstlane(c.it.first);
-        c.seen_low = __builtin_amdgcn_readfirstlane(span.x);
-        c.seen_high = __builtin_amdgcn_readfirstlane(span.y);
+        c.seen_low = __builtin_amdgcn_readfirstlane(low);
+        c.seen_high = __builtin_amdgcn_readfirstlane(high);
         c.a = __builtin_amdgcn_readfirstlane(a);
         c.nt = __builtin_amdgcn_readfirstlane(b - a);
         const bool whole = !p->stacked && c.nt == tiles;
@@ -983,6 +991,13 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
         else if (c.it.rows > 32) shared_piece<FP8, LAYOUT, false, 4>(hot, c, whole, slot, lds, wave, lane);
         else if (c.it.rows > 16) shared_piece<FP8, LAYOUT, false, 2>(hot, c, whole, slot, lds, wave, lane);
         else shared_piece<FP8, LAYOUT, false, 1>(hot, c, whole, slot, lds, wave, lane);
+        }
+        p = args_now();
+        if (end >= c1 || ++i >= p->items) break;
+        begin = end;
+        look_at(p, i, k);
+        low = __builtin_amdgcn_readfirstlane(k.low);
+        high = __builtin_amdgcn_readfirstlane(k.high);
     }
 }
 
@@ -1005,7 +1020,7 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams, in
     } else {
         const int chunks = kSharedRows / (2 * turns), i = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x % chunks;
         const int2 ends = p->ends[i];
-        if (p->costs[i] != p->costs[i + 1] && ends.x == ends.y) return;  // a whole item
+        if (ends.x == ends.y) return;  // a whole item
         it = item_rows(p, i);
         first = it.row0 + chunk * 2 * turns;
         count = min(2 * turns, it.row0 + it.rows - first);
@@ -1018,7 +1033,6 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams, in
         for (int part = STACKED ? 0 : 1; part < 2; ++part) {
             const int i = part == 0 ? row / kSharedRows : p->prefix_items + b * p->seq_blocks + in_seq / kSharedRows;
             const int hl = part == 0 ? row % kSharedRows : in_seq % kSharedRows;
-            if (p->costs[i] == p->costs[i + 1]) continue;  // none of its keys is seen
             const int2 ends = p->ends[i];
             for (int w = ends.x; w <= ends.y; w += kMergeBatch) {
                 float ms[kMergeBatch], ls[kMergeBatch];
@@ -1054,9 +1068,6 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams, in
 }  // namespace
 
 int launch_shared(const SharedParams& p, hipStream_t stream) {
-    hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
-    int rc = (int)hipGetLastError();
-    if (rc) return rc;
     const int layout = !p.block_table ? kRows : p.block_size % 4 == 0 ? kBlocks : kPages;
     auto* kernel = p.kv_fp8 ? (layout == kRows     ? shared_main_kernel<true, kRows>
                                : layout == kBlocks ? shared_main_kernel<true, kBlocks>
@@ -1065,7 +1076,7 @@ int launch_shared(const SharedParams& p, hipStream_t stream) {
                                : layout == kBlocks ? shared_main_kernel<false, kBlocks>
                                                    : shared_main_kernel<false, kPages>);
     hipLaunchKernelGGL(kernel, dim3(p.workgroups), dim3(kPPThreads), 0, stream, p);
-    rc = (int)hipGetLastError();
+    const int rc = (int)hipGetLastError();
     if (rc) return rc;
     // many rows are a prefill's, most of them there already: sixteen a workgroup
     const int rows = p.B * p.SQ * p.H, turns = rows >= 32768 ? 8 : 1;
