@@ -28,8 +28,12 @@ int finish(int rc, const char* what) {
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Query rows of a sequence from which its own blocks of kSharedRows are at least
-// this full; emptier ones make the prefix worth a pass over stacked rows.
+// Whether a sequence's query rows fill blocks of their own to seven eighths: then
+// those take the prefix too; emptier ones leave it to blocks of all sequences'
+// rows (stacked).  Measured with 16 sequences of bf16 rows, paged, 8192 rows
+// shared and up to 512 of their own, stacked and not: 16 rows a sequence 39 and
+// 44 us, 96 64 and 68, 112 70 and 70, 144 80 and 84, 224 106 and 99, 240 112 and
+// 99; with 1024 shared rows and up to 2048 own ones within 3 us of each other.
 bool fills_blocks(int64_t rows) {
     const int64_t blocks = (rows + dsa::kSharedRows - 1) / dsa::kSharedRows;
     return rows * 8 >= blocks * dsa::kSharedRows * 7;

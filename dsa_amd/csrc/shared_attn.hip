@@ -29,7 +29,6 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr int kKeys = kSharedKeys;
 constexpr int kFp8Row = 656, kFp8ScaleOff = 512, kFp8RopeOff = 528;
-constexpr int kThreads = 256;
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
@@ -84,18 +83,18 @@ __device__ __forceinline__ void item_tiles(ArgsPtr p, int i, int most, Item& it)
 // What an item costs, in tenths of a microsecond on a full chip: each tile, and
 // once the start and end of a piece (Q, the first tile's latency, the stores).
 // Measured on 64 to 256 sequences of their own rows, paged: up to 32 rows 1.5 us
-// a tile of bf16 rows (HBM, 6.4 TB/s) and 1.35 of fp8, up to 64 2.0 and 1.65,
-// up to 128 2.1 and 2.7; a piece 7.5, 10.5 and 12 us beside its tiles.
+// a tile of bf16 rows (HBM, 6.4 TB/s) and 1.4 of fp8, up to 64 2.0 and 1.65,
+// up to 128 2.1 and 2.7; a piece 8.5, 10.5 and 12 us beside its tiles.
 struct Cost {
     int tile, piece;
 };
 __device__ __forceinline__ Cost cost_of(int rows, int fp8) {
     if (rows > 64) return Cost{fp8 ? 27 : 21, 120};
     if (rows > 32) return Cost{fp8 ? 16 : 20, 105};
-    return Cost{fp8 ? 13 : 15, 75};
+    return Cost{fp8 ? 14 : 15, 85};
 }
 static_assert(kSharedMaxCost >= 27 && kSharedPieceCost >= 2 * 27 + 120, "the host's bound on an item's cost");
-constexpr int kMinShare = 40;  // least cost a workgroup is given: some tiles, and no less than one
+constexpr int kMinShare = 30;  // least cost a workgroup is given: more than a tile (16 heads, 3 sequences: 22.4 us at 40, 21.8 at 30)
 
 // Workgroup w computes the tiles that start in its share [w * total / groups,
 // (w + 1) * total / groups) of the summed costs; an item that starts at cost
@@ -1004,65 +1003,96 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
 // ------------------------------------------------------------------ merge
 // Rows of cut items joined, and rows without keys filled in; rows of whole items
 // are there already.  A workgroup owns 2 * turns rows of an item (stacked: of all
-// rows), two at a time; thread t of a row's 128 owns columns 4 t .. 4 t + 3.  Four
-// pieces are read at a time.
-constexpr int kMergeBatch = 4;
-template <bool STACKED>
-__global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams, int turns) {
+// rows), two at a time; thread t of a row's 128 owns columns 4 t .. 4 t + 3.  Eight
+// pieces are read at a time.  Where rows are few (SPLIT), a workgroup owns one, and
+// four groups of 128 threads take its pieces, eight at a time, in turn.
+constexpr int kMergeBatch = 8, kMergeSplit = 4, kMergeFewRows = 2048;
+template <bool STACKED, bool SPLIT>
+__global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_kernel(SharedParams, int turns) {
+    constexpr int ROWS = SPLIT ? 1 : 2, GROUPS = SPLIT ? kMergeSplit : 1;
+    __shared__ f32x4 parts[SPLIT ? 128 * (kMergeSplit - 1) : 1];
+    __shared__ float2 stats[SPLIT ? kMergeSplit - 1 : 1];  // maximum, sum
     const ArgsPtr p = args_now();
     const int rows = p->B * p->SQ * p->H, col = (threadIdx.x & 127) * 4;
-    const int seq_rows = p->SQ * p->H, half = threadIdx.x >> 7;
-    Item it;
+    const int seq_rows = p->SQ * p->H;
+    const int half = SPLIT ? 0 : threadIdx.x >> 7, group = SPLIT ? threadIdx.x >> 7 : 0;
     int first, count;  // the workgroup's rows
     if constexpr (STACKED) {
-        first = (int)blockIdx.x * 2 * turns;
-        count = min(2 * turns, rows - first);
+        first = (int)blockIdx.x * ROWS * turns;
+        count = min(ROWS * turns, rows - first);
     } else {
-        const int chunks = kSharedRows / (2 * turns), i = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x % chunks;
+        const int chunks = kSharedRows / (ROWS * turns), i = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x % chunks;
         const int2 ends = p->ends[i];
         if (ends.x == ends.y) return;  // a whole item
-        it = item_rows(p, i);
-        first = it.row0 + chunk * 2 * turns;
-        count = min(2 * turns, it.row0 + it.rows - first);
+        const Item it = item_rows(p, i);
+        first = it.row0 + chunk * ROWS * turns;
+        count = min(ROWS * turns, it.row0 + it.rows - first);
     }
-    for (int k = half; k < count; k += 2) {
-        const int row = first + k, b = row / seq_rows, in_seq = row - b * seq_rows;
+    for (int r = half; r < count; r += ROWS) {
+        const int row = first + r, b = row / seq_rows, in_seq = row - b * seq_rows;
         float m = -FLT_MAX, l = 0.f;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        auto join = [&](float top_of, float sum, const f32x4& u) __attribute__((always_inline)) {
+            const float top = fmaxf(m, top_of), keep = fast_exp2(m - top), add = fast_exp2(top_of - top);
+            l = l * keep + sum * add;
+            acc = acc * keep + u * add;
+            m = top;
+        };
+        // its pieces: of the stacked item first, then of the sequence's own
+        const int own = p->prefix_items + b * p->seq_blocks + in_seq / kSharedRows, shared = row / kSharedRows;
+        const int2 e1 = p->ends[own], e0 = STACKED ? p->ends[shared] : int2{0, -1};
+        const int n0 = e0.y - e0.x + 1, n = n0 + (e1.y - e1.x + 1);
+        for (int j0 = group * kMergeBatch; j0 < n; j0 += GROUPS * kMergeBatch) {
+            float ms[kMergeBatch], ls[kMergeBatch];
+            f32x4 u[kMergeBatch];
 #pragma unroll
-        for (int part = STACKED ? 0 : 1; part < 2; ++part) {
-            const int i = part == 0 ? row / kSharedRows : p->prefix_items + b * p->seq_blocks + in_seq / kSharedRows;
-            const int hl = part == 0 ? row % kSharedRows : in_seq % kSharedRows;
-            const int2 ends = p->ends[i];
-            for (int w = ends.x; w <= ends.y; w += kMergeBatch) {
-                float ms[kMergeBatch], ls[kMergeBatch];
-                f32x4 u[kMergeBatch];
-#pragma unroll
-                for (int n = 0; n < kMergeBatch; ++n) {
-                    const int64_t prow = slot_of(p, i, min(w + n, ends.y), w + n == ends.x) * kSharedRows + hl;
-                    ms[n] = p->part_m[prow];
-                    ls[n] = p->part_l[prow];
-                    u[n] = *reinterpret_cast<const f32x4*>(p->part_o + prow * 512 + col);
-                }
-#pragma unroll
-                for (int n = 0; n < kMergeBatch; ++n) {
-                    if (w + n > ends.y) break;
-                    const float top = fmaxf(m, ms[n]), keep = fast_exp2(m - top), add = fast_exp2(ms[n] - top);
-                    l = l * keep + ls[n] * add;
-                    acc = acc * keep + u[n] * add;
-                    m = top;
-                }
+            for (int k = 0; k < kMergeBatch; ++k) {
+                const int j = min(j0 + k, n - 1);
+                const int64_t prow = j < n0 ? slot_of(p, shared, e0.x + j, j == 0) * kSharedRows + row % kSharedRows
+                                            : slot_of(p, own, e1.x + (j - n0), j == n0) * kSharedRows + in_seq % kSharedRows;
+                ms[k] = p->part_m[prow];
+                ls[k] = p->part_l[prow];
+                u[k] = *reinterpret_cast<const f32x4*>(p->part_o + prow * 512 + col);
             }
+#pragma unroll
+            for (int k = 0; k < kMergeBatch; ++k) {
+                if (j0 + k >= n) break;
+                join(ms[k], ls[k], u[k]);
+            }
+        }
+        if constexpr (SPLIT) {
+            if (group > 0) {
+                parts[128 * (group - 1) + (threadIdx.x & 127)] = acc;
+                if (col == 0) stats[group - 1] = float2{m, l};
+            }
+            __syncthreads();
+            if (group > 0) return;
+            for (int g = 0; g < GROUPS - 1; ++g) join(stats[g].x, stats[g].y, parts[128 * g + threadIdx.x]);
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         bf16x4 v;
-        for (int r = 0; r < 4; ++r) v[r] = (__bf16)(acc[r] * inv);
+        for (int e = 0; e < 4; ++e) v[e] = (__bf16)(acc[e] * inv);
         *reinterpret_cast<bf16x4*>(p->out + (int64_t)row * 512 + col) = v;
         if (col == 0) {
             p->out_max[row] = l == 0.f ? -INFINITY : m * kLn2;
             p->out_sum[row] = l;
         }
     }
+}
+
+template <bool STACKED>
+void launch_merge(const SharedParams& p, hipStream_t stream) {
+    const int rows = p.B * p.SQ * p.H;
+    // Many rows are a prefill's, most of them there already: sixteen a workgroup
+    // (262,144 rows: 59 us for 121 with two).  Few: one, shared by four groups (48
+    // rows: 20.5 us a call for 21.8; 6144 rows: 155 for 147).
+    const bool split = rows <= kMergeFewRows;
+    const int turns = rows >= 32768 ? 8 : 1, own = split ? 1 : 2 * turns;
+    const int grid = STACKED ? (rows + own - 1) / own : p.items * (kSharedRows / own);
+    if (split)
+        hipLaunchKernelGGL((shared_merge_kernel<STACKED, true>), dim3(grid), dim3(128 * kMergeSplit), 0, stream, p, 1);
+    else
+        hipLaunchKernelGGL((shared_merge_kernel<STACKED, false>), dim3(grid), dim3(256), 0, stream, p, turns);
 }
 
 }  // namespace
@@ -1078,12 +1108,8 @@ int launch_shared(const SharedParams& p, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3(p.workgroups), dim3(kPPThreads), 0, stream, p);
     const int rc = (int)hipGetLastError();
     if (rc) return rc;
-    // many rows are a prefill's, most of them there already: sixteen a workgroup
-    const int rows = p.B * p.SQ * p.H, turns = rows >= 32768 ? 8 : 1;
-    if (p.stacked)
-        hipLaunchKernelGGL(shared_merge_kernel<true>, dim3((rows + 2 * turns - 1) / (2 * turns)), dim3(kThreads), 0, stream, p, turns);
-    else
-        hipLaunchKernelGGL(shared_merge_kernel<false>, dim3(p.items * (kSharedRows / (2 * turns))), dim3(kThreads), 0, stream, p, turns);
+    if (p.stacked) launch_merge<true>(p, stream);
+    else launch_merge<false>(p, stream);
     return (int)hipGetLastError();
 }
 
