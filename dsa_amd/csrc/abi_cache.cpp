@@ -42,7 +42,8 @@ bool fills_blocks(int64_t rows) {
 struct SharedPlan {
     bool stacked;
     int prefix_items, seq_blocks, items, workgroups;
-    int64_t ends_bytes, slots, bytes;
+    int own_rows;  // of a piece of a sequence's own rows
+    int64_t ends_bytes, part_rows, bytes;
 };
 
 int64_t round_256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -72,12 +73,15 @@ int shared_plan(const dsa_shared_args* a, SharedPlan* plan) {
     }
     // Pieces: every cut of an item's tiles starts a new one; a stacked call keeps
     // all of them, another only those of cut items, two at most a workgroup.
-    plan->slots = plan->stacked ? items + plan->workgroups : 2 * (int64_t)plan->workgroups;
+    plan->own_rows = (int)(seq_rows < dsa::kSharedRows ? seq_rows : dsa::kSharedRows);
+    const int64_t own_items = items - plan->prefix_items, wgs = plan->workgroups;
+    plan->part_rows = plan->stacked ? (plan->prefix_items + wgs) * dsa::kSharedRows + (own_items + wgs) * plan->own_rows
+                                    : 2 * wgs * plan->own_rows;
     // The kernel's sums: an item of at most 2^20 + 2 tiles costs less than 2^26, at
     // most 2^26 items times 2^12 workgroups stay in 64 bits.
     static_assert(dsa::kSharedMaxCost + (dsa::kSharedPieceCost >> 20) < 1 << 6, "an item's cost");
     plan->ends_bytes = round_256(8 * items);
-    plan->bytes = plan->ends_bytes + plan->slots * dsa::kSharedRows * (512 + 2) * 4;
+    plan->bytes = plan->ends_bytes + plan->part_rows * (512 + 2) * 4;
     return 0;
 }
 
@@ -181,8 +185,8 @@ int dsa_fwd_shared(const dsa_shared_args* a, void* stream) {
     char* ws = static_cast<char*>(a->workspace);
     p.ends = reinterpret_cast<int2*>(ws);
     p.part_o = reinterpret_cast<float*>(ws + plan.ends_bytes);
-    p.part_m = p.part_o + plan.slots * dsa::kSharedRows * 512;
-    p.part_l = p.part_m + plan.slots * dsa::kSharedRows;
+    p.part_m = p.part_o + plan.part_rows * 512;
+    p.part_l = p.part_m + plan.part_rows;
     p.B = a->B;
     p.SQ = a->SQ;
     p.H = a->H;
@@ -204,6 +208,7 @@ int dsa_fwd_shared(const dsa_shared_args* a, void* stream) {
     p.seq_blocks = plan.seq_blocks;
     p.items = plan.items;
     p.workgroups = plan.workgroups;
+    p.own_rows = plan.own_rows;
     return finish(dsa::launch_shared(p, static_cast<hipStream_t>(stream)), "shared attention launch");
 }
 

@@ -132,9 +132,14 @@ __device__ __forceinline__ void look_at(ArgsPtr p, int i, Look& k) {
     look_at(p, i, least, most, k);
 }
 
-// Slot of the piece of item i that workgroup w computes; `head`: it starts at the item's first tile.
-__device__ __forceinline__ int64_t slot_of(ArgsPtr p, int i, int w, bool head) {
-    return p->stacked ? (int64_t)i + w : 2 * (int64_t)w + (head ? 1 : 0);
+// First partial row of the piece of item i that workgroup w computes; `head`: it
+// starts at the item's first tile.  A stacked call keeps all its pieces, item i's
+// behind i - 1's; another only those of cut items, of which a workgroup has two at
+// most.  A sequence's own piece has own_rows rows.
+__device__ __forceinline__ int64_t piece_row(ArgsPtr p, int i, int w, bool head) {
+    if (!p->stacked) return (2 * (int64_t)w + (head ? 1 : 0)) * p->own_rows;
+    if (i < p->prefix_items) return ((int64_t)i + w) * kSharedRows;
+    return ((int64_t)p->prefix_items + p->workgroups) * kSharedRows + ((int64_t)(i - p->prefix_items) + w) * p->own_rows;
 }
 
 // ------------------------------------------------------------------ main
@@ -455,7 +460,7 @@ __device__ __forceinline__ void clear_specials(uint32_t stage, int gw, int lane)
 
 // One piece of an item, WIDE: up to 128 rows, else up to 16 NB (NB = 4 if WIDE).
 template <bool FP8, int LAYOUT, bool WIDE, int NB>
-__device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool whole, int64_t slot,
+__device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool whole, int64_t first_row,
                                              uint32_t lds, int wave, int lane) {
     static_assert(!WIDE || NB == 4, "a group's four row blocks");
     using X = PPLds<FP8>;
@@ -776,8 +781,8 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             out->out_max[c.it.row0 + hl] = sum == 0.f ? -INFINITY : top * kLn2;
             out->out_sum[c.it.row0 + hl] = sum;
         } else {
-            out->part_m[slot * kSharedRows + hl] = top;
-            out->part_l[slot * kSharedRows + hl] = sum;
+            out->part_m[first_row + hl] = top;
+            out->part_l[first_row + hl] = sum;
         }
     };
     // Staged rows [first, first + n) of the block, row r at HROW (bf16) or kPartRow (fp32) * (r - first), stored whole.
@@ -788,7 +793,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             for (int r = first + wave; r < end; r += 8)
                 *reinterpret_cast<bf16x8*>(base + (int64_t)r * 512) = lds_load<bf16x8>(lds + (r - first) * HROW + 16 * eln);
         } else {
-            float* base = out->part_o + slot * (kSharedRows * 512) + 4 * eln;
+            float* base = out->part_o + first_row * 512 + 4 * eln;
             for (int i = 2 * first + wave; i < 2 * end; i += 8)
                 *reinterpret_cast<f32x4*>(base + (i >> 1) * 512 + 256 * (i & 1)) =
                     lds_load<f32x4>(lds + (uint32_t)(((i >> 1) - first) * kPartRow + 1024 * (i & 1) + 16 * eln));
@@ -975,21 +980,21 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
         const int a = c0 <= tile0 ? 0 : ((int)(c0 - tile0) + k.each.tile - 1) / k.each.tile;
         const int b = c1 <= tile0 ? 0 : ((int)(min(c1, end) - tile0) + k.each.tile - 1) / k.each.tile;
         if (a < b) {
-        Piece c;
-        c.it = k.it;
-        c.it.first = __builtin_amdgcn_readfirstlane(c.it.first);
-        c.seen_low = __builtin_amdgcn_readfirstlane(low);
-        c.seen_high = __builtin_amdgcn_readfirstlane(high);
-        c.a = __builtin_amdgcn_readfirstlane(a);
-        c.nt = __builtin_amdgcn_readfirstlane(b - a);
-        const bool whole = !p->stacked && c.nt == tiles;
-        if (threadIdx.x == 0 && a == 0) p->ends[i].x = w;
-        if (threadIdx.x == 0 && b == tiles) p->ends[i].y = w;
-        const int64_t slot = slot_of(p, i, w, c.a == 0);
-        if (c.it.rows > 64) shared_piece<FP8, LAYOUT, true, 4>(hot, c, whole, slot, lds, wave, lane);
-        else if (c.it.rows > 32) shared_piece<FP8, LAYOUT, false, 4>(hot, c, whole, slot, lds, wave, lane);
-        else if (c.it.rows > 16) shared_piece<FP8, LAYOUT, false, 2>(hot, c, whole, slot, lds, wave, lane);
-        else shared_piece<FP8, LAYOUT, false, 1>(hot, c, whole, slot, lds, wave, lane);
+            Piece c;
+            c.it = k.it;
+            c.it.first = __builtin_amdgcn_readfirstlane(c.it.first);
+            c.seen_low = __builtin_amdgcn_readfirstlane(low);
+            c.seen_high = __builtin_amdgcn_readfirstlane(high);
+            c.a = __builtin_amdgcn_readfirstlane(a);
+            c.nt = __builtin_amdgcn_readfirstlane(b - a);
+            const bool whole = !p->stacked && c.nt == tiles;
+            if (threadIdx.x == 0 && a == 0) p->ends[i].x = w;
+            if (threadIdx.x == 0 && b == tiles) p->ends[i].y = w;
+            const int64_t first_row = piece_row(p, i, w, c.a == 0);
+            if (c.it.rows > 64) shared_piece<FP8, LAYOUT, true, 4>(hot, c, whole, first_row, lds, wave, lane);
+            else if (c.it.rows > 32) shared_piece<FP8, LAYOUT, false, 4>(hot, c, whole, first_row, lds, wave, lane);
+            else if (c.it.rows > 16) shared_piece<FP8, LAYOUT, false, 2>(hot, c, whole, first_row, lds, wave, lane);
+            else shared_piece<FP8, LAYOUT, false, 1>(hot, c, whole, first_row, lds, wave, lane);
         }
         p = args_now();
         if (end >= c1 || ++i >= p->items) break;
@@ -1048,8 +1053,8 @@ __global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_
 #pragma unroll
             for (int k = 0; k < kMergeBatch; ++k) {
                 const int j = min(j0 + k, n - 1);
-                const int64_t prow = j < n0 ? slot_of(p, shared, e0.x + j, j == 0) * kSharedRows + row % kSharedRows
-                                            : slot_of(p, own, e1.x + (j - n0), j == n0) * kSharedRows + in_seq % kSharedRows;
+                const int64_t prow = j < n0 ? piece_row(p, shared, e0.x + j, j == 0) + row % kSharedRows
+                                            : piece_row(p, own, e1.x + (j - n0), j == n0) + in_seq % kSharedRows;
                 ms[k] = p->part_m[prow];
                 ls[k] = p->part_l[prow];
                 u[k] = *reinterpret_cast<const f32x4*>(p->part_o + prow * 512 + col);

@@ -18,6 +18,9 @@ from .api import FP8_ROW, HEAD_DIM, ROPE_DIM, _check_scale, _device_cus, _on_dev
 
 
 def _check(q, kv, q_rope, k_rope, lengths, prefix, block_table):
+    optional = [t for t in (k_rope, block_table) if t is not None]
+    if not all(isinstance(t, torch.Tensor) for t in (q, kv, q_rope, lengths, *optional)):
+        raise ValueError("q, kv, q_rope, lengths (and k_rope, block_table) must be tensors")
     fp8 = kv.dtype == torch.uint8
     if fp8 and k_rope is not None:
         raise ValueError("with fp8 kv rows (uint8 [..., 656]) k_rope must be None: the rope values are in the rows")
@@ -73,8 +76,10 @@ def forward_shared(q, kv, q_rope, k_rope, lengths, prefix=0, *, scale=None, bloc
     its block table row) for every sequence.  The caller vouches that they are
     the same; it need not be a multiple of the block size.  0: nothing shared.
 
-    The output is finite for max|kv| < 2^38.  Outputs are fresh tensors, the
-    workspace is the caching allocator's, and nothing synchronises."""
+    The output is finite for max|kv| < 2^38.  Caches hold fewer than 2^25 rows.
+    Outputs are fresh tensors, which record no gradient (as
+    :func:`dsa_amd.forward`'s), the workspace is the caching allocator's, and
+    nothing synchronises."""
     scale = _check_scale(scale)
     batch, queries, heads, length, device, fp8 = _check(q, kv, q_rope, k_rope, lengths, prefix, block_table)
     args = _lib.DsaSharedArgs()

@@ -80,7 +80,8 @@ int dsa_rotary(const dsa_rotary_args* args, void* stream);
  * New rows into a cache: row slots[i] of the cache becomes token i's kv and
  * (rotated, where frequencies is given: as dsa_rotary over dim 64) k_rope.  A
  * token whose slot lies outside [0, cache_rows) is left out; slots that name a
- * row twice leave one of the two there, unspecified which.
+ * row twice leave one of the two there, unspecified which.  kv and k_rope must
+ * not lie in rows that the call writes.
  *
  *   kv [tokens, 512] bf16, kv_stride elements apart (a multiple of 8, 16-byte
  *   aligned); k_rope [tokens, 64] bf16, rope_stride apart (a multiple of 2,
@@ -125,7 +126,8 @@ int dsa_write_kv_rows(const dsa_write_args* args, void* stream);
  *   workspace: at least dsa_fwd_shared_ws_bytes bytes, 256-byte aligned, any
  *   contents; calls that can overlap need one each
  * Probabilities are rounded to bf16 before the second product, sums and
- * statistics are fp32; the output is finite for max|kv| < 2^38.
+ * statistics are fp32; the output is finite for max|kv| < 2^38.  L and
+ * num_blocks * block_size below 2^25, B * SQ * H at most 2^30.
  */
 typedef struct dsa_shared_args {
     const uint16_t* q;
@@ -142,7 +144,7 @@ typedef struct dsa_shared_args {
     int32_t B, SQ, H, L, prefix;
     int32_t block_size, max_blocks, num_blocks; /* paged: L = max_blocks * block_size */
     int32_t kv_format;          /* DSA_KV_BF16, DSA_KV_FP8 */
-    int32_t num_cus;            /* compute units to plan for; 0: the device's */
+    int32_t num_cus;            /* compute units to plan for, at most 4096; 0: the device's */
     float scale;                /* 0: 1/24 */
     int32_t reserved;           /* zero */
 } dsa_shared_args;

@@ -169,3 +169,58 @@ def test_c_table_refuses(at, value):
     args[at] = value
     assert lib.dsa_extend_block_table(*args) < 0
     assert lib.dsa_last_error()
+
+
+def _shared_args(**kw):
+    a = _lib.DsaSharedArgs()
+    for name in ("q", "kv", "q_rope", "k_rope", "lengths", "out", "out_max", "out_sum", "workspace"):
+        setattr(a, name, 4096)
+    a.workspace_bytes, a.num_cus = 1 << 40, 256
+    a.B, a.SQ, a.H, a.L, a.prefix = 3, 2, 16, 128, 64
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+SIZES = [dict(B=0), dict(SQ=0), dict(H=0), dict(H=24), dict(L=0), dict(L=1 << 25, prefix=0), dict(prefix=-1),
+         dict(prefix=129), dict(num_cus=-1), dict(num_cus=4097), dict(B=1 << 20, SQ=1 << 10, H=128)]
+
+
+@pytest.mark.parametrize("kw", SIZES + [
+    dict(q=None), dict(kv=None), dict(q_rope=None), dict(k_rope=None), dict(lengths=None), dict(out=None),
+    dict(out_max=None), dict(out_sum=None), dict(workspace=None), dict(q=4104), dict(kv=4104), dict(k_rope=4104),
+    dict(out=4104), dict(lengths=4098), dict(workspace=4112), dict(kv_format=2), dict(scale=-1.0), dict(scale=math.nan),
+    dict(block_table=4096), dict(block_table=4096, block_size=16, max_blocks=7, num_blocks=9),
+    dict(block_table=4096, block_size=16, max_blocks=8, num_blocks=0), dict(workspace_bytes=1 << 16),
+    dict(block_table=4096, block_size=16, max_blocks=8, num_blocks=1 << 21)])
+def test_c_shared_refuses(kw):
+    lib = _lib.load()
+    assert lib.dsa_fwd_shared(ctypes.byref(_shared_args(**kw)), None) < 0
+    assert lib.dsa_last_error()
+
+
+@pytest.mark.parametrize("kw", SIZES)
+def test_c_shared_workspace_refuses(kw):
+    assert _lib.load().dsa_fwd_shared_ws_bytes(ctypes.byref(_shared_args(**kw))) < 0
+
+
+def test_c_shared_workspace():
+    """Grows with the batch and the workgroups; a row of a piece is 512 + 2 floats."""
+    lib = _lib.load()
+    size = lambda **kw: lib.dsa_fwd_shared_ws_bytes(ctypes.byref(_shared_args(**kw)))  # noqa: E731
+    assert size(B=1, SQ=1, prefix=0) == 256 + 2 * 256 * 16 * 514 * 4
+    assert size(B=1, SQ=64, prefix=0) == 256 + 2 * 256 * 128 * 514 * 4
+    # 4 items of 128 stacked rows, 32 of 16 own ones, and a cut for each workgroup
+    assert size(B=32, SQ=1) == 512 + ((4 + 256) * 128 + (32 + 256) * 16) * 514 * 4
+    assert size(B=32, SQ=1, num_cus=8) < size(B=32, SQ=1) < size(B=4096, SQ=1)
+
+
+def test_shared_inputs_are_refused():
+    bf = torch.bfloat16
+    q, qr, lengths = torch.zeros(2, 1, 16, 512, dtype=bf), torch.zeros(2, 1, 16, 64, dtype=bf), torch.zeros(2, 1, dtype=torch.int32)
+    kv, kr = torch.zeros(2, 8, 1, 512, dtype=bf), torch.zeros(2, 8, 1, 64, dtype=bf)
+    for args in [(q, kv, qr, kr, lengths), (q, kv, qr, None, lengths), (None, kv, qr, kr, lengths),
+                 (q, kv, qr, kr, [8, 8]), (q[0], kv, qr, kr, lengths), (q, kv[..., :511], qr, kr, lengths),
+                 (q[:, :, :8], kv, qr[:, :, :8], kr, lengths), (q, kv, qr, kr, lengths, 9), (q, kv, qr, kr, lengths, True)]:
+        with pytest.raises(ValueError):
+            dsa_amd.forward_shared(*args)

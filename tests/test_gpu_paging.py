@@ -204,6 +204,28 @@ def test_write_strided_kv_and_empty():
     assert torch.equal(cache[slots.long()], kv)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_write_far_rows(fp8):
+    """Rows past 2^31 elements and 4 GiB of the cache."""
+    rows = (1 << 32) // 656 + 64 if fp8 else (1 << 31) // 512 + 64
+    kv, rope = rows_for(5)
+    slots = torch.tensor([rows - 1, 0, rows // 2 + 9, rows - 30, rows], dtype=torch.int32).cuda()
+    at = slots[:4].long()
+    if fp8:
+        cache = torch.zeros(rows, 656, dtype=torch.uint8, device="cuda")
+        dsa_amd.write_kv_rows(kv, rope, slots, cache)
+        assert torch.equal(cache[at], dsa_amd.quantize_kv_fp8(kv, rope.contiguous())[:4])
+        cache[at] = 0
+        assert not cache.view(torch.int64).any()
+    else:
+        cache = torch.zeros(rows, 512, dtype=torch.bfloat16, device="cuda")
+        rcache = torch.zeros(rows, 64, dtype=torch.bfloat16, device="cuda")
+        dsa_amd.write_kv_rows(kv, rope, slots, cache, rcache)
+        assert torch.equal(cache[at], kv[:4]) and torch.equal(rcache[at], rope[:4])
+        cache[at] = 0
+        assert not cache.any()
+
+
 def test_write_the_same_row_twice():
     """The row holds one of the two tokens; the other rows are right."""
     kv, rope = rows_for(64, 8)

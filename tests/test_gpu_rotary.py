@@ -140,6 +140,19 @@ def test_strides_groups_and_in_place():
     assert not cache[:, :10].any() and not cache[:, 15:].any()
 
 
+def test_far_offsets():
+    """Tokens past 2^31 elements of the input, and of the output."""
+    freq, positions = FREQ[64].cuda(), torch.tensor([3, 50, 7]).cuda()
+    big = torch.zeros((2 << 30) + 192, dtype=torch.bfloat16, device="cuda")
+    x = big.as_strided((3, 2, 96), (1 << 30, 96, 1))
+    x.copy_(make((3, 2, 96)))
+    near = x.contiguous()
+    want = dsa_amd.rotary(near, positions, freq, start=32)
+    assert torch.equal(dsa_amd.rotary(x, positions, freq, start=32), want)
+    dsa_amd.rotary(near, positions, freq, start=32, out=x)
+    assert torch.equal(x, want)
+
+
 def test_magnitude_and_round_trip():
     freq = FREQ[64].cuda()
     x, positions = make((6, 4, 64), torch.float32), torch.arange(6).cuda() * 1234

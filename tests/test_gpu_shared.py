@@ -145,6 +145,16 @@ def test_any_lengths(B, SQ, H, P, S, block):
     check(call(s, lengths), s, lengths)
 
 
+@pytest.mark.parametrize("B, SQ, H", [(2100, 1, 16), (700, 2, 64), (530, 1, 48)])
+def test_many_sequences(B, SQ, H):
+    """More blocks of rows than a workgroup has threads, some of them without keys."""
+    s = make(B, SQ, H, 45, 30, seed=B)
+    g = torch.Generator().manual_seed(1)
+    lengths = torch.randint(-20, 80, (B, SQ), generator=g).int().cuda()
+    lengths[100:300] = 0
+    check(call(s, lengths), s, lengths)
+
+
 @pytest.mark.parametrize("fp8", [False, True])
 def test_prefix_splits_change_nothing(fp8):
     """The same rows with any part of them called shared."""
