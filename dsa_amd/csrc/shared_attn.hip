@@ -99,7 +99,15 @@ constexpr int kMinShare = 30;  // least cost a workgroup is given: more than a t
 // Workgroup w computes the tiles that start in its share [w * total / groups,
 // (w + 1) * total / groups) of the summed costs; an item that starts at cost
 // `begin` has its tile t at begin + piece + t * tile.
-__device__ __forceinline__ int64_t share_of(int w, int64_t total, int groups) { return (int64_t)w * total / groups; }
+struct Shares {
+    int64_t each;
+    uint32_t rest, groups;
+    __device__ __forceinline__ Shares(int64_t total, uint32_t n) : groups(n) {  // a division of 64 bits only where it needs one
+        each = total >> 32 ? total / n : (uint32_t)total / n;
+        rest = (uint32_t)(total - each * n);
+    }
+    __device__ __forceinline__ int64_t start(uint32_t w) const { return w * each + w * rest / groups; }  // groups <= 2^12
+};
 
 // What an item's queries see (least and most), and with that its tiles and cost.
 struct Look {
@@ -917,16 +925,25 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
         const int items = p->items, run = (items + kPPThreads - 1) / kPPThreads;
         const int i0 = min((int)threadIdx.x * run, items), i1 = min(i0 + run, items);
         int64_t sum = 0;
+        Look k;
         for (int i = i0; i < i1; ++i) {
-            Look k;
             look_at(p, i, k);
             sum += k.cost;
             if (w == 0 && k.cost == 0) p->ends[i] = int2{0, -1};  // nobody's: for the merge
         }
         int64_t scan = sum;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t u = __shfl_up(scan, d);
-            if (lane >= d) scan += u;
+        if (run == 1) {  // 64 items cost less than 2^32
+            uint32_t s = (uint32_t)sum;
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t u = __shfl_up(s, d);
+                if (lane >= d) s += u;
+            }
+            scan = s;
+        } else {
+            for (int d = 1; d < 64; d <<= 1) {
+                const int64_t u = __shfl_up(scan, d);
+                if (lane >= d) scan += u;
+            }
         }
         int64_t* sums = reinterpret_cast<int64_t*>(smem);
         if (lane == 63) sums[wave] = scan;
@@ -940,12 +957,12 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
                 (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
         const int groups = (int)max((int64_t)1, min((int64_t)p->workgroups, total / kMinShare));
         if (total == 0 || w >= groups) return;
-        c0 = share_of(w, total, groups);
-        c1 = share_of(w + 1, total, groups);
+        const Shares shares(total, groups);
+        c0 = shares.start(w);
+        c1 = shares.start(w + 1);
         if (begin <= c0 && c0 < begin + sum) {
             for (int i = i0; i < i1; ++i) {
-                Look k;
-                look_at(p, i, k);
+                if (run > 1) look_at(p, i, k);
                 if (c0 < begin + k.cost) {
                     int* plan = reinterpret_cast<int*>(smem + X::PLAN_OFF);
                     plan[0] = i;
