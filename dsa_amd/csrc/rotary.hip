@@ -7,9 +7,13 @@
 // Bound by HBM (each element read and written once) and, for a decode step, by
 // the launch.  A head is cut into units: of the rotated part 16 bytes that hold
 // whole pairs (interleaved) or two times 16 bytes, dim / 2 apart; of the rest 16
-// bytes.  A workgroup owns a run of units, of some tokens or of a part of one
-// token's heads: it first loads them all, then forms its tokens' cosines and
-// sines once in LDS, for all heads, while the loads are on their way.
+// bytes; where sizes, strides or alignment forbid it a pair, or an element.  A
+// workgroup owns 256 units, of some tokens or of a part of one token's heads, one
+// a thread: it loads them, then forms its tokens' cosines and sines once in LDS,
+// for all heads, while the loads are on their way.  (Four units a thread were
+// slower throughout: 8 tokens x 128 heads x 64 of 192 bf16 4.1 us for 3.0, 4096
+// tokens 35.2 for 32.7 in a graph of them, 4.1 TB/s; 4096 x 64 heads x 64 of 128
+// fp32 in the half layout 59.4 for 51.5, 5.2 TB/s.)
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -22,7 +26,7 @@ namespace dsa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxAngles = 1024;  // cosines and sines a workgroup forms: four a thread, 8 KiB of LDS
+constexpr int kMaxAngles = 1024;  // cosines and sines a workgroup forms: four a thread at most, 8 KiB of LDS
 static_assert(DSA_ROTARY_MAX_DIM / 2 <= kMaxAngles, "a token's fit");
 
 // n / d, by a multiplication where magic = ceil(2^32 / d) gives it exactly (0: a division).
@@ -64,8 +68,8 @@ struct Vec {
     }
 };
 
-// WIDE: units of 16 bytes.  U units a thread.
-template <typename T, bool INTERLEAVED, bool WIDE, int U>
+// WIDE: units of 16 bytes.
+template <typename T, bool INTERLEAVED, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(dsa_rotary_args p, Shape s) {
     constexpr int W = WIDE ? 16 / (int)sizeof(T) : INTERLEAVED ? 2 : 1;  // elements of a vector
     constexpr int PAIRS = INTERLEAVED ? W / 2 : W;                       // pairs of a turning unit
@@ -77,16 +81,14 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(dsa_rotary_args p, Sha
     const uint32_t chunk = blockIdx.x - (uint32_t)group * s.chunks;
     const int64_t token0 = group * s.tokens;
     const int tokens = (int)min((int64_t)s.tokens, all - token0);
-    const uint32_t end = s.per_token * (uint32_t)tokens;
 
-    int64_t to[U];
-    int which[U];       // turning: its first angle; else -1; nothing there: -2
-    Vec<T, W> a[U], b[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-        const uint32_t n = (chunk * U + k) * kThreads + tid;
-        which[k] = -2;
-        if (n >= end) continue;
+    const uint32_t n = chunk * kThreads + tid;
+    const bool there = n < s.per_token * (uint32_t)tokens;
+    bool turns = false;
+    int first = 0;  // its first angle
+    int64_t to = 0;
+    Vec<T, W> a, b;
+    if (there) {
         const uint32_t t = s.tokens == 1 ? 0 : quotient(n, s.per_token, s.token_magic);
         const uint32_t in_token = n - t * s.per_token;
         const uint32_t h = s.units == 1 ? in_token : quotient(in_token, s.units, s.units_magic);
@@ -96,22 +98,20 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(dsa_rotary_args p, Sha
             outer = in_group / p.tokens;
             in_group -= outer * p.tokens;
         }
-        int e;
-        if (u < s.turning) {
-            which[k] = (int)t * pairs + u * PAIRS;
-            e = p.start + u * W;
-        } else {
-            which[k] = -1;
+        turns = u < s.turning;
+        first = (int)t * pairs + u * PAIRS;
+        int e = p.start + u * W;
+        if (!turns) {
             e = (u - s.turning) * COPY;
             e += e >= p.start ? p.dim : 0;
         }
-        to[k] = outer * p.out_stride[0] + in_group * p.out_stride[1] + h * p.out_stride[2] + e;
+        to = outer * p.out_stride[0] + in_group * p.out_stride[1] + h * p.out_stride[2] + e;
         const T* from = static_cast<const T*>(p.x) + outer * p.x_stride[0] + in_group * p.x_stride[1] + h * p.x_stride[2] + e;
-        if (WIDE || u < s.turning) {
-            a[k].load(from);
-            if (!INTERLEAVED && u < s.turning) b[k].load(from + pairs);
+        if (WIDE || turns) {
+            a.load(from);
+            if (!INTERLEAVED && turns) b.load(from + pairs);
         } else {
-            a[k].v[0] = from[0];
+            a.v[0] = from[0];
         }
     }
 
@@ -123,38 +123,35 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(dsa_rotary_args p, Sha
     }
     __syncthreads();
 
+    if (!there) return;
+    T* out = static_cast<T*>(p.out) + to;
+    if (!turns) {
+        if constexpr (WIDE) a.store(out);
+        else out[0] = a.v[0];
+        return;
+    }
+    const float2* cs = angles + first;
+    Vec<T, W> y;
+    if constexpr (INTERLEAVED) {
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-        if (which[k] == -2) continue;
-        T* out = static_cast<T*>(p.out) + to[k];
-        if (which[k] == -1) {
-            if constexpr (WIDE) a[k].store(out);
-            else out[0] = a[k].v[0];
-            continue;
+        for (int i = 0; i < PAIRS; ++i) {
+            float y0, y1;
+            rotary_pair((float)a.v[2 * i], (float)a.v[2 * i + 1], cs[i], y0, y1);
+            y.v[2 * i] = (T)y0;
+            y.v[2 * i + 1] = (T)y1;
         }
-        const float2* cs = angles + which[k];
-        Vec<T, W> y;
-        if constexpr (INTERLEAVED) {
+        y.store(out);
+    } else {
+        Vec<T, W> z;
 #pragma unroll
-            for (int i = 0; i < PAIRS; ++i) {
-                float y0, y1;
-                rotary_pair((float)a[k].v[2 * i], (float)a[k].v[2 * i + 1], cs[i], y0, y1);
-                y.v[2 * i] = (T)y0;
-                y.v[2 * i + 1] = (T)y1;
-            }
-            y.store(out);
-        } else {
-            Vec<T, W> z;
-#pragma unroll
-            for (int i = 0; i < PAIRS; ++i) {
-                float y0, y1;
-                rotary_pair((float)a[k].v[i], (float)b[k].v[i], cs[i], y0, y1);
-                y.v[i] = (T)y0;
-                z.v[i] = (T)y1;
-            }
-            y.store(out);
-            z.store(out + pairs);
+        for (int i = 0; i < PAIRS; ++i) {
+            float y0, y1;
+            rotary_pair((float)a.v[i], (float)b.v[i], cs[i], y0, y1);
+            y.v[i] = (T)y0;
+            z.v[i] = (T)y1;
         }
+        y.store(out);
+        z.store(out + pairs);
     }
 }
 
@@ -175,19 +172,14 @@ int launch(const dsa_rotary_args& p, hipStream_t stream) {
     s.units = s.turning + (in_place ? 0 : (p.width - p.dim) / (is_wide ? wide : 1));
     s.per_token = (uint32_t)p.heads * (uint32_t)s.units;
     const int64_t all = p.groups * p.tokens;
-    // Four units a thread where the chip is full all the same (256 workgroups),
-    // else one: 8 tokens of 128 heads.
-    const bool deep = all * s.per_token >= (int64_t)256 * 4 * kThreads;
-    const uint32_t units = (deep ? 4 : 1) * kThreads;
-    const int64_t fit = s.per_token < units ? units / s.per_token : 1, angles = kMaxAngles / pairs;
+    const int64_t fit = s.per_token < kThreads ? kThreads / s.per_token : 1, angles = kMaxAngles / pairs;
     s.tokens = (int)(fit < angles ? fit : angles);
-    s.chunks = (int)(((int64_t)s.per_token * s.tokens + units - 1) / units);
-    s.token_magic = magic_of(s.per_token, units);
+    s.chunks = (int)(((int64_t)s.per_token * s.tokens + kThreads - 1) / kThreads);
+    s.token_magic = magic_of(s.per_token, kThreads);
     s.units_magic = magic_of((uint32_t)s.units, s.per_token);
     const int64_t grid = (all + s.tokens - 1) / s.tokens * s.chunks;
     if (grid > 0x7fffffff) return (int)hipErrorInvalidConfiguration;
-    auto* kernel = is_wide ? (deep ? rotary_kernel<T, INTERLEAVED, true, 4> : rotary_kernel<T, INTERLEAVED, true, 1>)
-                           : (deep ? rotary_kernel<T, INTERLEAVED, false, 4> : rotary_kernel<T, INTERLEAVED, false, 1>);
+    auto* kernel = is_wide ? rotary_kernel<T, INTERLEAVED, true> : rotary_kernel<T, INTERLEAVED, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kThreads), 0, stream, p, s);
     return (int)hipGetLastError();
 }

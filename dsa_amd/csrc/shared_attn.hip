@@ -5,12 +5,19 @@
 // Every head of every sequence reads the same key rows in the prefix, so the
 // (token, head) pairs of the whole batch are rows of one product there: a block
 // of up to 128 such rows takes each tile of 32 key rows once from memory,
-// whatever sequences the rows belong to.  Three launches:
+// whatever sequences the rows belong to.  Two launches:
 //
-//   plan   cost of every item (kernels.h: SharedParams) from the lengths, summed
-//   main   the tiles of all items, cut evenly over the workgroups: one pass over
-//          a piece's keys with the sum of the softmax
+//   main   the tiles of all items (kernels.h: SharedParams), cut by cost evenly
+//          over the workgroups, one a CU: one pass over a piece's keys with the sum
+//          of the softmax
 //   merge  rows of cut items joined (FP32), rows without keys filled in
+//
+// With 128 heads bound by the matrix cores (52 % of cycles busy, 1.16 to 1.2
+// PFLOP/s over 4 prompts of 512 tokens behind 8192 rows: 2.1 us a tile of 128 rows,
+// 1.6 at the rate of a large matrix product), with 16 rows of their own by HBM
+// (6.4 TB/s), and for a decode step by what surrounds a piece's tiles: 4 us until
+// its share is found, 5 to 7 until its first tile and Q are there, 2 to 6 for its
+// rows, 4 to 16 for the merge.
 //
 // Tiles are laid out and swizzled in LDS as in the sparse kernels (mla_tiles.h).
 #include <hip/hip_runtime.h>
