@@ -688,8 +688,8 @@ def _fast_cache():
         return _fast_cache_state[0]
     with _fast_lock:
         if not _fast_cache_state:
-            _fast_cache_state.append(_load_fast("_fast_cache", ("dsa_extend_block_table", "dsa_rotary",
-                                                                "dsa_write_kv_rows")))
+            _fast_cache_state.append(_load_fast("_fast_cache", ("dsa_extend_block_table", "dsa_rotary", "dsa_write_kv_rows",
+                                                                "dsa_fwd_shared_ws_bytes", "dsa_fwd_shared")))
     return _fast_cache_state[0]
 
 

@@ -1,9 +1,9 @@
-// Host fast path of dsa_amd.extend_block_table, rotary and write_kv_rows (no
-// reference counterpart: the reference takes its cache as given,
-// dsa/api.py:30-33).
+// Host fast path of dsa_amd.extend_block_table, rotary, write_kv_rows and
+// forward_shared (no reference counterpart: the reference takes its cache as
+// given, dsa/api.py:30-33).
 //
-// A decode step's kernels take 3 to 4 us, their checks, output and launch in
-// Python 9 to 10.  Here the same work takes 2 to 4.  Nothing is raised for a bad
+// A decode step's kernels take 3 to 4 us (forward_shared's 20), their checks,
+// output and launch in Python 9 to 10 (15).  Here the same work takes 3 to 6.  Nothing is raised for a bad
 // input: whatever the Python path would reject, and what it does besides (a
 // gradient to record, nothing to do), returns None, and the caller goes on in
 // Python.  A failed launch returns the library's status code.  Nothing is
@@ -26,6 +26,8 @@ namespace {
 decltype(&dsa_extend_block_table) g_extend = nullptr;
 decltype(&dsa_rotary) g_rotary = nullptr;
 decltype(&dsa_write_kv_rows) g_write = nullptr;
+decltype(&dsa_fwd_shared_ws_bytes) g_shared_bytes = nullptr;
+decltype(&dsa_fwd_shared) g_shared = nullptr;
 
 const at::Tensor* tensor(py::handle h) { return THPVariable_Check(h.ptr()) ? &THPVariable_Unpack(h.ptr()) : nullptr; }
 
@@ -111,6 +113,7 @@ py::object extend_block_table(py::handle htable, py::handle hlengths, py::handle
                             (int)columns, (int)block, (int)free->size(0), (int)tokens,
                             c10::hip::getCurrentHIPStream(dev.index()).stream());
     if (rc != 0) return py::int_(rc);
+    at::AutoDispatchBelowADInplaceOrView plain;  // views of whole numbers: nothing to record
     return py::make_tuple(all.narrow(0, 0, tokens), all.narrow(0, tokens, tokens), all.narrow(0, 2 * tokens, B + 1),
                           all.narrow(0, 2 * tokens + B + 1, B), all.narrow(0, 2 * tokens + 2 * B + 1, 1));
 }
@@ -230,10 +233,84 @@ py::object write_kv_rows(py::handle hkv, py::handle hrope, py::handle hslots, py
     return py::int_(g_write(&a, c10::hip::getCurrentHIPStream(dev.index()).stream()));
 }
 
-void set_entry(uint64_t extend, uint64_t rotary_address, uint64_t write) {
+bool dims(const at::Tensor& t, std::initializer_list<int64_t> want) {
+    return t.sizes() == at::IntArrayRef(want.begin(), want.size());
+}
+
+py::object forward_shared(py::handle hq, py::handle hkv, py::handle hq_rope, py::handle hk_rope, py::handle hlengths,
+                          py::handle hprefix, py::handle hscale, py::handle htable) {
+    const at::Tensor *q = tensor(hq), *kv = tensor(hkv), *q_rope = tensor(hq_rope), *k_rope = tensor(hk_rope);
+    const at::Tensor *lengths = tensor(hlengths), *table = tensor(htable);
+    if (!q || !kv || !q_rope || !lengths || (!k_rope && !hk_rope.is_none()) || (!table && !htable.is_none()) ||
+        q->dim() != 4 || kv->dim() != 4)
+        return py::none();
+    const bool fp8 = kv->scalar_type() == at::kByte;
+    const auto bf16 = at::kBFloat16;
+    const int64_t B = q->size(0), SQ = q->size(1), H = q->size(2);
+    int64_t n = B, rows = kv->size(1), L = rows, prefix;  // kv [n, rows, 1, ..]
+    dsa_shared_args a{};
+    const c10::Device dev = q->device();
+    if (!dev.is_cuda()) return py::none();
+    if (table) {
+        if (table->dim() != 2 || table->size(0) != B || table->scalar_type() != at::kInt || table->device() != dev ||
+            !table->is_contiguous())
+            return py::none();
+        n = kv->size(0);
+        if (n <= 0 || rows <= 0 || n > 1 << 25 || rows > 1 << 25 || table->size(1) > 1 << 25) return py::none();
+        L = table->size(1) * rows;
+        a.block_table = static_cast<const int32_t*>(table->data_ptr());
+        a.block_size = (int32_t)rows;
+        a.max_blocks = (int32_t)table->size(1);
+        a.num_blocks = (int32_t)n;
+    }
+    if (fp8 != !k_rope || B <= 0 || SQ <= 0 || H <= 0 || L <= 0 || L >= 1 << 25 || B > 1 << 30 || SQ > 1 << 30 ||
+        H > 1 << 30 || !dims(*q, {B, SQ, H, 512}) || !dims(*q_rope, {B, SQ, H, 64}) || !dims(*lengths, {B, SQ}) ||
+        !dims(*kv, {n, rows, 1, fp8 ? 656 : 512}) || (!fp8 && !dims(*k_rope, {n, rows, 1, 64})) ||
+        q->scalar_type() != bf16 || q_rope->scalar_type() != bf16 || lengths->scalar_type() != at::kInt ||
+        (!fp8 && (kv->scalar_type() != bf16 || k_rope->scalar_type() != bf16)) || !integer(hprefix, 0, L, prefix))
+        return py::none();
+    for (const at::Tensor* t : {q, kv, q_rope, lengths, fp8 ? q : k_rope})
+        if (t->device() != dev || !t->is_contiguous()) return py::none();
+    if (!hscale.is_none()) {
+        if (!PyFloat_CheckExact(hscale.ptr())) return py::none();
+        a.scale = (float)PyFloat_AS_DOUBLE(hscale.ptr());
+        if (!(a.scale > 0.f) || !std::isfinite(a.scale)) return py::none();
+    }
+    a.B = (int32_t)B;
+    a.SQ = (int32_t)SQ;
+    a.H = (int32_t)H;
+    a.L = (int32_t)L;
+    a.prefix = (int32_t)prefix;
+    a.kv_format = fp8 ? 1 : 0;
+    a.q = static_cast<const uint16_t*>(q->data_ptr());
+    a.kv = kv->data_ptr();
+    a.q_rope = static_cast<const uint16_t*>(q_rope->data_ptr());
+    a.k_rope = fp8 ? nullptr : static_cast<const uint16_t*>(k_rope->data_ptr());
+    a.lengths = static_cast<const int32_t*>(lengths->data_ptr());
+    for (const void* p : {(const void*)a.q, a.kv, (const void*)a.q_rope, (const void*)a.k_rope})
+        if (!aligned(p, 16)) return py::none();
+    c10::DeviceGuard guard(dev);
+    a.workspace_bytes = g_shared_bytes(&a);
+    if (a.workspace_bytes < 0) return py::none();
+    const auto options = q->options().requires_grad(false);
+    at::Tensor out = at::empty(q->sizes(), options);
+    at::Tensor top = at::empty({B, 1, SQ, H}, options.dtype(at::kFloat)), sum = at::empty_like(top);
+    at::Tensor workspace = at::empty({a.workspace_bytes}, options.dtype(at::kByte));
+    a.out = static_cast<uint16_t*>(out.data_ptr());
+    a.out_max = static_cast<float*>(top.data_ptr());
+    a.out_sum = static_cast<float*>(sum.data_ptr());
+    a.workspace = workspace.data_ptr();
+    const int rc = g_shared(&a, c10::hip::getCurrentHIPStream(dev.index()).stream());
+    if (rc != 0) return py::int_(rc);
+    return py::make_tuple(out, top, sum);
+}
+
+void set_entry(uint64_t extend, uint64_t rotary_address, uint64_t write, uint64_t shared_bytes, uint64_t shared) {
     g_extend = reinterpret_cast<decltype(g_extend)>(extend);
     g_rotary = reinterpret_cast<decltype(g_rotary)>(rotary_address);
     g_write = reinterpret_cast<decltype(g_write)>(write);
+    g_shared_bytes = reinterpret_cast<decltype(g_shared_bytes)>(shared_bytes);
+    g_shared = reinterpret_cast<decltype(g_shared)>(shared);
 }
 
 }  // namespace
@@ -242,5 +319,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("extend_block_table", &extend_block_table, "dsa_amd.extend_block_table, or None");
     m.def("rotary", &rotary, "dsa_amd.rotary, or None");
     m.def("write_kv_rows", &write_kv_rows, "dsa_amd.write_kv_rows (0), or None");
-    m.def("set_entry", &set_entry, "addresses of the library's three entry points");
+    m.def("forward_shared", &forward_shared, "dsa_amd.forward_shared, or None");
+    m.def("set_entry", &set_entry, "addresses of the library's entry points");
 }

@@ -1032,10 +1032,10 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
 // ------------------------------------------------------------------ merge
 // Rows of cut items joined, and rows without keys filled in; rows of whole items
 // are there already.  A workgroup owns 2 * turns rows of an item (stacked: of all
-// rows), two at a time; thread t of a row's 128 owns columns 4 t .. 4 t + 3.  Eight
+// rows), two at a time; thread t of a row's 128 owns columns 4 t .. 4 t + 3.  Six
 // pieces are read at a time.  Where rows are few (SPLIT), a workgroup owns one, and
-// four groups of 128 threads take its pieces, eight at a time, in turn.
-constexpr int kMergeBatch = 8, kMergeSplit = 4, kMergeFewRows = 2048;
+// four groups of 128 threads take its pieces, six at a time, in turn.
+constexpr int kMergeBatch = 6, kMergeSplit = 4, kMergeFewRows = 2048;
 template <bool STACKED, bool SPLIT>
 __global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_kernel(SharedParams, int turns) {
     constexpr int ROWS = SPLIT ? 1 : 2, GROUPS = SPLIT ? kMergeSplit : 1;
@@ -1058,7 +1058,7 @@ __global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_
         count = min(ROWS * turns, it.row0 + it.rows - first);
     }
     for (int r = half; r < count; r += ROWS) {
-        const int row = first + r, b = row / seq_rows, in_seq = row - b * seq_rows;
+        const int row = __builtin_amdgcn_readfirstlane(first + r), b = row / seq_rows, in_seq = row - b * seq_rows;
         float m = -FLT_MAX, l = 0.f;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
         auto join = [&](float top_of, float sum, const f32x4& u) __attribute__((always_inline)) {
@@ -1069,14 +1069,19 @@ __global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_
         };
         // its pieces: of the stacked item first, then of the sequence's own
         const int own = p->prefix_items + b * p->seq_blocks + in_seq / kSharedRows, shared = row / kSharedRows;
-        const int2 e1 = p->ends[own], e0 = STACKED ? p->ends[shared] : int2{0, -1};
+        int2 e1 = p->ends[own], e0 = STACKED ? p->ends[shared] : int2{0, -1};
+        e1.x = __builtin_amdgcn_readfirstlane(e1.x);
+        e1.y = __builtin_amdgcn_readfirstlane(e1.y);
+        e0.x = __builtin_amdgcn_readfirstlane(e0.x);
+        e0.y = __builtin_amdgcn_readfirstlane(e0.y);
         const int n0 = e0.y - e0.x + 1, n = n0 + (e1.y - e1.x + 1);
-        for (int j0 = group * kMergeBatch; j0 < n; j0 += GROUPS * kMergeBatch) {
+        for (int j0 = __builtin_amdgcn_readfirstlane(group) * kMergeBatch; j0 < n; j0 += GROUPS * kMergeBatch) {
             float ms[kMergeBatch], ls[kMergeBatch];
             f32x4 u[kMergeBatch];
 #pragma unroll
             for (int k = 0; k < kMergeBatch; ++k) {
-                const int j = min(j0 + k, n - 1);
+                const int j = j0 + k;
+                if (j >= n) break;
                 const int64_t prow = j < n0 ? piece_row(p, shared, e0.x + j, j == 0) + row % kSharedRows
                                             : piece_row(p, own, e1.x + (j - n0), j == n0) + in_seq % kSharedRows;
                 ms[k] = p->part_m[prow];

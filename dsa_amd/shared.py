@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .api import FP8_ROW, HEAD_DIM, ROPE_DIM, _check_scale, _device_cus, _on_device
+from .api import FP8_ROW, HEAD_DIM, ROPE_DIM, _check_scale, _device_cus, _fast_cache, _on_device
 
 
 def _check(q, kv, q_rope, k_rope, lengths, prefix, block_table):
@@ -80,6 +80,13 @@ def forward_shared(q, kv, q_rope, k_rope, lengths, prefix=0, *, scale=None, bloc
     Outputs are fresh tensors, which record no gradient (as
     :func:`dsa_amd.forward`'s), the workspace is the caching allocator's, and
     nothing synchronises."""
+    fast = _fast_cache()
+    if fast is not None:  # checked, allocated and launched in C++ (None: not taken)
+        taken = fast.forward_shared(q, kv, q_rope, k_rope, lengths, prefix, scale, block_table)
+        if taken is not None:
+            if type(taken) is int:
+                _lib.check(taken, "dsa_fwd_shared")
+            return taken
     scale = _check_scale(scale)
     batch, queries, heads, length, device, fp8 = _check(q, kv, q_rope, k_rope, lengths, prefix, block_table)
     args = _lib.DsaSharedArgs()

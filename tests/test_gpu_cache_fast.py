@@ -43,6 +43,17 @@ def write_args(fp8=False, turned=True):
     return [kv[:, :512], kv[:, 512:], i32(3, -1, 11, 12, 0), *cache, *where, False, 1.0, True]
 
 
+def shared_args(layout="paged"):
+    bf = lambda *shape: torch.randn(shape, generator=torch.Generator().manual_seed(len(shape))).bfloat16().cuda()  # noqa: E731
+    q, kv, qr, kr = bf(2, 3, 16, 512), bf(6, 16, 1, 512), bf(2, 3, 16, 64), bf(6, 16, 1, 64)
+    lengths, table = i32(40, 41, 42, 7, 8, 9).view(2, 3), i32(0, 1, 2, 0, 4, 5).view(2, 3)
+    if layout == "rows":
+        return [q, kv.view(2, 48, 1, 512), qr, kr.view(2, 48, 1, 64), lengths, 0, None, None]
+    if layout == "fp8":
+        return [q, dsa_amd.quantize_kv_fp8(kv, kr), qr, None, lengths, 16, 0.05, table]
+    return [q, kv, qr, kr, lengths, 16, 192 ** -0.5, table]
+
+
 def test_taken_and_equal(fast, monkeypatch):
     module = sys.modules["dsa_amd.rotary"]
     for args in (rotary_args(), rotary_args(4), rotary_args(4, out=True)):
@@ -71,7 +82,22 @@ def test_taken_and_equal(fast, monkeypatch):
         assert torch.equal(args[3], again[3]) and (args[4] is None or torch.equal(args[4], again[4]))
 
 
+@pytest.mark.parametrize("layout", ["rows", "paged", "fp8"])
+def test_attention_taken_and_equal(fast, monkeypatch, layout):
+    args = shared_args(layout)
+    taken = fast.forward_shared(*args)
+    assert taken is not None
+    monkeypatch.setattr(sys.modules["dsa_amd.shared"], "_fast_cache", lambda: None)
+    for a, b in zip(taken, dsa_amd.forward_shared(*args[:6], scale=args[6], block_table=args[7])):
+        assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b)
+
+
 @pytest.mark.parametrize("call, make, bad", [
+    ("forward_shared", shared_args, {
+        0: [None, "cpu", "float", "short", "last", "empty", "unaligned"], 1: [None, "cpu", "float", "bytes", "unaligned"],
+        2: [None, "cpu", "float", "short", "last", "unaligned"], 3: [None, "cpu", "float", "short", "unaligned"],
+        4: [None, "cpu", "long", "short", "last"], 5: [-1, 49, 1.0, True, None], 6: [0.0, -1.0, float("nan"), float("inf"), 1, "x"],
+        7: [3, "cpu", "long", "short", "last"]}),
     ("extend_block_table", table_args, {
         0: [None, torch.zeros(12).int(), "cpu", "long", "apart", torch.zeros(4, 0).int()], 1: ["cpu", "long", "short"],
         2: ["cpu", "long", "short"], 3: ["cpu", "long", "apart"], 4: [0, -1, 2 ** 31, 4.0, True, None],
@@ -90,6 +116,7 @@ def test_declines(fast, call, make, bad):
     how = {"cpu": lambda t: t.cpu(), "long": lambda t: t.long(), "float": lambda t: t.float(), "short": lambda t: t[:-1],
            "apart": lambda t: torch.stack([t, t], -1)[..., 0], "last": lambda t: t.transpose(-1, -2),
            "grad": lambda t: t.clone().requires_grad_(), "empty": lambda t: t[:0], "bytes": lambda t: t.byte(),
+           "unaligned": lambda t: torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape),
            "odd": lambda t: torch.zeros(5, 577).bfloat16().cuda()[:, :512]}
     for at, values in bad.items():
         for value in values:
@@ -97,7 +124,7 @@ def test_declines(fast, call, make, bad):
             if isinstance(value, str) and value == "over":
                 args[7] = torch.zeros(args[0].numel() + 8).bfloat16().cuda()
                 args[0], args[7] = args[7][:-8].view(make()[0].shape), args[7][8:].view(make()[0].shape)
-            elif isinstance(value, str):
+            elif isinstance(value, str) and value in how:
                 args[at] = how[value](args[at] if args[at] is not None else torch.empty_like(args[0]))
             else:
                 args[at] = value
