@@ -622,14 +622,19 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
     };
 
     // fp8, every wave once a tile: its rows of tile u (issued two tiles ago) into
-    // the ring, and the gathers of tile u + 2 into their place.
-    auto advance = [&](int u) __attribute__((always_inline)) {
+    // the ring, and the gathers of tile u + 2, made ready before, into their place:
+    // every value read from there has been converted and stored by then.
+    auto expand = [&](int u) __attribute__((always_inline)) {
         if constexpr (FP8) {
             wait_vmcnt<G::LOADS>();
             if (u < nt) expand_rows(lds, u, wave, lane);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // raw is read before it is written again
-            gather.prepare(p, c, u + 2, bad, wave);
             gather.issue(p, lds, wave, lane);
+        }
+    };
+    auto advance = [&](int u) __attribute__((always_inline)) {
+        if constexpr (FP8) {
+            gather.prepare(p, c, u + 2, bad, wave);
+            expand(u);
             gather.fetch(p, c, u + 3, wave);
         }
     };
@@ -743,15 +748,14 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                     if constexpr (!FP8) wait_vmcnt<G::LOADS>();
                 }
                 turn_to(t + 1, [&]() __attribute__((always_inline)) {
-                    if constexpr (!FP8) {
-                        gather.prepare(p, c, t + 3, bad, wave);
-                        gather.fetch(p, c, t + 4, wave);
-                    }
+                    const int next = FP8 ? t + 3 + grp : t + 3;
+                    gather.prepare(p, c, next, bad, wave);
+                    gather.fetch(p, c, next + 1, wave);
                 });
                 lds_barrier();
                 if (grp == 0 && __builtin_expect(clears, 0)) lds_barrier();
                 pv(t, clears);
-                advance(t + 1 + grp);  // fp8: behind PV, when the other group's QK has left the LDS
+                expand(t + 1 + grp);  // fp8: behind PV, when the other group's QK has left the LDS
                 if constexpr (!FP8)
                     if (grp == 0) wait_vmcnt<2 * G::LOADS>();
                 lds_barrier();
