@@ -91,12 +91,12 @@ __device__ __forceinline__ void item_tiles(ArgsPtr p, int i, int most, Item& it)
 // once the start and end of a piece (Q, the first tile's latency, the stores).
 // Measured on 64 to 256 sequences of their own rows, paged: up to 32 rows 1.5 us
 // a tile of bf16 rows (HBM, 6.4 TB/s) and 1.4 of fp8, up to 64 2.0 and 1.65,
-// up to 128 2.1 and 2.7; a piece 8.5, 10.5 and 12 us beside its tiles.
+// up to 128 2.1 and 2.6; a piece 8.5, 10.5 and 12 us beside its tiles.
 struct Cost {
     int tile, piece;
 };
 __device__ __forceinline__ Cost cost_of(int rows, int fp8) {
-    if (rows > 64) return Cost{fp8 ? 27 : 21, 120};
+    if (rows > 64) return Cost{fp8 ? 26 : 21, 120};
     if (rows > 32) return Cost{fp8 ? 16 : 20, 105};
     return Cost{fp8 ? 14 : 15, 85};
 }
@@ -379,18 +379,26 @@ struct Gathers {
 // of the rotary part of row l / 8.  kv[d] = bf16(fp32(e4m3) * scale), both
 // roundings to nearest even; where all scales are powers of two (2^-100 ..
 // 2^100), one conversion a pair gives the same bits.
-__device__ __forceinline__ void expand_rows(uint32_t lds, int u, int wave, int lane) {
+struct RawRows {
+    u32x2 v[4];
+    float sc[4];
+    __device__ __forceinline__ void read(uint32_t lds, int u, int wave, int lane) {
+        asm volatile("" : "+v"(lane));
+        const uint32_t raw = PPLds<true>::raw(lds, u) + 4 * wave * kFp8Row;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            v[r] = lds_load<u32x2>(raw + r * kFp8Row + 8 * lane);
+            sc[r] = lds_load<float>(raw + r * kFp8Row + kFp8ScaleOff + 4 * (lane >> 4));
+        }
+    }
+};
+__device__ __forceinline__ void expand_rows(const RawRows& rows, uint32_t lds, int u, int wave, int lane) {
     using X = PPLds<true>;
     asm volatile("" : "+v"(lane));
     const uint32_t raw = X::raw(lds, u) + 4 * wave * kFp8Row;
     const uint32_t stage = X::stage(lds, u);
-    float sc[4];
-    u32x2 v[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        v[r] = lds_load<u32x2>(raw + r * kFp8Row + 8 * lane);
-        sc[r] = lds_load<float>(raw + r * kFp8Row + kFp8ScaleOff + 4 * (lane >> 4));
-    }
+    const float(&sc)[4] = rows.sc;
+    const u32x2(&v)[4] = rows.v;
     const int in4 = (lane >> 3) & 3, rope = 4 * wave + in4;
     const i32x4 turned = lds_load<i32x4>(raw + in4 * kFp8Row + kFp8RopeOff + 16 * (lane & 7));
     const uint32_t s0 = __float_as_uint(sc[0]), s1 = __float_as_uint(sc[1]), s2 = __float_as_uint(sc[2]);
@@ -592,6 +600,26 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         return key_mask(tile_at(p, c, u), c.seen_low, valid) != 0xffffffffu;
     };
 
+    // fp8, every wave once a tile: its rows of tile u (issued two tiles ago) into
+    // the ring, and the gathers of tile u + 2, made ready before, into their place:
+    // every value read from there has been converted and stored by then.
+    auto expand = [&](int u) __attribute__((always_inline)) {
+        if constexpr (FP8) {
+            wait_vmcnt<G::LOADS>();
+            RawRows landed;
+            landed.read(lds, u, wave, lane);  // of a tile behind the piece: not used
+            if (u < nt) expand_rows(landed, lds, u, wave, lane);
+            gather.issue(p, lds, wave, lane);
+        }
+    };
+    auto advance = [&](int u) __attribute__((always_inline)) {
+        if constexpr (FP8) {
+            gather.prepare(p, c, u + 2, bad, wave);
+            expand(u);
+            gather.fetch(p, c, u + 3, wave);
+        }
+    };
+
     auto pv = [&](int u, bool clears) __attribute__((always_inline)) {
         const uint32_t stage = X::stage(lds, u);
         asm volatile("" : "+v"(off_kv), "+v"(off_p));
@@ -618,24 +646,6 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                 oacc[hb][cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[cb % VD], pf[hb], oacc[hb][cb], 0, 0, 0);
             if (cb + VD < 8) vf[cb % VD] = vfrag(cb + VD);
             __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-
-    // fp8, every wave once a tile: its rows of tile u (issued two tiles ago) into
-    // the ring, and the gathers of tile u + 2, made ready before, into their place:
-    // every value read from there has been converted and stored by then.
-    auto expand = [&](int u) __attribute__((always_inline)) {
-        if constexpr (FP8) {
-            wait_vmcnt<G::LOADS>();
-            if (u < nt) expand_rows(lds, u, wave, lane);
-            gather.issue(p, lds, wave, lane);
-        }
-    };
-    auto advance = [&](int u) __attribute__((always_inline)) {
-        if constexpr (FP8) {
-            gather.prepare(p, c, u + 2, bad, wave);
-            expand(u);
-            gather.fetch(p, c, u + 3, wave);
         }
     };
 
