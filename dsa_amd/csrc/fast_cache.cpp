@@ -69,6 +69,11 @@ bool positions_ok(const at::Tensor* t, c10::Device dev) {
 
 bool aligned(const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+// Autograd is told of a tensor that a call writes in place.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // No two elements share memory: each dimension steps over the ones inside it.
 bool distinct(const at::Tensor& t) {
     std::array<std::pair<int64_t, int64_t>, 4> steps;
@@ -113,6 +118,7 @@ py::object extend_block_table(py::handle htable, py::handle hlengths, py::handle
                             (int)columns, (int)block, (int)free->size(0), (int)tokens,
                             c10::hip::getCurrentHIPStream(dev.index()).stream());
     if (rc != 0) return py::int_(rc);
+    written(*table);
     at::AutoDispatchBelowADInplaceOrView plain;  // views of whole numbers: nothing to record
     return py::make_tuple(all.narrow(0, 0, tokens), all.narrow(0, tokens, tokens), all.narrow(0, 2 * tokens, B + 1),
                           all.narrow(0, 2 * tokens + B + 1, B), all.narrow(0, 2 * tokens + 2 * B + 1, 1));
@@ -172,6 +178,7 @@ py::object rotary(py::handle hx, py::handle hpositions, py::handle hfrequencies,
     a.transposed = transposed;
     const int rc = g_rotary(&a, c10::hip::getCurrentHIPStream(dev.index()).stream());
     if (rc != 0) return py::int_(rc);
+    if (!fresh.defined()) written(*out);
     return fresh.defined() ? py::cast(fresh) : py::reinterpret_borrow<py::object>(hout);
 }
 
@@ -204,6 +211,7 @@ py::object write_kv_rows(py::handle hkv, py::handle hrope, py::handle hslots, py
             !rope_cache->is_contiguous() || rope_cache->dim() != n || rope_cache->size(n - 1) != 64 ||
             rope_cache->sizes().slice(0, n - 1) != cache->sizes().slice(0, n - 1))
             return py::none();
+        if (at::GradMode::is_enabled() && (cache->requires_grad() || rope_cache->requires_grad())) return py::none();
         a.rope_cache = static_cast<uint16_t*>(rope_cache->data_ptr());
     }
     if (frequencies) {
@@ -230,7 +238,12 @@ py::object write_kv_rows(py::handle hkv, py::handle hrope, py::handle hslots, py
     a.kv_format = fp8 ? 1 : 0;
     a.pow2_scales = pow2;
     a.interleaved = interleaved;
-    return py::int_(g_write(&a, c10::hip::getCurrentHIPStream(dev.index()).stream()));
+    const int rc = g_write(&a, c10::hip::getCurrentHIPStream(dev.index()).stream());
+    if (rc == 0) {
+        written(*cache);
+        if (rope_cache) written(*rope_cache);
+    }
+    return py::int_(rc);
 }
 
 bool dims(const at::Tensor& t, std::initializer_list<int64_t> want) {

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from .api import FP8_ROW, HEAD_DIM, ROPE_DIM, _fast_cache, _on_device
-from .rotary import check_frequencies, check_magnitude, check_positions
+from .rotary import check_frequencies, check_magnitude, check_positions, written
 
 MAX_SEQUENCES = 4096
 
@@ -87,6 +87,7 @@ def extend_block_table(block_table, lengths, new_tokens, free_blocks, block_size
             free_blocks.numel(), max_tokens, torch._C._cuda_getCurrentRawStream(device.index))
     if rc:
         _lib.check(rc, "dsa_extend_block_table")
+    written(block_table)
     return slots, positions, starts, totals, used
 
 
@@ -106,6 +107,8 @@ def write_kv_rows(kv, k_rope, slots, kv_cache, rope_cache=None, *, positions=Non
     ``kv_cache``: a bf16 cache or pool ``[..., 512]`` with its ``rope_cache
     [..., 64]``, or an fp8 one, uint8 ``[..., 656]``, whose rows become those of
     :func:`dsa_amd.quantize_kv_fp8` (``pow2_scales`` as there).
+
+    No gradient is recorded, and the caches must not require one.
 
     ``frequencies`` (float64 ``[32]``) with ``positions`` (int32 or int64
     ``[tokens]``) turns ``k_rope`` on its way as :func:`dsa_amd.rotary` does."""
@@ -146,6 +149,8 @@ def write_kv_rows(kv, k_rope, slots, kv_cache, rope_cache=None, *, positions=Non
             or (not fp8 and rope_cache.data_ptr() % 4)):
         raise ValueError("kv needs contiguous rows, 16-byte aligned and a multiple of 8 elements apart, k_rope rows "
                          "4-byte aligned and a multiple of 2 apart; the caches must be 16- and 4-byte aligned")
+    if not fp8 and torch.is_grad_enabled() and (kv_cache.requires_grad or rope_cache.requires_grad):
+        raise ValueError("the caches are written in place and must not require a gradient")
     _int32_vector(slots, "slots", device, tokens)
     if (frequencies is None) != (positions is None):
         raise ValueError("positions and frequencies go together")
@@ -171,3 +176,6 @@ def write_kv_rows(kv, k_rope, slots, kv_cache, rope_cache=None, *, positions=Non
         rc = _lib.load().dsa_write_kv_rows(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index))
     if rc:
         _lib.check(rc, "dsa_write_kv_rows")
+    written(kv_cache)
+    if not fp8:
+        written(rope_cache)

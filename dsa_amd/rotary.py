@@ -86,6 +86,12 @@ def check_magnitude(magnitude):
         raise ValueError("magnitude must be a finite 32-bit number")
 
 
+def written(t):
+    """Tells autograd of a tensor that a call has written in place."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _span(t):
     """Addresses [first, last) that the tensor's elements lie in."""
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
@@ -170,6 +176,7 @@ def rotary(x, positions, frequencies, *, interleaved=True, start=0, transposed=F
             (x0, x1), (y0, y1) = _span(x), _span(out)
             if x0 < y1 and y0 < x1:
                 raise ValueError("out must be x itself or lie apart from it")
+        written(out)
     elif wants_grad:
         return _Rotary.apply(x, positions, frequencies, interleaved, start, transposed, magnitude)
     else:

@@ -147,3 +147,32 @@ def test_a_gradient_is_recorded_all_the_same(fast):
     assert x.grad is not None
     with torch.no_grad():
         assert torch.equal(dsa_amd.rotary(x, positions, freq), y)
+
+
+@pytest.mark.parametrize("quick", [True, False])
+def test_autograd_is_told_of_writes(fast, monkeypatch, quick):
+    """A product that saved a cache for its gradient refuses once the cache has been written."""
+    if not quick:
+        for name in ("rotary", "paging"):
+            monkeypatch.setattr(sys.modules["dsa_amd." + name], "_fast_cache", lambda: None)
+    args = write_args()
+    w = torch.ones(512, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = (args[3] * w).sum()
+    dsa_amd.write_kv_rows(*args[:5])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    for t in args[3:5]:
+        with pytest.raises(ValueError, match="gradient"):
+            dsa_amd.write_kv_rows(*args[:3], *(c.clone().requires_grad_() if c is t else c for c in args[3:5]))
+    x, positions, freq = rotary_args()[:3]
+    before = x._version
+    dsa_amd.rotary(x, positions, freq, out=x)
+    assert x._version == before + 1
+    table = table_args()
+    dsa_amd.extend_block_table(*table)
+    assert table[0]._version == 1 + i32(*range(12)).view(3, 4)._version
+    with torch.inference_mode():
+        x, positions, freq = rotary_args()[:3]
+        dsa_amd.rotary(x, positions, freq, out=x)
+        dsa_amd.write_kv_rows(*write_args()[:5])
+    dsa_amd.rotary(x, positions, freq, out=x)
