@@ -362,9 +362,9 @@ struct Gathers {
             } else {
                 const rsrc_t rs = make_rsrc(p.kv + (first << 10), (uint32_t)rows << 10);
                 gather_at<0>(dst, rs, off);
-                gather_at<1024>(dst, rs, off ^ 64u);
-                gather_at<2048>(dst, rs, off ^ 128u);
-                gather_at<3072>(dst, rs, off ^ 192u);
+                gather_at<1 * 1024>(dst, rs, off ^ 64u);
+                gather_at<2 * 1024>(dst, rs, off ^ 128u);
+                gather_at<3 * 1024>(dst, rs, off ^ 192u);
                 const int in4 = lane >> 3;
                 if (lane < 32)
                     gather_at<0>(rope_dst, make_rsrc(p.k_rope + (first << 7), (uint32_t)rows << 7),
