@@ -203,10 +203,13 @@ __global__ __launch_bounds__(kThreads) void expand_rows_kernel(const uint8_t* __
 }
 
 // write_rows puts the new tokens' rows where a slot map says
-// (dsa_write_kv_rows), with the rotary part turned on the way.  A wave writes two
-// rows, so that all its lanes turn a pair each: lane l holds latent values 8 l ..
-// 8 l + 7 of both, and pair l % 32 of the rotary part of row l / 32.  All loads are
-// issued before the first is waited for, the rows' whatever their slots say.
+// (dsa_write_kv_rows), with the rotary part turned on the way.  A wave writes a
+// row: lane l holds latent values 8 l .. 8 l + 7, and of the rotary part
+// lane l < 32 holds pair l.  The loads are issued before the slot is looked at.
+// Bound by HBM, and in a decode step by the launch: 8191 fp8 rows 6.9 us in a
+// graph of them (2.1 TB/s), 65,536 33 us (3.6 TB/s), 33 rows 2.5 us.  Two rows a
+// wave, so that all lanes turn a pair, took 7.3, 31 and 3.0 us, and 20 us for 8191
+// bf16 rows in place of 7.1; one wave a workgroup 7.6, 39 and 2.4.
 template <bool FP8, bool POW2>
 __global__ __launch_bounds__(kThreads) void write_rows_kernel(dsa_write_args p) {
     const int lane = threadIdx.x & 63;
@@ -215,40 +218,34 @@ __global__ __launch_bounds__(kThreads) void write_rows_kernel(dsa_write_args p) 
     const int pair = lane & 31;
     const int e0 = p.interleaved ? 2 * pair : pair, e1 = p.interleaved ? e0 + 1 : pair + 32;
     const double freq = p.frequencies ? p.frequencies[pair] : 0.0;
-    for (int64_t r0 = 2 * wave; r0 < p.tokens; r0 += 2 * waves) {
-        const int64_t r1 = min(r0 + 1, p.tokens - 1);
-        const int64_t mine = lane < 32 ? r0 : r1;
-        const int slot[2] = {p.slots[r0], r1 > r0 ? p.slots[r1] : -1};  // uniform
-        const uint4 v[2] = {*reinterpret_cast<const uint4*>(p.kv + r0 * p.kv_stride + 8 * lane),
-                            *reinterpret_cast<const uint4*>(p.kv + r1 * p.kv_stride + 8 * lane)};
-        const __bf16* rope = reinterpret_cast<const __bf16*>(p.k_rope) + mine * p.rope_stride;
+    for (int64_t r = wave; r < p.tokens; r += waves) {
+        const int slot = p.slots[r];  // uniform
+        const uint4 v = *reinterpret_cast<const uint4*>(p.kv + r * p.kv_stride + 8 * lane);
+        const __bf16* rope = reinterpret_cast<const __bf16*>(p.k_rope) + r * p.rope_stride;
         __bf16 y0 = rope[e0], y1 = rope[e1];
         if (p.frequencies) {
             float a, b;
             rotary_pair((float)y0, (float)y1,
-                        rotary_turn(rotary_position(p.positions, mine, p.positions_64), freq, p.magnitude, 1.f), a, b);
+                        rotary_turn(rotary_position(p.positions, r, p.positions_64), freq, p.magnitude, 1.f), a, b);
             y0 = (__bf16)a;
             y1 = (__bf16)b;
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (slot[k] < 0 || slot[k] >= p.cache_rows) continue;
-            __bf16* turned;
-            if constexpr (FP8) {
-                uint8_t* row = static_cast<uint8_t*>(p.cache) + (int64_t)slot[k] * kRow;
-                float scale;
-                const uint2 code = encode8<POW2>(v[k], scale);
-                *reinterpret_cast<uint2*>(row + 8 * lane) = code;
-                if ((lane & 15) == 0) *reinterpret_cast<float*>(row + kScaleOff + (lane >> 2)) = scale;
-                turned = reinterpret_cast<__bf16*>(row + kRopeOff);
-            } else {
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.cache) + (int64_t)slot[k] * 512 + 8 * lane) = v[k];
-                turned = reinterpret_cast<__bf16*>(p.rope_cache) + (int64_t)slot[k] * 64;
-            }
-            if (lane >> 5 == k) {
-                turned[e0] = y0;
-                turned[e1] = y1;
-            }
+        if (slot < 0 || slot >= p.cache_rows) continue;
+        __bf16* turned;
+        if constexpr (FP8) {
+            uint8_t* row = static_cast<uint8_t*>(p.cache) + (int64_t)slot * kRow;
+            float scale;
+            const uint2 code = encode8<POW2>(v, scale);
+            *reinterpret_cast<uint2*>(row + 8 * lane) = code;
+            if ((lane & 15) == 0) *reinterpret_cast<float*>(row + kScaleOff + (lane >> 2)) = scale;
+            turned = reinterpret_cast<__bf16*>(row + kRopeOff);
+        } else {
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.cache) + (int64_t)slot * 512 + 8 * lane) = v;
+            turned = reinterpret_cast<__bf16*>(p.rope_cache) + (int64_t)slot * 64;
+        }
+        if (lane < 32) {
+            turned[e0] = y0;
+            turned[e1] = y1;
         }
     }
 }
@@ -262,7 +259,7 @@ int64_t grid_for(int64_t rows, int rows_per_wave) {
 }  // namespace
 
 int launch_write_rows(const dsa_write_args& p, hipStream_t stream) {
-    const dim3 grid((unsigned)grid_for(p.tokens, 2));
+    const dim3 grid((unsigned)grid_for(p.tokens, 1));
     auto* kernel = p.kv_format != DSA_KV_FP8 ? write_rows_kernel<false, false>
                    : p.pow2_scales           ? write_rows_kernel<true, true>
                                              : write_rows_kernel<true, false>;
