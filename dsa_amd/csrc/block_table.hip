@@ -2,7 +2,8 @@
 // (include/dsa_mi355x_cache.h: dsa_extend_block_table).  No reference
 // counterpart: the reference takes a contiguous cache (dsa/api.py:30-33).
 //
-// Bound by its launch: a step of 64 sequences moves about a kilobyte, one of
+// Bound by its launch (64 sequences 4.1 us, 48 prompts of up to 2047 tokens 4.3 in
+// a captured row of calls): a step of 64 sequences moves about a kilobyte, one of
 // 98,304 tokens 1.2 MB.  So it is one launch with no second pass: every
 // workgroup scans the sequences' token and block counts itself (at most 4096 of
 // them, kept in LDS) and then writes its share of the tokens and of the taken
@@ -19,7 +20,6 @@
 namespace dsa {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kMax = 0x7fffffff;
 
 // Sums of counts, held at 2^31 - 1 (associative, since no count is negative).
@@ -52,10 +52,12 @@ __device__ __forceinline__ int owner(const int* scan, int n, int i) {
     return low;
 }
 
+template <int kThreads>
 __global__ __launch_bounds__(kThreads) void extend_table_kernel(TableParams p) {
     extern __shared__ int smem[];
     int* tokens = smem;                // [B]: tokens of the sequences before
     int* blocks = smem + p.B;          // [B]: blocks taken by them
+    int* held = smem + 2 * p.B;        // [B]: tokens that a sequence holds
     __shared__ int wave_tokens[kThreads / 64], wave_blocks[kThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 
@@ -97,6 +99,7 @@ __global__ __launch_bounds__(kThreads) void extend_table_kernel(TableParams p) {
         const Counts c = counts_of(p, b);
         tokens[b] = bt;
         blocks[b] = bb;
+        held[b] = held_of(p, b);
         if (blockIdx.x == 0) {
             p.starts[b] = bt;
             p.totals[b] = sat_add(held_of(p, b), c.tokens);
@@ -113,15 +116,15 @@ __global__ __launch_bounds__(kThreads) void extend_table_kernel(TableParams p) {
     const int stride = gridDim.x * kThreads;
     for (int64_t k = blockIdx.x * kThreads + tid; k < total_blocks; k += stride) {
         const int b = owner(blocks, p.B, (int)k);
-        const int column = blocks_of(held_of(p, b), p.block_size) + ((int)k - blocks[b]);
+        const int column = blocks_of(held[b], p.block_size) + ((int)k - blocks[b]);
         p.block_table[(int64_t)b * p.max_blocks + column] = k < p.num_free ? p.free_blocks[k] : -1;
     }
     for (int64_t i = blockIdx.x * kThreads + tid; i < p.max_tokens; i += stride) {
         int slot = -1, position = 0;
         if (i < total_tokens) {
             const int b = owner(tokens, p.B, (int)i);
-            const int held = held_of(p, b), first = blocks_of(held, p.block_size);
-            position = sat_add(held, (int)i - tokens[b]);
+            const int first = blocks_of(held[b], p.block_size);
+            position = sat_add(held[b], (int)i - tokens[b]);
             const int column = position / p.block_size;
             int entry = -1;
             if (column < p.max_blocks) {
@@ -143,10 +146,14 @@ __global__ __launch_bounds__(kThreads) void extend_table_kernel(TableParams p) {
 }  // namespace
 
 int launch_extend_table(const TableParams& p, hipStream_t stream) {
-    // four tokens a thread, so that a large step's scans are few
-    const int64_t want = ((int64_t)p.max_tokens + 4 * kThreads - 1) / (4 * kThreads);
+    // One token a thread (four, with a quarter of the scans: 48 prompts 5.4 us for
+    // 4.3 in a captured row of calls); more threads where each has sequences to
+    // sum (2000 sequences 7.7 us with 512, 10.8 with 256; 64 4.15 and 4.06).
+    const int threads = p.B > 512 ? 512 : 256;
+    const int64_t want = ((int64_t)p.max_tokens + threads - 1) / threads;
     const int grid = want < 1 ? 1 : want < 512 ? (int)want : 512;
-    hipLaunchKernelGGL(extend_table_kernel, dim3(grid), dim3(kThreads), 2 * p.B * sizeof(int), stream, p);
+    auto* kernel = threads == 512 ? extend_table_kernel<512> : extend_table_kernel<256>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 3 * p.B * sizeof(int), stream, p);
     return (int)hipGetLastError();
 }
 
