@@ -254,3 +254,31 @@ def test_other_stream_and_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, dsa_amd.rotary(x[..., 128:], p, f))
+
+
+def test_captured_gradient():
+    """Forward and backward in one captured graph, replayed with new inputs between eager calls."""
+    freq, positions = FREQ[64].cuda(), torch.arange(9).cuda() * 31
+    x, w = make((9, 3, 96), torch.float32).requires_grad_(), make((9, 3, 96), torch.float32, seed=1)
+
+    def step(x):
+        y = dsa_amd.rotary(x, positions, freq, start=16, magnitude=1.5)
+        return y, torch.autograd.grad(y, x, w)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, dx = step(x)
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(make((9, 3, 96), torch.float32, seed=2 + k))
+            w.copy_(make((9, 3, 96), torch.float32, seed=20 + k))
+            positions.add_(1000)
+        graph.replay()
+        other = step(x.detach().clone().requires_grad_())
+        assert torch.equal(y, other[0]) and torch.equal(dx, other[1])
+        torch.cuda.synchronize()
