@@ -39,6 +39,26 @@ constexpr int kFp8Row = 656, kFp8ScaleOff = 512, kFp8RopeOff = 528;
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
+// Added to a row's sum for each tile while it has keys but no score above -inf.  Its
+// maximum counts as -FLT_MAX there, so that beside any finite score this is scaled
+// to 0.  2^20 tiles of 2^12 pieces, eight lanes a row: less than 2^-64 in all, and a
+// sum of real weights, whose greatest is 1, stays above.
+constexpr float kOnlyMinusInf = 0x1p-100f;
+
+// A row's sum and maximum (log2 units) as they are returned, and what its weighted
+// rows are to be multiplied by.  0: no key, all zeros and -inf.  Scores that are
+// all -inf, or one of +inf or NaN among them: the sum is NaN, by its formula, and
+// the maximum NaN too unless an infinity is it.
+struct Returned {
+    float max, sum, inv;
+};
+__device__ __forceinline__ Returned returned(float top, float sum) {
+    if (sum == 0.f) return Returned{-INFINITY, 0.f, 0.f};
+    if (sum <= 0x1p-64f) return Returned{-INFINITY, NAN, NAN};
+    if (sum != sum && top != INFINITY) return Returned{NAN, sum, sum};
+    return Returned{top * kLn2, sum, 1.f / sum};
+}
+
 // The kernel's arguments, read from memory here and now.  As ordinary arguments
 // the compiler holds all of them in scalar registers from the start, spills
 // those into vector registers, and these, in the loop, into memory -- where the
@@ -571,6 +591,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         m_lane = fmaxf(m_lane, top * p.scale_log2);
         if (__builtin_expect(__any(m_ref == -FLT_MAX), 0)) {  // a row's first keys: O and l are still zero
             const float m = max_xor32(max_xor16(m_lane));
+            if (mask != 0 && m == -FLT_MAX) l_run += kOnlyMinusInf;
             m_ref = m_ref == -FLT_MAX ? m : m_ref;
         }
         const bool ovf = m_lane > m_ref + kRestartLog2;
@@ -807,8 +828,9 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
     auto put_stats = [&](int hl, float top, float sum) __attribute__((always_inline)) {
         if (hl >= c.it.rows) return;
         if (whole) {
-            out->out_max[c.it.row0 + hl] = sum == 0.f ? -INFINITY : top * kLn2;
-            out->out_sum[c.it.row0 + hl] = sum;
+            const Returned r = returned(top, sum);
+            out->out_max[c.it.row0 + hl] = r.max;
+            out->out_sum[c.it.row0 + hl] = r.sum;
         } else {
             out->part_m[first_row + hl] = top;
             out->part_l[first_row + hl] = sum;
@@ -849,7 +871,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             const float top = lds_load<float>(ml + 4 * (256 + hl));
             const float to_true = fast_exp2(mr - top), sum = l * to_true;
             scale[hb] = to_true;
-            if (whole) scale[hb] *= sum == 0.f ? 0.f : 1.f / sum;
+            if (whole) scale[hb] *= returned(top, sum).inv;
             if (gw == 0 && eg == 0) put_stats(hl, top, sum);
         }
         auto stage = [&](int at) __attribute__((always_inline)) {
@@ -895,7 +917,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             const float f0 = fast_exp2(mr[0] - top), f1 = fast_exp2(mr[1] - top);
             const float sum = fmaf(l[0], f0, l[1] * f1);
             scale[hb] = grp == 0 ? f0 : f1;
-            if (whole) scale[hb] *= sum == 0.f ? 0.f : 1.f / sum;
+            if (whole) scale[hb] *= returned(top, sum).inv;
             if (wave == 0 && eg == 0) put_stats(hl, top, sum);
         }
         auto finish = [&](auto kept) __attribute__((always_inline)) {  // kept: 0 (blocks 0-3) or 4 (blocks 4-7)
@@ -1117,13 +1139,13 @@ __global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_
             if (group > 0) return;
             for (int g = 0; g < GROUPS - 1; ++g) join(stats[g].x, stats[g].y, parts[128 * g + threadIdx.x]);
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const Returned got = returned(m, l);
         bf16x4 v;
-        for (int e = 0; e < 4; ++e) v[e] = (__bf16)(acc[e] * inv);
+        for (int e = 0; e < 4; ++e) v[e] = (__bf16)(acc[e] * got.inv);
         *reinterpret_cast<bf16x4*>(p->out + (int64_t)row * 512 + col) = v;
         if (col == 0) {
-            p->out_max[row] = l == 0.f ? -INFINITY : m * kLn2;
-            p->out_sum[row] = l;
+            p->out_max[row] = got.max;
+            p->out_sum[row] = got.sum;
         }
     }
 }

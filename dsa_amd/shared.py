@@ -70,7 +70,10 @@ def forward_shared(q, kv, q_rope, k_rope, lengths, prefix=0, *, scale=None, bloc
     ``b`` sees rows ``[0, lengths[b, t])``, clamped to ``[0, L]``; a causal step
     gives each query its position plus one.  A query that sees none (padding)
     gives output 0, max -inf and sum 0.  Rows a query does not see may hold
-    anything, infinities and NaN included.
+    anything, infinities and NaN included.  In rows that it sees they do what the
+    formulas say: a score of +inf or NaN, or no score above -inf, makes its output
+    and sum NaN (max too, where a score is NaN and none +inf); beside finite scores,
+    one of -inf is a weight of 0.
 
     ``prefix``: rows ``[0, prefix)`` are read from sequence 0's cache (or through
     its block table row) for every sequence.  The caller vouches that they are
