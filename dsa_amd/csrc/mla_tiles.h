@@ -23,6 +23,10 @@ template <typename T>
 __device__ __forceinline__ void lds_store(uint32_t addr, T v) {
     *reinterpret_cast<__attribute__((address_space(3))) T*>(addr) = v;
 }
+__device__ __forceinline__ void lds_or(uint32_t addr, uint32_t v) {
+    __hip_atomic_fetch_or(reinterpret_cast<__attribute__((address_space(3))) uint32_t*>(addr), v, __ATOMIC_RELAXED,
+                          __HIP_MEMORY_SCOPE_WORKGROUP);
+}
 // ds_read_b64_tr_b16: within each 16-lane group, lane l supplies the address
 // of 4 consecutive bf16 of "row" l/4, columns 4*(l%4)..+3 of a 4x16 block;
 // lane n receives column n of that block (rows 0..3).

@@ -204,6 +204,7 @@ __device__ __forceinline__ int64_t piece_row(ArgsPtr p, int i, int w, bool head)
 // masked: their scores become -inf, their weights 0 (see clear_specials).
 constexpr int kPPThreads = 512;
 constexpr float kRestartLog2 = 64.0f;
+constexpr int kPoisonBytes = kSharedRows / 16 * 512 / 8;
 
 // Each wave brings in four rows of every tile.  bf16 rows are gathered straight
 // into a ring of four tiles; fp8 rows land as stored (656 bytes) in one of two
@@ -218,7 +219,9 @@ struct PPLds {
     static constexpr int FLAG_OFF = P_OFF + 2 * P_GROUP;  // a second pass is needed
     static constexpr int BAD_OFF = FLAG_OFF + 4;          // some block entry of the piece lies outside the pool
     static constexpr int PLAN_OFF = FLAG_OFF + 16;        // the workgroup's first item: number, begin, low, high
-    static constexpr int LDS_BYTES = PLAN_OFF + 32;
+    static constexpr int MASK_OFF = PLAN_OFF + 32;        // of either group: the keys of a tile that its four row blocks see
+    static constexpr int POISON_OFF = MASK_OFF + 32;      // columns of each row block to become NaN, and whether there is one
+    static constexpr int LDS_BYTES = POISON_OFF + kPoisonBytes + 16;
     static constexpr int ML_OFF = P_OFF;  // [3][128] floats, at the end: l, reference and maximum
     static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
     __device__ static uint32_t stage(uint32_t lds, int u) { return lds + (uint32_t)(u % NSTAGE) * STAGE_BYTES; }
@@ -482,22 +485,35 @@ __device__ __forceinline__ uint32_t lane_rows(uint32_t mask, int g) {
 
 // Infinities and NaN in a wave's 128 columns of a tile become zeros, where some
 // query row does not see all of the tile: a hidden row's weight is 0, which they
-// would turn into NaN.  A query row that does see such a value has a score, a
-// sum and so a whole result that are NaN already, as the key row that it lies in
-// is the value row too.  Both groups are past QK of the tile; the wave's own LDS
-// accesses are in order, and no other wave of its group reads these columns.
-__device__ __forceinline__ void clear_specials(uint32_t stage, int gw, int lane) {
+// would turn into NaN.  Query rows that do see one have NaN in that column (its
+// score may be -inf and so its weight 0, too): the row blocks that do, by their
+// masks of the tile's keys, are noted in LDS, a bit a column, and their columns
+// made NaN at the end.  All groups that read the columns are past QK of the tile;
+// the wave's own LDS accesses are in order, and no other wave writes these columns.
+template <int BLOCKS>
+__device__ __forceinline__ void clear_specials(uint32_t stage, uint32_t masks, uint32_t poison, int gw, int lane) {
     asm volatile("" : "+v"(lane));
     const uint32_t at = stage + (uint32_t)((lane >> 4) * 1024 + gw * 256 + (lane & 15) * 16);
 #pragma unroll 1
     for (int r = 0; r < kKeys; r += 4) {
         i32x4 v = lds_load<i32x4>(at + r * 1024);
+        uint32_t any = 0;  // an exponent of all ones carries into its sign bit
+#pragma unroll
+        for (int d = 0; d < 4; ++d) any |= ((uint32_t)v[d] & 0x7f807f80u) + 0x00800080u;
+        if (__builtin_expect((any & 0x80008000u) == 0, 1)) continue;
+        uint32_t columns = 0;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-            if ((v[d] & 0x7f80) == 0x7f80) v[d] &= 0xffff0000;
-            if ((v[d] & 0x7f800000) == 0x7f800000) v[d] &= 0xffff;
+            if ((v[d] & 0x7f80) == 0x7f80) v[d] &= 0xffff0000, columns |= 1u << (2 * d);
+            if ((v[d] & 0x7f800000) == 0x7f800000) v[d] &= 0xffff, columns |= 2u << (2 * d);
         }
         lds_store<i32x4>(at + r * 1024, v);
+        const int row = r + (lane >> 4), byte = 16 * gw + ((lane & 15) ^ sw_kv(row));  // of the 512 columns' bits
+#pragma unroll 1
+        for (int b = 0; b < BLOCKS; ++b)
+            if (lds_load<uint32_t>(masks + 4 * b) >> row & 1)
+                lds_or(poison + 64 * b + (byte & ~3), columns << (8 * (byte & 3)));
+        lds_store<int>(poison + kPoisonBytes, 1);
     }
 }
 
@@ -517,6 +533,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
     const ArgsPtr args = args_now();
     int seen = seen_by(args, row / args->H);  // in a scalar register from the first wait on
     const uint32_t p_lds = lds + X::P_OFF + grp * X::P_GROUP, bad = lds + X::BAD_OFF;
+    const uint32_t masks = lds + X::MASK_OFF + 16 * grp, poison = lds + X::POISON_OFF;
 
     bf16x8 qf[18];
     {
@@ -616,9 +633,13 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         lds_store<bf16x8>(p_lds + (off_p >> 16), pk);
     };
 
-    // Whether some query row of the block does not see all keys of tile u, the wave's last scored (every wave agrees).
+    // Whether some query row of the block does not see all keys of tile u, the wave's
+    // last scored (every wave agrees); which ones its own rows see is left for PV then.
     auto partial = [&](int u) __attribute__((always_inline)) -> bool {
-        return key_mask(tile_at(p, c, u), c.seen_low, valid) != 0xffffffffu;
+        const Tile k = tile_at(p, c, u);
+        const bool some = key_mask(k, c.seen_low, valid) != 0xffffffffu;
+        if (__builtin_expect(some, 0)) lds_store<uint32_t>(masks + 4 * gw, key_mask(k, seen, valid));
+        return some;
     };
 
     // fp8, every wave once a tile: its rows of tile u (issued two tiles ago) into
@@ -651,7 +672,10 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             const bf16x4 v1 = lds_load_tr(a + 16 * 1024);
             return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
         };
-        if (__builtin_expect(clears, 0)) clear_specials(stage, gw, lane);
+        if (__builtin_expect(clears, 0)) {
+            if constexpr (!WIDE) clear_specials<NB>(stage, masks, poison, gw, lane);
+            else if (grp == 0) clear_specials<8>(stage, masks, poison, gw, lane);  // of both groups' rows
+        }
         bf16x8 pf[NB];
 #pragma unroll
         for (int hb = 0; hb < NB; ++hb) pf[hb] = lds_load<bf16x8>(p_lds + (off_p & 0xffffu) + 1024 * hb);
@@ -684,6 +708,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         gather.fetch(p, c, 0, wave);
         behind.fetch(p, c, 1, wave);
         if (threadIdx.x == 0) lds_store<int>(bad, 0);
+        if (threadIdx.x <= kPoisonBytes / 4) lds_store<int>(poison + 4 * threadIdx.x, 0);
         lds_barrier();
         gather.prepare(p, c, 0, bad, wave);
         gather.issue(p, lds, wave, lane);
@@ -759,7 +784,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             // bf16: tile t + 3 is issued in PV of tile t, into the stage of tile
             // t - 1, which both groups are past.  A tile in which some row sees
             // less than all has one barrier more, between group 1's QK and group
-            // 0's clear_specials of it.
+            // 0's clear_specials of it; group 1 meets it cleared.
             if constexpr (!FP8)
                 if (grp == 0) gather.issue(p, lds, wave, lane);
             lds_barrier();
@@ -819,6 +844,17 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         lds_store<float>(ml + 4 * hl, l_run);
         lds_store<float>(ml + 4 * (128 + hl), m_ref);
         lds_store<float>(ml + 4 * (256 + hl), m_true);
+    }
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(lds_load<int>(poison + kPoisonBytes)), 0)) {
+#pragma unroll
+        for (int hb = 0; hb < NB; ++hb)
+#pragma unroll
+            for (int cb = 0; cb < 8; ++cb) {
+                const uint32_t word = lds_load<uint32_t>(poison + 64 * ((WIDE ? 4 * grp : 0) + hb) + 16 * gw + (cb >> 1) * 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (word >> (16 * (cb & 1) + 4 * eg + j) & 1) oacc[hb][cb][j] = NAN;
+            }
     }
     lds_barrier();
     constexpr int HROW = 1040;      // bytes of a staged bf16 row (16 more: rows spread over the banks)

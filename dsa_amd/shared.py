@@ -73,7 +73,8 @@ def forward_shared(q, kv, q_rope, k_rope, lengths, prefix=0, *, scale=None, bloc
     anything, infinities and NaN included.  In rows that it sees they do what the
     formulas say: a score of +inf or NaN, or no score above -inf, makes its output
     and sum NaN (max too, where a score is NaN and none +inf); beside finite scores,
-    one of -inf is a weight of 0.
+    one of -inf is a weight of 0, and 0 times an infinite latent value NaN in that
+    value's column.
 
     ``prefix``: rows ``[0, prefix)`` are read from sequence 0's cache (or through
     its block table row) for every sequence.  The caller vouches that they are

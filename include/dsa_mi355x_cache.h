@@ -120,8 +120,9 @@ int dsa_write_kv_rows(const dsa_write_args* args, void* stream);
  * query with no row left gives out 0, max -inf, sum 0.  Any other takes
  * infinities and NaN as the formulas do: a score of +inf or NaN, or none above
  * -inf, makes its sum and out NaN (max: NaN where a score is and none is +inf); a
- * score of -inf beside finite ones is a weight of 0.  Rows a query does not see,
- * whatever their bits, do not touch its result.
+ * score of -inf beside finite ones is a weight of 0, whose product with an
+ * infinite element of kv_j makes that column of out NaN.  Rows a query does not
+ * see, whatever their bits, do not touch its result.
  *
  *   q [B, SQ, H, 512], q_rope [B, SQ, H, 64] bf16, H a multiple of 16
  *   lengths [B, SQ] int32: rows each query sees, clamped to [0, L]

@@ -78,7 +78,8 @@ def check(s, lengths, prefix, scale=1 / 24):
                 assert not got[0].any() and (got[1] == -INF).all() and not got[2].any()
                 continue
             score = (s["both"][b, t][:, None] * rows[:n]).sum(-1) * scale
-            peak = score.amax(-1)
+            peak = score.amax(-1)  # NaN where a score is; with +inf beside it, +inf is returned
+            peak[(score == INF).any(-1)] = INF
             w = torch.exp(score - peak[:, None])
             norm = w.sum(-1)
             want = (w[:, :, None] * rows[:n, :512]).sum(1) / norm[:, None]
@@ -104,6 +105,48 @@ def steps(*ends, queries):
 
 # B, SQ, H: 16, 32, 48, 64 and 128 query rows a block; stacked ones of a prefix and a sequence's own
 SHAPES = [(1, 1, 16), (1, 2, 16), (2, 3, 16), (1, 2, 32), (3, 1, 64), (1, 8, 16), (2, 2, 64), (1, 3, 128), (5, 1, 16)]
+
+
+@pytest.mark.parametrize("layout", ["rows", "paged16", "paged7"])
+@pytest.mark.parametrize("value", [INF, -INF])
+@pytest.mark.parametrize("B, SQ, H", SHAPES)
+def test_a_seen_infinity(B, SQ, H, value, layout):
+    """One infinite element of a row: NaN in every column of the heads whose
+    product with it is +inf, and in its own column (0 times an infinity) of the
+    others, whether or not the tile that it lies in is seen whole."""
+    prefix, L = 70, 150
+    ends = [149, 131, 97, 71, 128][:B]
+    lengths = steps(*ends, queries=SQ)
+    last = int(lengths[0, -1]) - 1
+    # the first tile, the prefix's last rows and the first behind it, a whole tile, the last tile, the newest row (of the last query only)
+    for row, column in zip((3, 64, 69, 70, 75, 100, 127, 128, last - SQ, last), (0, 131, 511, 7, 64, 300, 255, 90, 128, 399)):
+        def edit(kv, kr):
+            kv[0, row, column] = value
+        check(make(B, SQ, H, L, layout, edit, seed=row), lengths, prefix)
+
+
+@pytest.mark.parametrize("layout", ["rows", "paged7"])
+@pytest.mark.parametrize("B, SQ, H", SHAPES)
+def test_seen_infinities_do_not_depend_on_other_queries(B, SQ, H, layout):
+    """A query's result is the same bits alone, whatever the rest of its block sees."""
+    def edit(kv, kr):
+        kv[:, 40, 17], kv[:, 100, 300], kv[:, 75, 5] = INF, -INF, NAN
+
+    s = make(B, SQ, H, 150, layout, edit, seed=5)
+    for others in (150, 101, 75, 41, 20, 0):
+        lengths = torch.full((B, SQ), others)
+        lengths[0, 0] = 74
+        check(s, lengths, 0)
+
+
+@pytest.mark.parametrize("layout", ["rows", "paged16"])
+@pytest.mark.parametrize("B, SQ, H", [(1, 1, 16), (2, 2, 64), (2, 3, 16)])
+def test_a_seen_infinity_in_the_rotary_part(B, SQ, H, layout):
+    """No value of the output is infinite there: a score of -inf is a weight of 0."""
+    def edit(kv, kr):
+        kr[0, 20, 3] = kr[0, 90, 40] = INF
+
+    check(make(B, SQ, H, 130, layout, edit, seed=1), steps(*[128, 111][:B], queries=SQ), 64)
 
 
 @pytest.mark.parametrize("layout", ["rows", "paged16", "paged7"])
@@ -134,3 +177,58 @@ def test_a_seen_nan(B, SQ, H, layout):
     check(make(B, SQ, H, 110, layout, lambda kv, kr: kv.fill_(NAN), seed=4), steps(*(110, 33, 64, 85, 81)[:B], queries=SQ), 0)
 
 
+@pytest.mark.parametrize("layout", ["fp8", "fp8_paged16", "fp8_paged7"])
+@pytest.mark.parametrize("B, SQ, H", SHAPES)
+def test_seen_specials_of_fp8_rows(B, SQ, H, layout):
+    """A NaN code; an infinite scale over codes that are 0 but for one; a scale that is NaN."""
+    def code(rows):
+        rows[0, 5, 300] = 0x7F
+
+    def scale(rows):
+        rows[0, 66, :512], rows[-1, 97, :512] = 0, 0
+        rows[0, 66, 130], rows[-1, 97, 131] = 0x38, 0xB8
+        for b, r, block in ((0, 66, 1), (-1, 97, 2)):
+            rows[b, r, 512 + 4 * block:516 + 4 * block].view(torch.float32).fill_(INF)
+
+    def bad_scale(rows):
+        rows[-1, 90, 512:516].view(torch.float32).fill_(NAN)
+
+    def alone(rows):  # every code of an infinite block of one sign: +inf or NaN scores but for heads of the other sign
+        rows[0, 97, 128:256] = 0x38
+        rows[0, 97, 516:520].view(torch.float32).fill_(INF)
+
+    for edit in (code, scale, bad_scale, alone):
+        s = make(B, SQ, H, 110, layout, edit, seed=6)
+        if edit is alone:  # one head of one sign there: its score is -inf, and the block's 128 columns NaN
+            for t in (s["q"], s["both"]):
+                t[0, :, 3, 128:256] = -t[0, :, 3, 128:256].abs()
+        check(s, steps(*(110, 33, 64, 98, 101)[:B], queries=SQ), 32)
+        check(s, steps(*(98, 33, 64, 110, 101)[:B], queries=SQ), 0)
+
+
+@pytest.mark.parametrize("layout", ["paged7", "fp8", "fp8_paged16", "fp8_paged7"])
+@pytest.mark.parametrize("B, SQ, H", [(4, 1, 16), (3, 4, 16), (2, 2, 64), (2, 1, 128)])
+def test_unseen_specials(B, SQ, H, layout):
+    """Codes, scales and rotary parts of every kind in rows that no query of a sequence sees."""
+    P, L = 70, 128
+    lengths = steps(*[115, 73, 70, 101][:B], queries=SQ)
+    clean = call(make(B, SQ, H, L, layout, lambda *t: None, seed=8), lengths, P)
+
+    def edit(*store):
+        g = torch.Generator().manual_seed(0)
+        for b in range(B):
+            n = max(P, int(lengths[b].max()))
+            for t in store:
+                hidden = t[b, n:]
+                if t.dtype == torch.uint8:
+                    hidden.copy_(torch.randint(0, 256, hidden.shape, generator=g, dtype=torch.uint8))
+                    hidden[::3, :512] = 0x7F
+                    hidden[1::3, 512:528].view(torch.float32).fill_(INF)
+                    hidden[2::3, 512:528].view(torch.float32).fill_(NAN)
+                else:
+                    hidden[::2], hidden[1::2] = INF, NAN
+                if b > 0:  # of the prefix only sequence 0's rows count
+                    t[b, :P] = 0xFF if t.dtype == torch.uint8 else NAN
+
+    for a, b in zip(clean, call(make(B, SQ, H, L, layout, edit, seed=8), lengths, P)):
+        assert torch.equal(a, b)
