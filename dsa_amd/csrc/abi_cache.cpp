@@ -202,7 +202,8 @@ int dsa_fwd_shared(const dsa_shared_args* a, void* stream) {
         p.block_magic = (uint32_t)((num + d - 1) / d);
     }
     p.kv_fp8 = fp8;
-    p.scale_log2 = (a->scale == 0.f ? 1.f / 24.f : a->scale) * 1.4426950408889634f;
+    p.scale = a->scale == 0.f ? 1.f / 24.f : a->scale;
+    p.scale_log2 = p.scale * 1.4426950408889634f;
     p.stacked = plan.stacked;
     p.prefix_items = plan.prefix_items;
     p.seq_blocks = plan.seq_blocks;

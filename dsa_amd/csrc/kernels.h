@@ -207,14 +207,14 @@ struct SharedParams {
     float *out_max, *out_sum;
     int2* ends;       // [items]: workgroups that compute an item's first and last tile
     float* part_o;    // [partial rows, 512] of the pieces of cut items
-    float* part_m;    // [partial rows] (log2 units)
+    float* part_m;    // [partial rows], before the scale
     float* part_l;    // [partial rows]
     int B, SQ, H, L, prefix;
     int block_size, max_blocks, num_blocks;
     uint32_t block_magic;  // key / block_size = mulhi(key, block_magic) >> block_shift for block_size > 1
     int block_shift;
     int kv_fp8;
-    float scale_log2;
+    float scale, scale_log2;
     int stacked, prefix_items, seq_blocks, items;
     int workgroups, own_rows;  // own_rows: of a piece of a sequence's own rows
 };

@@ -33,7 +33,6 @@ namespace {
 
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr float kLn2 = 0.69314718055994531f;
 constexpr int kKeys = kSharedKeys;
 constexpr int kFp8Row = 656, kFp8ScaleOff = 512, kFp8RopeOff = 528;
 
@@ -45,18 +44,18 @@ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; 
 // sum of real weights, whose greatest is 1, stays above.
 constexpr float kOnlyMinusInf = 0x1p-100f;
 
-// A row's sum and maximum (log2 units) as they are returned, and what its weighted
-// rows are to be multiplied by.  0: no key, all zeros and -inf.  Scores that are
-// all -inf, or one of +inf or NaN among them: the sum is NaN, by its formula, and
-// the maximum NaN too unless an infinity is it.
+// A row's sum and maximum as they are returned (`top`: the largest product, before
+// the scale), and what its weighted rows are to be multiplied by.  Sum 0: no key, all
+// zeros and -inf.  Scores that are all -inf, or one of +inf or NaN among them: the
+// sum is NaN, by its formula, and the maximum NaN too unless an infinity is it.
 struct Returned {
     float max, sum, inv;
 };
-__device__ __forceinline__ Returned returned(float top, float sum) {
+__device__ __forceinline__ Returned returned(float top, float sum, float scale) {
     if (sum == 0.f) return Returned{-INFINITY, 0.f, 0.f};
     if (sum <= 0x1p-64f) return Returned{-INFINITY, NAN, NAN};
     if (sum != sum && top != INFINITY) return Returned{NAN, sum, sum};
-    return Returned{top * kLn2, sum, 1.f / sum};
+    return Returned{top * scale, sum, 1.f / sum};
 }
 
 // The kernel's arguments, read from memory here and now.  As ordinary arguments
@@ -198,7 +197,9 @@ __device__ __forceinline__ int64_t piece_row(ArgsPtr p, int i, int w, bool head)
 //
 // P is formed against a reference maximum, a row's from its first tile, and a
 // piece whose scores pass it by 64 (log2 units) is computed once more against
-// the exact one, so O is never rescaled in the loop.
+// the exact one, so O is never rescaled in the loop.  The maximum is taken off
+// the products and the difference scaled: scaled first, a product of 2^31 and its
+// rounded maximum would differ by more than weights of 32 bits hold.
 //
 // A query row sees keys [0, seen) only, and rows behind a bad block entry are
 // masked: their scores become -inf, their weights 0 (see clear_specials).
@@ -546,7 +547,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
     }
 
     f32x4 oacc[NB][8];
-    // log2 units; the maximum of this lane's own scores
+    // products, not scaled yet; the maximum of this lane's own
     float m_ref = -FLT_MAX, m_lane = -FLT_MAX, l_run = 0.f;
 
     // This lane's LDS offsets in the loop, packed as in the sparse ping-pong kernel.
@@ -605,23 +606,22 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         float top = -INFINITY;
 #pragma unroll
         for (int r = 0; r < 8; ++r) top = fmaxf(top, x[r]);
-        m_lane = fmaxf(m_lane, top * p.scale_log2);
+        m_lane = fmaxf(m_lane, top);
         if (__builtin_expect(__any(m_ref == -FLT_MAX), 0)) {  // a row's first keys: O and l are still zero
             const float m = max_xor32(max_xor16(m_lane));
             if (mask != 0 && m == -FLT_MAX) l_run += kOnlyMinusInf;
             m_ref = m_ref == -FLT_MAX ? m : m_ref;
         }
-        const bool ovf = m_lane > m_ref + kRestartLog2;
+        const bool ovf = (m_lane - m_ref) * p.scale_log2 > kRestartLog2;
         overflow |= ovf;
-        const float neg_ref = -m_ref;
         float psum = 0.f;
         bf16x8 pk;
         if (__builtin_expect(__any(ovf), 0)) {  // this pass is to be discarded: the clamp keeps it free of inf
 #pragma unroll
-            for (int r = 0; r < 8; ++r) x[r] = fminf(fmaf(x[r], p.scale_log2, neg_ref), kRestartLog2);
+            for (int r = 0; r < 8; ++r) x[r] = fminf((x[r] - m_ref) * p.scale_log2, kRestartLog2);
         } else {
 #pragma unroll
-            for (int r = 0; r < 8; ++r) x[r] = fmaf(x[r], p.scale_log2, neg_ref);
+            for (int r = 0; r < 8; ++r) x[r] = (x[r] - m_ref) * p.scale_log2;
         }
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
@@ -864,7 +864,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
     auto put_stats = [&](int hl, float top, float sum) __attribute__((always_inline)) {
         if (hl >= c.it.rows) return;
         if (whole) {
-            const Returned r = returned(top, sum);
+            const Returned r = returned(top, sum, out->scale);
             out->out_max[c.it.row0 + hl] = r.max;
             out->out_sum[c.it.row0 + hl] = r.sum;
         } else {
@@ -905,9 +905,9 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
             const int hl = 64 * grp + 16 * hb + en16;
             const float l = lds_load<float>(ml + 4 * hl), mr = lds_load<float>(ml + 4 * (128 + hl));
             const float top = lds_load<float>(ml + 4 * (256 + hl));
-            const float to_true = fast_exp2(mr - top), sum = l * to_true;
+            const float to_true = fast_exp2((mr - top) * p.scale_log2), sum = l * to_true;
             scale[hb] = to_true;
-            if (whole) scale[hb] *= returned(top, sum).inv;
+            if (whole) scale[hb] *= returned(top, sum, 1.f).inv;
             if (gw == 0 && eg == 0) put_stats(hl, top, sum);
         }
         auto stage = [&](int at) __attribute__((always_inline)) {
@@ -950,10 +950,10 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
                 mt[k] = lds_load<float>(ml + 4 * (256 + 64 * k + hl));
             }
             const float top = fmaxf(mt[0], mt[1]);
-            const float f0 = fast_exp2(mr[0] - top), f1 = fast_exp2(mr[1] - top);
+            const float f0 = fast_exp2((mr[0] - top) * p.scale_log2), f1 = fast_exp2((mr[1] - top) * p.scale_log2);
             const float sum = fmaf(l[0], f0, l[1] * f1);
             scale[hb] = grp == 0 ? f0 : f1;
-            if (whole) scale[hb] *= returned(top, sum).inv;
+            if (whole) scale[hb] *= returned(top, sum, 1.f).inv;
             if (wave == 0 && eg == 0) put_stats(hl, top, sum);
         }
         auto finish = [&](auto kept) __attribute__((always_inline)) {  // kept: 0 (blocks 0-3) or 4 (blocks 4-7)
@@ -1134,7 +1134,8 @@ __global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_
         float m = -FLT_MAX, l = 0.f;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
         auto join = [&](float top_of, float sum, const f32x4& u) __attribute__((always_inline)) {
-            const float top = fmaxf(m, top_of), keep = fast_exp2(m - top), add = fast_exp2(top_of - top);
+            const float top = fmaxf(m, top_of);
+            const float keep = fast_exp2((m - top) * p->scale_log2), add = fast_exp2((top_of - top) * p->scale_log2);
             l = l * keep + sum * add;
             acc = acc * keep + u * add;
             m = top;
@@ -1175,7 +1176,7 @@ __global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_
             if (group > 0) return;
             for (int g = 0; g < GROUPS - 1; ++g) join(stats[g].x, stats[g].y, parts[128 * g + threadIdx.x]);
         }
-        const Returned got = returned(m, l);
+        const Returned got = returned(m, l, p->scale);
         bf16x4 v;
         for (int e = 0; e < 4; ++e) v[e] = (__bf16)(acc[e] * got.inv);
         *reinterpret_cast<bf16x4*>(p->out + (int64_t)row * 512 + col) = v;

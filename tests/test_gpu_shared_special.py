@@ -232,3 +232,32 @@ def test_unseen_specials(B, SQ, H, layout):
 
     for a, b in zip(clean, call(make(B, SQ, H, L, layout, edit, seed=8), lengths, P)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("layout", ["rows", "paged16", "paged7"])
+@pytest.mark.parametrize("rows_a_block", [16, 32, 64, 128])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_huge_scores(sign, rows_a_block, layout):
+    """Scores up to 2^37, exact in 32 bits (one product each, scale 1), more than
+    200 apart: all the weight is the largest one's.  The output is its row, the sum
+    1 and max the score itself, all exact."""
+    L, keys = 140, 131
+
+    def edit(kv, kr):
+        kv.mul_(2.0 ** 30)
+        # distinct bf16 values, 128 in each power of two
+        order = torch.randperm(L, generator=torch.Generator().manual_seed(2))[:kv.shape[1]].double()
+        order = torch.cat([order, torch.zeros(kv.shape[1] - order.numel(), dtype=torch.float64)])
+        kv[0, :, 0] = (sign * 2.0 ** (36 + order // 128) * (1 + order % 128 / 128)).bfloat16()
+
+    s = make(1, rows_a_block // 16, 16, L, layout, edit, seed=9)
+    s["q"].zero_(), s["q_rope"].zero_()
+    s["q"][..., 0] = 1
+    lengths = torch.full((1, rows_a_block // 16), keys)
+    out, top, total = call(s, lengths, 0, scale=1.0)
+    score = s["rows"][0, :keys, 0].cpu()
+    best = int(score.argmax())
+    assert (score == score[best]).sum() == 1
+    assert torch.equal(out.double(), s["rows"][0, best, :512].expand(out.shape))
+    assert (total == 1).all()
+    assert (top.cpu().double() == score[best]).all()
