@@ -74,6 +74,9 @@ void written(const at::Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// Whether it carries a forward-mode derivative, or is one of a function transform's stand-ins (they hold no memory).
+bool differentiated(const at::Tensor& t) { return t._fw_grad(0).defined() || !t.has_storage(); }
+
 // No two elements share memory: each dimension steps over the ones inside it.
 bool distinct(const at::Tensor& t) {
     std::array<std::pair<int64_t, int64_t>, 4> steps;
@@ -143,6 +146,8 @@ py::object rotary(py::handle hx, py::handle hpositions, py::handle hfrequencies,
         !integer(hstart, 0, width - 2 * frequencies->size(0), start) || x->stride(n - 1) != 1)
         return py::none();
     if (at::GradMode::is_enabled() && (x->requires_grad() || (out && out->requires_grad()))) return py::none();
+    if (differentiated(*x) || (out && differentiated(*out)) || !positions->has_storage() || !frequencies->has_storage())
+        return py::none();
     if (out) {
         if (out->sizes() != x->sizes() || out->scalar_type() != type || out->device() != dev || out->stride(n - 1) != 1 ||
             !distinct(*out))

@@ -108,19 +108,34 @@ def _elements_distinct(t):
     return True
 
 
+def has_tangent(t):
+    """Whether the tensor carries a forward-mode derivative."""
+    return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
 class _Rotary(torch.autograd.Function):
+    """Linear in x: the tangent takes the same turn, the gradient the opposite one."""
+
     @staticmethod
     def forward(ctx, x, positions, frequencies, interleaved, start, transposed, magnitude):
         ctx.save_for_backward(positions, frequencies)
-        ctx.how = (interleaved, start, not transposed, magnitude)
+        ctx.save_for_forward(positions, frequencies)
+        ctx.how = (interleaved, start, transposed, magnitude)
         return _launch(x, positions, frequencies, interleaved, start, transposed, magnitude,
                        torch.empty(x.shape, device=x.device, dtype=x.dtype))
 
     @staticmethod
+    def _turned(ctx, t, back):
+        return rotary(t if t.stride(-1) == 1 else t.contiguous(), *ctx.saved_tensors, interleaved=ctx.how[0],
+                      start=ctx.how[1], transposed=bool(ctx.how[2]) != back, magnitude=ctx.how[3])
+
+    @staticmethod
     def backward(ctx, grad):
-        grad = grad if grad.stride(-1) == 1 else grad.contiguous()
-        return (rotary(grad, *ctx.saved_tensors, interleaved=ctx.how[0], start=ctx.how[1], transposed=ctx.how[2],
-                       magnitude=ctx.how[3]), None, None, None, None, None, None)
+        return _Rotary._turned(ctx, grad, True), None, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        return _Rotary._turned(ctx, tangent, False)
 
 
 def rotary(x, positions, frequencies, *, interleaved=True, start=0, transposed=False, magnitude=1.0, out=None):
@@ -140,8 +155,8 @@ def rotary(x, positions, frequencies, *, interleaved=True, start=0, transposed=F
 
     ``out``: where the result goes (``x`` itself: in place, the rest of each head
     untouched), else a new contiguous tensor.  ``transposed`` turns the other
-    way, which is the gradient for ``x``; where ``x`` requires a gradient the
-    call records that itself (not with ``out``)."""
+    way, which is the gradient for ``x``; where ``x`` requires a gradient or
+    carries a forward-mode tangent the call records that itself (not with ``out``)."""
     fast = _fast_cache()
     if fast is not None:  # checked and launched in C++ (None: not taken)
         taken = fast.rotary(x, positions, frequencies, interleaved, start, transposed, magnitude, out)
@@ -163,13 +178,13 @@ def rotary(x, positions, frequencies, *, interleaved=True, start=0, transposed=F
         raise ValueError(f"start must be an int with start + {dim} inside the head of {x.shape[-1]}")
     if x.stride(-1) != 1:
         raise ValueError("x's last stride must be 1")
-    wants_grad = torch.is_grad_enabled() and x.requires_grad
+    wants_grad = (torch.is_grad_enabled() and x.requires_grad) or has_tangent(x)
     if out is not None:
         if not isinstance(out, torch.Tensor) or out.shape != x.shape or out.dtype != x.dtype or out.device != device:
             raise ValueError("out must have x's shape, type and device")
         if out.stride(-1) != 1 or not _elements_distinct(out):
             raise ValueError("out's last stride must be 1 and no two of its elements share memory")
-        if wants_grad or (torch.is_grad_enabled() and out.requires_grad):
+        if wants_grad or (torch.is_grad_enabled() and out.requires_grad) or has_tangent(out):
             raise ValueError("out cannot be given where a gradient is recorded")
         same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
         if not same and x.numel() > 0:
