@@ -145,8 +145,10 @@ py::object rotary(py::handle hx, py::handle hpositions, py::handle hfrequencies,
         positions->sizes() != x->sizes().slice(0, n - 2) || width > 0x7fffffff || x->size(n - 2) > 0x7fffffff ||
         !integer(hstart, 0, width - 2 * frequencies->size(0), start) || x->stride(n - 1) != 1)
         return py::none();
-    if (at::GradMode::is_enabled() && (x->requires_grad() || (out && out->requires_grad()))) return py::none();
-    if (differentiated(*x) || (out && differentiated(*out)) || !positions->has_storage() || !frequencies->has_storage())
+    if (at::GradMode::is_enabled() &&
+        (x->requires_grad() || frequencies->requires_grad() || (out && out->requires_grad())))
+        return py::none();
+    if (differentiated(*x) || (out && differentiated(*out)) || differentiated(*frequencies) || !positions->has_storage())
         return py::none();
     if (out) {
         if (out->sizes() != x->sizes() || out->scalar_type() != type || out->device() != dev || out->stride(n - 1) != 1 ||

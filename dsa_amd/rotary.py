@@ -156,7 +156,8 @@ def rotary(x, positions, frequencies, *, interleaved=True, start=0, transposed=F
     ``out``: where the result goes (``x`` itself: in place, the rest of each head
     untouched), else a new contiguous tensor.  ``transposed`` turns the other
     way, which is the gradient for ``x``; where ``x`` requires a gradient or
-    carries a forward-mode tangent the call records that itself (not with ``out``)."""
+    carries a forward-mode tangent the call records that itself (not with ``out``).
+    There is no gradient for ``frequencies``, and none may be asked of them."""
     fast = _fast_cache()
     if fast is not None:  # checked and launched in C++ (None: not taken)
         taken = fast.rotary(x, positions, frequencies, interleaved, start, transposed, magnitude, out)
@@ -172,6 +173,8 @@ def rotary(x, positions, frequencies, *, interleaved=True, start=0, transposed=F
     if x.dtype not in DTYPES:
         raise ValueError("x must be bfloat16, float16 or float32")
     dim = check_frequencies(frequencies, device)
+    if (torch.is_grad_enabled() and frequencies.requires_grad) or has_tangent(frequencies):
+        raise ValueError("frequencies must not require a gradient: there is none for them")
     check_positions(positions, x.shape[:-2], device)
     check_magnitude(magnitude)
     if type(start) is not int or start < 0 or start + dim > x.shape[-1]:

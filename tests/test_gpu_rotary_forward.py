@@ -92,3 +92,18 @@ def test_no_tangent_into_out(host):
         with torch.no_grad(), pytest.raises(ValueError, match="gradient"):
             dsa_amd.rotary(dual, positions, freq, out=torch.empty_like(x))
     assert torch.equal(x, make((5, 3, 64)))
+
+
+def test_frequencies_have_no_gradient(host):
+    """Asked for one, the call refuses; it does not return a zero."""
+    x, t, positions, freq = inputs((5, 3, 64))
+    wanted = freq.clone().requires_grad_()
+    for kw in ({}, dict(out=torch.empty_like(x))):
+        with pytest.raises(ValueError, match="frequencies"):
+            dsa_amd.rotary(x, positions, wanted, **kw)
+    with pytest.raises(ValueError, match="frequencies"):
+        dsa_amd.rotary(x.clone().requires_grad_(), positions, wanted)
+    with torch.no_grad():
+        assert torch.equal(dsa_amd.rotary(x, positions, wanted), dsa_amd.rotary(x, positions, freq))
+    with fw.dual_level(), pytest.raises(ValueError, match="frequencies"):
+        dsa_amd.rotary(x, positions, fw.make_dual(freq, torch.ones_like(freq)))
