@@ -219,6 +219,7 @@ py::object write_kv_rows(py::handle hkv, py::handle hrope, py::handle hslots, py
             rope_cache->sizes().slice(0, n - 1) != cache->sizes().slice(0, n - 1))
             return py::none();
         if (at::GradMode::is_enabled() && (cache->requires_grad() || rope_cache->requires_grad())) return py::none();
+        if (differentiated(*cache) || differentiated(*rope_cache)) return py::none();
         a.rope_cache = static_cast<uint16_t*>(rope_cache->data_ptr());
     }
     if (frequencies) {

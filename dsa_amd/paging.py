@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from .api import FP8_ROW, HEAD_DIM, ROPE_DIM, _fast_cache, _on_device
-from .rotary import check_frequencies, check_magnitude, check_positions, written
+from .rotary import check_frequencies, check_magnitude, check_positions, has_tangent, written
 
 MAX_SEQUENCES = 4096
 
@@ -108,7 +108,8 @@ def write_kv_rows(kv, k_rope, slots, kv_cache, rope_cache=None, *, positions=Non
     [..., 64]``, or an fp8 one, uint8 ``[..., 656]``, whose rows become those of
     :func:`dsa_amd.quantize_kv_fp8` (``pow2_scales`` as there).
 
-    No gradient is recorded, and the caches must not require one.
+    No gradient is recorded, and the caches must not require one or carry a
+    forward-mode tangent.
 
     ``frequencies`` (float64 ``[32]``) with ``positions`` (int32 or int64
     ``[tokens]``) turns ``k_rope`` on its way as :func:`dsa_amd.rotary` does."""
@@ -149,7 +150,7 @@ def write_kv_rows(kv, k_rope, slots, kv_cache, rope_cache=None, *, positions=Non
             or (not fp8 and rope_cache.data_ptr() % 4)):
         raise ValueError("kv needs contiguous rows, 16-byte aligned and a multiple of 8 elements apart, k_rope rows "
                          "4-byte aligned and a multiple of 2 apart; the caches must be 16- and 4-byte aligned")
-    if not fp8 and torch.is_grad_enabled() and (kv_cache.requires_grad or rope_cache.requires_grad):
+    if not fp8 and any((torch.is_grad_enabled() and t.requires_grad) or has_tangent(t) for t in (kv_cache, rope_cache)):
         raise ValueError("the caches are written in place and must not require a gradient")
     _int32_vector(slots, "slots", device, tokens)
     if (frequencies is None) != (positions is None):

@@ -107,3 +107,19 @@ def test_frequencies_have_no_gradient(host):
         assert torch.equal(dsa_amd.rotary(x, positions, wanted), dsa_amd.rotary(x, positions, freq))
     with fw.dual_level(), pytest.raises(ValueError, match="frequencies"):
         dsa_amd.rotary(x, positions, fw.make_dual(freq, torch.ones_like(freq)))
+
+
+def test_caches_have_no_tangent(host):
+    """A cache that carries a tangent would keep the old one over its new rows."""
+    bf16 = lambda *s: torch.randn(s, generator=torch.Generator().manual_seed(0)).bfloat16().cuda()  # noqa: E731
+    kv, rope, cache, rcache = bf16(3, 512), bf16(3, 64), bf16(8, 512), bf16(8, 64)
+    slots = torch.tensor([1, 4, 6], dtype=torch.int32).cuda()
+    kept = cache.clone(), rcache.clone()
+    with fw.dual_level():
+        dual = [fw.make_dual(c, torch.ones_like(c)) for c in (cache, rcache)]
+        for pair in ((dual[0], rcache), (cache, dual[1])):
+            with torch.no_grad(), pytest.raises(ValueError, match="gradient"):
+                dsa_amd.write_kv_rows(kv, rope, slots, *pair)
+            with pytest.raises(ValueError, match="gradient"):
+                dsa_amd.write_kv_rows(kv, rope, slots, *pair)
+    assert torch.equal(cache, kept[0]) and torch.equal(rcache, kept[1])
