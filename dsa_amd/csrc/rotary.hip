@@ -43,7 +43,10 @@ struct Shape {
     int chunks;              // workgroups of one token's units (tokens > 1: one)
     uint32_t per_token;      // units of a token
     uint32_t units_magic, token_magic;
+    int64_t group0;          // first group of tokens (of `chunks` workgroups) of this launch
 };
+// Workgroups of a launch: the grid's threads are counted in 32 bits.
+constexpr int64_t kMaxGrid = (int64_t)1 << 23;
 
 // W elements at a time: 16 bytes, or as few as a unit can have, which need no alignment.
 template <typename T, int W>
@@ -77,9 +80,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(dsa_rotary_args p, Sha
     __shared__ float2 angles[kMaxAngles];
     const int tid = threadIdx.x, pairs = p.dim >> 1;
     const int64_t all = p.groups * p.tokens;
-    const int64_t group = blockIdx.x / (uint32_t)s.chunks;
-    const uint32_t chunk = blockIdx.x - (uint32_t)group * s.chunks;
-    const int64_t token0 = group * s.tokens;
+    const uint32_t group = blockIdx.x / (uint32_t)s.chunks;
+    const uint32_t chunk = blockIdx.x - group * s.chunks;
+    const int64_t token0 = (s.group0 + group) * s.tokens;
     const int tokens = (int)min((int64_t)s.tokens, all - token0);
 
     const uint32_t n = chunk * kThreads + tid;
@@ -177,11 +180,15 @@ int launch(const dsa_rotary_args& p, hipStream_t stream) {
     s.chunks = (int)(((int64_t)s.per_token * s.tokens + kThreads - 1) / kThreads);
     s.token_magic = magic_of(s.per_token, kThreads);
     s.units_magic = magic_of((uint32_t)s.units, s.per_token);
-    const int64_t grid = (all + s.tokens - 1) / s.tokens * s.chunks;
-    if (grid > 0x7fffffff) return (int)hipErrorInvalidConfiguration;
     auto* kernel = is_wide ? rotary_kernel<T, INTERLEAVED, true> : rotary_kernel<T, INTERLEAVED, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kThreads), 0, stream, p, s);
-    return (int)hipGetLastError();
+    // heads * width <= 2^31, so a token has at most 2^23 chunks
+    const int64_t groups = (all + s.tokens - 1) / s.tokens, most = kMaxGrid / s.chunks;
+    for (s.group0 = 0; s.group0 < groups; s.group0 += most) {
+        const int64_t n = groups - s.group0 < most ? groups - s.group0 : most;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(n * s.chunks)), dim3(kThreads), 0, stream, p, s);
+        if (const int rc = (int)hipGetLastError()) return rc;
+    }
+    return 0;
 }
 
 template <typename T>
