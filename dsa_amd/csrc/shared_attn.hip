@@ -1109,20 +1109,20 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
 // four groups of 128 threads take its pieces, six at a time, in turn.
 constexpr int kMergeBatch = 6, kMergeSplit = 4, kMergeFewRows = 2048;
 template <bool STACKED, bool SPLIT>
-__global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_kernel(SharedParams, int turns) {
+__global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_kernel(SharedParams, int turns, int block0) {
     constexpr int ROWS = SPLIT ? 1 : 2, GROUPS = SPLIT ? kMergeSplit : 1;
     __shared__ f32x4 parts[SPLIT ? 128 * (kMergeSplit - 1) : 1];
     __shared__ float2 stats[SPLIT ? kMergeSplit - 1 : 1];  // maximum, sum
     const ArgsPtr p = args_now();
     const int rows = p->B * p->SQ * p->H, col = (threadIdx.x & 127) * 4;
-    const int seq_rows = p->SQ * p->H;
+    const int seq_rows = p->SQ * p->H, block = block0 + (int)blockIdx.x;
     const int half = SPLIT ? 0 : threadIdx.x >> 7, group = SPLIT ? threadIdx.x >> 7 : 0;
     int first, count;  // the workgroup's rows
     if constexpr (STACKED) {
-        first = (int)blockIdx.x * ROWS * turns;
+        first = block * ROWS * turns;
         count = min(ROWS * turns, rows - first);
     } else {
-        const int chunks = kSharedRows / (ROWS * turns), i = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x % chunks;
+        const int chunks = kSharedRows / (ROWS * turns), i = block / chunks, chunk = block % chunks;
         const int2 ends = p->ends[i];
         if (ends.x == ends.y) return;  // a whole item
         const Item it = item_rows(p, i);
@@ -1188,7 +1188,7 @@ __global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_
 }
 
 template <bool STACKED>
-void launch_merge(const SharedParams& p, hipStream_t stream) {
+int launch_merge(const SharedParams& p, hipStream_t stream) {
     const int rows = p.B * p.SQ * p.H;
     // Many rows are a prefill's, most of them there already: sixteen a workgroup
     // (262,144 rows: 59 us for 121 with two).  Few: one, shared by four groups (48
@@ -1196,10 +1196,14 @@ void launch_merge(const SharedParams& p, hipStream_t stream) {
     const bool split = rows <= kMergeFewRows;
     const int turns = rows >= 32768 ? 8 : 1, own = split ? 1 : 2 * turns;
     const int grid = STACKED ? (rows + own - 1) / own : p.items * (kSharedRows / own);
-    if (split)
-        hipLaunchKernelGGL((shared_merge_kernel<STACKED, true>), dim3(grid), dim3(128 * kMergeSplit), 0, stream, p, 1);
-    else
-        hipLaunchKernelGGL((shared_merge_kernel<STACKED, false>), dim3(grid), dim3(256), 0, stream, p, turns);
+    auto* kernel = split ? shared_merge_kernel<STACKED, true> : shared_merge_kernel<STACKED, false>;
+    constexpr int kMaxGrid = 1 << 22;  // a grid's threads, 512 a workgroup, are counted in 32 bits
+    for (int first = 0; first < grid; first += kMaxGrid) {
+        const int n = grid - first < kMaxGrid ? grid - first : kMaxGrid;
+        hipLaunchKernelGGL(kernel, dim3(n), dim3(split ? 128 * kMergeSplit : 256), 0, stream, p, turns, first);
+        if (const int rc = (int)hipGetLastError()) return rc;
+    }
+    return 0;
 }
 
 }  // namespace
@@ -1215,9 +1219,7 @@ int launch_shared(const SharedParams& p, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3(p.workgroups), dim3(kPPThreads), 0, stream, p);
     const int rc = (int)hipGetLastError();
     if (rc) return rc;
-    if (p.stacked) launch_merge<true>(p, stream);
-    else launch_merge<false>(p, stream);
-    return (int)hipGetLastError();
+    return p.stacked ? launch_merge<true>(p, stream) : launch_merge<false>(p, stream);
 }
 
 }  // namespace dsa
