@@ -99,10 +99,11 @@ def write_kv_rows(kv, k_rope, slots, kv_cache, rope_cache=None, *, positions=Non
     ``kv [tokens, 512]`` and ``k_rope [tokens, 64]`` bf16, each row contiguous and
     any distance apart (so the two slices of a projection's output go in as they
     are); ``slots`` int32 ``[tokens]``, rows of the cache with its leading
-    dimensions flattened.  A token whose slot lies outside the cache is left out;
-    a row that two tokens name holds one of them, unspecified which.  ``kv`` and
-    ``k_rope`` may be rows of the cache themselves, but not ones that the call
-    writes.
+    dimensions flattened.  A token whose slot lies outside the cache is left out.
+    No row may be named twice: nothing orders the two tokens' writes, and the row
+    holds parts of either (as :func:`extend_block_table` gives them, slots are
+    distinct).  ``kv`` and ``k_rope`` may be rows of the cache themselves, but not
+    ones that the call writes.
 
     ``kv_cache``: a bf16 cache or pool ``[..., 512]`` with its ``rope_cache
     [..., 64]``, or an fp8 one, uint8 ``[..., 656]``, whose rows become those of

@@ -79,9 +79,9 @@ int dsa_rotary(const dsa_rotary_args* args, void* stream);
 /*
  * New rows into a cache: row slots[i] of the cache becomes token i's kv and
  * (rotated, where frequencies is given: as dsa_rotary over dim 64) k_rope.  A
- * token whose slot lies outside [0, cache_rows) is left out; slots that name a
- * row twice leave one of the two there, unspecified which.  kv and k_rope must
- * not lie in rows that the call writes.
+ * token whose slot lies outside [0, cache_rows) is left out.  No row may be named
+ * twice: nothing orders the two tokens' writes, and the row holds parts of
+ * either.  kv and k_rope must not lie in rows that the call writes.
  *
  *   kv [tokens, 512] bf16, kv_stride elements apart (a multiple of 8, 16-byte
  *   aligned); k_rope [tokens, 64] bf16, rope_stride apart (a multiple of 2,
