@@ -204,8 +204,9 @@ __global__ __launch_bounds__(kThreads) void expand_rows_kernel(const uint8_t* __
 
 // write_rows puts the new tokens' rows where a slot map says
 // (dsa_write_kv_rows), with the rotary part turned on the way.  A wave writes a
-// row, in several stores that nothing orders against another wave's: lane l holds latent values 8 l .. 8 l + 7, and of the rotary part
-// lane l < 32 holds pair l.  The loads are issued before the slot is looked at.
+// row, in several stores that nothing orders against another wave's: lane l holds
+// latent values 8 l .. 8 l + 7, and of the rotary part lane l < 32 holds pair l.
+// The loads are issued before the slot is looked at.
 // Bound by HBM, and in a decode step by the launch: 8191 fp8 rows 6.9 us in a
 // graph of them (2.1 TB/s), 65,536 33 us (3.6 TB/s), 33 rows 2.5 us.  Two rows a
 // wave, so that all lanes turn a pair, took 7.3, 31 and 3.0 us, and 20 us for 8191

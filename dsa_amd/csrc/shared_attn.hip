@@ -14,8 +14,9 @@
 //
 // With 128 heads bound by the matrix cores (52 % of cycles busy, 1.16 to 1.2
 // PFLOP/s over 4 prompts of 512 tokens behind 8192 rows: 2.1 us a tile of 128 rows,
-// 1.6 at the rate of a large matrix product), with 16 rows of their own by HBM
-// (6.4 TB/s), and for a decode step by what surrounds a piece's tiles: 4 us until
+// 1.6 at the rate of a large matrix product), with 16 to 64 rows of their own by HBM
+// (256 sequences of 4096 bf16 rows 235 us, 5.1 TB/s), and for a decode step by what
+// surrounds a piece's tiles: 4 us until
 // its share is found, 5 to 7 until its first tile and Q are there, 2 to 6 for its
 // rows, 4 to 16 for the merge.
 //
@@ -108,9 +109,13 @@ __device__ __forceinline__ void item_tiles(ArgsPtr p, int i, int most, Item& it)
 
 // What an item costs, in tenths of a microsecond on a full chip: each tile, and
 // once the start and end of a piece (Q, the first tile's latency, the stores).
-// Measured on 64 to 256 sequences of their own rows, paged: up to 32 rows 1.5 us
-// a tile of bf16 rows (HBM, 6.4 TB/s) and 1.4 of fp8, up to 64 2.0 and 1.65,
-// up to 128 2.1 and 2.6; a piece 8.5, 10.5 and 12 us beside its tiles.
+// Set from the kernel's own clock readings on 64 to 256 sequences of their own rows,
+// in blocks of 64.  Whole calls of 256 sequences, a workgroup each (2048 to 4096 rows,
+// us a tile; contiguous, blocks, pages): 16 query rows 1.65, 1.60, 1.61 for bf16 and
+// 1.06, 1.29, 1.49 for fp8, 64 rows 1.56, 1.60, 2.55 and 1.48, 1.84, 1.90, 128 rows
+// 2.37, 2.44, 2.87 and 2.54, 2.53, 3.29.  The items of a call differ in rows only, so
+// what counts is the ratio of 128 rows to 16: 1.4 here, 1.5 measured, fp8 1.9 and 2.0;
+// of pages 1.8 and 2.2, for which no costs of their own have been tried.
 struct Cost {
     int tile, piece;
 };
@@ -120,7 +125,11 @@ __device__ __forceinline__ Cost cost_of(int rows, int fp8) {
     return Cost{fp8 ? 14 : 15, 85};
 }
 static_assert(kSharedMaxCost >= 27 && kSharedPieceCost >= 2 * 27 + 120, "the host's bound on an item's cost");
-constexpr int kMinShare = 30;  // least cost a workgroup is given: more than a tile (16 heads, 3 sequences: 22.4 us at 40, 21.8 at 30)
+// Least cost a workgroup is given, more than a tile's.  At 20, 30, 40 and 60: 3
+// sequences of 16 heads behind 500 rows 21.4, 21.3, 22.0 and 22.9 us, 16 of them behind
+// 600 29.6, 27.9, 27.8 and 27.7, 8 of 1000 rows 23.2, 22.5, 23.3 and 23.8, one query of
+// 300 18.3, 19.1, 19.7 and 20.9, of 2000 21.0, 20.7, 20.0 and 21.0 (in a graph of calls).
+constexpr int kMinShare = 30;
 
 // Workgroup w computes the tiles that start in its share [w * total / groups,
 // (w + 1) * total / groups) of the summed costs; an item that starts at cost
@@ -1190,9 +1199,11 @@ __global__ __launch_bounds__(SPLIT ? 128 * kMergeSplit : 256) void shared_merge_
 template <bool STACKED>
 int launch_merge(const SharedParams& p, hipStream_t stream) {
     const int rows = p.B * p.SQ * p.H;
-    // Many rows are a prefill's, most of them there already: sixteen a workgroup
-    // (262,144 rows: 59 us for 121 with two).  Few: one, shared by four groups (48
-    // rows: 20.5 us a call for 21.8; 6144 rows: 155 for 147).
+    // Many rows are a prefill's, most of them there already: sixteen a workgroup (262,144
+    // rows: 59 us for 121 with two; from 8192 to 65,536 a call is within 3 % either way:
+    // 32,768 stacked 461 and 457 us, whole items 302 and 302).  Few: one, shared by four
+    // groups (stacked, behind 8192 rows: 48 rows 20.5 us a call for 21.8, 512 47 for 50,
+    // 1024 58 and 58, 2048 82 and 80, 4096 127 for 121; whole items 1024 49 for 46).
     const bool split = rows <= kMergeFewRows;
     const int turns = rows >= 32768 ? 8 : 1, own = split ? 1 : 2 * turns;
     const int grid = STACKED ? (rows + own - 1) / own : p.items * (kSharedRows / own);
