@@ -2,8 +2,8 @@
 // (include/dsa_mi355x_cache.h: dsa_extend_block_table).  No reference
 // counterpart: the reference takes a contiguous cache (dsa/api.py:30-33).
 //
-// Bound by its launch (64 sequences 4.1 us, 48 prompts of up to 2047 tokens 4.3 in
-// a captured row of calls): a step of 64 sequences moves about a kilobyte, one of
+// Bound by its launch (64 sequences 4.1 us, 48 prompts of up to 2047 tokens 4.3 in a
+// captured row of calls; 3.6 and 4.6 as traced): a step of 64 sequences moves about a kilobyte, one of
 // 98,304 tokens 1.2 MB.  So it is one launch with no second pass: every
 // workgroup scans the sequences' token and block counts itself (at most 4096 of
 // them, kept in LDS) and then writes its share of the tokens and of the taken

@@ -3,10 +3,10 @@
 // given, dsa/api.py:30-33).
 //
 // A decode step's kernels take 3 to 4 us (forward_shared's 20), their checks,
-// output and launch in Python 9 to 10 (15).  Here the same work takes 3 to 6.  Nothing is raised for a bad
-// input: whatever the Python path would reject, and what it does besides (a
-// gradient to record, nothing to do), returns None, and the caller goes on in
-// Python.  A failed launch returns the library's status code.  Nothing is
+// output and launch in Python 9 to 10 (15).  Here the same work takes 3 to 6.
+// Nothing is raised for a bad input: whatever the Python path would reject, and
+// what it does besides (a gradient or tangent to record, nothing to do), returns
+// None, and the caller goes on in Python.  A failed launch returns the library's status code.  Nothing is
 // allocated or launched before every check has passed.
 #include <torch/extension.h>
 #include <ATen/core/grad_mode.h>

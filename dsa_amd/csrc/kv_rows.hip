@@ -207,10 +207,11 @@ __global__ __launch_bounds__(kThreads) void expand_rows_kernel(const uint8_t* __
 // row, in several stores that nothing orders against another wave's: lane l holds
 // latent values 8 l .. 8 l + 7, and of the rotary part lane l < 32 holds pair l.
 // The loads are issued before the slot is looked at.
-// Bound by HBM, and in a decode step by the launch: 8191 fp8 rows 6.9 us in a
-// graph of them (2.1 TB/s), 65,536 33 us (3.6 TB/s), 33 rows 2.5 us.  Two rows a
-// wave, so that all lanes turn a pair, took 7.3, 31 and 3.0 us, and 20 us for 8191
-// bf16 rows in place of 7.1; one wave a workgroup 7.6, 39 and 2.4.
+// Bound by HBM, and in a decode step by the launch: 8191 fp8 rows 7.1 us in a
+// graph of calls on other inputs (2.1 TB/s), 65,536 32 us (3.7 TB/s), 33 rows 2.4
+// us; bf16 7.0, 32.5 (4.7 TB/s) and 2.1.  Two rows a wave, so that all lanes turn a
+// pair, took 7.3, 31 and 3.0 us, and 20 us for 8191 bf16 rows; one wave a workgroup
+// 7.6, 39 and 2.4; the rotary part in dwords 7.2, 30.5 and 2.4, bf16 7.1, 34 and 2.1.
 template <bool FP8, bool POW2>
 __global__ __launch_bounds__(kThreads) void write_rows_kernel(dsa_write_args p) {
     const int lane = threadIdx.x & 63;

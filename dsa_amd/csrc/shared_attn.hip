@@ -12,7 +12,7 @@
 //          of the softmax
 //   merge  rows of cut items joined (FP32), rows without keys filled in
 //
-// With 128 heads bound by the matrix cores (52 % of cycles busy, 1.16 to 1.2
+// With 128 heads bound by the matrix cores (54 % of cycles busy, 1.17 to 1.22
 // PFLOP/s over 4 prompts of 512 tokens behind 8192 rows: 2.1 us a tile of 128 rows,
 // 1.6 at the rate of a large matrix product), with 16 to 64 rows of their own by HBM
 // (256 sequences of 4096 bf16 rows 235 us, 5.1 TB/s), and for a decode step by what
