@@ -109,8 +109,8 @@ def write_kv_rows(kv, k_rope, slots, kv_cache, rope_cache=None, *, positions=Non
     [..., 64]``, or an fp8 one, uint8 ``[..., 656]``, whose rows become those of
     :func:`dsa_amd.quantize_kv_fp8` (``pow2_scales`` as there).
 
-    No gradient is recorded, and the caches must not require one or carry a
-    forward-mode tangent.
+    No gradient is recorded and no forward-mode tangent, and the caches must not
+    require the one or carry the other.
 
     ``frequencies`` (float64 ``[32]``) with ``positions`` (int32 or int64
     ``[tokens]``) turns ``k_rope`` on its way as :func:`dsa_amd.rotary` does."""

@@ -81,8 +81,8 @@ def forward_shared(q, kv, q_rope, k_rope, lengths, prefix=0, *, scale=None, bloc
     the same; it need not be a multiple of the block size.  0: nothing shared.
 
     The output is finite for max|kv| < 2^38.  Caches hold fewer than 2^25 rows.
-    Outputs are fresh tensors, which record no gradient (as
-    :func:`dsa_amd.forward`'s), the workspace is the caching allocator's, and
+    Outputs are fresh tensors, which record no gradient and no forward-mode tangent
+    (as :func:`dsa_amd.forward`'s), the workspace is the caching allocator's, and
     nothing synchronises."""
     fast = _fast_cache()
     if fast is not None:  # checked, allocated and launched in C++ (None: not taken)
