@@ -1,5 +1,5 @@
-"""ctypes binding of ``libdsa_mi355x.so`` (C ABI: include/dsa_mi355x.h and
-include/dsa_mi355x_cache.h).
+"""ctypes binding of ``libdsa_mi355x.so`` (C ABI: include/dsa_mi355x.h,
+include/dsa_mi355x_cache.h and include/dsa_mi355x_layer.h).
 
 The library is required: there is no fallback path.  Loading it touches no
 GPU (the planning entry points are pure host logic), so the binding also works
@@ -107,6 +107,40 @@ class DsaSharedArgs(ctypes.Structure):
                 + [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)])
 
 
+class DsaTreeArgs(ctypes.Structure):
+    """Mirror of ``struct dsa_tree_args`` (include/dsa_mi355x_cache.h)."""
+
+    _fields_ = [("shared", DsaSharedArgs), ("tree", ctypes.c_void_p), ("words", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+class DsaNormArgs(ctypes.Structure):
+    """Mirror of ``struct dsa_norm_args`` (include/dsa_mi355x_layer.h)."""
+
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("x", "residual", "weight", "out", "sum", "scales", "inverse")]
+                + [(name, ctypes.c_int64) for name in ("rows", "x_stride", "residual_stride")]
+                + [(name, ctypes.c_int32) for name in ("dim", "dtype", "weight_f32", "pow2_scales")]
+                + [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)])
+
+
+class DsaNormGradArgs(ctypes.Structure):
+    """Mirror of ``struct dsa_norm_grad_args`` (include/dsa_mi355x_layer.h)."""
+
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("h", "inverse", "weight", "grad_out", "grad_sum", "grad_in",
+                                                      "grad_weight", "workspace")]
+                + [(name, ctypes.c_int64) for name in ("workspace_bytes", "rows", "h_stride")]
+                + [(name, ctypes.c_int32) for name in ("dim", "dtype", "weight_f32", "reserved")])
+
+
+class DsaProductArgs(ctypes.Structure):
+    """Mirror of ``struct dsa_product_args`` (include/dsa_mi355x_layer.h)."""
+
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("a", "a_scales", "b", "b_scales", "out", "workspace")]
+                + [("workspace_bytes", ctypes.c_int64)]
+                + [(name, ctypes.c_int32) for name in ("M", "N", "K", "dtype")])
+
+
+BF16, F16, F32 = 0, 1, 2  # DSA_BF16, DSA_F16, DSA_F32
 KV_BF16 = 0  # DSA_KV_BF16
 KV_FP8 = 1   # DSA_KV_FP8: 656-byte rows (512 e4m3, 4 fp32 scales, 64 bf16 rope)
 
@@ -149,6 +183,19 @@ CACHE_SIGNATURES = {
     "dsa_fwd_shared_ws_bytes": (_i64, [ctypes.POINTER(DsaSharedArgs)]),
     "dsa_fwd_shared": (_i32, [ctypes.POINTER(DsaSharedArgs), _vp]),
     "dsa_write_kv_rows": (_i32, [ctypes.POINTER(DsaWriteArgs), _vp]),
+    "dsa_draft_tree": (_i32, [_vp] * 4 + [_i32] * 2 + [_vp]),
+    "dsa_fwd_tree_ws_bytes": (_i64, [ctypes.POINTER(DsaTreeArgs)]),
+    "dsa_fwd_tree": (_i32, [ctypes.POINTER(DsaTreeArgs), _vp]),
+}
+
+# Entry points of include/dsa_mi355x_layer.h.
+LAYER_SIGNATURES = {
+    "dsa_rms_norm": (_i32, [ctypes.POINTER(DsaNormArgs), _vp]),
+    "dsa_rms_norm_fp8": (_i32, [ctypes.POINTER(DsaNormArgs), _vp]),
+    "dsa_rms_norm_grad_ws_bytes": (_i64, [_i64, _i32]),
+    "dsa_rms_norm_grad": (_i32, [ctypes.POINTER(DsaNormGradArgs), _vp]),
+    "dsa_matmul_fp8_ws_bytes": (_i64, [ctypes.POINTER(DsaProductArgs)]),
+    "dsa_matmul_fp8": (_i32, [ctypes.POINTER(DsaProductArgs), _vp]),
 }
 
 # Entry points of csrc/host_entry.h, called by this package only.
@@ -172,7 +219,7 @@ def load() -> ctypes.CDLL:
                     f"{LIB_PATH} is missing: build it with `python -m dsa_amd.build` "
                     "(dsa_amd has no CPU or fallback path)")
             lib = ctypes.CDLL(str(LIB_PATH))
-            for name, (res, args) in {**SIGNATURES, **CACHE_SIGNATURES, **PRIVATE_SIGNATURES}.items():
+            for name, (res, args) in {**SIGNATURES, **CACHE_SIGNATURES, **LAYER_SIGNATURES, **PRIVATE_SIGNATURES}.items():
                 fn = getattr(lib, name)
                 fn.restype = res
                 fn.argtypes = args

@@ -689,8 +689,23 @@ def _fast_cache():
     with _fast_lock:
         if not _fast_cache_state:
             _fast_cache_state.append(_load_fast("_fast_cache", ("dsa_extend_block_table", "dsa_rotary", "dsa_write_kv_rows",
-                                                                "dsa_fwd_shared_ws_bytes", "dsa_fwd_shared")))
+                                                                "dsa_fwd_shared_ws_bytes", "dsa_fwd_shared", "dsa_draft_tree",
+                                                                "dsa_fwd_tree")))
     return _fast_cache_state[0]
+
+
+# And for the norms and 8-bit products (csrc/fast_layer.cpp).
+_fast_layer_state = []
+
+
+def _fast_layer():
+    if _fast_layer_state:
+        return _fast_layer_state[0]
+    with _fast_lock:
+        if not _fast_layer_state:
+            _fast_layer_state.append(_load_fast("_fast_layer", ("dsa_rms_norm", "dsa_rms_norm_fp8",
+                                                                "dsa_matmul_fp8_ws_bytes", "dsa_matmul_fp8")))
+    return _fast_layer_state[0]
 
 
 def _register_fast(device, shape, plan, partials):

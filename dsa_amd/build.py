@@ -2,10 +2,10 @@
 
 Usage: ``python -m dsa_amd.build`` (or ``__graft_entry__.build()``).  Compiles
 the kernel sources in ``dsa_amd/csrc`` with ``hipcc --offload-arch=gfx950`` and
-links one shared library exporting the C ABI of ``include/dsa_mi355x.h`` and
-``include/dsa_mi355x_cache.h``, and builds ``dsa_amd/_fast*.so``, the host fast
-paths of ``forward`` and of the paged cache's operators (g++ against the
-installed PyTorch-ROCm; no device code).
+links one shared library exporting the C ABI of ``include/dsa_mi355x.h``,
+``dsa_mi355x_cache.h`` and ``dsa_mi355x_layer.h``, and builds ``dsa_amd/_fast*.so``, the host fast
+paths of ``forward``, of the paged cache's operators and of the norms and
+products (g++ against the installed PyTorch-ROCm; no device code).
 """
 from __future__ import annotations
 
@@ -23,8 +23,8 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libdsa_mi355x.so"
 OBJ_DIR = PKG / "_build"
 SOURCES = ["sparse_mla_fwd.hip", "merge.hip", "project_uv.hip", "indexer.hip", "fwd_scratch.hip", "bucket_rows.hip",
-           "kv_rows.hip", "rotary.hip", "block_table.hip", "shared_attn.hip",
-           "abi.cpp", "abi_cache.cpp"]
+           "kv_rows.hip", "rotary.hip", "block_table.hip", "shared_attn.hip", "draft_tree.hip",
+           "norm.hip", "product.hip", "abi.cpp", "abi_cache.cpp", "abi_layer.cpp"]
 ARCH = "gfx950"
 ROCM_INCLUDE = Path(os.environ.get("ROCM_PATH", "/opt/rocm")) / "include"
 
@@ -59,7 +59,7 @@ def _compile(src: str, verbose: bool) -> Path:
     return obj
 
 
-FAST_SOURCES = {"_fast": "fast_forward.cpp", "_fast_cache": "fast_cache.cpp"}
+FAST_SOURCES = {"_fast": "fast_forward.cpp", "_fast_cache": "fast_cache.cpp", "_fast_layer": "fast_layer.cpp"}
 
 
 def fast_path_module(name: str = "_fast") -> Path:

@@ -87,6 +87,73 @@ int shared_plan(const dsa_shared_args* a, SharedPlan* plan) {
 
 bool aligned(const void* p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
+// dsa_fwd_shared, or with a tree dsa_fwd_tree.
+int run_shared(const dsa_shared_args* a, const int32_t* tree, int words, void* stream) {
+    SharedPlan plan;
+    if (const int rc = shared_plan(a, &plan)) return rc;
+    if (a->kv_format != DSA_KV_BF16 && a->kv_format != DSA_KV_FP8) return fail(-1, "unknown kv_format %d", a->kv_format);
+    const bool fp8 = a->kv_format == DSA_KV_FP8;
+    if (!a->q || !a->kv || !a->q_rope || (!fp8 && !a->k_rope) || !a->lengths || !a->out || !a->out_max || !a->out_sum ||
+        !a->workspace)
+        return fail(-1, "NULL pointer argument");
+    if (!aligned(a->q, 16) || !aligned(a->kv, 16) || !aligned(a->q_rope, 16) || (!fp8 && !aligned(a->k_rope, 16)) ||
+        !aligned(a->out, 16) || !aligned(a->lengths, 4) || !aligned(a->block_table, 4) || !aligned(a->out_max, 4) ||
+        !aligned(a->out_sum, 4) || !aligned(a->workspace, 256))
+        return fail(-1, "tensors must be 16-byte (lengths, block_table, max and sum 4-byte, workspace 256-byte) aligned");
+    if (!(a->scale >= 0.f) || !std::isfinite(a->scale)) return fail(-1, "scale must be a positive finite number, or 0");
+    if (a->block_table) {
+        if (a->block_size <= 0 || a->max_blocks <= 0 || a->num_blocks <= 0 ||
+            (int64_t)a->block_size * a->max_blocks != a->L)
+            return fail(-1, "paged kv: block_size, max_blocks and num_blocks must be positive, L = max_blocks * block_size");
+        if ((int64_t)a->num_blocks * a->block_size >= 1 << 25)
+            return fail(-1, "paged kv: num_blocks * block_size must be below 33554432");
+    }
+    if (a->workspace_bytes < plan.bytes)
+        return fail(-1, "workspace of %lld bytes is below the %lld needed", (long long)a->workspace_bytes,
+                    (long long)plan.bytes);
+    dsa::SharedParams p{};
+    p.q = a->q;
+    p.kv = static_cast<const char*>(a->kv);
+    p.q_rope = a->q_rope;
+    p.k_rope = a->k_rope;
+    p.lengths = a->lengths;
+    p.block_table = a->block_table;
+    p.tree = tree;
+    p.words = words;
+    p.out = a->out;
+    p.out_max = a->out_max;
+    p.out_sum = a->out_sum;
+    char* ws = static_cast<char*>(a->workspace);
+    p.ends = reinterpret_cast<int2*>(ws);
+    p.part_o = reinterpret_cast<float*>(ws + plan.ends_bytes);
+    p.part_m = p.part_o + plan.part_rows * 512;
+    p.part_l = p.part_m + plan.part_rows;
+    p.B = a->B;
+    p.SQ = a->SQ;
+    p.H = a->H;
+    p.L = a->L;
+    p.prefix = a->prefix;
+    p.block_size = a->block_size;
+    p.max_blocks = a->max_blocks;
+    p.num_blocks = a->num_blocks;
+    // d in (2^s, 2^(s+1)]: ceil(2^(32+s) / d) d < 2^(32+s) + d, so the quotient is exact for keys below 2^31
+    if (a->block_table && a->block_size > 1) {
+        while ((int64_t)2 << p.block_shift < a->block_size) ++p.block_shift;
+        const uint64_t num = (uint64_t)1 << (32 + p.block_shift), d = (uint64_t)a->block_size;
+        p.block_magic = (uint32_t)((num + d - 1) / d);
+    }
+    p.kv_fp8 = fp8;
+    p.scale = a->scale == 0.f ? 1.f / 24.f : a->scale;
+    p.scale_log2 = p.scale * 1.4426950408889634f;
+    p.stacked = plan.stacked;
+    p.prefix_items = plan.prefix_items;
+    p.seq_blocks = plan.seq_blocks;
+    p.items = plan.items;
+    p.workgroups = plan.workgroups;
+    p.own_rows = plan.own_rows;
+    return finish(dsa::launch_shared(p, static_cast<hipStream_t>(stream)), "shared attention launch");
+}
+
 }  // namespace
 
 extern "C" {
@@ -149,68 +216,27 @@ int64_t dsa_fwd_shared_ws_bytes(const dsa_shared_args* a) {
     return plan.bytes;
 }
 
-int dsa_fwd_shared(const dsa_shared_args* a, void* stream) {
-    SharedPlan plan;
-    if (const int rc = shared_plan(a, &plan)) return rc;
-    if (a->kv_format != DSA_KV_BF16 && a->kv_format != DSA_KV_FP8) return fail(-1, "unknown kv_format %d", a->kv_format);
-    const bool fp8 = a->kv_format == DSA_KV_FP8;
-    if (!a->q || !a->kv || !a->q_rope || (!fp8 && !a->k_rope) || !a->lengths || !a->out || !a->out_max || !a->out_sum ||
-        !a->workspace)
-        return fail(-1, "NULL pointer argument");
-    if (!aligned(a->q, 16) || !aligned(a->kv, 16) || !aligned(a->q_rope, 16) || (!fp8 && !aligned(a->k_rope, 16)) ||
-        !aligned(a->out, 16) || !aligned(a->lengths, 4) || !aligned(a->block_table, 4) || !aligned(a->out_max, 4) ||
-        !aligned(a->out_sum, 4) || !aligned(a->workspace, 256))
-        return fail(-1, "tensors must be 16-byte (lengths, block_table, max and sum 4-byte, workspace 256-byte) aligned");
-    if (!(a->scale >= 0.f) || !std::isfinite(a->scale)) return fail(-1, "scale must be a positive finite number, or 0");
-    if (a->block_table) {
-        if (a->block_size <= 0 || a->max_blocks <= 0 || a->num_blocks <= 0 ||
-            (int64_t)a->block_size * a->max_blocks != a->L)
-            return fail(-1, "paged kv: block_size, max_blocks and num_blocks must be positive, L = max_blocks * block_size");
-        if ((int64_t)a->num_blocks * a->block_size >= 1 << 25)
-            return fail(-1, "paged kv: num_blocks * block_size must be below 33554432");
-    }
-    if (a->workspace_bytes < plan.bytes)
-        return fail(-1, "workspace of %lld bytes is below the %lld needed", (long long)a->workspace_bytes,
-                    (long long)plan.bytes);
-    dsa::SharedParams p{};
-    p.q = a->q;
-    p.kv = static_cast<const char*>(a->kv);
-    p.q_rope = a->q_rope;
-    p.k_rope = a->k_rope;
-    p.lengths = a->lengths;
-    p.block_table = a->block_table;
-    p.out = a->out;
-    p.out_max = a->out_max;
-    p.out_sum = a->out_sum;
-    char* ws = static_cast<char*>(a->workspace);
-    p.ends = reinterpret_cast<int2*>(ws);
-    p.part_o = reinterpret_cast<float*>(ws + plan.ends_bytes);
-    p.part_m = p.part_o + plan.part_rows * 512;
-    p.part_l = p.part_m + plan.part_rows;
-    p.B = a->B;
-    p.SQ = a->SQ;
-    p.H = a->H;
-    p.L = a->L;
-    p.prefix = a->prefix;
-    p.block_size = a->block_size;
-    p.max_blocks = a->max_blocks;
-    p.num_blocks = a->num_blocks;
-    // d in (2^s, 2^(s+1)]: ceil(2^(32+s) / d) d < 2^(32+s) + d, so the quotient is exact for keys below 2^31
-    if (a->block_table && a->block_size > 1) {
-        while ((int64_t)2 << p.block_shift < a->block_size) ++p.block_shift;
-        const uint64_t num = (uint64_t)1 << (32 + p.block_shift), d = (uint64_t)a->block_size;
-        p.block_magic = (uint32_t)((num + d - 1) / d);
-    }
-    p.kv_fp8 = fp8;
-    p.scale = a->scale == 0.f ? 1.f / 24.f : a->scale;
-    p.scale_log2 = p.scale * 1.4426950408889634f;
-    p.stacked = plan.stacked;
-    p.prefix_items = plan.prefix_items;
-    p.seq_blocks = plan.seq_blocks;
-    p.items = plan.items;
-    p.workgroups = plan.workgroups;
-    p.own_rows = plan.own_rows;
-    return finish(dsa::launch_shared(p, static_cast<hipStream_t>(stream)), "shared attention launch");
+int dsa_fwd_shared(const dsa_shared_args* a, void* stream) { return run_shared(a, nullptr, 0, stream); }
+
+int64_t dsa_fwd_tree_ws_bytes(const dsa_tree_args* a) { return dsa_fwd_shared_ws_bytes(a ? &a->shared : nullptr); }
+
+int dsa_fwd_tree(const dsa_tree_args* a, void* stream) {
+    if (!a || !a->tree) return fail(-1, "NULL pointer argument");
+    if (a->words <= 0 || a->words > DSA_TREE_MAX_WORDS)
+        return fail(-1, "words must be in [1, %d] (got %d)", DSA_TREE_MAX_WORDS, a->words);
+    if (!aligned(a->tree, 4)) return fail(-1, "tree must be 4-byte aligned");
+    return run_shared(&a->shared, a->tree, a->words, stream);
+}
+
+int dsa_draft_tree(const int32_t* parents, const int32_t* lengths, int32_t* tree, int32_t* positions, int B, int SQ,
+                   void* stream) {
+    if (!parents || !lengths || !tree || !positions) return fail(-1, "NULL pointer argument");
+    if (B <= 0 || B > 1 << 20 || SQ <= 0 || SQ > 32 * DSA_TREE_MAX_WORDS)
+        return fail(-1, "B must be in [1, 2^20] and SQ in [1, %d] (got %d, %d)", 32 * DSA_TREE_MAX_WORDS, B, SQ);
+    if (!aligned(parents, 4) || !aligned(lengths, 4) || !aligned(tree, 4) || !aligned(positions, 4))
+        return fail(-1, "pointers must be aligned to their elements");
+    return finish(dsa::launch_draft_tree(parents, lengths, tree, positions, B, SQ, static_cast<hipStream_t>(stream)),
+                  "draft tree launch");
 }
 
 }  // extern "C"

@@ -1,6 +1,6 @@
-// Host fast path of dsa_amd.extend_block_table, rotary, write_kv_rows and
-// forward_shared (no reference counterpart: the reference takes its cache as
-// given, dsa/api.py:30-33).
+// Host fast path of dsa_amd.extend_block_table, rotary, write_kv_rows,
+// forward_shared, draft_tree and forward_tree (no reference counterpart: the
+// reference takes its cache as given, dsa/api.py:30-33).
 //
 // A decode step's kernels take 3 to 4 us (forward_shared's 20), their checks,
 // output and launch in Python 9 to 10 (15).  Here the same work takes 3 to 6.
@@ -8,11 +8,6 @@
 // what it does besides (a gradient or tangent to record, nothing to do), returns
 // None, and the caller goes on in Python.  A failed launch returns the library's status code.  Nothing is
 // allocated or launched before every check has passed.
-#include <torch/extension.h>
-#include <ATen/core/grad_mode.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-
 #include <algorithm>
 #include <array>
 #include <cmath>
@@ -20,6 +15,7 @@
 #include <utility>
 
 #include "dsa_mi355x_cache.h"
+#include "fast_args.h"
 
 namespace {
 
@@ -28,22 +24,8 @@ decltype(&dsa_rotary) g_rotary = nullptr;
 decltype(&dsa_write_kv_rows) g_write = nullptr;
 decltype(&dsa_fwd_shared_ws_bytes) g_shared_bytes = nullptr;
 decltype(&dsa_fwd_shared) g_shared = nullptr;
-
-const at::Tensor* tensor(py::handle h) { return THPVariable_Check(h.ptr()) ? &THPVariable_Unpack(h.ptr()) : nullptr; }
-
-// An int of exactly that type in [low, high].
-bool integer(py::handle h, int64_t low, int64_t high, int64_t& value) {
-    if (!PyLong_CheckExact(h.ptr())) return false;
-    int overflow = 0;
-    value = PyLong_AsLongLongAndOverflow(h.ptr(), &overflow);
-    return overflow == 0 && value >= low && value <= high;
-}
-
-bool flag(py::handle h, bool& value) {
-    if (!PyBool_Check(h.ptr())) return false;
-    value = h.ptr() == Py_True;
-    return true;
-}
+decltype(&dsa_draft_tree) g_draft = nullptr;
+decltype(&dsa_fwd_tree) g_tree = nullptr;
 
 bool magnitude_of(py::handle h, float& value) {
     if (!PyFloat_CheckExact(h.ptr())) return false;
@@ -51,11 +33,6 @@ bool magnitude_of(py::handle h, float& value) {
     if (!(std::abs(d) <= 3.4028234663852886e38)) return false;
     value = (float)d;
     return true;
-}
-
-bool vector(const at::Tensor* t, at::ScalarType type, c10::Device dev, int64_t size) {
-    return t && t->dim() == 1 && (size < 0 || t->size(0) == size) && t->scalar_type() == type && t->device() == dev &&
-           t->is_contiguous();
 }
 
 bool frequencies_ok(const at::Tensor* t, c10::Device dev) {
@@ -66,16 +43,6 @@ bool positions_ok(const at::Tensor* t, c10::Device dev) {
     return t && (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && t->device() == dev &&
            t->is_contiguous();
 }
-
-bool aligned(const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
-
-// Autograd is told of a tensor that a call writes in place.
-void written(const at::Tensor& t) {
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-
-// Whether it carries a forward-mode derivative, or is one of a function transform's stand-ins (they hold no memory).
-bool differentiated(const at::Tensor& t) { return t._fw_grad(0).defined() || !t.has_storage(); }
 
 // No two elements share memory: each dimension steps over the ones inside it.
 bool distinct(const at::Tensor& t) {
@@ -254,12 +221,9 @@ py::object write_kv_rows(py::handle hkv, py::handle hrope, py::handle hslots, py
     return py::int_(rc);
 }
 
-bool dims(const at::Tensor& t, std::initializer_list<int64_t> want) {
-    return t.sizes() == at::IntArrayRef(want.begin(), want.size());
-}
-
-py::object forward_shared(py::handle hq, py::handle hkv, py::handle hq_rope, py::handle hk_rope, py::handle hlengths,
-                          py::handle hprefix, py::handle hscale, py::handle htable) {
+// forward_shared, or with a tree (of `words` words a token) forward_tree.
+py::object attend(py::handle hq, py::handle hkv, py::handle hq_rope, py::handle hk_rope, py::handle hlengths,
+                  const at::Tensor* tree, py::handle hprefix, py::handle hscale, py::handle htable) {
     const at::Tensor *q = tensor(hq), *kv = tensor(hkv), *q_rope = tensor(hq_rope), *k_rope = tensor(hk_rope);
     const at::Tensor *lengths = tensor(hlengths), *table = tensor(htable);
     if (!q || !kv || !q_rope || !lengths || (!k_rope && !hk_rope.is_none()) || (!table && !htable.is_none()) ||
@@ -269,7 +233,8 @@ py::object forward_shared(py::handle hq, py::handle hkv, py::handle hq_rope, py:
     const auto bf16 = at::kBFloat16;
     const int64_t B = q->size(0), SQ = q->size(1), H = q->size(2);
     int64_t n = B, rows = kv->size(1), L = rows, prefix;  // kv [n, rows, 1, ..]
-    dsa_shared_args a{};
+    dsa_tree_args with_tree{};
+    dsa_shared_args& a = with_tree.shared;
     const c10::Device dev = q->device();
     if (!dev.is_cuda()) return py::none();
     if (table) {
@@ -285,13 +250,21 @@ py::object forward_shared(py::handle hq, py::handle hkv, py::handle hq_rope, py:
         a.num_blocks = (int32_t)n;
     }
     if (fp8 != !k_rope || B <= 0 || SQ <= 0 || H <= 0 || L <= 0 || L >= 1 << 25 || B > 1 << 30 || SQ > 1 << 30 ||
-        H > 1 << 30 || !dims(*q, {B, SQ, H, 512}) || !dims(*q_rope, {B, SQ, H, 64}) || !dims(*lengths, {B, SQ}) ||
+        H > 1 << 30 || !dims(*q, {B, SQ, H, 512}) || !dims(*q_rope, {B, SQ, H, 64}) || !(tree ? dims(*lengths, {B}) : dims(*lengths, {B, SQ})) ||
         !dims(*kv, {n, rows, 1, fp8 ? 656 : 512}) || (!fp8 && !dims(*k_rope, {n, rows, 1, 64})) ||
         q->scalar_type() != bf16 || q_rope->scalar_type() != bf16 || lengths->scalar_type() != at::kInt ||
         (!fp8 && (kv->scalar_type() != bf16 || k_rope->scalar_type() != bf16)) || !integer(hprefix, 0, L, prefix))
         return py::none();
     for (const at::Tensor* t : {q, kv, q_rope, lengths, fp8 ? q : k_rope})
         if (t->device() != dev || !t->is_contiguous()) return py::none();
+    if (tree) {
+        if (tree->dim() != 3 || tree->size(0) != B || tree->size(1) != SQ || tree->size(2) < 1 ||
+            tree->size(2) > DSA_TREE_MAX_WORDS || tree->scalar_type() != at::kInt || tree->device() != dev ||
+            !tree->is_contiguous())
+            return py::none();
+        with_tree.tree = static_cast<const int32_t*>(tree->data_ptr());
+        with_tree.words = (int32_t)tree->size(2);
+    }
     if (!hscale.is_none()) {
         if (!PyFloat_CheckExact(hscale.ptr())) return py::none();
         a.scale = (float)PyFloat_AS_DOUBLE(hscale.ptr());
@@ -321,17 +294,51 @@ py::object forward_shared(py::handle hq, py::handle hkv, py::handle hq_rope, py:
     a.out_max = static_cast<float*>(top.data_ptr());
     a.out_sum = static_cast<float*>(sum.data_ptr());
     a.workspace = workspace.data_ptr();
-    const int rc = g_shared(&a, c10::hip::getCurrentHIPStream(dev.index()).stream());
+    auto* stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    const int rc = tree ? g_tree(&with_tree, stream) : g_shared(&a, stream);
     if (rc != 0) return py::int_(rc);
     return py::make_tuple(out, top, sum);
 }
 
-void set_entry(uint64_t extend, uint64_t rotary_address, uint64_t write, uint64_t shared_bytes, uint64_t shared) {
+py::object forward_shared(py::handle hq, py::handle hkv, py::handle hq_rope, py::handle hk_rope, py::handle hlengths,
+                          py::handle hprefix, py::handle hscale, py::handle htable) {
+    return attend(hq, hkv, hq_rope, hk_rope, hlengths, nullptr, hprefix, hscale, htable);
+}
+
+py::object forward_tree(py::handle hq, py::handle hkv, py::handle hq_rope, py::handle hk_rope, py::handle hlengths,
+                        py::handle htree, py::handle hprefix, py::handle hscale, py::handle htable) {
+    const at::Tensor* tree = tensor(htree);
+    if (!tree) return py::none();
+    return attend(hq, hkv, hq_rope, hk_rope, hlengths, tree, hprefix, hscale, htable);
+}
+
+py::object draft_tree(py::handle hparents, py::handle hlengths) {
+    const at::Tensor *parents = tensor(hparents), *lengths = tensor(hlengths);
+    if (!parents || parents->dim() != 2) return py::none();
+    const int64_t B = parents->size(0), SQ = parents->size(1);
+    const c10::Device dev = parents->device();
+    if (B < 1 || B > 1 << 20 || SQ < 1 || SQ > 32 * DSA_TREE_MAX_WORDS || !dev.is_cuda() || !parents->is_contiguous() ||
+        parents->scalar_type() != at::kInt || !vector(lengths, at::kInt, dev, B))
+        return py::none();
+    c10::DeviceGuard guard(dev);
+    const auto options = parents->options().requires_grad(false);
+    at::Tensor tree = at::empty({B, SQ, (SQ + 31) / 32}, options), positions = at::empty({B, SQ}, options);
+    const int rc = g_draft(static_cast<const int32_t*>(parents->data_ptr()), static_cast<const int32_t*>(lengths->data_ptr()),
+                           static_cast<int32_t*>(tree.data_ptr()), static_cast<int32_t*>(positions.data_ptr()), (int)B,
+                           (int)SQ, c10::hip::getCurrentHIPStream(dev.index()).stream());
+    if (rc != 0) return py::int_(rc);
+    return py::make_tuple(tree, positions);
+}
+
+void set_entry(uint64_t extend, uint64_t rotary_address, uint64_t write, uint64_t shared_bytes, uint64_t shared,
+               uint64_t draft, uint64_t tree) {
     g_extend = reinterpret_cast<decltype(g_extend)>(extend);
     g_rotary = reinterpret_cast<decltype(g_rotary)>(rotary_address);
     g_write = reinterpret_cast<decltype(g_write)>(write);
     g_shared_bytes = reinterpret_cast<decltype(g_shared_bytes)>(shared_bytes);
     g_shared = reinterpret_cast<decltype(g_shared)>(shared);
+    g_draft = reinterpret_cast<decltype(g_draft)>(draft);
+    g_tree = reinterpret_cast<decltype(g_tree)>(tree);
 }
 
 }  // namespace
@@ -341,5 +348,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("rotary", &rotary, "dsa_amd.rotary, or None");
     m.def("write_kv_rows", &write_kv_rows, "dsa_amd.write_kv_rows (0), or None");
     m.def("forward_shared", &forward_shared, "dsa_amd.forward_shared, or None");
+    m.def("draft_tree", &draft_tree, "dsa_amd.draft_tree, or None");
+    m.def("forward_tree", &forward_tree, "dsa_amd.forward_tree, or None");
     m.def("set_entry", &set_entry, "addresses of the library's entry points");
 }

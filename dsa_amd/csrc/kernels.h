@@ -7,6 +7,7 @@
 
 #include "../../include/dsa_mi355x.h"
 #include "../../include/dsa_mi355x_cache.h"
+#include "../../include/dsa_mi355x_layer.h"
 
 namespace dsa {
 
@@ -201,8 +202,9 @@ struct SharedParams {
     const char* kv;
     const uint16_t* q_rope;
     const uint16_t* k_rope;
-    const int32_t* lengths;      // [B, SQ]
+    const int32_t* lengths;      // [B, SQ], with a tree [B]
     const int32_t* block_table;  // [B, max_blocks] or NULL
+    const int32_t* tree;         // [B, SQ, words] or NULL
     uint16_t* out;
     float *out_max, *out_sum;
     int2* ends;       // [items]: workgroups that compute an item's first and last tile
@@ -217,7 +219,22 @@ struct SharedParams {
     float scale, scale_log2;
     int stacked, prefix_items, seq_blocks, items;
     int workgroups, own_rows;  // own_rows: of a piece of a sequence's own rows
+    int words;                 // of a token's bits (tree)
 };
 int launch_shared(const SharedParams& p, hipStream_t stream);
+
+// Ancestors and positions of drafted tokens (draft_tree.hip).
+int launch_draft_tree(const int32_t* parents, const int32_t* lengths, int32_t* tree, int32_t* positions, int B, int SQ,
+                      hipStream_t stream);
+
+// Norms and their gradients (norm.hip).  `vector`: all rows can be read and written
+// 16 bytes at a time.
+int launch_norm(const dsa_norm_args& p, bool codes, bool vector, hipStream_t stream);
+int launch_norm_grad(const dsa_norm_grad_args& p, bool vector, hipStream_t stream);
+int64_t norm_grad_teams(int64_t rows, int dim);  // rows of 32-bit sums in the workspace
+
+// 8-bit products (product.hip).
+int64_t product_ws_bytes(const dsa_product_args& p);
+int launch_product(const dsa_product_args& p, hipStream_t stream);
 
 }  // namespace dsa

@@ -1,0 +1,411 @@
+// Root-mean-square norms of a residual stream, and 8-bit codes
+// (include/dsa_mi355x_layer.h).  No reference counterpart: the reference takes q
+// and kv as given (README.md:19-21).
+//
+// A row is held in registers by a team of one, four or sixteen waves, eight values
+// a thread and chunk, so that it is read once: the sum of squares needs all of it
+// before the first output.  Bound by HBM, and in a decode step by the launch and two
+// trips to memory.
+#include <hip/hip_runtime.h>
+#include <hip/hip_fp16.h>
+#include <stdint.h>
+
+#include "kernels.h"
+
+namespace dsa {
+namespace {
+
+constexpr int kBlock = 128;  // values that share a scale: 16 lanes of eight
+
+typedef _Float16 f16;
+
+template <typename T>
+struct Eight {
+    uint4 v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ float at(int i) const {
+        const uint32_t w = i < 4 ? (i < 2 ? v.x : v.y) : (i < 6 ? v.z : v.w);
+        const uint16_t half = (uint16_t)(i & 1 ? w >> 16 : w);
+        return (float)__builtin_bit_cast(T, half);
+    }
+};
+template <>
+struct Eight<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = reinterpret_cast<const float4*>(p)[0];
+        b = reinterpret_cast<const float4*>(p)[1];
+    }
+    __device__ __forceinline__ float at(int i) const {
+        const float4& v = i < 4 ? a : b;
+        return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+    }
+};
+
+// Values [e, e + 8) of a row of dim, zeros behind its end.  `vector`: the row is
+// 16-byte aligned and dim a multiple of eight.
+template <typename T>
+__device__ __forceinline__ void load8(float (&f)[8], const T* row, int e, int dim, bool vector) {
+    if (vector) {
+        if (e < dim) {
+            Eight<T> v;
+            v.load(row + e);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = v.at(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = 0.f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = e + i < dim ? (float)row[e + i] : 0.f;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* row, const float (&f)[8], int e, int dim, bool vector) {
+    T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = (T)f[i];
+    if (vector) {
+        if (e < dim) {
+            typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+            constexpr int N = 16 / sizeof(T);
+#pragma unroll
+            for (int k = 0; k < 8 / N; ++k) {
+                vec v;
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = t[N * k + i];
+                reinterpret_cast<vec*>(row + e)[k] = v;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (e + i < dim) row[e + i] = t[i];
+    }
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// Sum over a team; `turn` alternates, so that one barrier a sum is enough.
+template <int WAVES>
+__device__ __forceinline__ float team_sum(float v, float (*parts)[WAVES], int turn) {
+    v = wave_sum(v);
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) parts[turn & 1][threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v += parts[turn & 1][w];
+    }
+    return v;
+}
+
+// max over the 16 lanes of this lane's DPP row.
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true));  // row_ror:8
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x124, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x122, 0xf, 0xf, true));
+    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x121, 0xf, 0xf, true));
+}
+
+// e4m3 code of v clamped to +-448, NaN kept (0x7f with v's sign).
+__device__ __forceinline__ uint32_t code_special(float v) {
+    if (v != v) return 0x7fu | (__float_as_uint(v) >> 31 << 7);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fminf(fmaxf(v, -448.f), 448.f), 0.f, 0, false) & 0xffu;
+}
+
+// Codes of this lane's eight values and the scale that its 16 lanes share.  The
+// quotient by 448 is a product with its rounded reciprocal (1.2e-7 of the scale); by
+// the scale, an exponent shift where that is a power of two, and else a product with
+// its reciprocal: 2^-23 of a value, so that only one so near to the middle of two
+// codes takes the other.  Either stays below 464, and e4m3 rounds that to 448.
+__device__ __forceinline__ uint2 encode8(const float (&f)[8], bool pow2, float& scale) {
+    uint32_t m = 0;  // |f| as bits: a NaN's exceed infinity's
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+    m = row16_max(m);
+    const float top = __uint_as_float(m);
+    scale = top > 0.f ? top * (1.f / 448.f) : 1.f;
+    if (!(scale > 0.f)) scale = __uint_as_float(1);  // the product of the least numbers underflows
+    float x[8];
+    if (pow2) {
+        const int k = __builtin_amdgcn_frexp_expf(scale) - (__builtin_amdgcn_frexp_mantf(scale) == 0.5f ? 1 : 0);
+        if (m < 0x7f800000u) scale = ldexpf(1.f, k);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = ldexpf(f[i], -k);
+    } else if (scale >= 0x1p-126f) {
+        const float by = 1.f / scale;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = f[i] * by;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = f[i] / scale;
+    }
+    uint2 c;
+    if (__builtin_expect(m >= 0x7f800000u || scale < 0x1p-126f, 0)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = f[i] / scale;
+        c.x = code_special(x[0]) | code_special(x[1]) << 8 | code_special(x[2]) << 16 | code_special(x[3]) << 24;
+        c.y = code_special(x[4]) | code_special(x[5]) << 8 | code_special(x[6]) << 16 | code_special(x[7]) << 24;
+    } else {
+        c.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(
+            x[2], x[3], __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false), true);
+        c.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(
+            x[6], x[7], __builtin_amdgcn_cvt_pk_fp8_f32(x[4], x[5], 0, false), true);
+    }
+    return c;
+}
+
+__device__ __forceinline__ void load_weight(float (&f)[8], const void* weight, int e, int dim, bool f32, bool vector,
+                                            const __bf16*) {
+    if (f32) load8(f, static_cast<const float*>(weight), e, dim, vector);
+    else load8(f, static_cast<const __bf16*>(weight), e, dim, vector);
+}
+__device__ __forceinline__ void load_weight(float (&f)[8], const void* weight, int e, int dim, bool f32, bool vector,
+                                            const f16*) {
+    if (f32) load8(f, static_cast<const float*>(weight), e, dim, vector);
+    else load8(f, static_cast<const f16*>(weight), e, dim, vector);
+}
+__device__ __forceinline__ void load_weight(float (&f)[8], const void* weight, int e, int dim, bool, bool vector,
+                                            const float*) {
+    load8(f, static_cast<const float*>(weight), e, dim, vector);
+}
+
+template <typename T, bool CODES, int WAVES, int CH>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void norm_kernel(dsa_norm_args p, int vector_) {
+    constexpr int TEAM = WAVES * 64, TEAMS = WAVES == 1 ? 4 : 1;
+    __shared__ float parts[2][WAVES];
+    const bool vector = vector_;
+    const int tid = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int team = WAVES == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+    const int dim = p.dim, blocks = (dim + kBlock - 1) / kBlock;
+    const bool normed = !CODES || p.weight != nullptr;
+    float w[CH][8];
+    if (normed) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            load_weight(w[c], p.weight, (c * TEAM + tid) * 8, dim, p.weight_f32, vector, (const T*)nullptr);
+    }
+    int turn = 0;
+    for (int64_t r = (int64_t)blockIdx.x * TEAMS + team; r < p.rows; r += (int64_t)gridDim.x * TEAMS, ++turn) {
+        const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
+        float h[CH][8];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) load8(h[c], x, (c * TEAM + tid) * 8, dim, vector);
+        if (p.residual) {
+            const T* residual = static_cast<const T*>(p.residual) + r * p.residual_stride;
+            T* sum = static_cast<T*>(p.sum) + r * dim;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                float add[8];
+                load8(add, residual, (c * TEAM + tid) * 8, dim, vector);
+                // rounded here, as the stream is kept: its norm, its gradients and a
+                // model that adds first all see the same values
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[c][i] = (float)(T)(h[c][i] + add[i]);
+            }
+#pragma unroll
+            for (int c = 0; c < CH; ++c) store8(sum, h[c], (c * TEAM + tid) * 8, dim, vector);
+        }
+        if (normed) {
+            float squares = 0.f;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) squares = fmaf(h[c][i], h[c][i], squares);
+            squares = team_sum<WAVES>(squares, parts, turn);
+            const float inverse = 1.f / sqrtf(squares / (float)dim + p.eps);
+            if (!CODES && p.inverse && tid == 0) p.inverse[r] = inverse;
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * inverse * w[c][i];
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int e = (c * TEAM + tid) * 8;
+            if constexpr (CODES) {
+                float scale;
+                const uint2 code = encode8(h[c], p.pow2_scales, scale);
+                if (e < dim) {
+                    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + r * dim + e) = code;
+                    if ((tid & 15) == 0) p.scales[r * blocks + e / kBlock] = scale;
+                }
+            } else {
+                store8(static_cast<T*>(p.out) + r * dim, h[c], e, dim, vector);
+            }
+        }
+    }
+}
+
+// Gradients: a team goes over rows team, team + teams, .. and keeps its columns'
+// sums of the weight's gradient in registers; they are added up, in a fixed order,
+// by norm_weight_kernel.
+template <typename T, int WAVES, int CH>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void norm_grad_kernel(dsa_norm_grad_args p, int vector_) {
+    constexpr int TEAM = WAVES * 64, TEAMS = WAVES == 1 ? 4 : 1;
+    __shared__ float parts[2][WAVES];
+    const bool vector = vector_;
+    const int tid = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int64_t team = (int64_t)blockIdx.x * TEAMS + (WAVES == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+    const int64_t teams = (int64_t)gridDim.x * TEAMS;
+    const int dim = p.dim;
+    float w[CH][8], sums[CH][8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        load_weight(w[c], p.weight, (c * TEAM + tid) * 8, dim, p.weight_f32, vector, (const T*)nullptr);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[c][i] = 0.f;
+    }
+    int turn = 0;
+    for (int64_t r = team; r < p.rows; r += teams, ++turn) {
+        const float inverse = p.inverse[r];
+        float u[CH][8], b[CH][8], mean = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int e = (c * TEAM + tid) * 8;
+            load8(u[c], static_cast<const T*>(p.h) + r * p.h_stride, e, dim, vector);
+            load8(b[c], static_cast<const T*>(p.grad_out) + r * dim, e, dim, vector);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                u[c][i] *= inverse;
+                sums[c][i] = fmaf(b[c][i], u[c][i], sums[c][i]);
+                b[c][i] *= w[c][i];
+                mean = fmaf(b[c][i], u[c][i], mean);
+            }
+        mean = team_sum<WAVES>(mean, parts, turn) / (float)dim;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int e = (c * TEAM + tid) * 8;
+            float given[8];
+            if (p.grad_sum) load8(given, static_cast<const T*>(p.grad_sum) + r * dim, e, dim, vector);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float v = (b[c][i] - u[c][i] * mean) * inverse;
+                if (p.grad_sum) v += given[i];
+                b[c][i] = v;
+            }
+            store8(static_cast<T*>(p.grad_in) + r * dim, b[c], e, dim, vector);
+        }
+    }
+    if (p.grad_weight) {
+        float* out = static_cast<float*>(p.workspace) + team * dim;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) store8(out, sums[c], (c * TEAM + tid) * 8, dim, (dim & 3) == 0 && (dim & 7) == 0);
+    }
+}
+
+constexpr int kSumColumns = 64, kSumGroups = 16;
+template <typename W>
+__global__ __launch_bounds__(kSumColumns* kSumGroups) void norm_weight_kernel(const float* parts, W* out, int teams, int dim) {
+    __shared__ float sums[kSumGroups][kSumColumns];
+    const int column = threadIdx.x & 63, group = threadIdx.x >> 6, at = blockIdx.x * kSumColumns + column;
+    float s = 0.f;
+    if (at < dim)
+        for (int t = group; t < teams; t += kSumGroups) s += parts[(int64_t)t * dim + at];
+    sums[group][column] = s;
+    __syncthreads();
+    if (group == 0 && at < dim) {
+        for (int g = 1; g < kSumGroups; ++g) s += sums[g][column];
+        out[at] = (W)s;
+    }
+}
+
+// Waves a row and chunks a thread.
+struct Shape {
+    int waves, chunks;
+};
+Shape shape_of(int64_t rows, int dim) {
+    if (dim <= 512) return {1, 1};
+    if (dim <= 1024) return {1, 2};
+    if (rows <= 512) return {16, dim <= 8192 ? 1 : 2};
+    if (dim <= 2048) return {4, 1};
+    if (dim <= 4096) return {4, 2};
+    if (dim <= 8192) return {4, 4};
+    return {16, 2};
+}
+
+constexpr int64_t kMaxGrid = 4096;
+
+template <typename T, bool CODES>
+int launch_typed(const dsa_norm_args& p, int vector, hipStream_t stream) {
+    const Shape s = shape_of(p.rows, p.dim);
+    const int64_t teams = s.waves == 1 ? 4 : 1, want = (p.rows + teams - 1) / teams;
+    const dim3 grid((unsigned)(want < kMaxGrid ? want : kMaxGrid)), block(s.waves == 1 ? 256 : 64 * s.waves);
+#define DSA_NORM(W, C) \
+    if (s.waves == W && s.chunks == C) hipLaunchKernelGGL((norm_kernel<T, CODES, W, C>), grid, block, 0, stream, p, vector)
+    DSA_NORM(1, 1);
+    DSA_NORM(1, 2);
+    DSA_NORM(4, 1);
+    DSA_NORM(4, 2);
+    DSA_NORM(4, 4);
+    DSA_NORM(16, 1);
+    DSA_NORM(16, 2);
+#undef DSA_NORM
+    return (int)hipGetLastError();
+}
+
+Shape grad_shape_of(int dim) {
+    if (dim <= 512) return {1, 1};
+    if (dim <= 1024) return {1, 2};
+    if (dim <= 2048) return {4, 1};
+    if (dim <= 4096) return {4, 2};
+    return {16, dim <= 8192 ? 1 : 2};
+}
+int64_t grad_groups(int64_t rows, int dim) {
+    const int64_t teams = grad_shape_of(dim).waves == 1 ? 4 : 1, want = (rows + teams - 1) / teams;
+    return want < 512 ? want : 512;
+}
+
+template <typename T>
+int launch_grad_typed(const dsa_norm_grad_args& p, int vector, hipStream_t stream) {
+    const Shape s = grad_shape_of(p.dim);
+    const int64_t groups = grad_groups(p.rows, p.dim);
+    const dim3 grid((unsigned)groups), block(s.waves == 1 ? 256 : 64 * s.waves);
+#define DSA_NORM(W, C) \
+    if (s.waves == W && s.chunks == C) hipLaunchKernelGGL((norm_grad_kernel<T, W, C>), grid, block, 0, stream, p, vector)
+    DSA_NORM(1, 1);
+    DSA_NORM(1, 2);
+    DSA_NORM(4, 1);
+    DSA_NORM(4, 2);
+    DSA_NORM(16, 1);
+    DSA_NORM(16, 2);
+#undef DSA_NORM
+    if (const int rc = (int)hipGetLastError()) return rc;
+    if (!p.grad_weight) return 0;
+    const int teams = (int)groups * (s.waves == 1 ? 4 : 1);
+    const dim3 columns((unsigned)((p.dim + kSumColumns - 1) / kSumColumns)), threads(kSumColumns * kSumGroups);
+    const float* parts = static_cast<const float*>(p.workspace);
+    if (p.weight_f32) hipLaunchKernelGGL((norm_weight_kernel<float>), columns, threads, 0, stream, parts, static_cast<float*>(p.grad_weight), teams, p.dim);
+    else hipLaunchKernelGGL((norm_weight_kernel<T>), columns, threads, 0, stream, parts, static_cast<T*>(p.grad_weight), teams, p.dim);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+int64_t norm_grad_teams(int64_t rows, int dim) {
+    return grad_groups(rows, dim) * (grad_shape_of(dim).waves == 1 ? 4 : 1);
+}
+
+int launch_norm(const dsa_norm_args& p, bool codes, bool vector, hipStream_t stream) {
+    if (p.dtype == DSA_BF16) return codes ? launch_typed<__bf16, true>(p, vector, stream) : launch_typed<__bf16, false>(p, vector, stream);
+    if (p.dtype == DSA_F16) return codes ? launch_typed<f16, true>(p, vector, stream) : launch_typed<f16, false>(p, vector, stream);
+    return codes ? launch_typed<float, true>(p, vector, stream) : launch_typed<float, false>(p, vector, stream);
+}
+
+int launch_norm_grad(const dsa_norm_grad_args& p, bool vector, hipStream_t stream) {
+    if (p.dtype == DSA_BF16) return launch_grad_typed<__bf16>(p, vector, stream);
+    if (p.dtype == DSA_F16) return launch_grad_typed<f16>(p, vector, stream);
+    return launch_grad_typed<float>(p, vector, stream);
+}
+
+}  // namespace dsa

@@ -1,6 +1,7 @@
 // Dense MLA attention of a batch whose sequences share their first rows
-// (include/dsa_mi355x_cache.h: dsa_fwd_shared).  No reference counterpart: the
-// reference attends to given indices (dsa/api.py:76-132).
+// (include/dsa_mi355x_cache.h: dsa_fwd_shared), or ends with a tree of drafted
+// tokens (dsa_fwd_tree).  No reference counterpart: the reference attends to given
+// indices (dsa/api.py:76-132).
 //
 // Every head of every sequence reads the same key rows in the prefix, so the
 // (token, head) pairs of the whole batch are rows of one product there: a block
@@ -79,8 +80,11 @@ struct Item {
     int first, second;  // tiles over the prefix, over the own rows
 };
 
+// Rows that a token sees: all of the first so many.  With a tree that is its
+// sequence's length, and some of the 32 * words rows behind it.
+template <bool TREE>
 __device__ __forceinline__ int seen_by(ArgsPtr p, int token) {
-    return min(max(p->lengths[token], 0), p->L);
+    return min(max(p->lengths[TREE ? token / p->SQ : token], 0), p->L);
 }
 
 // Rows and sequence of item i, without its tiles.
@@ -159,19 +163,24 @@ __device__ __forceinline__ void look_at(ArgsPtr p, int i, int low, int high, Loo
     const int tiles = k.it.first + k.it.second;
     k.cost = tiles == 0 ? 0 : k.each.piece + tiles * k.each.tile;
 }
+template <bool TREE>
 __device__ __forceinline__ void look_at(ArgsPtr p, int i, Look& k) {
     const Item it = item_rows(p, i);
     // a block has eight times 16 rows at most, each of one token: as many lengths, read together
     const int first = it.row0 / p->H, last = (it.row0 + it.rows - 1) / p->H;
     int seen[kSharedRows / 16], most = 0, least = p->L;
 #pragma unroll
-    for (int n = 0; n < kSharedRows / 16; ++n) seen[n] = p->lengths[min(first + n, last)];
+    for (int n = 0; n < kSharedRows / 16; ++n) {
+        const int token = min(first + n, last);
+        seen[n] = p->lengths[TREE ? token / p->SQ : token];
+    }
 #pragma unroll
     for (int n = 0; n < kSharedRows / 16; ++n) {
         const int v = min(max(seen[n], 0), p->L);
         most = max(most, v);
         least = min(least, v);
     }
+    if constexpr (TREE) most = min(most + 32 * p->words, p->L);
     look_at(p, i, least, most, k);
 }
 
@@ -257,7 +266,7 @@ struct Tile {
 struct Piece {
     Item it;
     int a, nt;      // first tile of the item, and how many
-    int seen_low, seen_high;  // least and greatest number of rows a query row of the block sees
+    int seen_low, seen_high;  // all rows of the block see the rows below the one, none a row from the other on
 };
 __device__ __forceinline__ Tile tile_at(const Hot& p, const Piece& c, int u) {
     const int t = c.a + u;
@@ -488,6 +497,17 @@ __device__ __forceinline__ uint32_t key_mask(const Tile& k, int seen, uint32_t v
     return valid & (n == kKeys ? 0xffffffffu : (1u << n) - 1) & (0xffffffffu << skip);
 }
 
+// The same with a tree: and the rows `seen` + j of the set bits j of the token's
+// words.  A tile takes 32 bits from bit key0 - seen on, from two words.
+__device__ __forceinline__ uint32_t tree_mask(ArgsPtr p, const Tile& k, int token, int seen, uint32_t valid) {
+    const int at = k.key0 - seen, w = at >> 5;
+    const auto* words = (const __attribute__((address_space(4))) int32_t*)(uint64_t)p->tree + (int64_t)token * p->words;
+    const uint32_t lo = w >= 0 && w < p->words ? (uint32_t)words[w] : 0u;
+    const uint32_t hi = w >= -1 && w + 1 < p->words ? (uint32_t)words[w + 1] : 0u;
+    const uint32_t drafted = (uint32_t)(((uint64_t)hi << 32 | lo) >> (at & 31));
+    return key_mask(k, seen, valid) | (key_mask(k, p->L, valid) & drafted);
+}
+
 // Lane group g's rows of a tile -- 4 g + j (j < 4) and 16 + 4 g + j -- from a key mask: bit j, bit 4 + j.
 __device__ __forceinline__ uint32_t lane_rows(uint32_t mask, int g) {
     return (mask >> (4 * g) & 15u) | (mask >> (16 + 4 * g) & 15u) << 4;
@@ -528,7 +548,7 @@ __device__ __forceinline__ void clear_specials(uint32_t stage, uint32_t masks, u
 }
 
 // One piece of an item, WIDE: up to 128 rows, else up to 16 NB (NB = 4 if WIDE).
-template <bool FP8, int LAYOUT, bool WIDE, int NB>
+template <bool FP8, int LAYOUT, bool TREE, bool WIDE, int NB>
 __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool whole, int64_t first_row,
                                              uint32_t lds, int wave, int lane) {
     static_assert(!WIDE || NB == 4, "a group's four row blocks");
@@ -541,7 +561,8 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
     const int row = c.it.row0 + (live ? block : 0);
     const int nt = c.nt;
     const ArgsPtr args = args_now();
-    int seen = seen_by(args, row / args->H);  // in a scalar register from the first wait on
+    const int token = TREE ? __builtin_amdgcn_readfirstlane(row / args->H) : 0;
+    int seen = seen_by<TREE>(args, row / args->H);  // in a scalar register from the first wait on
     const uint32_t p_lds = lds + X::P_OFF + grp * X::P_GROUP, bad = lds + X::BAD_OFF;
     const uint32_t masks = lds + X::MASK_OFF + 16 * grp, poison = lds + X::POISON_OFF;
 
@@ -571,11 +592,18 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         off_p = pp_pchunk(n16, g) | (pp_pchunk(16 * gw + n16, g) << 16);
     }
 
+    uint32_t valid = 0;
+
+    // The keys of tile u that this wave's rows see, where `mask` is not all of them.
+    auto seen_mask = [&](int u, uint32_t mask) __attribute__((always_inline)) -> uint32_t {
+        if constexpr (TREE) mask = tree_mask(args_now(), tile_at(p, c, u), token, seen, valid);
+        return mask;
+    };
+
     // Made ready behind QK, the shorter turn of the two: the gathers (behind:
     // narrow, those of the next QK), and the rows of its next tile that are in
     // the pool.
     G gather, behind;
-    uint32_t valid = 0;
     auto qk_softmax = [&](int u, bool& overflow) __attribute__((always_inline)) {
         const uint32_t stage = X::stage(lds, u);
         asm volatile("" : "+v"(off_kv), "+v"(off_rope), "+v"(off_p));
@@ -603,8 +631,9 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
         float x[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) x[r] = sacc[r >> 2][r & 3];
-        const uint32_t mask = key_mask(tile_at(p, c, u), seen, valid);
+        uint32_t mask = key_mask(tile_at(p, c, u), seen, valid);
         if (__builtin_expect(mask != 0xffffffffu, 0)) {
+            mask = seen_mask(u, mask);
             int ln = lane;
             asm volatile("" : "+v"(ln));
             const uint32_t mine = lane_rows(mask, ln >> 4);
@@ -647,7 +676,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
     auto partial = [&](int u) __attribute__((always_inline)) -> bool {
         const Tile k = tile_at(p, c, u);
         const bool some = key_mask(k, c.seen_low, valid) != 0xffffffffu;
-        if (__builtin_expect(some, 0)) lds_store<uint32_t>(masks + 4 * gw, key_mask(k, seen, valid));
+        if (__builtin_expect(some, 0)) lds_store<uint32_t>(masks + 4 * gw, seen_mask(u, key_mask(k, seen, valid)));
         return some;
     };
 
@@ -993,7 +1022,7 @@ __device__ __forceinline__ void shared_piece(const Hot& p, const Piece& c, bool 
     lds_barrier();  // LDS is free for the next piece
 }
 
-template <bool FP8, int LAYOUT>
+template <bool FP8, int LAYOUT, bool TREE>
 __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams arguments) {
     using X = PPLds<FP8>;
     __shared__ __attribute__((aligned(1024))) char smem[X::LDS_BYTES];
@@ -1015,7 +1044,7 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
         int64_t sum = 0;
         Look k;
         for (int i = i0; i < i1; ++i) {
-            look_at(p, i, k);
+            look_at<TREE>(p, i, k);
             sum += k.cost;
             if (w == 0 && k.cost == 0) p->ends[i] = int2{0, -1};  // nobody's: for the merge
         }
@@ -1050,7 +1079,7 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
         c1 = shares.start(w + 1);
         if (begin <= c0 && c0 < begin + sum) {
             for (int i = i0; i < i1; ++i) {
-                if (run > 1) look_at(p, i, k);
+                if (run > 1) look_at<TREE>(p, i, k);
                 if (c0 < begin + k.cost) {
                     int* plan = reinterpret_cast<int*>(smem + X::PLAN_OFF);
                     plan[0] = i;
@@ -1096,15 +1125,15 @@ __global__ __launch_bounds__(kPPThreads, 1) void shared_main_kernel(SharedParams
             if (threadIdx.x == 0 && a == 0) p->ends[i].x = w;
             if (threadIdx.x == 0 && b == tiles) p->ends[i].y = w;
             const int64_t first_row = piece_row(p, i, w, c.a == 0);
-            if (c.it.rows > 64) shared_piece<FP8, LAYOUT, true, 4>(hot, c, whole, first_row, lds, wave, lane);
-            else if (c.it.rows > 32) shared_piece<FP8, LAYOUT, false, 4>(hot, c, whole, first_row, lds, wave, lane);
-            else if (c.it.rows > 16) shared_piece<FP8, LAYOUT, false, 2>(hot, c, whole, first_row, lds, wave, lane);
-            else shared_piece<FP8, LAYOUT, false, 1>(hot, c, whole, first_row, lds, wave, lane);
+            if (c.it.rows > 64) shared_piece<FP8, LAYOUT, TREE, true, 4>(hot, c, whole, first_row, lds, wave, lane);
+            else if (c.it.rows > 32) shared_piece<FP8, LAYOUT, TREE, false, 4>(hot, c, whole, first_row, lds, wave, lane);
+            else if (c.it.rows > 16) shared_piece<FP8, LAYOUT, TREE, false, 2>(hot, c, whole, first_row, lds, wave, lane);
+            else shared_piece<FP8, LAYOUT, TREE, false, 1>(hot, c, whole, first_row, lds, wave, lane);
         }
         p = args_now();
         if (end >= c1 || ++i >= p->items) break;
         begin = end;
-        look_at(p, i, k);
+        look_at<TREE>(p, i, k);
         low = __builtin_amdgcn_readfirstlane(k.low);
         high = __builtin_amdgcn_readfirstlane(k.high);
     }
@@ -1219,14 +1248,19 @@ int launch_merge(const SharedParams& p, hipStream_t stream) {
 
 }  // namespace
 
-int launch_shared(const SharedParams& p, hipStream_t stream) {
+template <bool TREE>
+auto* main_kernel(const SharedParams& p) {
     const int layout = !p.block_table ? kRows : p.block_size % 4 == 0 ? kBlocks : kPages;
-    auto* kernel = p.kv_fp8 ? (layout == kRows     ? shared_main_kernel<true, kRows>
-                               : layout == kBlocks ? shared_main_kernel<true, kBlocks>
-                                                   : shared_main_kernel<true, kPages>)
-                            : (layout == kRows     ? shared_main_kernel<false, kRows>
-                               : layout == kBlocks ? shared_main_kernel<false, kBlocks>
-                                                   : shared_main_kernel<false, kPages>);
+    return p.kv_fp8 ? (layout == kRows     ? shared_main_kernel<true, kRows, TREE>
+                       : layout == kBlocks ? shared_main_kernel<true, kBlocks, TREE>
+                                           : shared_main_kernel<true, kPages, TREE>)
+                    : (layout == kRows     ? shared_main_kernel<false, kRows, TREE>
+                       : layout == kBlocks ? shared_main_kernel<false, kBlocks, TREE>
+                                           : shared_main_kernel<false, kPages, TREE>);
+}
+
+int launch_shared(const SharedParams& p, hipStream_t stream) {
+    auto* kernel = p.tree ? main_kernel<true>(p) : main_kernel<false>(p);
     hipLaunchKernelGGL(kernel, dim3(p.workgroups), dim3(kPPThreads), 0, stream, p);
     const int rc = (int)hipGetLastError();
     if (rc) return rc;

@@ -4,8 +4,8 @@ counterpart: the reference attends to given indices, dsa/api.py:76-132).
 Beside :func:`dsa_amd.forward`, over the same caches: contexts shorter than the
 indexer's top-k, a model's dense layers, and batches whose sequences start with
 the same rows -- a system prompt, a document -- which are then read, and their
-products formed, once for the whole batch (``csrc/shared_attn.hip``).  There is
-no CPU path.
+products formed, once for the whole batch (``csrc/shared_attn.hip``); and steps
+that verify a tree of drafted tokens behind each sequence.  There is no CPU path.
 """
 from __future__ import annotations
 
@@ -15,10 +15,11 @@ import torch
 
 from . import _lib
 from .api import FP8_ROW, HEAD_DIM, ROPE_DIM, _check_scale, _device_cus, _fast_cache, _on_device
+from .tree import TREE_MAX_WORDS
 
 
-def _check(q, kv, q_rope, k_rope, lengths, prefix, block_table):
-    optional = [t for t in (k_rope, block_table) if t is not None]
+def _check(q, kv, q_rope, k_rope, lengths, prefix, block_table, tree=None):
+    optional = [t for t in (k_rope, block_table, tree) if t is not None]
     if not all(isinstance(t, torch.Tensor) for t in (q, kv, q_rope, lengths, *optional)):
         raise ValueError("q, kv, q_rope, lengths (and k_rope, block_table) must be tensors")
     fp8 = kv.dtype == torch.uint8
@@ -29,6 +30,11 @@ def _check(q, kv, q_rope, k_rope, lengths, prefix, block_table):
     if q.dim() != 4 or kv.dim() != 4:
         raise ValueError("q and kv must be 4-D tensors")
     batch, queries, heads, width = q.shape
+    if tree is not None and (tree.dim() != 3 or tree.shape[:2] != (batch, queries)
+                             or not 1 <= tree.shape[2] <= TREE_MAX_WORDS):
+        raise ValueError(f"tree must be [B, SQ, words] of up to {TREE_MAX_WORDS} words (draft_tree)")
+    if tree is not None and lengths.shape != (batch,):
+        raise ValueError("with a tree lengths must be [B]")
     if block_table is None:
         pool, length = (batch, kv.shape[1]), kv.shape[1]
     else:
@@ -37,7 +43,7 @@ def _check(q, kv, q_rope, k_rope, lengths, prefix, block_table):
         pool, length = tuple(kv.shape[:2]), block_table.shape[1] * kv.shape[1]
     if (width != HEAD_DIM or kv.shape != (*pool, 1, FP8_ROW if fp8 else HEAD_DIM)
             or q_rope.shape != (batch, queries, heads, ROPE_DIM)
-            or (not fp8 and k_rope.shape != (*pool, 1, ROPE_DIM)) or lengths.shape != (batch, queries)
+            or (not fp8 and k_rope.shape != (*pool, 1, ROPE_DIM)) or (tree is None and lengths.shape != (batch, queries))
             or min(batch, queries, heads, length, *pool) <= 0):
         raise ValueError("expected q[B,SQ,H,512], q_rope[B,SQ,H,64], lengths[B,SQ], kv[B,L,1,512] and k_rope[B,L,1,64] "
                          "or fp8 kv[B,L,1,656] (or pools [N,BS,1,...] with block_table[B,M])")
@@ -47,13 +53,14 @@ def _check(q, kv, q_rope, k_rope, lengths, prefix, block_table):
         raise ValueError(f"prefix must be an int in [0, {length}]")
     device = q.device
     tensors = [q, kv, q_rope, lengths] + ([] if fp8 else [k_rope]) + ([] if block_table is None else [block_table])
+    tensors += [] if tree is None else [tree]
     if device.type != "cuda" or torch.version.hip is None or any(
             t.device != device or not t.is_contiguous() for t in tensors):
         raise ValueError("all inputs must be contiguous and on the same ROCm GPU")
     bf16 = torch.bfloat16
     if (q.dtype != bf16 or q_rope.dtype != bf16 or (not fp8 and (kv.dtype != bf16 or k_rope.dtype != bf16))
-            or lengths.dtype != torch.int32 or (block_table is not None and block_table.dtype != torch.int32)):
-        raise ValueError("q/kv/q_rope/k_rope must be bfloat16, lengths (and block_table) int32")
+            or any(t is not None and t.dtype != torch.int32 for t in (lengths, block_table, tree))):
+        raise ValueError("q/kv/q_rope/k_rope must be bfloat16, lengths (and block_table, tree) int32")
     return batch, queries, heads, length, device, fp8
 
 
@@ -91,15 +98,49 @@ def forward_shared(q, kv, q_rope, k_rope, lengths, prefix=0, *, scale=None, bloc
             if type(taken) is int:
                 _lib.check(taken, "dsa_fwd_shared")
             return taken
+    return _run(q, kv, q_rope, k_rope, lengths, None, prefix, scale, block_table)
+
+
+def forward_tree(q, kv, q_rope, k_rope, lengths, tree, prefix=0, *, scale=None, block_table=None):
+    """:func:`forward_shared` for a step that verifies drafted tokens: query ``t`` of
+    sequence ``b`` sees rows ``[0, lengths[b])`` and, of the rows behind them, those
+    that its words of ``tree`` name -- row ``lengths[b] + j`` where bit ``j % 32`` of
+    ``tree[b, t, j // 32]`` is set (:func:`dsa_amd.draft_tree`: the token itself and
+    its ancestors).
+
+    ``lengths`` int32 ``[B]``, clamped to ``[0, L]``; ``tree`` int32 ``[B, SQ, words]``,
+    up to 64 words, any bits (bits of rows from ``L`` on are left out).  The drafted
+    tokens' rows have to be in the cache: token ``j``'s at row ``lengths[b] + j``
+    (:func:`dsa_amd.write_kv_rows`), rotated by its own position.  A query with no row
+    gives output 0, max -inf and sum 0.
+
+    All else, and the three results, as :func:`forward_shared`'s; rows below ``prefix``
+    are sequence 0's."""
+    fast = _fast_cache()
+    if fast is not None:  # checked, allocated and launched in C++ (None: not taken)
+        taken = fast.forward_tree(q, kv, q_rope, k_rope, lengths, tree, prefix, scale, block_table)
+        if taken is not None:
+            if type(taken) is int:
+                _lib.check(taken, "dsa_fwd_tree")
+            return taken
+    if not isinstance(tree, torch.Tensor):
+        raise ValueError("tree must be a tensor")
+    return _run(q, kv, q_rope, k_rope, lengths, tree, prefix, scale, block_table)
+
+
+def _run(q, kv, q_rope, k_rope, lengths, tree, prefix, scale, block_table):
     scale = _check_scale(scale)
-    batch, queries, heads, length, device, fp8 = _check(q, kv, q_rope, k_rope, lengths, prefix, block_table)
-    args = _lib.DsaSharedArgs()
+    batch, queries, heads, length, device, fp8 = _check(q, kv, q_rope, k_rope, lengths, prefix, block_table,
+                                                          tree)
+    call = "dsa_fwd_shared" if tree is None else "dsa_fwd_tree"
+    whole = _lib.DsaTreeArgs()
+    args = whole.shared
     args.B, args.SQ, args.H, args.L, args.prefix = batch, queries, heads, length, prefix
     args.num_cus = _device_cus(device)
     lib = _lib.load()
     size = lib.dsa_fwd_shared_ws_bytes(ctypes.byref(args))
     if size < 0:
-        _lib.check(-1, "dsa_fwd_shared")
+        _lib.check(-1, call)
     output = torch.empty_like(q)
     maximum = torch.empty((batch, 1, queries, heads), device=device, dtype=torch.float32)
     denominator = torch.empty_like(maximum)
@@ -113,8 +154,11 @@ def forward_shared(q, kv, q_rope, k_rope, lengths, prefix=0, *, scale=None, bloc
     if block_table is not None:
         args.block_table, args.max_blocks = block_table.data_ptr(), block_table.shape[1]
         args.block_size, args.num_blocks = kv.shape[1], kv.shape[0]
+    if tree is not None:
+        whole.tree, whole.words = tree.data_ptr(), tree.shape[2]
     with _on_device(device):
-        rc = lib.dsa_fwd_shared(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index))
+        stream = torch._C._cuda_getCurrentRawStream(device.index)
+        rc = getattr(lib, call)(ctypes.byref(args if tree is None else whole), stream)
     if rc:
-        _lib.check(rc, "dsa_fwd_shared")
+        _lib.check(rc, call)
     return output, maximum, denominator

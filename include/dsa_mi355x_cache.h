@@ -1,7 +1,7 @@
 /*
  * dsa_mi355x_cache.h -- C ABI of the operators around a paged MLA cache: block
  * tables and slot maps, rotary positions, cache row writes, and dense attention
- * of a batch that shares a prefix.  Part of the same library as dsa_mi355x.h
+ * of a batch that shares a prefix or ends with trees of drafted tokens.  Part of the same library as dsa_mi355x.h
  * and of the same conventions: device pointers, a stream, nothing allocated,
  * no synchronisation, 0 / < 0 (invalid argument, nothing enqueued) / > 0 (a
  * hipError_t) with dsa_last_error().  No reference counterpart: the reference
@@ -155,6 +155,38 @@ typedef struct dsa_shared_args {
 /* < 0: the sizes are refused (dsa_last_error).  Reads no pointer of args. */
 int64_t dsa_fwd_shared_ws_bytes(const dsa_shared_args* args);
 int dsa_fwd_shared(const dsa_shared_args* args, void* stream);
+
+/*
+ * Drafted tokens behind B sequences, SQ each: token t follows token
+ * parents[b, t] < t, or the sequence's last row (-1).  Any other value, or an
+ * ancestor with one, makes it no token (padding).
+ *
+ *   parents [B, SQ], lengths [B] int32
+ *   tree    [B, SQ, ceil(SQ / 32)] int32: bit j % 32 of word j / 32 is set where
+ *           drafted token j is t itself or an ancestor of it; none for padding
+ *   positions [B, SQ] int32: lengths[b] (negative counts as 0) + the number of t's
+ *           ancestors, at most 2^31 - 1; 0 for padding
+ * B <= 2^20, SQ <= 32 * DSA_TREE_MAX_WORDS.
+ */
+#define DSA_TREE_MAX_WORDS 64
+int dsa_draft_tree(const int32_t* parents, const int32_t* lengths, int32_t* tree, int32_t* positions, int B, int SQ,
+                   void* stream);
+
+/*
+ * dsa_fwd_shared where the rows a query sees end with a tree: query t of sequence
+ * b sees rows [0, shared.lengths[b]) and rows shared.lengths[b] + j below L for
+ * every bit j of its `words` words that is set (word j / 32, bit j % 32).
+ * shared.lengths is [B] here; all else is as there (rows below the prefix are
+ * sequence 0's).  dsa_fwd_tree_ws_bytes reads shared's sizes only.
+ */
+typedef struct dsa_tree_args {
+    dsa_shared_args shared;
+    const int32_t* tree;        /* [B, SQ, words] */
+    int32_t words;              /* at most DSA_TREE_MAX_WORDS */
+    int32_t reserved;           /* zero */
+} dsa_tree_args;
+int64_t dsa_fwd_tree_ws_bytes(const dsa_tree_args* args);
+int dsa_fwd_tree(const dsa_tree_args* args, void* stream);
 
 #ifdef __cplusplus
 }

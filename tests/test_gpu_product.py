@@ -1,0 +1,184 @@
+"""8-bit products against a plain form in 64 bits.
+
+Tolerances.  32-bit outputs: a block's 128 products are exact in 32 bits and summed in
+four steps, then scaled and added block after block, and joined over at most 64 parts:
+(40 + blocks + 64) x 2^-24 of the sum of the products' sizes.  16-bit outputs are summed
+by the 8-bit matrix instructions, which keep products to a fraction of the largest:
+a single sum of 128 was off by at most 2^-13.8 of its largest product where it was
+measured, and 2^-12 of max|a| max|b| is allowed for each block; half a step of the
+output's type beside it.
+"""
+import math
+
+import pytest
+import torch
+
+import dsa_amd
+
+pytestmark = pytest.mark.gpu
+
+BF, HALF, FULL, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no ROCm GPU")
+    torch.cuda.init()
+
+
+def make(M, N, K, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    blocks = -(-K // 128)
+    a = (torch.randn(M, K, generator=g) * 100).clamp(-448, 448).to(E4M3)
+    b = (torch.randn(N, K, generator=g) * 100).clamp(-448, 448).to(E4M3)
+    a_scales = torch.exp(torch.randn(M, blocks, generator=g))
+    b_scales = torch.exp(torch.randn(-(-N // 128), blocks, generator=g)) / 1024
+    return [t.cuda() for t in (a, a_scales, b, b_scales)]
+
+
+def check(out, a, a_scales, b, b_scales):
+    M, K = a.shape
+    N = b.shape[0]
+    want = torch.zeros(M, N, dtype=torch.float64, device="cuda")
+    size, coarse = torch.zeros_like(want), torch.zeros_like(want)
+    band = torch.arange(N, device="cuda") // 128
+    for k in range(a_scales.shape[1]):
+        part = slice(128 * k, 128 * k + 128)
+        x, y = a[:, part].double(), b[:, part].double()
+        s = a_scales[:, k, None].double() * b_scales[band, k].double()
+        want += (x @ y.t()) * s
+        size += (x.abs() @ y.abs().t()) * s
+        coarse += x.abs().amax(1)[:, None] * y.abs().amax(1) * s
+    assert out.shape == want.shape and out.is_contiguous()
+    deep = 40 + a_scales.shape[1] + 64
+    bound = deep * 2.0 ** -24 * size
+    if out.dtype != FULL:
+        bound += 2.0 ** -12 * coarse
+    bound = bound * (1 + 2.0 ** -7) + torch.finfo(out.dtype).eps / 2 * want.abs() + torch.finfo(out.dtype).tiny
+    # past the largest number of the type by more than half its last step a value rounds to infinity
+    most = torch.finfo(out.dtype).max
+    over = (want.abs() + bound > most) & (out.double() * want.sign() == math.inf)
+    assert (((out.double() - want).abs() <= bound) | over).all()
+    assert not (over & (want.abs() + bound < most * (1 + torch.finfo(out.dtype).eps / 4))).any()
+
+
+@pytest.mark.parametrize("dtype", [BF, HALF, FULL])
+@pytest.mark.parametrize("M, N, K", [
+    (1, 1, 16), (1, 16, 32), (2, 17, 112), (3, 100, 128), (15, 127, 144), (16, 128, 256), (17, 129, 272), (1, 576, 7168),
+    (8, 2112, 1536), (31, 300, 512), (33, 64, 1040), (48, 1000, 640), (64, 257, 1536), (65, 2112, 512), (77, 640, 1552),
+    (100, 33, 384), (127, 200, 1024), (128, 128, 128), (129, 384, 2048), (200, 1, 256), (255, 255, 272), (257, 513, 640),
+    (300, 2112, 1536), (600, 700, 128), (1000, 130, 4096), (513, 1024, 16), (1500, 1200, 400), (2, 5, 16384)])
+def test_against_64_bits(M, N, K, dtype):
+    args = make(M, N, K, seed=M + N)
+    check(dsa_amd.matmul_fp8(*args, dtype=dtype), *args)
+
+
+@pytest.mark.parametrize("dtype", [BF, FULL])
+@pytest.mark.parametrize("M, N, K", [(2048, 1536, 7168), (4100, 2112, 1040), (1025, 4097, 2064), (777, 7168, 1536)])
+def test_large(M, N, K, dtype):
+    args = make(M, N, K, seed=1)
+    check(dsa_amd.matmul_fp8(*args, dtype=dtype), *args)
+
+
+def test_leading_dimensions_and_empty():
+    a, sa, b, sb = make(24, 100, 256)
+    want = dsa_amd.matmul_fp8(a, sa, b, sb)
+    assert torch.equal(dsa_amd.matmul_fp8(a.view(2, 3, 4, 256), sa.view(2, 3, 4, 2), b, sb), want.view(2, 3, 4, 100))
+    assert torch.equal(dsa_amd.matmul_fp8(a[0], sa[0], b, sb), want[0])
+    assert dsa_amd.matmul_fp8(a[:0], sa[:0], b, sb, dtype=FULL).shape == (0, 100)
+
+
+@pytest.mark.parametrize("M, N, K", [(5, 40, 272), (150, 300, 400)])
+@pytest.mark.parametrize("dtype", [BF, FULL])
+def test_special_codes_and_scales_stay_in_their_row(M, N, K, dtype):
+    """NaN codes of a row or column, and scales of 0, infinity and NaN, reach their own outputs only."""
+    a, sa, b, sb = make(M, N, K)
+    clean = dsa_amd.matmul_fp8(a, sa, b, sb, dtype=dtype)
+    bits_a, bits_b = a.view(torch.uint8), b.view(torch.uint8)
+    bits_a[1, K - 1] = 0x7F
+    bits_b[7, 130] = 0xFF
+    sa[2, 1], sa[3] = math.inf, 0.0
+    out = dsa_amd.matmul_fp8(a, sa, b, sb, dtype=dtype)
+    assert out[1].isnan().all() and out[:, 7].isnan().all()
+    rest = torch.ones(N, dtype=torch.bool, device="cuda")
+    rest[7] = False
+    assert not out[2, rest].isfinite().any() and not out[3, rest].any()
+    keep = [i for i in range(M) if i not in (1, 2, 3)]
+    assert torch.equal(out[keep][:, rest], clean[keep][:, rest])
+
+
+def test_what_lies_behind_is_not_read():
+    """Rows behind the last and columns behind K hold NaN: views into larger storage."""
+    M, N, K = 37, 200, 1040
+    a, sa, b, sb = make(M, N, K)
+    want = dsa_amd.matmul_fp8(a, sa, b, sb)
+    nan = lambda t, extra: torch.cat([t, torch.full((extra, t.shape[1]), 0x7F, dtype=torch.uint8, device="cuda").view(t.dtype)  # noqa: E731
+                                      if t.dtype == E4M3 else t.new_full((extra, t.shape[1]), math.nan)])
+    got = dsa_amd.matmul_fp8(nan(a, 300)[:M], nan(sa, 300)[:M], nan(b, 300)[:N], nan(sb, 9)[:sb.shape[0]])
+    assert torch.equal(got, want)
+
+
+def test_far_offsets():
+    """Outputs and codes beyond 2^31 elements."""
+    M, N, K = 70000, 32768, 16
+    a, sa, b, sb = make(1, 64, K)
+    a, sa = a.expand(M, K).contiguous(), torch.arange(M, device="cuda").float()[:, None].contiguous()
+    b, sb = b.repeat(N // 64, 1), torch.ones(N // 128, 1, device="cuda")
+    out = dsa_amd.matmul_fp8(a, sa, b, sb)
+    for m in (1, 35000, 65536, 69999):
+        check(out[m:m + 1].contiguous(), a[m:m + 1], sa[m:m + 1], b, sb)
+    del out
+    M, N, K = 140000, 16, 16384
+    a = torch.zeros(M, K, dtype=torch.uint8, device="cuda")
+    sa = torch.ones(M, K // 128, device="cuda")
+    x, sx, b, sb = make(64, N, K)
+    for m in (0, 131050, M - 64):
+        a[m:m + 64], sa[m:m + 64] = x.view(torch.uint8), sx
+    out = dsa_amd.matmul_fp8(a.view(E4M3), sa, b, sb)
+    for m in (0, 131050, M - 64):
+        check(out[m:m + 64].contiguous(), x, sx, b, sb)
+    assert not out[64:131050].any()
+
+
+@pytest.mark.parametrize("M, N, K", [(3, 2112, 7168), (100, 576, 7168), (700, 2112, 1536)])
+def test_repeats_streams_and_graphs(M, N, K):
+    args, more = make(M, N, K), make(M, N, K, seed=5)
+    want = dsa_amd.matmul_fp8(*args)
+    for _ in range(5):
+        assert torch.equal(dsa_amd.matmul_fp8(*args), want)
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    for side in sides:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            outs.append([dsa_amd.matmul_fp8(*args) for _ in range(4)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for few in outs for o in few)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = dsa_amd.matmul_fp8(*args)
+        two = dsa_amd.matmul_fp8(*more)
+    for k in range(4):
+        for t, u in zip(args, make(M, N, K, seed=10 + k)):
+            t.copy_(u)
+        graph.replay()
+        assert torch.equal(out, dsa_amd.matmul_fp8(*args)) and torch.equal(two, dsa_amd.matmul_fp8(*more))
+        torch.cuda.synchronize()
+
+
+def test_refusals():
+    a, sa, b, sb = make(4, 200, 256)
+    good = dict(a=a, a_scales=sa, b=b, b_scales=sb)
+    dsa_amd.matmul_fp8(**good)
+    off = torch.zeros(4 * 256 + 1, dtype=torch.uint8, device="cuda").view(E4M3)[1:].view(4, 256)
+    bad = [dict(a=a.float()), dict(a=a.view(torch.uint8)), dict(b=b.view(torch.float8_e5m2)), dict(a=a.cpu()), dict(b=b.cpu()),
+           dict(a=a[:, :240]), dict(b=b[:, :240]), dict(b=b[None]), dict(a=None), dict(b=None), dict(a_scales=None),
+           dict(b_scales=None), dict(a_scales=sa[:3]), dict(a_scales=sa[:, :1]), dict(a_scales=sa.double()),
+           dict(b_scales=sb[:1]), dict(b_scales=sb[:, :1]), dict(b_scales=sb.half()), dict(a_scales=sa.cpu()),
+           dict(b_scales=sb.t().contiguous().t()), dict(a=a.t().contiguous().t()), dict(b=b.t().contiguous().t()),
+           dict(dtype=torch.float64), dict(dtype="bf16"), dict(b=b[:0], b_scales=sb[:0]), dict(a=off),
+           dict(a=a[:, :8].contiguous(), b=b[:, :8].contiguous(), a_scales=sa[:, :1].contiguous(), b_scales=sb[:, :1].contiguous())]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            dsa_amd.matmul_fp8(**{**good, **kw})
