@@ -17,13 +17,12 @@
 #include <stdint.h>
 
 #include "kernels.h"
+#include "mla_tiles.h"
 
 namespace dsa {
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
 typedef _Float16 f16;
 
 constexpr int kBlock = 128;
@@ -49,6 +48,19 @@ __device__ __forceinline__ f32x4 dot128(const i32x8& a, const i32x8& b) {
     } else {
         return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
     }
+}
+
+// Four bytes a lane straight into LDS: lane l's at lds_base + 4 l.
+__device__ __forceinline__ void gather_word(uint32_t lds_base, rsrc_t rsrc, uint32_t off) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "buffer_load_dword %1, %2, 0 offen lds"
+        :
+        : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(off), "s"(rsrc)
+        : "memory", "m0");
+#pragma clang diagnostic pop
 }
 
 // Lane (r, g)'s part of a row's block of 128: chunks g and 4 + g of 16 bytes.
@@ -115,14 +127,149 @@ __global__ __launch_bounds__(64 * WAVES) void product_few_kernel(dsa_product_arg
     }
 }
 
+
+// ------------------------------------------------------------------ tiles
+// Many rows of a: a workgroup of eight waves computes TN columns by TM rows, a wave
+// 16 NT by 16 MT of them, from stages of 128 of K in LDS, of which there are two: the
+// next one's rows come straight into LDS while one is multiplied.
+//
+// A row's 128 bytes lie in LDS as eight chunks of 16, chunk c of row r at c ^ swizzle(r):
+// a fragment read takes chunks g and 4 + g of 16 rows, and the 16 lanes of a
+// ds_read_b128 pass (quads 0, 3, 5, 6 or 1, 2, 4, 7 of a half-wave: rows 0-3 and 12-15
+// of one lane group, 4-11 of the next) meet 16 different bank groups.
+__device__ __forceinline__ uint32_t swizzle(int row) { return (uint32_t)(row >> 1) & 7u; }
+
+template <bool EXACT, int NT, int MT, int WN, int WM>
+struct Tile {
+    static constexpr int TN = 16 * NT * WN, TM = 16 * MT * WM, WAVES = WN * WM, THREADS = 64 * WAVES;
+    static constexpr int B_BYTES = TN * kBlock, A_BYTES = TM * kBlock, S_BYTES = TM * 4;
+    static constexpr int A_OFF = B_BYTES, S_OFF = B_BYTES + A_BYTES, STAGE = S_OFF + S_BYTES;
+    static constexpr int LDS_BYTES = 2 * STAGE;
+    static constexpr int B_LOADS = TN / 8 / WAVES, A_LOADS = TM / 8 / WAVES;  // a wave, each of 8 rows
+    static constexpr int S_WAVES = TM / 64;                                   // waves that bring in the scales, 64 each
+    static_assert(TN % (8 * WAVES) == 0 && TM % (8 * WAVES) == 0 && S_WAVES <= WAVES, "loads split evenly");
+    static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
+    // a wave's columns lie in one block of weights
+    static_assert(kBlock % (16 * NT) == 0, "one scale a wave");
+};
+
+template <bool EXACT, int NT, int MT, int WN, int WM>
+__global__ __launch_bounds__(64 * WN * WM, 2) void product_tile_kernel(dsa_product_args p, int tiles_m, int tiles_n) {
+    using T = Tile<EXACT, NT, MT, WN, WM>;
+    __shared__ __attribute__((aligned(1024))) char smem[T::LDS_BYTES];
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int tile_m = blockIdx.x % tiles_m, tile_n = blockIdx.x / tiles_m;
+    const int m0 = tile_m * T::TM, n0 = tile_n * T::TN;
+    const int K = p.K, blocks = (K + kBlock - 1) / kBlock;
+    const int rows_m = min(T::TM, p.M - m0), rows_n = min(T::TN, p.N - n0);
+    const char* b_base = reinterpret_cast<const char*>(p.b) + (int64_t)n0 * K;
+    const char* a_base = reinterpret_cast<const char*>(p.a) + (int64_t)m0 * K;
+    const char* s_base = reinterpret_cast<const char*>(p.a_scales + (int64_t)m0 * blocks);
+    // Lane l of a load brings in chunk l % 8 of row l / 8: rows 8 apart have the same
+    // swizzle but for bit 2.
+    const int in8 = lane >> 3;
+    const uint32_t chunk = 16u * ((uint32_t)(lane & 7) ^ swizzle(in8));
+    auto issue = [&](int k) __attribute__((always_inline)) {
+        const uint32_t stage = lds + (uint32_t)(k & 1) * T::STAGE;
+        const int at = k * kBlock, left = K - at;  // bytes of a row from here on
+        const rsrc_t rb = make_rsrc(b_base + at, (uint32_t)(rows_n * K - at));
+        const rsrc_t ra = make_rsrc(a_base + at, (uint32_t)(rows_m * K - at));
+#pragma unroll
+        for (int i = 0; i < T::B_LOADS; ++i) {
+            const int first = (wave * T::B_LOADS + i) * 8;
+            uint32_t off = (uint32_t)((first + in8) * K) + (chunk ^ (first & 8 ? 64u : 0u));
+            if (left < kBlock && (int)(chunk ^ (first & 8 ? 64u : 0u)) >= left) off = 0x80000000u;  // behind the row: zeros
+            gather_lanes(stage + (uint32_t)first * kBlock, rb, off);
+        }
+#pragma unroll
+        for (int i = 0; i < T::A_LOADS; ++i) {
+            const int first = (wave * T::A_LOADS + i) * 8;
+            uint32_t off = (uint32_t)((first + in8) * K) + (chunk ^ (first & 8 ? 64u : 0u));
+            if (left < kBlock && (int)(chunk ^ (first & 8 ? 64u : 0u)) >= left) off = 0x80000000u;
+            gather_lanes(stage + T::A_OFF + (uint32_t)first * kBlock, ra, off);
+        }
+        if (wave < T::S_WAVES)
+            gather_word(stage + T::S_OFF + (uint32_t)wave * 256u, make_rsrc(s_base + 4 * k, (uint32_t)(4 * (rows_m * blocks - k))),
+                        (uint32_t)(4 * (64 * wave + lane) * blocks));
+    };
+    const int wn = wave % WN, wm = wave / WN;
+    const int band = min(n0 + 16 * NT * wn, p.N - 1) / kBlock;
+    const float* b_scale = p.b_scales + (int64_t)band * blocks;
+    // fragment reads: chunk g (and 4 + g: ^ 64) of row r of a 16-row tile
+    const uint32_t frag = (uint32_t)r * kBlock + 16u * ((uint32_t)g ^ swizzle(r));
+    const uint32_t b_frag = frag + (uint32_t)wn * NT * 16 * kBlock, a_frag = frag + T::A_OFF + (uint32_t)wm * MT * 16 * kBlock;
+    const uint32_t s_frag = T::S_OFF + 4u * (uint32_t)(wm * MT * 16 + r);
+    auto read = [&](uint32_t at) __attribute__((always_inline)) -> i32x8 {
+        const i32x4 lo = lds_load<i32x4>(at), hi = lds_load<i32x4>(at ^ 64u);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    issue(0);
+    for (int k = 0; k < blocks; ++k) {
+        wait_vmcnt<0>();
+        lds_barrier();  // stage k is there, and every wave is done with stage k - 1
+        if (k + 1 < blocks) issue(k + 1);
+        const uint32_t stage = lds + (uint32_t)(k & 1) * T::STAGE;
+        const float sb = b_scale[k];
+        i32x8 af[MT];
+        float s[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            af[i] = read(stage + a_frag + i * 16 * kBlock);
+            s[i] = lds_load<float>(stage + s_frag + 64 * i) * sb;
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const i32x8 bf = read(stage + b_frag + j * 16 * kBlock);
+            f32x4 u[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) u[i] = dot128<EXACT>(bf, af[i]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[j][i] += u[i] * s[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int m = m0 + (wm * MT + i) * 16 + r;
+        if (m >= p.M) continue;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int n = n0 + (wn * NT + j) * 16 + 4 * g;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < p.N) store_out(p.out, p.dtype, (int64_t)m * p.N + n + e, acc[j][i][e]);
+        }
+    }
+}
+
+template <bool EXACT, int NT, int MT, int WN, int WM>
+void launch_tile(const dsa_product_args& p, hipStream_t stream) {
+    using T = Tile<EXACT, NT, MT, WN, WM>;
+    const int tiles_m = (p.M + T::TM - 1) / T::TM, tiles_n = (p.N + T::TN - 1) / T::TN;
+    hipLaunchKernelGGL((product_tile_kernel<EXACT, NT, MT, WN, WM>), dim3(tiles_m * tiles_n), dim3(T::THREADS), 0, stream, p,
+                       tiles_m, tiles_n);
+}
+
 }  // namespace
 
 int64_t product_ws_bytes(const dsa_product_args&) { return 0; }
 
 int launch_product(const dsa_product_args& p, hipStream_t stream) {
-    const dim3 grid((p.N + 15) / 16, (p.M + 63) / 64);
-    if (p.dtype == DSA_F32) hipLaunchKernelGGL((product_few_kernel<true, 4, 4>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((product_few_kernel<false, 4, 4>), grid, dim3(256), 0, stream, p);
+    const bool exact = p.dtype == DSA_F32;
+    if (p.M > 128) {
+        if (exact) launch_tile<true, 4, 4, 2, 4>(p, stream);
+        else launch_tile<false, 8, 4, 2, 4>(p, stream);
+    } else {
+        const dim3 grid((p.N + 15) / 16, (p.M + 63) / 64);
+        if (exact) hipLaunchKernelGGL((product_few_kernel<true, 4, 4>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((product_few_kernel<false, 4, 4>), grid, dim3(256), 0, stream, p);
+    }
     return (int)hipGetLastError();
 }
 
