@@ -71,20 +71,24 @@ __device__ __forceinline__ i32x8 load_part(const uint8_t* row, int k, int K, int
     return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
 }
 
-template <typename T>
-__device__ __forceinline__ void store_out(void* out, int64_t at, float v) {
-    static_cast<T*>(out)[at] = (T)v;
-}
-__device__ __forceinline__ void store_out(void* out, int dtype, int64_t at, float v) {
-    if (dtype == DSA_BF16) store_out<__bf16>(out, at, v);
-    else if (dtype == DSA_F16) store_out<f16>(out, at, v);
-    else store_out<float>(out, at, v);
+// Columns n .. n + 3 of a row of N; `wide`: the four are aligned together.
+template <typename OUT>
+__device__ __forceinline__ void store4(OUT* row, int n, int N, bool wide, const f32x4& v) {
+    typedef OUT out4 __attribute__((ext_vector_type(4)));
+    if (wide) {
+        if (n < N) *reinterpret_cast<out4*>(row + n) = out4{(OUT)v[0], (OUT)v[1], (OUT)v[2], (OUT)v[3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < N) row[n + e] = (OUT)v[e];
+    }
 }
 
 // Few rows of a: a workgroup's waves take the blocks of K in turn, 16 columns by
 // 16 MB rows each, and join their sums in LDS.
-template <bool EXACT, int MB, int WAVES>
+template <typename OUT, int MB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void product_few_kernel(dsa_product_args p) {
+    constexpr bool EXACT = sizeof(OUT) == 4;
     __shared__ f32x4 sums[WAVES][MB][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
@@ -119,11 +123,9 @@ __global__ __launch_bounds__(64 * WAVES) void product_few_kernel(dsa_product_arg
     for (int i = wave; i < MB; i += WAVES) {
         f32x4 t = sums[0][i][lane];
         for (int w = 1; w < WAVES; ++w) t += sums[w][i][lane];
-        const int m = m0 + 16 * i + r, n = n0 + 4 * g;
-        if (m < p.M)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n + j < p.N) store_out(p.out, p.dtype, (int64_t)m * p.N + n + j, t[j]);
+        const int m = m0 + 16 * i + r;
+        const bool wide = (p.N & 3) == 0 && ((uintptr_t)p.out & (4 * sizeof(OUT) - 1)) == 0;
+        if (m < p.M) store4(static_cast<OUT*>(p.out) + (int64_t)m * p.N, n0 + 4 * g, p.N, wide, t);
     }
 }
 
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(64 * WAVES) void product_few_kernel(dsa_product_arg
 // of one lane group, 4-11 of the next) meet 16 different bank groups.
 __device__ __forceinline__ uint32_t swizzle(int row) { return (uint32_t)(row >> 1) & 7u; }
 
-template <bool EXACT, int NT, int MT, int WN, int WM>
+template <int NT, int MT, int WN, int WM>
 struct Tile {
     static constexpr int TN = 16 * NT * WN, TM = 16 * MT * WM, WAVES = WN * WM, THREADS = 64 * WAVES;
     static constexpr int B_BYTES = TN * kBlock, A_BYTES = TM * kBlock, S_BYTES = TM * 4;
@@ -153,9 +155,10 @@ struct Tile {
     static_assert(kBlock % (16 * NT) == 0, "one scale a wave");
 };
 
-template <bool EXACT, int NT, int MT, int WN, int WM>
+template <typename OUT, int NT, int MT, int WN, int WM>
 __global__ __launch_bounds__(64 * WN * WM, 2) void product_tile_kernel(dsa_product_args p, int tiles_m, int tiles_n) {
-    using T = Tile<EXACT, NT, MT, WN, WM>;
+    constexpr bool EXACT = sizeof(OUT) == 4;
+    using T = Tile<NT, MT, WN, WM>;
     __shared__ __attribute__((aligned(1024))) char smem[T::LDS_BYTES];
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -196,64 +199,79 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void product_tile_kernel(dsa_produ
     };
     const int wn = wave % WN, wm = wave / WN;
     const int band = min(n0 + 16 * NT * wn, p.N - 1) / kBlock;
-    const float* b_scale = p.b_scales + (int64_t)band * blocks;
+    // a scalar load: the compiler does not count the loads to LDS, and would wait for all of them with one of its own
+    const auto* b_scale = (const __attribute__((address_space(4))) float*)(uint64_t)p.b_scales + (int64_t)band * blocks;
     // fragment reads: chunk g (and 4 + g: ^ 64) of row r of a 16-row tile
     const uint32_t frag = (uint32_t)r * kBlock + 16u * ((uint32_t)g ^ swizzle(r));
     const uint32_t b_frag = frag + (uint32_t)wn * NT * 16 * kBlock, a_frag = frag + T::A_OFF + (uint32_t)wm * MT * 16 * kBlock;
     const uint32_t s_frag = T::S_OFF + 4u * (uint32_t)(wm * MT * 16 + r);
-    auto read = [&](uint32_t at) __attribute__((always_inline)) -> i32x8 {
-        const i32x4 lo = lds_load<i32x4>(at), hi = lds_load<i32x4>(at ^ 64u);
-        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
     f32x4 acc[NT][MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     issue(0);
+    float sb = b_scale[0];
+#pragma unroll 1
     for (int k = 0; k < blocks; ++k) {
         wait_vmcnt<0>();
         lds_barrier();  // stage k is there, and every wave is done with stage k - 1
         if (k + 1 < blocks) issue(k + 1);
         const uint32_t stage = lds + (uint32_t)(k & 1) * T::STAGE;
-        const float sb = b_scale[k];
-        i32x8 af[MT];
+        const uint32_t b_lo = stage + b_frag, b_hi = b_lo ^ 64u, a_lo = stage + a_frag, a_hi = a_lo ^ 64u;
+        auto read = [&](uint32_t lo, uint32_t hi, int tile) __attribute__((always_inline)) -> i32x8 {
+            const i32x4 l = lds_load<i32x4>(lo + tile * 16 * kBlock), h = lds_load<i32x4>(hi + tile * 16 * kBlock);
+            return __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        i32x8 af[MT], bf[2];
         float s[MT];
+        bf[0] = read(b_lo, b_hi, 0);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            af[i] = read(stage + a_frag + i * 16 * kBlock);
-            s[i] = lds_load<float>(stage + s_frag + 64 * i) * sb;
-        }
+        for (int i = 0; i < MT; ++i) af[i] = read(a_lo, a_hi, i);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const i32x8 bf = read(stage + b_frag + j * 16 * kBlock);
-            f32x4 u[MT];
+        for (int i = 0; i < MT; ++i) s[i] = lds_load<float>(stage + s_frag + 64 * i) * sb;
+        sb = b_scale[min(k + 1, blocks - 1)];
+        // products of tile j beside the sums of tile j - 1
+        f32x4 u[2][MT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) u[i] = dot128<EXACT>(bf, af[i]);
+        for (int j = 0; j <= NT; ++j) {
+            if (j + 1 < NT) bf[(j + 1) & 1] = read(b_lo, b_hi, j + 1);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) acc[j][i] += u[i] * s[i];
+            for (int i = 0; i < MT; ++i) {
+                if (j < NT) u[j & 1][i] = dot128<EXACT>(bf[j & 1], af[i]);
+                if (j > 0) acc[j - 1][i] += u[(j - 1) & 1][i] * s[i];
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
+    const bool wide = (p.N & 3) == 0 && ((uintptr_t)p.out & (4 * sizeof(OUT) - 1)) == 0;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int m = m0 + (wm * MT + i) * 16 + r;
         if (m >= p.M) continue;
+        OUT* row = static_cast<OUT*>(p.out) + (int64_t)m * p.N;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int n = n0 + (wn * NT + j) * 16 + 4 * g;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < p.N) store_out(p.out, p.dtype, (int64_t)m * p.N + n + e, acc[j][i][e]);
-        }
+        for (int j = 0; j < NT; ++j) store4(row, n0 + (wn * NT + j) * 16 + 4 * g, p.N, wide, acc[j][i]);
     }
 }
 
-template <bool EXACT, int NT, int MT, int WN, int WM>
+template <typename OUT, int NT, int MT, int WN, int WM>
 void launch_tile(const dsa_product_args& p, hipStream_t stream) {
-    using T = Tile<EXACT, NT, MT, WN, WM>;
+    using T = Tile<NT, MT, WN, WM>;
     const int tiles_m = (p.M + T::TM - 1) / T::TM, tiles_n = (p.N + T::TN - 1) / T::TN;
-    hipLaunchKernelGGL((product_tile_kernel<EXACT, NT, MT, WN, WM>), dim3(tiles_m * tiles_n), dim3(T::THREADS), 0, stream, p,
+    hipLaunchKernelGGL((product_tile_kernel<OUT, NT, MT, WN, WM>), dim3(tiles_m * tiles_n), dim3(T::THREADS), 0, stream, p,
                        tiles_m, tiles_n);
+}
+
+template <typename OUT>
+void launch_typed(const dsa_product_args& p, hipStream_t stream) {
+    if (p.M > 128) {
+        if constexpr (sizeof(OUT) == 4) launch_tile<OUT, 4, 4, 2, 4>(p, stream);
+        else launch_tile<OUT, 8, 4, 2, 4>(p, stream);
+    } else {
+        const dim3 grid((p.N + 15) / 16, (p.M + 63) / 64);
+        hipLaunchKernelGGL((product_few_kernel<OUT, 4, 4>), grid, dim3(256), 0, stream, p);
+    }
 }
 
 }  // namespace
@@ -261,15 +279,9 @@ void launch_tile(const dsa_product_args& p, hipStream_t stream) {
 int64_t product_ws_bytes(const dsa_product_args&) { return 0; }
 
 int launch_product(const dsa_product_args& p, hipStream_t stream) {
-    const bool exact = p.dtype == DSA_F32;
-    if (p.M > 128) {
-        if (exact) launch_tile<true, 4, 4, 2, 4>(p, stream);
-        else launch_tile<false, 8, 4, 2, 4>(p, stream);
-    } else {
-        const dim3 grid((p.N + 15) / 16, (p.M + 63) / 64);
-        if (exact) hipLaunchKernelGGL((product_few_kernel<true, 4, 4>), grid, dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL((product_few_kernel<false, 4, 4>), grid, dim3(256), 0, stream, p);
-    }
+    if (p.dtype == DSA_BF16) launch_typed<__bf16>(p, stream);
+    else if (p.dtype == DSA_F16) launch_typed<f16>(p, stream);
+    else launch_typed<float>(p, stream);
     return (int)hipGetLastError();
 }
 
