@@ -84,51 +84,100 @@ __device__ __forceinline__ void store4(OUT* row, int n, int N, bool wide, const 
     }
 }
 
-// Few rows of a: a workgroup's waves take the blocks of K in turn, 16 columns by
-// 16 MB rows each, and join their sums in LDS.
-template <typename OUT, int MB, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void product_few_kernel(dsa_product_args p) {
+// ------------------------------------------------------------------ few rows
+// Up to 128 rows of a: the weights are read once, by one wave, so they go from memory
+// straight into registers.  A wave takes 16 NT columns by all 16 MB rows, over every
+// WAVES-th block of K, DEPTH blocks ahead; the workgroup's waves join their sums in
+// LDS, in the order of the waves.
+template <typename OUT, int NT, int MB, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 1) void product_few_kernel(dsa_product_args p) {
     constexpr bool EXACT = sizeof(OUT) == 4;
-    __shared__ f32x4 sums[WAVES][MB][64];
+    constexpr int DEPTH = NT + MB <= 4 ? 4 : NT + MB <= 6 ? 3 : 2;
+    __shared__ f32x4 sums[WAVES][NT * MB][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MB;
-    const int blocks = (p.K + kBlock - 1) / kBlock;
-    const uint8_t* b = p.b + (int64_t)min(n0 + r, p.N - 1) * p.K;
-    const float* b_scale = p.b_scales + (int64_t)(n0 / kBlock) * blocks;
+    const int n0 = blockIdx.x * 16 * NT;
+    const int K = p.K, blocks = (K + kBlock - 1) / kBlock;
+    const auto* b_scale = (const __attribute__((address_space(4))) float*)(uint64_t)p.b_scales + (int64_t)(n0 / kBlock) * blocks;
+    const uint8_t* b[NT];
     const uint8_t* a[MB];
     const float* a_scale[MB];
 #pragma unroll
+    for (int j = 0; j < NT; ++j) b[j] = p.b + (int64_t)min(n0 + 16 * j + r, p.N - 1) * K;
+#pragma unroll
     for (int i = 0; i < MB; ++i) {
-        const int m = min(m0 + 16 * i + r, p.M - 1);
-        a[i] = p.a + (int64_t)m * p.K;
+        const int m = min(16 * i + r, p.M - 1);
+        a[i] = p.a + (int64_t)m * K;
         a_scale[i] = p.a_scales + (int64_t)m * blocks;
     }
-    f32x4 acc[MB];
+    f32x4 acc[NT][MB];
 #pragma unroll
-    for (int i = 0; i < MB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k = wave; k < blocks; k += WAVES) {
-        const i32x8 weights = load_part(b, k * kBlock, p.K, g);
-        const float sb = b_scale[k];
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    struct Ahead {
+        i32x8 b[NT], a[MB];
+        float s[MB], sb;
+    } ahead[DEPTH];
+    auto fetch = [&](Ahead& x, int k) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) x.b[j] = load_part(b[j], k * kBlock, K, g);
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
-            const f32x4 t = dot128<EXACT>(weights, load_part(a[i], k * kBlock, p.K, g));
-            const float s = a_scale[i][k] * sb;
-            acc[i] += t * s;
+            x.a[i] = load_part(a[i], k * kBlock, K, g);
+            x.s[i] = a_scale[i][k];
+        }
+        x.sb = b_scale[k];
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (wave + d * WAVES < blocks) fetch(ahead[d], wave + d * WAVES);
+    for (int k = wave; k < blocks; k += DEPTH * WAVES) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const int at = k + d * WAVES;
+            if (at >= blocks) break;
+            Ahead& x = ahead[d];
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                const float s = x.s[i] * x.sb;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[j][i] += dot128<EXACT>(x.b[j], x.a[i]) * s;
+            }
+            if (at + DEPTH * WAVES < blocks) fetch(x, at + DEPTH * WAVES);
         }
     }
 #pragma unroll
-    for (int i = 0; i < MB; ++i) sums[wave][i][lane] = acc[i];
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) sums[wave][j * MB + i][lane] = acc[j][i];
     __syncthreads();
-    for (int i = wave; i < MB; i += WAVES) {
-        f32x4 t = sums[0][i][lane];
-        for (int w = 1; w < WAVES; ++w) t += sums[w][i][lane];
-        const int m = m0 + 16 * i + r;
-        const bool wide = (p.N & 3) == 0 && ((uintptr_t)p.out & (4 * sizeof(OUT) - 1)) == 0;
-        if (m < p.M) store4(static_cast<OUT*>(p.out) + (int64_t)m * p.N, n0 + 4 * g, p.N, wide, t);
+    const bool wide = (p.N & 3) == 0 && ((uintptr_t)p.out & (4 * sizeof(OUT) - 1)) == 0;
+#pragma unroll 1
+    for (int t = wave; t < NT * MB; t += WAVES) {
+        f32x4 v = sums[0][t][lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v += sums[w][t][lane];
+        const int m = t % MB * 16 + r;
+        if (m < p.M) store4(static_cast<OUT*>(p.out) + (int64_t)m * p.N, n0 + t / MB * 16 + 4 * g, p.N, wide, v);
     }
 }
 
+template <typename OUT, int NT, int MB>
+void launch_few(const dsa_product_args& p, hipStream_t stream) {
+    const dim3 grid((p.N + 16 * NT - 1) / (16 * NT));
+    if (p.K <= 16 * kBlock) hipLaunchKernelGGL((product_few_kernel<OUT, NT, MB, 4>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((product_few_kernel<OUT, NT, MB, 8>), grid, dim3(512), 0, stream, p);
+}
+
+template <typename OUT, int NT>
+void launch_few(const dsa_product_args& p, hipStream_t stream) {
+    if (p.M <= 16) launch_few<OUT, NT, 1>(p, stream);
+    else if (p.M <= 32) launch_few<OUT, NT, 2>(p, stream);
+    else if (p.M <= 64) launch_few<OUT, NT, 4>(p, stream);
+    else if (p.M <= 96) launch_few<OUT, NT, 6>(p, stream);
+    else launch_few<OUT, NT, 8>(p, stream);
+}
 
 // ------------------------------------------------------------------ tiles
 // Many rows of a: a workgroup of eight waves computes TN columns by TM rows, a wave
@@ -269,8 +318,8 @@ void launch_typed(const dsa_product_args& p, hipStream_t stream) {
         if constexpr (sizeof(OUT) == 4) launch_tile<OUT, 4, 4, 2, 4>(p, stream);
         else launch_tile<OUT, 8, 4, 2, 4>(p, stream);
     } else {
-        const dim3 grid((p.N + 15) / 16, (p.M + 63) / 64);
-        hipLaunchKernelGGL((product_few_kernel<OUT, 4, 4>), grid, dim3(256), 0, stream, p);
+        if (p.N >= 32 * 224) launch_few<OUT, 2>(p, stream);
+        else launch_few<OUT, 1>(p, stream);
     }
 }
 
