@@ -89,10 +89,9 @@ __device__ __forceinline__ void store4(OUT* row, int n, int N, bool wide, const 
 // straight into registers.  A wave takes 16 NT columns by all 16 MB rows, over every
 // WAVES-th block of K, DEPTH blocks ahead; the workgroup's waves join their sums in
 // LDS, in the order of the waves.
-template <typename OUT, int NT, int MB, int WAVES>
+template <typename OUT, int NT, int MB, int WAVES, int DEPTH>
 __global__ __launch_bounds__(64 * WAVES, 1) void product_few_kernel(dsa_product_args p) {
     constexpr bool EXACT = sizeof(OUT) == 4;
-    constexpr int DEPTH = NT + MB <= 4 ? 4 : NT + MB <= 6 ? 3 : 2;
     __shared__ f32x4 sums[WAVES][NT * MB][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
@@ -163,11 +162,17 @@ __global__ __launch_bounds__(64 * WAVES, 1) void product_few_kernel(dsa_product_
     }
 }
 
-template <typename OUT, int NT, int MB>
+template <typename OUT, int NT, int MB, int WAVES, int DEPTH>
 void launch_few(const dsa_product_args& p, hipStream_t stream) {
     const dim3 grid((p.N + 16 * NT - 1) / (16 * NT));
-    if (p.K <= 16 * kBlock) hipLaunchKernelGGL((product_few_kernel<OUT, NT, MB, 4>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((product_few_kernel<OUT, NT, MB, 8>), grid, dim3(512), 0, stream, p);
+    hipLaunchKernelGGL((product_few_kernel<OUT, NT, MB, WAVES, DEPTH>), grid, dim3(64 * WAVES), 0, stream, p);
+}
+
+template <typename OUT, int NT, int MB>
+void launch_few(const dsa_product_args& p, hipStream_t stream) {
+    constexpr int DEPTH = NT + MB <= 4 ? 4 : NT + MB <= 6 ? 3 : 2;
+    if (p.K <= 16 * kBlock) launch_few<OUT, NT, MB, 4, DEPTH>(p, stream);
+    else launch_few<OUT, NT, MB, 8, DEPTH>(p, stream);
 }
 
 template <typename OUT, int NT>
@@ -190,31 +195,48 @@ void launch_few(const dsa_product_args& p, hipStream_t stream) {
 // of one lane group, 4-11 of the next) meet 16 different bank groups.
 __device__ __forceinline__ uint32_t swizzle(int row) { return (uint32_t)(row >> 1) & 7u; }
 
-template <int NT, int MT, int WN, int WM>
+// A workgroup's tile.  Every eighth workgroup is on the same XCD: each XCD gets a run of
+// tiles, ordered in bands of up to eight tiles of rows, so that the tiles that run
+// there together share rows and columns in its L2.
+__device__ __forceinline__ void place(int tiles_m, int tiles_n, int& m, int& n) {
+    const uint32_t total = (uint32_t)(tiles_m * tiles_n), each = total / 8, rest = total % 8;
+    const uint32_t xcd = blockIdx.x % 8, t = xcd * each + min(xcd, rest) + blockIdx.x / 8;
+    const uint32_t band = t / (uint32_t)(8 * tiles_n), in_band = t % (uint32_t)(8 * tiles_n);
+    const uint32_t high = min(8u, (uint32_t)tiles_m - 8 * band);
+    m = (int)(8 * band + in_band % high);
+    n = (int)(in_band / high);
+}
+
+template <int NT, int MT, int WN, int WM, int KS, int STAGES>
 struct Tile {
-    static constexpr int TN = 16 * NT * WN, TM = 16 * MT * WM, WAVES = WN * WM, THREADS = 64 * WAVES;
-    static constexpr int B_BYTES = TN * kBlock, A_BYTES = TM * kBlock, S_BYTES = TM * 4;
-    static constexpr int A_OFF = B_BYTES, S_OFF = B_BYTES + A_BYTES, STAGE = S_OFF + S_BYTES;
-    static constexpr int LDS_BYTES = 2 * STAGE;
-    static constexpr int B_LOADS = TN / 8 / WAVES, A_LOADS = TM / 8 / WAVES;  // a wave, each of 8 rows
-    static constexpr int S_WAVES = TM / 64;                                   // waves that bring in the scales, 64 each
-    static_assert(TN % (8 * WAVES) == 0 && TM % (8 * WAVES) == 0 && S_WAVES <= WAVES, "loads split evenly");
+    static constexpr int TN = 16 * NT * WN, TM = 16 * MT * WM, GROUP = WN * WM, WAVES = GROUP * KS, THREADS = 64 * WAVES;
+    static constexpr int B_LOADS = (TN + 8 * GROUP - 1) / (8 * GROUP), A_LOADS = (TM + 8 * GROUP - 1) / (8 * GROUP);  // a wave, of 8 rows each
+    static constexpr int S_WAVES = (TM + 63) / 64;  // loads of 64 scales each
+    static constexpr int LOADS = B_LOADS + A_LOADS + 1;
+    static constexpr int A_OFF = B_LOADS * GROUP * 8 * kBlock, S_OFF = A_OFF + A_LOADS * GROUP * 8 * kBlock;
+    static constexpr int BLOCK = S_OFF + S_WAVES * 256, STAGE = BLOCK * KS;
+    static constexpr int JOIN_BYTES = KS > 1 ? WAVES * NT * MT * 1024 : 0;
+    static constexpr int LDS_BYTES = STAGES * STAGE > JOIN_BYTES ? STAGES * STAGE : JOIN_BYTES;
+    static_assert(S_WAVES <= GROUP, "a scale load a wave");
     static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
+    static_assert((STAGES - 1) * LOADS < 64, "loads in flight are counted in six bits");
     // a wave's columns lie in one block of weights
     static_assert(kBlock % (16 * NT) == 0, "one scale a wave");
 };
 
-template <typename OUT, int NT, int MT, int WN, int WM>
-__global__ __launch_bounds__(64 * WN * WM, 2) void product_tile_kernel(dsa_product_args p, int tiles_m, int tiles_n) {
+template <typename OUT, int NT, int MT, int WN, int WM, int KS, int STAGES>
+__global__ __launch_bounds__(64 * WN * WM * KS, 1) void product_tile_kernel(dsa_product_args p, int tiles_m, int tiles_n) {
     constexpr bool EXACT = sizeof(OUT) == 4;
-    using T = Tile<NT, MT, WN, WM>;
+    using T = Tile<NT, MT, WN, WM, KS, STAGES>;
     __shared__ __attribute__((aligned(1024))) char smem[T::LDS_BYTES];
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = KS > 1 ? wave / T::GROUP : 0, in_group = KS > 1 ? wave % T::GROUP : wave;
     const int r = lane & 15, g = lane >> 4;
-    const int tile_m = blockIdx.x % tiles_m, tile_n = blockIdx.x / tiles_m;
+    int tile_m, tile_n;
+    place(tiles_m, tiles_n, tile_m, tile_n);
     const int m0 = tile_m * T::TM, n0 = tile_n * T::TN;
-    const int K = p.K, blocks = (K + kBlock - 1) / kBlock;
+    const int K = p.K, blocks = (K + kBlock - 1) / kBlock, steps = (blocks + KS - 1) / KS;
     const int rows_m = min(T::TM, p.M - m0), rows_n = min(T::TN, p.N - n0);
     const char* b_base = reinterpret_cast<const char*>(p.b) + (int64_t)n0 * K;
     const char* a_base = reinterpret_cast<const char*>(p.a) + (int64_t)m0 * K;
@@ -223,30 +245,35 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void product_tile_kernel(dsa_produ
     // swizzle but for bit 2.
     const int in8 = lane >> 3;
     const uint32_t chunk = 16u * ((uint32_t)(lane & 7) ^ swizzle(in8));
-    auto issue = [&](int k) __attribute__((always_inline)) {
-        const uint32_t stage = lds + (uint32_t)(k & 1) * T::STAGE;
-        const int at = k * kBlock, left = K - at;  // bytes of a row from here on
-        const rsrc_t rb = make_rsrc(b_base + at, (uint32_t)(rows_n * K - at));
-        const rsrc_t ra = make_rsrc(a_base + at, (uint32_t)(rows_m * K - at));
+    // A group's block of step t: behind the last one nothing is read, but the loads are
+    // the same, so that they can be counted on.  Rows behind the last are out of the
+    // descriptors' range, and so zeros.
+    auto issue = [&](int t) __attribute__((always_inline)) {
+        const uint32_t stage = lds + (uint32_t)(t % STAGES) * T::STAGE + (uint32_t)group * T::BLOCK;
+        const int k = t * KS + group, at = k * kBlock, left = K - at;  // bytes of a row from here on
+        const bool on = k < blocks;
+        const rsrc_t rb = make_rsrc(b_base + at, on ? (uint32_t)(rows_n * K - at) : 0u);
+        const rsrc_t ra = make_rsrc(a_base + at, on ? (uint32_t)(rows_m * K - at) : 0u);
+        auto offset = [&](int first) __attribute__((always_inline)) -> uint32_t {
+            const uint32_t c = chunk ^ (first & 8 ? 64u : 0u);
+            return (int)c < left ? (uint32_t)((first + in8) * K) + c : 0x80000000u;  // behind the row's end: zeros
+        };
 #pragma unroll
         for (int i = 0; i < T::B_LOADS; ++i) {
-            const int first = (wave * T::B_LOADS + i) * 8;
-            uint32_t off = (uint32_t)((first + in8) * K) + (chunk ^ (first & 8 ? 64u : 0u));
-            if (left < kBlock && (int)(chunk ^ (first & 8 ? 64u : 0u)) >= left) off = 0x80000000u;  // behind the row: zeros
-            gather_lanes(stage + (uint32_t)first * kBlock, rb, off);
+            const int first = (in_group * T::B_LOADS + i) * 8;
+            gather_lanes(stage + (uint32_t)first * kBlock, rb, offset(first));
         }
 #pragma unroll
         for (int i = 0; i < T::A_LOADS; ++i) {
-            const int first = (wave * T::A_LOADS + i) * 8;
-            uint32_t off = (uint32_t)((first + in8) * K) + (chunk ^ (first & 8 ? 64u : 0u));
-            if (left < kBlock && (int)(chunk ^ (first & 8 ? 64u : 0u)) >= left) off = 0x80000000u;
-            gather_lanes(stage + T::A_OFF + (uint32_t)first * kBlock, ra, off);
+            const int first = (in_group * T::A_LOADS + i) * 8;
+            gather_lanes(stage + T::A_OFF + (uint32_t)first * kBlock, ra, offset(first));
         }
-        if (wave < T::S_WAVES)
-            gather_word(stage + T::S_OFF + (uint32_t)wave * 256u, make_rsrc(s_base + 4 * k, (uint32_t)(4 * (rows_m * blocks - k))),
-                        (uint32_t)(4 * (64 * wave + lane) * blocks));
+        const int part = in_group % T::S_WAVES;  // some are loaded twice, the same
+        gather_word(stage + T::S_OFF + (uint32_t)part * 256u,
+                    make_rsrc(s_base + 4 * k, on ? (uint32_t)(4 * (rows_m * blocks - k)) : 0u),
+                    (uint32_t)(4 * (64 * part + lane) * blocks));
     };
-    const int wn = wave % WN, wm = wave / WN;
+    const int wn = in_group % WN, wm = in_group / WN;
     const int band = min(n0 + 16 * NT * wn, p.N - 1) / kBlock;
     // a scalar load: the compiler does not count the loads to LDS, and would wait for all of them with one of its own
     const auto* b_scale = (const __attribute__((address_space(4))) float*)(uint64_t)p.b_scales + (int64_t)band * blocks;
@@ -259,14 +286,17 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void product_tile_kernel(dsa_produ
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    issue(0);
-    float sb = b_scale[0];
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t) issue(t);
+    float sb = b_scale[min(group, blocks - 1)];
 #pragma unroll 1
-    for (int k = 0; k < blocks; ++k) {
-        wait_vmcnt<0>();
-        lds_barrier();  // stage k is there, and every wave is done with stage k - 1
-        if (k + 1 < blocks) issue(k + 1);
-        const uint32_t stage = lds + (uint32_t)(k & 1) * T::STAGE;
+    for (int t = 0; t < steps; ++t) {
+        wait_vmcnt<(STAGES - 2) * T::LOADS>();
+        lds_barrier();  // stage t is there, and every wave is done with stage t - 1
+        issue(t + STAGES - 1);
+        const int k = t * KS + group;
+        if (KS > 1 && k >= blocks) break;  // the last step, of a group that has none: no barrier follows but the one below
+        const uint32_t stage = lds + (uint32_t)(t % STAGES) * T::STAGE + (uint32_t)group * T::BLOCK;
         const uint32_t b_lo = stage + b_frag, b_hi = b_lo ^ 64u, a_lo = stage + a_frag, a_hi = a_lo ^ 64u;
         auto read = [&](uint32_t lo, uint32_t hi, int tile) __attribute__((always_inline)) -> i32x8 {
             const i32x4 l = lds_load<i32x4>(lo + tile * 16 * kBlock), h = lds_load<i32x4>(hi + tile * 16 * kBlock);
@@ -279,7 +309,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void product_tile_kernel(dsa_produ
         for (int i = 0; i < MT; ++i) af[i] = read(a_lo, a_hi, i);
 #pragma unroll
         for (int i = 0; i < MT; ++i) s[i] = lds_load<float>(stage + s_frag + 64 * i) * sb;
-        sb = b_scale[min(k + 1, blocks - 1)];
+        sb = b_scale[min(k + KS, blocks - 1)];
         // products of tile j beside the sums of tile j - 1
         f32x4 u[2][MT];
 #pragma unroll
@@ -293,30 +323,50 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void product_tile_kernel(dsa_produ
             }
         }
     }
+    wait_vmcnt<0>();  // loads behind the last block write zeros into LDS
     const bool wide = (p.N & 3) == 0 && ((uintptr_t)p.out & (4 * sizeof(OUT) - 1)) == 0;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    auto store = [&](int j, int i, const f32x4& v) __attribute__((always_inline)) {
         const int m = m0 + (wm * MT + i) * 16 + r;
-        if (m >= p.M) continue;
-        OUT* row = static_cast<OUT*>(p.out) + (int64_t)m * p.N;
+        if (m < p.M) store4(static_cast<OUT*>(p.out) + (int64_t)m * p.N, n0 + (wn * NT + j) * 16 + 4 * g, p.N, wide, v);
+    };
+    if constexpr (KS == 1) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) store4(row, n0 + (wn * NT + j) * 16 + 4 * g, p.N, wide, acc[j][i]);
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) store(j, i, acc[j][i]);
+    } else {  // the groups' sums, in their order: a group joins every KS-th tile
+        lds_barrier();
+        auto at = [&](int of, int tile) __attribute__((always_inline)) -> uint32_t {
+            return lds + (uint32_t)(((of * T::GROUP + in_group) * NT * MT + tile) * 1024 + 16 * lane);
+        };
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) lds_store<f32x4>(at(group, j * MT + i), acc[j][i]);
+        lds_barrier();
+#pragma unroll 1
+        for (int tile = group; tile < NT * MT; tile += KS) {
+            f32x4 v = lds_load<f32x4>(at(0, tile));
+#pragma unroll
+            for (int of = 1; of < KS; ++of) v += lds_load<f32x4>(at(of, tile));
+            store(tile / MT, tile % MT, v);
+        }
     }
 }
 
-template <typename OUT, int NT, int MT, int WN, int WM>
+template <typename OUT, int NT, int MT, int WN, int WM, int KS, int STAGES>
 void launch_tile(const dsa_product_args& p, hipStream_t stream) {
-    using T = Tile<NT, MT, WN, WM>;
+    using T = Tile<NT, MT, WN, WM, KS, STAGES>;
     const int tiles_m = (p.M + T::TM - 1) / T::TM, tiles_n = (p.N + T::TN - 1) / T::TN;
-    hipLaunchKernelGGL((product_tile_kernel<OUT, NT, MT, WN, WM>), dim3(tiles_m * tiles_n), dim3(T::THREADS), 0, stream, p,
+    hipLaunchKernelGGL((product_tile_kernel<OUT, NT, MT, WN, WM, KS, STAGES>), dim3(tiles_m * tiles_n), dim3(T::THREADS), 0, stream, p,
                        tiles_m, tiles_n);
 }
 
 template <typename OUT>
 void launch_typed(const dsa_product_args& p, hipStream_t stream) {
     if (p.M > 128) {
-        if constexpr (sizeof(OUT) == 4) launch_tile<OUT, 4, 4, 2, 4>(p, stream);
-        else launch_tile<OUT, 8, 4, 2, 4>(p, stream);
+        if constexpr (sizeof(OUT) == 4) launch_tile<OUT, 4, 4, 2, 4, 1, 2>(p, stream);
+        else launch_tile<OUT, 8, 4, 2, 4, 1, 2>(p, stream);
     } else {
         if (p.N >= 32 * 224) launch_few<OUT, 2>(p, stream);
         else launch_few<OUT, 1>(p, stream);
