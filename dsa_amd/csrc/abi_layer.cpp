@@ -129,7 +129,11 @@ int dsa_matmul_fp8(const dsa_product_args* a, void* stream) {
         return fail(-1, "codes must be 16-byte aligned, scales and out to their elements, the workspace to 256 bytes");
     if (a->workspace_bytes < need)
         return fail(-1, "workspace of %lld bytes is below the %lld needed", (long long)a->workspace_bytes, (long long)need);
-    return finish(dsa::launch_product(*a, static_cast<hipStream_t>(stream)), "product launch");
+    int device = 0, cus = 0;
+    int rc = (int)hipGetDevice(&device);
+    if (!rc) rc = (int)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
+    if (rc) return fail(rc, "device query: %s", hipGetErrorString((hipError_t)rc));
+    return finish(dsa::launch_product(*a, cus, static_cast<hipStream_t>(stream)), "product launch");
 }
 
 }  // extern "C"

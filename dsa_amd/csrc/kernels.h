@@ -235,6 +235,6 @@ int64_t norm_grad_teams(int64_t rows, int dim);  // rows of 32-bit sums in the w
 
 // 8-bit products (product.hip).
 int64_t product_ws_bytes(const dsa_product_args& p);
-int launch_product(const dsa_product_args& p, hipStream_t stream);
+int launch_product(const dsa_product_args& p, int cus, hipStream_t stream);  // cus: compute units to plan for
 
 }  // namespace dsa

@@ -63,14 +63,6 @@ __device__ __forceinline__ void gather_word(uint32_t lds_base, rsrc_t rsrc, uint
 #pragma clang diagnostic pop
 }
 
-// Lane (r, g)'s part of a row's block of 128: chunks g and 4 + g of 16 bytes.
-__device__ __forceinline__ i32x8 load_part(const uint8_t* row, int k, int K, int g) {
-    uint4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-    if (k + 16 * g < K) lo = *reinterpret_cast<const uint4*>(row + k + 16 * g);
-    if (k + 64 + 16 * g < K) hi = *reinterpret_cast<const uint4*>(row + k + 64 + 16 * g);
-    return i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-}
-
 // Columns n .. n + 3 of a row of N; `wide`: the four are aligned together.
 template <typename OUT>
 __device__ __forceinline__ void store4(OUT* row, int n, int N, bool wide, const f32x4& v) {
@@ -82,106 +74,6 @@ __device__ __forceinline__ void store4(OUT* row, int n, int N, bool wide, const 
         for (int e = 0; e < 4; ++e)
             if (n + e < N) row[n + e] = (OUT)v[e];
     }
-}
-
-// ------------------------------------------------------------------ few rows
-// Up to 128 rows of a: the weights are read once, by one wave, so they go from memory
-// straight into registers.  A wave takes 16 NT columns by all 16 MB rows, over every
-// WAVES-th block of K, DEPTH blocks ahead; the workgroup's waves join their sums in
-// LDS, in the order of the waves.
-template <typename OUT, int NT, int MB, int WAVES, int DEPTH>
-__global__ __launch_bounds__(64 * WAVES, 1) void product_few_kernel(dsa_product_args p) {
-    constexpr bool EXACT = sizeof(OUT) == 4;
-    __shared__ f32x4 sums[WAVES][NT * MB][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16 * NT;
-    const int K = p.K, blocks = (K + kBlock - 1) / kBlock;
-    const auto* b_scale = (const __attribute__((address_space(4))) float*)(uint64_t)p.b_scales + (int64_t)(n0 / kBlock) * blocks;
-    const uint8_t* b[NT];
-    const uint8_t* a[MB];
-    const float* a_scale[MB];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) b[j] = p.b + (int64_t)min(n0 + 16 * j + r, p.N - 1) * K;
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-        const int m = min(16 * i + r, p.M - 1);
-        a[i] = p.a + (int64_t)m * K;
-        a_scale[i] = p.a_scales + (int64_t)m * blocks;
-    }
-    f32x4 acc[NT][MB];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MB; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    struct Ahead {
-        i32x8 b[NT], a[MB];
-        float s[MB], sb;
-    } ahead[DEPTH];
-    auto fetch = [&](Ahead& x, int k) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) x.b[j] = load_part(b[j], k * kBlock, K, g);
-#pragma unroll
-        for (int i = 0; i < MB; ++i) {
-            x.a[i] = load_part(a[i], k * kBlock, K, g);
-            x.s[i] = a_scale[i][k];
-        }
-        x.sb = b_scale[k];
-    };
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d)
-        if (wave + d * WAVES < blocks) fetch(ahead[d], wave + d * WAVES);
-    for (int k = wave; k < blocks; k += DEPTH * WAVES) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            const int at = k + d * WAVES;
-            if (at >= blocks) break;
-            Ahead& x = ahead[d];
-#pragma unroll
-            for (int i = 0; i < MB; ++i) {
-                const float s = x.s[i] * x.sb;
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[j][i] += dot128<EXACT>(x.b[j], x.a[i]) * s;
-            }
-            if (at + DEPTH * WAVES < blocks) fetch(x, at + DEPTH * WAVES);
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MB; ++i) sums[wave][j * MB + i][lane] = acc[j][i];
-    __syncthreads();
-    const bool wide = (p.N & 3) == 0 && ((uintptr_t)p.out & (4 * sizeof(OUT) - 1)) == 0;
-#pragma unroll 1
-    for (int t = wave; t < NT * MB; t += WAVES) {
-        f32x4 v = sums[0][t][lane];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) v += sums[w][t][lane];
-        const int m = t % MB * 16 + r;
-        if (m < p.M) store4(static_cast<OUT*>(p.out) + (int64_t)m * p.N, n0 + t / MB * 16 + 4 * g, p.N, wide, v);
-    }
-}
-
-template <typename OUT, int NT, int MB, int WAVES, int DEPTH>
-void launch_few(const dsa_product_args& p, hipStream_t stream) {
-    const dim3 grid((p.N + 16 * NT - 1) / (16 * NT));
-    hipLaunchKernelGGL((product_few_kernel<OUT, NT, MB, WAVES, DEPTH>), grid, dim3(64 * WAVES), 0, stream, p);
-}
-
-template <typename OUT, int NT, int MB>
-void launch_few(const dsa_product_args& p, hipStream_t stream) {
-    constexpr int DEPTH = NT + MB <= 4 ? 4 : NT + MB <= 6 ? 3 : 2;
-    if (p.K <= 16 * kBlock) launch_few<OUT, NT, MB, 4, DEPTH>(p, stream);
-    else launch_few<OUT, NT, MB, 8, DEPTH>(p, stream);
-}
-
-template <typename OUT, int NT>
-void launch_few(const dsa_product_args& p, hipStream_t stream) {
-    if (p.M <= 16) launch_few<OUT, NT, 1>(p, stream);
-    else if (p.M <= 32) launch_few<OUT, NT, 2>(p, stream);
-    else if (p.M <= 64) launch_few<OUT, NT, 4>(p, stream);
-    else if (p.M <= 96) launch_few<OUT, NT, 6>(p, stream);
-    else launch_few<OUT, NT, 8>(p, stream);
 }
 
 // ------------------------------------------------------------------ tiles
@@ -211,13 +103,20 @@ template <int NT, int MT, int WN, int WM, int KS, int STAGES>
 struct Tile {
     static constexpr int TN = 16 * NT * WN, TM = 16 * MT * WM, GROUP = WN * WM, WAVES = GROUP * KS, THREADS = 64 * WAVES;
     static constexpr int B_LOADS = (TN + 8 * GROUP - 1) / (8 * GROUP), A_LOADS = (TM + 8 * GROUP - 1) / (8 * GROUP);  // a wave, of 8 rows each
-    static constexpr int S_WAVES = (TM + 63) / 64;  // loads of 64 scales each
-    static constexpr int LOADS = B_LOADS + A_LOADS + 1;
-    static constexpr int A_OFF = B_LOADS * GROUP * 8 * kBlock, S_OFF = A_OFF + A_LOADS * GROUP * 8 * kBlock;
-    static constexpr int BLOCK = S_OFF + S_WAVES * 256, STAGE = BLOCK * KS;
+    static constexpr int LOADS = B_LOADS + A_LOADS;
+    static constexpr int A_OFF = B_LOADS * GROUP * 8 * kBlock, BLOCK = A_OFF + A_LOADS * GROUP * 8 * kBlock, STAGE = BLOCK * KS;
+    // Scales come 8 or 16 blocks of a row at a time, a row's 32 or 64 bytes, four or eight rows a load.
+    static constexpr int S_BLOCKS = KS * (STAGES - 1) > 8 ? 16 : 8, S_STEPS = S_BLOCKS / KS, S_ROWS = 64 / S_BLOCKS;
+    static constexpr int S_LOADS = (TM + S_ROWS * WAVES - 1) / (S_ROWS * WAVES);
+    static constexpr int S_OFF = STAGES * STAGE, SB_OFF = S_LOADS * WAVES * 256, S_BYTES = SB_OFF + 256;
     static constexpr int JOIN_BYTES = KS > 1 ? WAVES * NT * MT * 1024 : 0;
-    static constexpr int LDS_BYTES = STAGES * STAGE > JOIN_BYTES ? STAGES * STAGE : JOIN_BYTES;
-    static_assert(S_WAVES <= GROUP, "a scale load a wave");
+    static constexpr int RING_BYTES = S_OFF + 2 * S_BYTES, LDS_BYTES = RING_BYTES > JOIN_BYTES ? RING_BYTES : JOIN_BYTES;
+    // With two stages, the part of a stage that is read first -- the rows of a, and of
+    // the weights half of each wave's -- is loaded again within the step that reads it.
+    static constexpr bool HALVES = STAGES == 2 && NT % 2 == 0 && B_LOADS % 2 == 0 && TN % (8 * GROUP) == 0 && KS == 1;
+    static constexpr int EARLY = A_LOADS + B_LOADS / 2;
+    static constexpr int AHEAD = HALVES ? EARLY : (STAGES - 2) * LOADS;  // loads that may be in flight when a step begins
+    static_assert(S_BLOCKS % KS == 0 && S_STEPS >= STAGES - 1, "scales have landed by the step that needs them");
     static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
     static_assert((STAGES - 1) * LOADS < 64, "loads in flight are counted in six bits");
     // a wave's columns lie in one block of weights
@@ -245,83 +144,124 @@ __global__ __launch_bounds__(64 * WN * WM * KS, 1) void product_tile_kernel(dsa_
     // swizzle but for bit 2.
     const int in8 = lane >> 3;
     const uint32_t chunk = 16u * ((uint32_t)(lane & 7) ^ swizzle(in8));
-    // A group's block of step t: behind the last one nothing is read, but the loads are
-    // the same, so that they can be counted on.  Rows behind the last are out of the
-    // descriptors' range, and so zeros.
-    auto issue = [&](int t) __attribute__((always_inline)) {
-        const uint32_t stage = lds + (uint32_t)(t % STAGES) * T::STAGE + (uint32_t)group * T::BLOCK;
-        const int k = t * KS + group, at = k * kBlock, left = K - at;  // bytes of a row from here on
+    // Load i of a group's block of step t: behind the last one nothing is read, but the
+    // loads are the same, so that they can be counted on.  Rows behind the last are out
+    // of the descriptors' range, and so zeros.
+    struct Next {
+        rsrc_t b, a;
+        uint32_t stage;
+        int left;  // bytes of a row from the block on
+    };
+    auto next_at = [&](int t, uint32_t stage) __attribute__((always_inline)) -> Next {
+        const int k = t * KS + group, at = k * kBlock;
         const bool on = k < blocks;
-        const rsrc_t rb = make_rsrc(b_base + at, on ? (uint32_t)(rows_n * K - at) : 0u);
-        const rsrc_t ra = make_rsrc(a_base + at, on ? (uint32_t)(rows_m * K - at) : 0u);
-        auto offset = [&](int first) __attribute__((always_inline)) -> uint32_t {
-            const uint32_t c = chunk ^ (first & 8 ? 64u : 0u);
-            return (int)c < left ? (uint32_t)((first + in8) * K) + c : 0x80000000u;  // behind the row's end: zeros
-        };
-#pragma unroll
-        for (int i = 0; i < T::B_LOADS; ++i) {
-            const int first = (in_group * T::B_LOADS + i) * 8;
-            gather_lanes(stage + (uint32_t)first * kBlock, rb, offset(first));
+        return Next{make_rsrc(b_base + at, on ? (uint32_t)(rows_n * K - at) : 0u),
+                    make_rsrc(a_base + at, on ? (uint32_t)(rows_m * K - at) : 0u), lds + stage + (uint32_t)group * T::BLOCK, K - at};
+    };
+    auto issue = [&](const Next& n, int i) __attribute__((always_inline)) {
+        const bool of_b = i >= T::A_LOADS;
+        int first = of_b ? (in_group * T::B_LOADS + i - T::A_LOADS) * 8 : (in_group * T::A_LOADS + i) * 8;
+        if (T::HALVES && of_b) {  // first the rows 0 .. 8 NT - 1 of each 16 NT, then the others
+            const int half = i - T::A_LOADS >= T::B_LOADS / 2, at = in_group * (T::B_LOADS / 2) + (i - T::A_LOADS) % (T::B_LOADS / 2);
+            first = at / NT * 16 * NT + half * 8 * NT + at % NT * 8;
         }
+        const uint32_t c = chunk ^ (first & 8 ? 64u : 0u);
+        const uint32_t off = (int)c < n.left ? (uint32_t)((first + in8) * K) + c : 0x80000000u;  // behind the row's end: zeros
+        gather_lanes(n.stage + (of_b ? 0 : T::A_OFF) + (uint32_t)first * kBlock, of_b ? n.b : n.a, off);
+    };
+    const rsrc_t rs = make_rsrc(s_base, (uint32_t)(4 * rows_m * blocks));
+    const rsrc_t rsb = make_rsrc(p.b_scales + (int64_t)(n0 / kBlock) * blocks, (uint32_t)(4 * ((rows_n + kBlock - 1) / kBlock) * blocks));
+    const int s_row = lane / T::S_BLOCKS, s_block = lane % T::S_BLOCKS;
+    auto issue_scales = [&](int c) __attribute__((always_inline)) {  // of blocks c * S_BLOCKS on
+        const uint32_t to = lds + T::S_OFF + (uint32_t)(c & 1) * T::S_BYTES;
+        const int k = c * T::S_BLOCKS + s_block;
+        if (wave == 0)  // the weights': those of 128 columns as those of a row
+            gather_word(to + T::SB_OFF, rsb, k < blocks ? (uint32_t)(4 * (s_row * blocks + k)) : 0x80000000u);
 #pragma unroll
-        for (int i = 0; i < T::A_LOADS; ++i) {
-            const int first = (in_group * T::A_LOADS + i) * 8;
-            gather_lanes(stage + T::A_OFF + (uint32_t)first * kBlock, ra, offset(first));
+        for (int i = 0; i < T::S_LOADS; ++i) {
+            const int first = (wave * T::S_LOADS + i) * T::S_ROWS;
+            gather_word(to + (uint32_t)first * (4 * T::S_BLOCKS), rs,
+                        k < blocks ? (uint32_t)(4 * ((first + s_row) * blocks + k)) : 0x80000000u);
         }
-        const int part = in_group % T::S_WAVES;  // some are loaded twice, the same
-        gather_word(stage + T::S_OFF + (uint32_t)part * 256u,
-                    make_rsrc(s_base + 4 * k, on ? (uint32_t)(4 * (rows_m * blocks - k)) : 0u),
-                    (uint32_t)(4 * (64 * part + lane) * blocks));
     };
     const int wn = in_group % WN, wm = in_group / WN;
-    const int band = min(n0 + 16 * NT * wn, p.N - 1) / kBlock;
-    // a scalar load: the compiler does not count the loads to LDS, and would wait for all of them with one of its own
-    const auto* b_scale = (const __attribute__((address_space(4))) float*)(uint64_t)p.b_scales + (int64_t)band * blocks;
     // fragment reads: chunk g (and 4 + g: ^ 64) of row r of a 16-row tile
     const uint32_t frag = (uint32_t)r * kBlock + 16u * ((uint32_t)g ^ swizzle(r));
     const uint32_t b_frag = frag + (uint32_t)wn * NT * 16 * kBlock, a_frag = frag + T::A_OFF + (uint32_t)wm * MT * 16 * kBlock;
-    const uint32_t s_frag = T::S_OFF + 4u * (uint32_t)(wm * MT * 16 + r);
+    const uint32_t s_frag = lds + T::S_OFF + 4u * T::S_BLOCKS * (uint32_t)(wm * MT * 16 + r);
+    const uint32_t sb_frag = lds + T::S_OFF + T::SB_OFF + 4u * T::S_BLOCKS * (uint32_t)((n0 % kBlock + 16 * NT * wn) / kBlock);
     f32x4 acc[NT][MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    issue_scales(0);
 #pragma unroll
-    for (int t = 0; t < STAGES - 1; ++t) issue(t);
-    float sb = b_scale[min(group, blocks - 1)];
+    for (int t = 0; t < STAGES - 1; ++t) {
+        const Next n = next_at(t, (uint32_t)t * T::STAGE);
+#pragma unroll
+        for (int i = 0; i < T::LOADS; ++i) issue(n, i);
+    }
+    if (T::HALVES) {
+        const Next n = next_at(1, T::STAGE);
+#pragma unroll
+        for (int i = 0; i < T::EARLY; ++i) issue(n, i);
+    }
+    uint32_t at = 0, ahead = (STAGES - 1) * T::STAGE;
 #pragma unroll 1
     for (int t = 0; t < steps; ++t) {
-        wait_vmcnt<(STAGES - 2) * T::LOADS>();
+        wait_vmcnt<T::AHEAD>();
         lds_barrier();  // stage t is there, and every wave is done with stage t - 1
-        issue(t + STAGES - 1);
         const int k = t * KS + group;
-        if (KS > 1 && k >= blocks) break;  // the last step, of a group that has none: no barrier follows but the one below
-        const uint32_t stage = lds + (uint32_t)(t % STAGES) * T::STAGE + (uint32_t)group * T::BLOCK;
+        const uint32_t stage = lds + at + (uint32_t)group * T::BLOCK;
         const uint32_t b_lo = stage + b_frag, b_hi = b_lo ^ 64u, a_lo = stage + a_frag, a_hi = a_lo ^ 64u;
         auto read = [&](uint32_t lo, uint32_t hi, int tile) __attribute__((always_inline)) -> i32x8 {
             const i32x4 l = lds_load<i32x4>(lo + tile * 16 * kBlock), h = lds_load<i32x4>(hi + tile * 16 * kBlock);
             return __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7);
         };
+        if (KS > 1 && k >= blocks) break;  // the last step, of a group that has no block: only the barriers of the end follow
         i32x8 af[MT], bf[2];
         float s[MT];
         bf[0] = read(b_lo, b_hi, 0);
 #pragma unroll
         for (int i = 0; i < MT; ++i) af[i] = read(a_lo, a_hi, i);
+        const uint32_t chunk_at = (uint32_t)(k / T::S_BLOCKS & 1) * T::S_BYTES + 4u * (uint32_t)(k % T::S_BLOCKS);
+        const float sb = lds_load<float>(sb_frag + chunk_at);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) s[i] = lds_load<float>(stage + s_frag + 64 * i) * sb;
-        sb = b_scale[min(k + KS, blocks - 1)];
-        // products of tile j beside the sums of tile j - 1
+        for (int i = 0; i < MT; ++i) s[i] = lds_load<float>(s_frag + chunk_at + 64 * T::S_BLOCKS * i);
+        if (t % T::S_STEPS == 0) issue_scales(t / T::S_STEPS + 1);
+        const Next n = next_at(t + STAGES - 1, ahead);
+        const Next n2 = next_at(t + 2, at);
+        // products of tile j beside the sums of tile j - 1, and a few loads
         f32x4 u[2][MT];
 #pragma unroll
         for (int j = 0; j <= NT; ++j) {
             if (j + 1 < NT) bf[(j + 1) & 1] = read(b_lo, b_hi, j + 1);
+            if constexpr (T::HALVES) {
+                // the last loads of stage t + 1, then, when all waves have read the first
+                // part of stage t (tiles up to NT / 2 - 1 are in registers), those of t + 2
+#pragma unroll
+                for (int i = T::EARLY; i < T::LOADS; ++i)
+                    if (i - T::EARLY == j) issue(n, i);
+                if (j == NT / 2 - 1) lds_barrier();
+#pragma unroll
+                for (int i = 0; i < T::EARLY; ++i)
+                    if (j >= NT / 2 - 1 && j < NT && i * (NT / 2 + 1) / T::EARLY == j - (NT / 2 - 1)) issue(n2, i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < T::LOADS; ++i)
+                    if (i * NT / T::LOADS == j) issue(n, i);
+            }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
+                if (j == 0) s[i] *= sb;
                 if (j < NT) u[j & 1][i] = dot128<EXACT>(bf[j & 1], af[i]);
                 if (j > 0) acc[j - 1][i] += u[(j - 1) & 1][i] * s[i];
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        at = at + T::STAGE == T::S_OFF ? 0 : at + T::STAGE;
+        ahead = ahead + T::STAGE == T::S_OFF ? 0 : ahead + T::STAGE;
     }
     wait_vmcnt<0>();  // loads behind the last block write zeros into LDS
     const bool wide = (p.N & 3) == 0 && ((uintptr_t)p.out & (4 * sizeof(OUT) - 1)) == 0;
@@ -336,19 +276,19 @@ __global__ __launch_bounds__(64 * WN * WM * KS, 1) void product_tile_kernel(dsa_
             for (int j = 0; j < NT; ++j) store(j, i, acc[j][i]);
     } else {  // the groups' sums, in their order: a group joins every KS-th tile
         lds_barrier();
-        auto at = [&](int of, int tile) __attribute__((always_inline)) -> uint32_t {
+        auto part = [&](int of, int tile) __attribute__((always_inline)) -> uint32_t {
             return lds + (uint32_t)(((of * T::GROUP + in_group) * NT * MT + tile) * 1024 + 16 * lane);
         };
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) lds_store<f32x4>(at(group, j * MT + i), acc[j][i]);
+            for (int i = 0; i < MT; ++i) lds_store<f32x4>(part(group, j * MT + i), acc[j][i]);
         lds_barrier();
 #pragma unroll 1
         for (int tile = group; tile < NT * MT; tile += KS) {
-            f32x4 v = lds_load<f32x4>(at(0, tile));
+            f32x4 v = lds_load<f32x4>(part(0, tile));
 #pragma unroll
-            for (int of = 1; of < KS; ++of) v += lds_load<f32x4>(at(of, tile));
+            for (int of = 1; of < KS; ++of) v += lds_load<f32x4>(part(of, tile));
             store(tile / MT, tile % MT, v);
         }
     }
@@ -362,25 +302,49 @@ void launch_tile(const dsa_product_args& p, hipStream_t stream) {
                        tiles_m, tiles_n);
 }
 
-template <typename OUT>
-void launch_typed(const dsa_product_args& p, hipStream_t stream) {
-    if (p.M > 128) {
-        if constexpr (sizeof(OUT) == 4) launch_tile<OUT, 4, 4, 2, 4, 1, 2>(p, stream);
-        else launch_tile<OUT, 8, 4, 2, 4, 1, 2>(p, stream);
-    } else {
-        if (p.N >= 32 * 224) launch_few<OUT, 2>(p, stream);
-        else launch_few<OUT, 1>(p, stream);
-    }
-}
+// Tiles by the size of the call.  With one workgroup a CU (their stages fill the
+// LDS) a call takes as many rounds as its tiles fill CUs; a round takes its steps and
+// a start and end of about 2 us.  Microseconds a step, measured on 33 to 256
+// workgroups (K 1536 to 16384): what follows `step`.  Small tiles split K over their
+// waves, which makes fewer steps of few columns.  Whole calls, us, smallest tile to
+// largest that were tried (rows, columns, K):
+//   16, 2112, 7168     16x16 9.7, 32x32 11.8, 64x32 15.4, 64x64 16.6, 128x64 30.6
+//   64, 2112, 7168     16x16 16, 32x32 12.3, 64x32 16.1, 64x64 20, 128x64 31.7, 128x128 35
+//   16, 24576, 1536    32x32 14, 64x32 12.1, 128x32 9.8, 128x64 10.3, 128x128 10.8
+//   256, 2112, 7168    32x32 30, 64x32 29, 64x64 19, 128x32 25, 128x64 31, 128x128 38
+//   1024, 2112, 7168   64x64 50, 128x64 61, 128x80 35, 128x128 38, 128x256 63, 256x256 88
+//   1024, 7168, 16384  64x64 239, 128x80 216, 128x128 168, 128x256 149, 256x256 189
+//   1024, 24576, 1536  128x128 76, 128x256 65, 256x256 63
+struct Variant {
+    int columns, rows, blocks;  // of a tile, and blocks of K a step
+    float step;
+    void (*launch[3])(const dsa_product_args&, hipStream_t);  // by type
+};
+#define DSA_TILE(...) {launch_tile<__bf16, __VA_ARGS__>, launch_tile<f16, __VA_ARGS__>, launch_tile<float, __VA_ARGS__>}
+const Variant kVariants[] = {
+    {16, 16, 8, 0.90f, DSA_TILE(1, 1, 1, 1, 8, 2)},  {32, 16, 4, 0.60f, DSA_TILE(1, 1, 2, 1, 4, 3)},
+    {32, 32, 4, 0.70f, DSA_TILE(1, 2, 2, 1, 4, 3)},  {64, 32, 2, 0.48f, DSA_TILE(1, 2, 4, 1, 2, 4)},
+    {64, 64, 2, 0.59f, DSA_TILE(2, 2, 2, 2, 2, 4)},  {128, 32, 1, 0.39f, DSA_TILE(1, 2, 8, 1, 1, 4)},
+    {128, 64, 1, 0.51f, DSA_TILE(1, 4, 8, 1, 1, 4)}, {128, 80, 1, 0.55f, DSA_TILE(1, 5, 8, 1, 1, 4)},
+    {128, 128, 1, 0.61f, DSA_TILE(2, 4, 4, 2, 1, 4)}, {128, 256, 1, 1.07f, DSA_TILE(4, 4, 2, 4, 1, 2)},
+    {256, 256, 1, 1.60f, DSA_TILE(8, 4, 2, 4, 1, 2)},
+};
 
 }  // namespace
 
 int64_t product_ws_bytes(const dsa_product_args&) { return 0; }
 
-int launch_product(const dsa_product_args& p, hipStream_t stream) {
-    if (p.dtype == DSA_BF16) launch_typed<__bf16>(p, stream);
-    else if (p.dtype == DSA_F16) launch_typed<f16>(p, stream);
-    else launch_typed<float>(p, stream);
+int launch_product(const dsa_product_args& p, int cus, hipStream_t stream) {
+    const int blocks = (p.K + kBlock - 1) / kBlock;
+    const Variant* best = nullptr;
+    float least = 0.f;
+    for (const Variant& v : kVariants) {
+        if (p.dtype == DSA_F32 && v.rows * v.columns > 128 * 256) continue;  // the widened codes need its registers
+        const int64_t tiles = (int64_t)((p.M + v.rows - 1) / v.rows) * ((p.N + v.columns - 1) / v.columns);
+        const float time = (float)((tiles + cus - 1) / cus) * (2.f + v.step * (float)((blocks + v.blocks - 1) / v.blocks));
+        if (!best || time < least) best = &v, least = time;
+    }
+    best->launch[p.dtype](p, stream);
     return (int)hipGetLastError();
 }
 
