@@ -42,6 +42,25 @@ struct Eight<float> {
     }
 };
 
+// Values [e, e + 8) of a row as they lie in memory, zeros behind its end: half the
+// registers of their 32-bit values, for what is loaded ahead.
+template <typename T>
+struct Ahead {
+    Eight<T> v;
+    __device__ __forceinline__ void load(const T* row, int e, int dim, bool vector) {
+        if (vector) {
+            if (e < dim) v.load(row + e);
+            else v = Eight<T>{};
+        } else {
+            T t[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = e + i < dim ? row[e + i] : (T)0.f;
+            __builtin_memcpy(&v, t, sizeof t);
+        }
+    }
+    __device__ __forceinline__ float at(int i) const { return v.at(i); }
+};
+
 // Values [e, e + 8) of a row of dim, zeros behind its end.  `vector`: the row is
 // 16-byte aligned and dim a multiple of eight.
 template <typename T>
@@ -263,21 +282,42 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void norm_grad_kerne
 #pragma unroll
         for (int i = 0; i < 8; ++i) sums[c][i] = 0.f;
     }
-    int turn = 0;
-    for (int64_t r = team; r < p.rows; r += teams, ++turn) {
-        const float inverse = p.inverse[r];
-        float u[CH][8], b[CH][8], mean = 0.f;
+    // a row ahead, where there are registers for it: its loads are on their way while the
+    // one before is summed and stored
+    constexpr bool AHEAD = WAVES * CH < 32;
+    Ahead<T> next_h[CH], next_out[CH], next_sum[CH];
+    float next_inverse = 0.f;
+    auto fetch = [&](int64_t r) __attribute__((always_inline)) {
+        next_inverse = p.inverse[r];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int e = (c * TEAM + tid) * 8;
-            load8(u[c], static_cast<const T*>(p.h) + r * p.h_stride, e, dim, vector);
-            load8(b[c], static_cast<const T*>(p.grad_out) + r * dim, e, dim, vector);
+            next_h[c].load(static_cast<const T*>(p.h) + r * p.h_stride, e, dim, vector);
+            next_out[c].load(static_cast<const T*>(p.grad_out) + r * dim, e, dim, vector);
+            if (p.grad_sum) next_sum[c].load(static_cast<const T*>(p.grad_sum) + r * dim, e, dim, vector);
         }
+    };
+    if (AHEAD && team < p.rows) fetch(team);
+    int turn = 0;
+    for (int64_t r = team; r < p.rows; r += teams, ++turn) {
+        if (!AHEAD) fetch(r);
+        const float inverse = next_inverse;
+        float u[CH][8], b[CH][8], mean = 0.f;
+        Ahead<T> given[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            given[c] = next_sum[c];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                u[c][i] = next_h[c].at(i) * inverse;
+                b[c][i] = next_out[c].at(i);
+            }
+        }
+        if (AHEAD && r + teams < p.rows) fetch(r + teams);
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                u[c][i] *= inverse;
                 sums[c][i] = fmaf(b[c][i], u[c][i], sums[c][i]);
                 b[c][i] *= w[c][i];
                 mean = fmaf(b[c][i], u[c][i], mean);
@@ -285,16 +325,13 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void norm_grad_kerne
         mean = team_sum<WAVES>(mean, parts, turn) / (float)dim;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int e = (c * TEAM + tid) * 8;
-            float given[8];
-            if (p.grad_sum) load8(given, static_cast<const T*>(p.grad_sum) + r * dim, e, dim, vector);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float v = (b[c][i] - u[c][i] * mean) * inverse;
-                if (p.grad_sum) v += given[i];
+                if (p.grad_sum) v += given[c].at(i);
                 b[c][i] = v;
             }
-            store8(static_cast<T*>(p.grad_in) + r * dim, b[c], e, dim, vector);
+            store8(static_cast<T*>(p.grad_in) + r * dim, b[c], (c * TEAM + tid) * 8, dim, vector);
         }
     }
     if (p.grad_weight) {
@@ -304,17 +341,22 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void norm_grad_kerne
     }
 }
 
-constexpr int kSumColumns = 64, kSumGroups = 16;
+// The teams' sums of 32 columns: 32 groups of threads take every 32nd team, and are
+// added in their order.
+constexpr int kSumColumns = 32, kSumGroups = 32;
 template <typename W>
 __global__ __launch_bounds__(kSumColumns* kSumGroups) void norm_weight_kernel(const float* parts, W* out, int teams, int dim) {
     __shared__ float sums[kSumGroups][kSumColumns];
-    const int column = threadIdx.x & 63, group = threadIdx.x >> 6, at = blockIdx.x * kSumColumns + column;
+    const int column = threadIdx.x % kSumColumns, group = threadIdx.x / kSumColumns, at = blockIdx.x * kSumColumns + column;
     float s = 0.f;
-    if (at < dim)
+    if (at < dim) {
+#pragma unroll 16
         for (int t = group; t < teams; t += kSumGroups) s += parts[(int64_t)t * dim + at];
+    }
     sums[group][column] = s;
     __syncthreads();
     if (group == 0 && at < dim) {
+#pragma unroll
         for (int g = 1; g < kSumGroups; ++g) s += sums[g][column];
         out[at] = (W)s;
     }
