@@ -87,12 +87,15 @@ __device__ __forceinline__ void store4(OUT* row, int n, int N, bool wide, const 
 // of one lane group, 4-11 of the next) meet 16 different bank groups.
 __device__ __forceinline__ uint32_t swizzle(int row) { return (uint32_t)(row >> 1) & 7u; }
 
-// A workgroup's tile.  Every eighth workgroup is on the same XCD: each XCD gets a run of
-// tiles, ordered in bands of up to eight tiles of rows, so that the tiles that run
-// there together share rows and columns in its L2.
-__device__ __forceinline__ void place(int tiles_m, int tiles_n, int& m, int& n) {
-    const uint32_t total = (uint32_t)(tiles_m * tiles_n), each = total / 8, rest = total % 8;
-    const uint32_t xcd = blockIdx.x % 8, t = xcd * each + min(xcd, rest) + blockIdx.x / 8;
+// Workgroup i of `total` counted along the XCDs: every eighth is on the same one, and
+// each XCD gets a run of them.
+__device__ __forceinline__ uint32_t along_xcds(uint32_t i, uint32_t total) {
+    const uint32_t each = total / 8, rest = total % 8, xcd = i % 8;
+    return xcd * each + min(xcd, rest) + i / 8;
+}
+// Tile t, in bands of up to eight tiles of rows, so that the tiles that run together on
+// an XCD share rows and columns in its L2.
+__device__ __forceinline__ void place(uint32_t t, int tiles_m, int tiles_n, int& m, int& n) {
     const uint32_t band = t / (uint32_t)(8 * tiles_n), in_band = t % (uint32_t)(8 * tiles_n);
     const uint32_t high = min(8u, (uint32_t)tiles_m - 8 * band);
     m = (int)(8 * band + in_band % high);
@@ -124,17 +127,12 @@ struct Tile {
 };
 
 template <typename OUT, int NT, int MT, int WN, int WM, int KS, int STAGES>
-__global__ __launch_bounds__(64 * WN * WM * KS, 1) void product_tile_kernel(dsa_product_args p, int tiles_m, int tiles_n) {
+__device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t lds, int m0, int n0) {
     constexpr bool EXACT = sizeof(OUT) == 4;
     using T = Tile<NT, MT, WN, WM, KS, STAGES>;
-    __shared__ __attribute__((aligned(1024))) char smem[T::LDS_BYTES];
-    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int group = KS > 1 ? wave / T::GROUP : 0, in_group = KS > 1 ? wave % T::GROUP : wave;
     const int r = lane & 15, g = lane >> 4;
-    int tile_m, tile_n;
-    place(tiles_m, tiles_n, tile_m, tile_n);
-    const int m0 = tile_m * T::TM, n0 = tile_n * T::TN;
     const int K = p.K, blocks = (K + kBlock - 1) / kBlock, steps = (blocks + KS - 1) / KS;
     const int rows_m = min(T::TM, p.M - m0), rows_n = min(T::TN, p.N - n0);
     const char* b_base = reinterpret_cast<const char*>(p.b) + (int64_t)n0 * K;
@@ -295,11 +293,51 @@ __global__ __launch_bounds__(64 * WN * WM * KS, 1) void product_tile_kernel(dsa_
 }
 
 template <typename OUT, int NT, int MT, int WN, int WM, int KS, int STAGES>
+__global__ __launch_bounds__(64 * WN * WM * KS, 1) void product_tile_kernel(dsa_product_args p, int tiles_m, int tiles_n) {
+    using T = Tile<NT, MT, WN, WM, KS, STAGES>;
+    __shared__ __attribute__((aligned(1024))) char smem[T::LDS_BYTES];
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+    int m, n;
+    place(along_xcds(blockIdx.x, tiles_m * tiles_n), tiles_m, tiles_n, m, n);
+    product_tile<OUT, NT, MT, WN, WM, KS, STAGES>(p, lds, m * T::TM, n * T::TN);
+}
+
+// Tiles of 256 by 256 for whole rounds of them, and those left over cut in two: a last
+// round of 128 columns by 256 rows, of two thirds the time.
+using Whole = Tile<8, 4, 2, 4, 1, 2>;
+using Half = Tile<4, 4, 2, 4, 1, 2>;
+template <typename OUT>
+__global__ __launch_bounds__(Whole::THREADS, 1) void product_mixed_kernel(dsa_product_args p, int tiles_m, int tiles_n, int whole) {
+    static_assert(Whole::THREADS == Half::THREADS && Whole::TM == Half::TM && Whole::TN == 2 * Half::TN, "two halves");
+    __shared__ __attribute__((aligned(1024))) char smem[Whole::LDS_BYTES];
+    static_assert(Half::LDS_BYTES <= Whole::LDS_BYTES, "one LDS");
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+    int m, n;
+    if ((int)blockIdx.x < whole) {
+        place(along_xcds(blockIdx.x, whole), tiles_m, tiles_n, m, n);
+        product_tile<OUT, 8, 4, 2, 4, 1, 2>(p, lds, m * Whole::TM, n * Whole::TN);
+    } else {
+        const uint32_t i = along_xcds(blockIdx.x - whole, 2 * (tiles_m * tiles_n - whole));
+        place(whole + i / 2, tiles_m, tiles_n, m, n);
+        const int n0 = n * Whole::TN + (int)(i & 1) * Half::TN;
+        if (n0 < p.N) product_tile<OUT, 4, 4, 2, 4, 1, 2>(p, lds, m * Half::TM, n0);
+    }
+}
+
+template <typename OUT, int NT, int MT, int WN, int WM, int KS, int STAGES>
 void launch_tile(const dsa_product_args& p, hipStream_t stream) {
     using T = Tile<NT, MT, WN, WM, KS, STAGES>;
     const int tiles_m = (p.M + T::TM - 1) / T::TM, tiles_n = (p.N + T::TN - 1) / T::TN;
     hipLaunchKernelGGL((product_tile_kernel<OUT, NT, MT, WN, WM, KS, STAGES>), dim3(tiles_m * tiles_n), dim3(T::THREADS), 0, stream, p,
                        tiles_m, tiles_n);
+}
+
+template <typename OUT>
+void launch_mixed(const dsa_product_args& p, int cus, hipStream_t stream) {
+    const int tiles_m = (p.M + Whole::TM - 1) / Whole::TM, tiles_n = (p.N + Whole::TN - 1) / Whole::TN;
+    const int tiles = tiles_m * tiles_n, whole = tiles / cus * cus;
+    hipLaunchKernelGGL((product_mixed_kernel<OUT>), dim3(whole + 2 * (tiles - whole)), dim3(Whole::THREADS), 0, stream, p, tiles_m,
+                       tiles_n, whole);
 }
 
 // Tiles by the size of the call.  With one workgroup a CU (their stages fill the
@@ -327,8 +365,8 @@ const Variant kVariants[] = {
     {64, 64, 2, 0.59f, DSA_TILE(2, 2, 2, 2, 2, 4)},  {128, 32, 1, 0.39f, DSA_TILE(1, 2, 8, 1, 1, 4)},
     {128, 64, 1, 0.51f, DSA_TILE(1, 4, 8, 1, 1, 4)}, {128, 80, 1, 0.55f, DSA_TILE(1, 5, 8, 1, 1, 4)},
     {128, 128, 1, 0.61f, DSA_TILE(2, 4, 4, 2, 1, 4)}, {128, 256, 1, 1.07f, DSA_TILE(4, 4, 2, 4, 1, 2)},
-    {256, 256, 1, 1.60f, DSA_TILE(8, 4, 2, 4, 1, 2)},
 };
+constexpr float kWholeStep = 1.70f, kHalfStep = 1.07f;  // of the mixed kernel
 
 }  // namespace
 
@@ -339,10 +377,19 @@ int launch_product(const dsa_product_args& p, int cus, hipStream_t stream) {
     const Variant* best = nullptr;
     float least = 0.f;
     for (const Variant& v : kVariants) {
-        if (p.dtype == DSA_F32 && v.rows * v.columns > 128 * 256) continue;  // the widened codes need its registers
         const int64_t tiles = (int64_t)((p.M + v.rows - 1) / v.rows) * ((p.N + v.columns - 1) / v.columns);
         const float time = (float)((tiles + cus - 1) / cus) * (2.f + v.step * (float)((blocks + v.blocks - 1) / v.blocks));
         if (!best || time < least) best = &v, least = time;
+    }
+    if (p.dtype != DSA_F32) {  // the widened codes of 32-bit outputs would need more registers
+        const int64_t tiles = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256), rest = tiles % cus;
+        const float time = (float)(tiles / cus) * (2.f + kWholeStep * (float)blocks) +
+                           (float)((2 * rest + cus - 1) / cus) * (2.f + kHalfStep * (float)blocks);
+        if (time < least) {
+            if (p.dtype == DSA_BF16) launch_mixed<__bf16>(p, cus, stream);
+            else launch_mixed<f16>(p, cus, stream);
+            return (int)hipGetLastError();
+        }
     }
     best->launch[p.dtype](p, stream);
     return (int)hipGetLastError();
