@@ -340,31 +340,33 @@ void launch_mixed(const dsa_product_args& p, int cus, hipStream_t stream) {
                        tiles_n, whole);
 }
 
-// Tiles by the size of the call.  With one workgroup a CU (their stages fill the
-// LDS) a call takes as many rounds as its tiles fill CUs; a round takes its steps and
-// a start and end of about 2 us.  Microseconds a step, measured on 33 to 256
-// workgroups (K 1536 to 16384): what follows `step`.  Small tiles split K over their
-// waves, which makes fewer steps of few columns.  Whole calls, us, smallest tile to
-// largest that were tried (rows, columns, K):
-//   16, 2112, 7168     16x16 9.7, 32x32 11.8, 64x32 15.4, 64x64 16.6, 128x64 30.6
-//   64, 2112, 7168     16x16 16, 32x32 12.3, 64x32 16.1, 64x64 20, 128x64 31.7, 128x128 35
-//   16, 24576, 1536    32x32 14, 64x32 12.1, 128x32 9.8, 128x64 10.3, 128x128 10.8
-//   256, 2112, 7168    32x32 30, 64x32 29, 64x64 19, 128x32 25, 128x64 31, 128x128 38
-//   1024, 2112, 7168   64x64 50, 128x64 61, 128x80 35, 128x128 38, 128x256 63, 256x256 88
+// Tiles by the size of the call: a call takes as many rounds as its tiles fill CUs, and
+// a round its steps, and a start and end of about 2 us.  What a step takes was measured
+// on 17 to 256 workgroups with K from 1536 to 16384, and, where the stages of two
+// workgroups fit a CU's LDS, on 264 to 512.  Small tiles split K over their waves, so
+// that there are fewer steps.  Whole calls, us (rows, columns, K; columns x rows of a
+// tile, in `kVariants`' order):
+//   8, 2112, 7168      16x16 7.3, 32x16 10.4, 32x32 11.7, 64x32 14
+//   64, 2112, 7168     16x16 14.3, 32x32 11.5, 64x32 16.3, 64x64 20.5 and 21.4, 128x64 31.6
+//   16, 24576, 1536    16x16 13.4, 32x32 14.4, 64x32 12.4, 64x64 13.2 and 10.5, 128x32 10.0, 128x64 10.4
+//   512, 2112, 7168    32x32 45, 64x64 33.8 and 28.0, 128x32 46, 128x64 31.4, 128x128 37.3
+//   1000, 2112, 7168   64x64 49.0 and 45.5, 128x64 60.6, 128x80 34.4, 128x128 37.3, 128x256 63
 //   1024, 7168, 16384  64x64 239, 128x80 216, 128x128 168, 128x256 149, 256x256 189
 //   1024, 24576, 1536  128x128 76, 128x256 65, 256x256 63
+// Over 44 drawn calls of these ranges the chosen tile took 3 % longer than the best one.
 struct Variant {
     int columns, rows, blocks;  // of a tile, and blocks of K a step
-    float step;
+    float step, both;           // us a step, alone on a CU and beside another; 0: does not fit beside another
     void (*launch[3])(const dsa_product_args&, hipStream_t);  // by type
 };
 #define DSA_TILE(...) {launch_tile<__bf16, __VA_ARGS__>, launch_tile<f16, __VA_ARGS__>, launch_tile<float, __VA_ARGS__>}
 const Variant kVariants[] = {
-    {16, 16, 8, 0.90f, DSA_TILE(1, 1, 1, 1, 8, 2)},  {32, 16, 4, 0.60f, DSA_TILE(1, 1, 2, 1, 4, 3)},
-    {32, 32, 4, 0.70f, DSA_TILE(1, 2, 2, 1, 4, 3)},  {64, 32, 2, 0.48f, DSA_TILE(1, 2, 4, 1, 2, 4)},
-    {64, 64, 2, 0.59f, DSA_TILE(2, 2, 2, 2, 2, 4)},  {128, 32, 1, 0.39f, DSA_TILE(1, 2, 8, 1, 1, 4)},
-    {128, 64, 1, 0.51f, DSA_TILE(1, 4, 8, 1, 1, 4)}, {128, 80, 1, 0.55f, DSA_TILE(1, 5, 8, 1, 1, 4)},
-    {128, 128, 1, 0.61f, DSA_TILE(2, 4, 4, 2, 1, 4)}, {128, 256, 1, 1.07f, DSA_TILE(4, 4, 2, 4, 1, 2)},
+    {16, 16, 4, 0.31f, 0.58f, DSA_TILE(1, 1, 1, 1, 4, 4)},  {32, 16, 4, 0.53f, 0.70f, DSA_TILE(1, 1, 2, 1, 4, 3)},
+    {32, 32, 4, 0.63f, 0.00f, DSA_TILE(1, 2, 2, 1, 4, 4)},  {64, 32, 2, 0.48f, 0.00f, DSA_TILE(1, 2, 4, 1, 2, 4)},
+    {64, 64, 2, 0.59f, 0.00f, DSA_TILE(2, 2, 2, 2, 2, 4)},  {64, 64, 1, 0.33f, 0.45f, DSA_TILE(2, 2, 2, 2, 1, 4)},
+    {128, 32, 1, 0.39f, 0.00f, DSA_TILE(1, 2, 8, 1, 1, 4)}, {128, 64, 1, 0.51f, 0.00f, DSA_TILE(1, 4, 8, 1, 1, 4)},
+    {128, 80, 1, 0.55f, 0.00f, DSA_TILE(1, 5, 8, 1, 1, 4)}, {128, 128, 1, 0.61f, 0.00f, DSA_TILE(2, 4, 4, 2, 1, 4)},
+    {128, 256, 1, 1.07f, 0.00f, DSA_TILE(4, 4, 2, 4, 1, 2)},
 };
 constexpr float kWholeStep = 1.70f, kHalfStep = 1.07f;  // of the mixed kernel
 
@@ -378,7 +380,10 @@ int launch_product(const dsa_product_args& p, int cus, hipStream_t stream) {
     float least = 0.f;
     for (const Variant& v : kVariants) {
         const int64_t tiles = (int64_t)((p.M + v.rows - 1) / v.rows) * ((p.N + v.columns - 1) / v.columns);
-        const float time = (float)((tiles + cus - 1) / cus) * (2.f + v.step * (float)((blocks + v.blocks - 1) / v.blocks));
+        const bool pairs = v.both > 0.f && tiles > cus;
+        const int64_t fit = pairs ? 2 * cus : cus;
+        const float time = (float)((tiles + fit - 1) / fit) *
+                           (2.f + (pairs ? v.both : v.step) * (float)((blocks + v.blocks - 1) / v.blocks));
         if (!best || time < least) best = &v, least = time;
     }
     if (p.dtype != DSA_F32) {  // the widened codes of 32-bit outputs would need more registers

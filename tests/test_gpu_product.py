@@ -81,6 +81,16 @@ def test_large(M, N, K, dtype):
     check(dsa_amd.matmul_fp8(*args, dtype=dtype), *args)
 
 
+@pytest.mark.parametrize("dtype", [BF, FULL])
+@pytest.mark.parametrize("M, N, K", [
+    (8, 2112, 7184), (13, 7168, 7152), (60, 2112, 7184), (55, 6376, 2224), (100, 7168, 7184), (512, 2112, 7184), (18, 24570, 1552),
+    (64, 24576, 1520), (1000, 2112, 7184), (115, 24570, 1552), (3639, 2112, 7184), (1024, 24576, 1552), (4100, 4300, 272)])
+def test_every_tile(M, N, K, dtype):
+    """Sizes for which tiles of 16 by 16 to 256 by 256 are chosen, K ending inside a block."""
+    args = make(M, N, K, seed=3)
+    check(dsa_amd.matmul_fp8(*args, dtype=dtype), *args)
+
+
 def test_leading_dimensions_and_empty():
     a, sa, b, sb = make(24, 100, 256)
     want = dsa_amd.matmul_fp8(a, sa, b, sb)
