@@ -135,8 +135,7 @@ class DsaNormGradArgs(ctypes.Structure):
 class DsaProductArgs(ctypes.Structure):
     """Mirror of ``struct dsa_product_args`` (include/dsa_mi355x_layer.h)."""
 
-    _fields_ = ([(name, ctypes.c_void_p) for name in ("a", "a_scales", "b", "b_scales", "out", "workspace")]
-                + [("workspace_bytes", ctypes.c_int64)]
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("a", "a_scales", "b", "b_scales", "out")]
                 + [(name, ctypes.c_int32) for name in ("M", "N", "K", "dtype")])
 
 
@@ -194,7 +193,6 @@ LAYER_SIGNATURES = {
     "dsa_rms_norm_fp8": (_i32, [ctypes.POINTER(DsaNormArgs), _vp]),
     "dsa_rms_norm_grad_ws_bytes": (_i64, [_i64, _i32]),
     "dsa_rms_norm_grad": (_i32, [ctypes.POINTER(DsaNormGradArgs), _vp]),
-    "dsa_matmul_fp8_ws_bytes": (_i64, [ctypes.POINTER(DsaProductArgs)]),
     "dsa_matmul_fp8": (_i32, [ctypes.POINTER(DsaProductArgs), _vp]),
 }
 

@@ -704,9 +704,8 @@ def _fast_layer():
     with _fast_lock:
         if not _fast_layer_state:
             _fast_layer_state.append(_load_fast("_fast_layer", ("dsa_rms_norm", "dsa_rms_norm_fp8",
-                                                                "dsa_matmul_fp8_ws_bytes", "dsa_matmul_fp8",
-                                                                "dsa_rms_norm_grad_ws_bytes", "dsa_rms_norm_grad",
-                                                                "dsa_last_error")))
+                                                                "dsa_matmul_fp8", "dsa_rms_norm_grad_ws_bytes",
+                                                                "dsa_rms_norm_grad", "dsa_last_error")))
     return _fast_layer_state[0]
 
 

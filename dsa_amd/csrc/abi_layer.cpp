@@ -69,6 +69,7 @@ int check_product(const dsa_product_args* a) {
     if (a->M <= 0 || a->N <= 0 || a->K <= 0) return fail(-1, "M, N, K must be positive (got %d, %d, %d)", a->M, a->N, a->K);
     if (a->K % 16 || a->K >= 1 << 20) return fail(-1, "K must be a multiple of 16 below 2^20 (got %d)", a->K);
     if (a->M > 1 << 24 || a->N > 1 << 24) return fail(-1, "M and N must be at most 2^24 (got %d, %d)", a->M, a->N);
+    if ((int64_t)a->M * a->N > (int64_t)1 << 37) return fail(-1, "M * N must be at most 2^37 (got %d, %d)", a->M, a->N);
     if (!known(a->dtype)) return fail(-1, "unknown dtype %d", a->dtype);
     return 0;
 }
@@ -113,22 +114,13 @@ int dsa_rms_norm_grad(const dsa_norm_grad_args* a, void* stream) {
     return finish(dsa::launch_norm_grad(*a, vector, static_cast<hipStream_t>(stream)), "norm gradient launch");
 }
 
-int64_t dsa_matmul_fp8_ws_bytes(const dsa_product_args* a) {
-    if (const int rc = check_product(a)) return rc;
-    dsa::set_error(0, "%s", "");
-    return dsa::product_ws_bytes(*a);
-}
-
 int dsa_matmul_fp8(const dsa_product_args* a, void* stream) {
     if (const int rc = check_product(a)) return rc;
-    const int64_t need = dsa::product_ws_bytes(*a);
-    if (!a->a || !a->a_scales || !a->b || !a->b_scales || !a->out || (need > 0 && !a->workspace))
+    if (!a->a || !a->a_scales || !a->b || !a->b_scales || !a->out)
         return fail(-1, "NULL pointer argument");
     if (!aligned(a->a, 16) || !aligned(a->b, 16) || !aligned(a->a_scales, 4) || !aligned(a->b_scales, 4) ||
-        !aligned(a->out, a->dtype == DSA_F32 ? 4 : 2) || !aligned(a->workspace, 256))
-        return fail(-1, "codes must be 16-byte aligned, scales and out to their elements, the workspace to 256 bytes");
-    if (a->workspace_bytes < need)
-        return fail(-1, "workspace of %lld bytes is below the %lld needed", (long long)a->workspace_bytes, (long long)need);
+        !aligned(a->out, a->dtype == DSA_F32 ? 4 : 2))
+        return fail(-1, "codes must be 16-byte aligned, scales and out to their elements");
     int device = 0, cus = 0;
     int rc = (int)hipGetDevice(&device);
     if (!rc) rc = (int)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);

@@ -25,7 +25,6 @@ namespace {
 
 decltype(&dsa_rms_norm) g_norm = nullptr;
 decltype(&dsa_rms_norm_fp8) g_norm_fp8 = nullptr;
-decltype(&dsa_matmul_fp8_ws_bytes) g_product_bytes = nullptr;
 decltype(&dsa_matmul_fp8) g_product = nullptr;
 decltype(&dsa_rms_norm_grad_ws_bytes) g_grad_bytes = nullptr;
 decltype(&dsa_rms_norm_grad) g_grad = nullptr;
@@ -233,7 +232,7 @@ py::object matmul_fp8(py::handle ha, py::handle ha_scales, py::handle hb, py::ha
     dsa_product_args p{};
     p.dtype = code_of(type);
     if (!dev.is_cuda() || p.dtype < 0 || K <= 0 || K % 16 || K >= 1 << 20 || N <= 0 || N > 1 << 24 || a->size(-1) != K ||
-        a->numel() / K > 1 << 24 || a_scales->dim() != a->dim() || a_scales->size(-1) != blocks ||
+        a->numel() / K > 1 << 24 || a->numel() / K * N > (int64_t)1 << 37 || a_scales->dim() != a->dim() || a_scales->size(-1) != blocks ||
         a_scales->sizes().slice(0, a->dim() - 1) != a->sizes().slice(0, a->dim() - 1) ||
         !dims(*b_scales, {(N + 127) / 128, blocks}) || a->scalar_type() != at::kFloat8_e4m3fn ||
         b->scalar_type() != at::kFloat8_e4m3fn || a_scales->scalar_type() != at::kFloat ||
@@ -250,27 +249,20 @@ py::object matmul_fp8(py::handle ha, py::handle ha_scales, py::handle hb, py::ha
     p.N = (int32_t)N;
     p.K = (int32_t)K;
     c10::DeviceGuard guard(dev);
-    p.workspace_bytes = g_product_bytes(&p);
-    if (p.workspace_bytes < 0) return py::none();
     auto shape = a->sizes().vec();
     shape.back() = N;
     const auto options = a->options().requires_grad(false).memory_format(std::nullopt);
-    at::Tensor out = at::empty(shape, options.dtype(type)), workspace;
-    if (p.workspace_bytes > 0) {
-        workspace = at::empty({p.workspace_bytes}, options.dtype(at::kByte));
-        p.workspace = workspace.data_ptr();
-    }
+    at::Tensor out = at::empty(shape, options.dtype(type));
     p.out = out.data_ptr();
     const int rc = g_product(&p, stream_of(dev));
     if (rc != 0) return py::int_(rc);
     return py::cast(out);
 }
 
-void set_entry(uint64_t norm_address, uint64_t norm_fp8, uint64_t product_bytes, uint64_t product, uint64_t grad_bytes,
-               uint64_t grad, uint64_t error) {
+void set_entry(uint64_t norm_address, uint64_t norm_fp8, uint64_t product, uint64_t grad_bytes, uint64_t grad,
+               uint64_t error) {
     g_norm = reinterpret_cast<decltype(g_norm)>(norm_address);
     g_norm_fp8 = reinterpret_cast<decltype(g_norm_fp8)>(norm_fp8);
-    g_product_bytes = reinterpret_cast<decltype(g_product_bytes)>(product_bytes);
     g_product = reinterpret_cast<decltype(g_product)>(product);
     g_grad_bytes = reinterpret_cast<decltype(g_grad_bytes)>(grad_bytes);
     g_grad = reinterpret_cast<decltype(g_grad)>(grad);

@@ -234,7 +234,6 @@ int launch_norm_grad(const dsa_norm_grad_args& p, bool vector, hipStream_t strea
 int64_t norm_grad_teams(int64_t rows, int dim);  // rows of 32-bit sums in the workspace
 
 // 8-bit products (product.hip).
-int64_t product_ws_bytes(const dsa_product_args& p);
 int launch_product(const dsa_product_args& p, int cus, hipStream_t stream);  // cus: compute units to plan for
 
 }  // namespace dsa

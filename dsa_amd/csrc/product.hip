@@ -372,14 +372,13 @@ constexpr float kWholeStep = 1.70f, kHalfStep = 1.07f;  // of the mixed kernel
 
 }  // namespace
 
-int64_t product_ws_bytes(const dsa_product_args&) { return 0; }
-
 int launch_product(const dsa_product_args& p, int cus, hipStream_t stream) {
     const int blocks = (p.K + kBlock - 1) / kBlock;
     const Variant* best = nullptr;
     float least = 0.f;
     for (const Variant& v : kVariants) {
         const int64_t tiles = (int64_t)((p.M + v.rows - 1) / v.rows) * ((p.N + v.columns - 1) / v.columns);
+        if (tiles > 1 << 22) continue;  // a grid's threads are counted in 32 bits
         const bool pairs = v.both > 0.f && tiles > cus;
         const int64_t fit = pairs ? 2 * cus : cus;
         const float time = (float)((tiles + fit - 1) / fit) *

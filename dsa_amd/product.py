@@ -29,10 +29,11 @@ def matmul_fp8(a, a_scales, b, b_scales, *, dtype=torch.bfloat16):
 
     The products of 128 are summed in 32 bits, multiplied by their two scales,
     summed in 32 bits and rounded once to ``dtype`` (bfloat16, float16 or float32).
-    The same inputs give the same bits.  K is a multiple of 16 below 2^20.  All
-    inputs are contiguous.  The output is a fresh tensor, which records no gradient and no
-    forward-mode tangent, the workspace is the caching allocator's, and nothing
-    synchronises."""
+    For the 16-bit ones the matrix cores keep products to about 2^-14 of a block's
+    largest; for float32 whole, at half their rate.  The same inputs give the same
+    bits.  K is a multiple of 16 below 2^20.  All inputs are contiguous, the codes
+    16-byte aligned.  The output is a fresh tensor, which records no gradient and no
+    forward-mode tangent, and nothing synchronises."""
     fast = _fast_layer()
     if fast is not None:  # checked, allocated and launched in C++ (None: not taken)
         taken = fast.matmul_fp8(a, a_scales, b, b_scales, dtype)
@@ -45,9 +46,10 @@ def matmul_fp8(a, a_scales, b, b_scales, *, dtype=torch.bfloat16):
     if a.dim() < 1 or b.dim() != 2 or a.shape[-1] != b.shape[1]:
         raise ValueError("expected a[..., K] and b[N, K]")
     columns, inner = b.shape
-    if inner <= 0 or inner % 16 or inner >= 1 << 20 or not 0 < columns <= 1 << 24 or a.numel() > inner << 24:
-        raise ValueError("K must be a positive multiple of 16 below 2^20, N in [1, 2^24] and there be at most 2^24 rows "
-                         f"(got {inner}, {columns} and {list(a.shape[:-1])})")
+    if inner <= 0 or inner % 16 or inner >= 1 << 20 or not 0 < columns <= 1 << 24 or a.numel() > inner << 24 or (
+            a.numel() // inner * columns > 1 << 37):
+        raise ValueError("K must be a positive multiple of 16 below 2^20, N in [1, 2^24], and there be at most 2^24 rows and "
+                         f"2^37 outputs (got {inner}, {columns} and {list(a.shape[:-1])})")
     blocks = -(-inner // SCALE_BLOCK)
     if a_scales.shape != (*a.shape[:-1], blocks) or b_scales.shape != (-(-columns // SCALE_BLOCK), blocks):
         raise ValueError(f"expected a_scales[..., {blocks}] and b_scales[{-(-columns // SCALE_BLOCK)}, {blocks}]")
@@ -69,12 +71,6 @@ def matmul_fp8(a, a_scales, b, b_scales, *, dtype=torch.bfloat16):
     args.M, args.N, args.K = a.numel() // inner, columns, inner
     lib = _lib.load()
     with _on_device(device):
-        size = lib.dsa_matmul_fp8_ws_bytes(ctypes.byref(args))
-        if size < 0:
-            _lib.check(-1, "dsa_matmul_fp8")
-        if size > 0:
-            workspace = torch.empty(size, device=device, dtype=torch.uint8)
-            args.workspace, args.workspace_bytes = workspace.data_ptr(), size
         rc = lib.dsa_matmul_fp8(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index))
     if rc:
         _lib.check(rc, "dsa_matmul_fp8")

@@ -98,29 +98,21 @@ def test_c_norm_grad_refuses(kw):
 
 def _product_args(**kw):
     a = _lib.DsaProductArgs()
-    a.a = a.a_scales = a.b = a.b_scales = a.out = a.workspace = 4096
-    a.M, a.N, a.K, a.workspace_bytes = 5, 100, 256, 1 << 40
+    a.a = a.a_scales = a.b = a.b_scales = a.out = 4096
+    a.M, a.N, a.K = 5, 100, 256
     return _fill(a, **kw)
 
 
-SIZES = [dict(M=0), dict(N=0), dict(K=0), dict(K=8), dict(K=250), dict(K=1 << 20), dict(M=(1 << 24) + 1),
-         dict(N=(1 << 24) + 1), dict(dtype=3)]
-
-
-@pytest.mark.parametrize("kw", SIZES + [dict(a=None), dict(a_scales=None), dict(b=None), dict(b_scales=None), dict(out=None),
-                                        dict(a=4104), dict(b=4104), dict(a_scales=4098), dict(b_scales=4098), dict(out=4097),
-                                        dict(out=4098, dtype=2), dict(workspace=4112)])
+@pytest.mark.parametrize("kw", [dict(M=0), dict(N=0), dict(K=0), dict(K=8), dict(K=250), dict(K=1 << 20), dict(M=(1 << 24) + 1),
+                                dict(N=(1 << 24) + 1), dict(M=1 << 19, N=(1 << 18) + 1), dict(dtype=3), dict(a=None),
+                                dict(a_scales=None), dict(b=None), dict(b_scales=None), dict(out=None),
+                                dict(a=4104), dict(b=4104), dict(a_scales=4098), dict(b_scales=4098), dict(out=4097),
+                                dict(out=4098, dtype=2)])
 def test_c_product_refuses(kw):
     lib = _lib.load()
     assert lib.dsa_matmul_fp8(ctypes.byref(_product_args(**kw)), None) < 0
     assert lib.dsa_last_error()
-
-
-@pytest.mark.parametrize("kw", SIZES)
-def test_c_product_workspace_refuses(kw):
-    lib = _lib.load()
-    assert lib.dsa_matmul_fp8_ws_bytes(ctypes.byref(_product_args(**kw))) < 0
-    assert lib.dsa_matmul_fp8_ws_bytes(None) < 0
+    assert lib.dsa_matmul_fp8(None, None) < 0
 
 
 def _tree_args(**kw):
