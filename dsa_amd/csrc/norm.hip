@@ -2,15 +2,16 @@
 // (include/dsa_mi355x_layer.h).  No reference counterpart: the reference takes q
 // and kv as given (README.md:19-21).
 //
-// A row is held in registers by a team of one, four or sixteen waves, eight values
-// a thread and chunk, so that it is read once: the sum of squares needs all of it
-// before the first output.  Bound by HBM, and in a decode step by the launch and two
-// trips to memory.
+// A row is held in registers by a team of one to sixteen waves, eight values a thread
+// (sixteen above 8192), so that it is read once: the sum of squares needs all of it
+// before the first output.  Bound by HBM, and in a decode step by the launch and a trip
+// to memory.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>
 
 #include "kernels.h"
+#include "mla_tiles.h"
 
 namespace dsa {
 namespace {
@@ -105,10 +106,18 @@ __device__ __forceinline__ void store8(T* row, const float (&f)[8], int e, int d
     }
 }
 
+// Over the 16 lanes of a DPP row by rotations, then over the four rows by lane swaps:
+// no trip through LDS.
+template <int CONTROL>
+__device__ __forceinline__ float rotated(float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CONTROL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
+    v += rotated<0x128>(v);  // row_ror:8
+    v += rotated<0x124>(v);
+    v += rotated<0x122>(v);
+    v += rotated<0x121>(v);
+    return sum_xor32(sum_xor16(v));
 }
 
 // Sum over a team; `turn` alternates, so that one barrier a sum is enough.
@@ -362,83 +371,75 @@ __global__ __launch_bounds__(kSumColumns* kSumGroups) void norm_weight_kernel(co
     }
 }
 
-// Waves a row and chunks a thread.
-struct Shape {
-    int waves, chunks;
-};
-Shape shape_of(int64_t rows, int dim) {
-    if (dim <= 512) return {1, 1};
-    if (dim <= 1024) return {1, 2};
-    if (rows <= 512) return {16, dim <= 8192 ? 1 : 2};
-    if (dim <= 2048) return {4, 1};
-    if (dim <= 4096) return {4, 2};
-    if (dim <= 8192) return {4, 4};
-    return {16, 2};
-}
+// Waves a row: as many as hold it with eight values a thread, sixteen at most (then 16).
+// Fewer waves with more values each were slower for 8 to 8192 rows: rows of 7168 with
+// a residual, by 16, 8 and 4 waves, 8 rows 3.2, 3.7 and 5.1 us, 400 7.6, 7.9 and 10.4,
+// 8192 84, 88 and 97; rows of 4096 by 16, 8 and 4, 8 rows 3.0, 2.8 and 3.5, 8192 57, 49
+// and 52; of 1024 by 4, 2 and 1, 8 rows 2.6, 2.6 and 3.2, 8192 16.8, 14.6 and 16.0.
+int waves_of(int dim) { return dim <= 512 ? 1 : dim <= 1024 ? 2 : dim <= 2048 ? 4 : dim <= 4096 ? 8 : 16; }
 
 constexpr int64_t kMaxGrid = 4096;
 
 template <typename T, bool CODES>
 int launch_typed(const dsa_norm_args& p, int vector, hipStream_t stream) {
-    const Shape s = shape_of(p.rows, p.dim);
-    const int64_t teams = s.waves == 1 ? 4 : 1, want = (p.rows + teams - 1) / teams;
-    const dim3 grid((unsigned)(want < kMaxGrid ? want : kMaxGrid)), block(s.waves == 1 ? 256 : 64 * s.waves);
-#define DSA_NORM(W, C) \
-    if (s.waves == W && s.chunks == C) hipLaunchKernelGGL((norm_kernel<T, CODES, W, C>), grid, block, 0, stream, p, vector)
-    DSA_NORM(1, 1);
-    DSA_NORM(1, 2);
-    DSA_NORM(4, 1);
-    DSA_NORM(4, 2);
-    DSA_NORM(4, 4);
-    DSA_NORM(16, 1);
-    DSA_NORM(16, 2);
-#undef DSA_NORM
+    const int waves = waves_of(p.dim);
+    const int64_t teams = waves == 1 ? 4 : 1, want = (p.rows + teams - 1) / teams;
+    const dim3 grid((unsigned)(want < kMaxGrid ? want : kMaxGrid)), block(waves == 1 ? 256 : 64 * waves);
+    auto* kernel = waves == 1   ? norm_kernel<T, CODES, 1, 1>
+                   : waves == 2 ? norm_kernel<T, CODES, 2, 1>
+                   : waves == 4 ? norm_kernel<T, CODES, 4, 1>
+                   : waves == 8 ? norm_kernel<T, CODES, 8, 1>
+                   : p.dim <= 8192 ? norm_kernel<T, CODES, 16, 1>
+                                   : norm_kernel<T, CODES, 16, 2>;
+    hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, vector);
     return (int)hipGetLastError();
 }
 
-Shape grad_shape_of(int dim) {
-    if (dim <= 512) return {1, 1};
-    if (dim <= 1024) return {1, 2};
-    if (dim <= 2048) return {4, 1};
-    if (dim <= 4096) return {4, 2};
-    return {16, dim <= 8192 ? 1 : 2};
-}
+// Workgroups of the gradient: two a CU keep their columns' sums over 8 rows of 4095.
 int64_t grad_groups(int64_t rows, int dim) {
-    const int64_t teams = grad_shape_of(dim).waves == 1 ? 4 : 1, want = (rows + teams - 1) / teams;
+    const int64_t teams = waves_of(dim) == 1 ? 4 : 1, want = (rows + teams - 1) / teams;
     return want < 512 ? want : 512;
 }
 
 template <typename T>
 int launch_grad_typed(const dsa_norm_grad_args& p, int vector, hipStream_t stream) {
-    const Shape s = grad_shape_of(p.dim);
+    const int waves = waves_of(p.dim);
     const int64_t groups = grad_groups(p.rows, p.dim);
-    const dim3 grid((unsigned)groups), block(s.waves == 1 ? 256 : 64 * s.waves);
-#define DSA_NORM(W, C) \
-    if (s.waves == W && s.chunks == C) hipLaunchKernelGGL((norm_grad_kernel<T, W, C>), grid, block, 0, stream, p, vector)
-    DSA_NORM(1, 1);
-    DSA_NORM(1, 2);
-    DSA_NORM(4, 1);
-    DSA_NORM(4, 2);
-    DSA_NORM(16, 1);
-    DSA_NORM(16, 2);
-#undef DSA_NORM
+    const dim3 grid((unsigned)groups), block(waves == 1 ? 256 : 64 * waves);
+    auto* kernel = waves == 1   ? norm_grad_kernel<T, 1, 1>
+                   : waves == 2 ? norm_grad_kernel<T, 2, 1>
+                   : waves == 4 ? norm_grad_kernel<T, 4, 1>
+                   : waves == 8 ? norm_grad_kernel<T, 8, 1>
+                   : p.dim <= 8192 ? norm_grad_kernel<T, 16, 1>
+                                   : norm_grad_kernel<T, 16, 2>;
+    hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, vector);
     if (const int rc = (int)hipGetLastError()) return rc;
     if (!p.grad_weight) return 0;
-    const int teams = (int)groups * (s.waves == 1 ? 4 : 1);
+    const int teams = (int)norm_grad_teams(p.rows, p.dim);
     const dim3 columns((unsigned)((p.dim + kSumColumns - 1) / kSumColumns)), threads(kSumColumns * kSumGroups);
     const float* parts = static_cast<const float*>(p.workspace);
-    if (p.weight_f32) hipLaunchKernelGGL((norm_weight_kernel<float>), columns, threads, 0, stream, parts, static_cast<float*>(p.grad_weight), teams, p.dim);
-    else hipLaunchKernelGGL((norm_weight_kernel<T>), columns, threads, 0, stream, parts, static_cast<T*>(p.grad_weight), teams, p.dim);
+    if (p.weight_f32)
+        hipLaunchKernelGGL((norm_weight_kernel<float>), columns, threads, 0, stream, parts, static_cast<float*>(p.grad_weight), teams,
+                           p.dim);
+    else
+        hipLaunchKernelGGL((norm_weight_kernel<T>), columns, threads, 0, stream, parts, static_cast<T*>(p.grad_weight), teams, p.dim);
     return (int)hipGetLastError();
 }
 
 }  // namespace
 
 int64_t norm_grad_teams(int64_t rows, int dim) {
-    return grad_groups(rows, dim) * (grad_shape_of(dim).waves == 1 ? 4 : 1);
+    return grad_groups(rows, dim) * (waves_of(dim) == 1 ? 4 : 1);
 }
 
-int launch_norm(const dsa_norm_args& p, bool codes, bool vector, hipStream_t stream) {
+int launch_norm(const dsa_norm_args& args, bool codes, bool vector, hipStream_t stream) {
+    dsa_norm_args p = args;
+    // Codes of rows that follow each other, without a norm, are those of pieces of them:
+    // a wave then holds 512 values and waits for no other.
+    if (codes && !p.weight && p.dim > 512 && p.dim % 512 == 0 && p.x_stride == p.dim) {
+        p.rows *= p.dim / 512;
+        p.x_stride = p.dim = 512;
+    }
     if (p.dtype == DSA_BF16) return codes ? launch_typed<__bf16, true>(p, vector, stream) : launch_typed<__bf16, false>(p, vector, stream);
     if (p.dtype == DSA_F16) return codes ? launch_typed<f16, true>(p, vector, stream) : launch_typed<f16, false>(p, vector, stream);
     return codes ? launch_typed<float, true>(p, vector, stream) : launch_typed<float, false>(p, vector, stream);
