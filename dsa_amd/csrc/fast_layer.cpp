@@ -12,6 +12,8 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <hip/hip_runtime_api.h>
+
 #include <cmath>
 #include <cstdint>
 #include <memory>
@@ -48,6 +50,9 @@ bool row_stride(const at::Tensor& t, int64_t& stride) {
     }
     return true;
 }
+
+// Whether the fast path takes it: its memory holds its values as they are.
+bool plain(const at::Tensor& t) { return !differentiated(t) && !t.is_neg(); }
 
 bool wants_grad(const at::Tensor* t) { return t && at::GradMode::is_enabled() && t->requires_grad(); }
 
@@ -99,12 +104,12 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
             const c10::Device dev = h.device();
             c10::DeviceGuard guard(dev);
             const auto options = h.options().requires_grad(false).memory_format(std::nullopt);
-            const at::Tensor grad_y = grads[0].defined() ? grads[0].contiguous() : at::zeros(h.sizes(), options);
+            const at::Tensor grad_y = grads[0].defined() ? grads[0].resolve_neg().contiguous() : at::zeros(h.sizes(), options);
             at::Tensor grad_sum, workspace;
             grad_h = at::empty(h.sizes(), options);
             dsa_norm_grad_args a{};
             if (grads.size() > 1 && grads[1].defined()) {
-                grad_sum = grads[1].contiguous();
+                grad_sum = grads[1].resolve_neg().contiguous();
                 a.grad_sum = grad_sum.data_ptr();
             }
             a.h = h.data_ptr();
@@ -142,6 +147,25 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     }
 };
 
+// A leaf that some eager graph on the default stream still uses has its sums there, and
+// a capture of the gradient, which runs on a stream of its own, would end in an error
+// that no caller can catch.  Refused here, before anything of it is captured.
+void check_capture(std::initializer_list<const at::Tensor*> leaves) {
+    bool lives = false;
+    for (const at::Tensor* t : leaves) {
+        if (!wants_grad(t) || !t->is_leaf()) continue;
+        const auto sums = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto stream = sums ? sums->stream() : std::nullopt;
+        lives |= stream && stream->id() == 0;
+    }
+    if (!lives) return;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const int rc = (int)hipStreamIsCapturing(c10::hip::getCurrentHIPStream().stream(), &status);
+    if (rc == 0 && status != hipStreamCaptureStatusNone)
+        throw py::value_error("the gradient of a leaf cannot be captured while results that it was used for on the "
+                              "default stream are kept: drop them first");
+}
+
 // Without a weight: codes of x itself.
 py::object norm(py::handle hx, const at::Tensor* weight, const at::Tensor* residual, double eps, bool codes, bool pow2) {
     const at::Tensor* x = tensor(hx);
@@ -152,18 +176,18 @@ py::object norm(py::handle hx, const at::Tensor* weight, const at::Tensor* resid
     dsa_norm_args a{};
     a.dtype = code_of(type);
     if (!dev.is_cuda() || a.dtype < 0 || dim > DSA_NORM_MAX_DIM || (codes && dim % 16) ||
-        !(eps >= 0.0 && eps <= 3.4028234663852886e38) || !row_stride(*x, a.x_stride) || differentiated(*x))
+        !(eps >= 0.0 && eps <= 3.4028234663852886e38) || !row_stride(*x, a.x_stride) || !plain(*x))
         return py::none();
     if (weight) {
         if (weight->dim() != 1 || weight->size(0) != dim || weight->device() != dev || !weight->is_contiguous() ||
-            (weight->scalar_type() != type && weight->scalar_type() != at::kFloat) || differentiated(*weight))
+            (weight->scalar_type() != type && weight->scalar_type() != at::kFloat) || !plain(*weight))
             return py::none();
         a.weight = weight->data_ptr();
         a.weight_f32 = weight->scalar_type() == at::kFloat;
     }
     if (residual) {
         if (residual->sizes() != x->sizes() || residual->scalar_type() != type || residual->device() != dev ||
-            !row_stride(*residual, a.residual_stride) || differentiated(*residual))
+            !row_stride(*residual, a.residual_stride) || !plain(*residual))
             return py::none();
         a.residual = residual->data_ptr();
     }
@@ -171,6 +195,7 @@ py::object norm(py::handle hx, const at::Tensor* weight, const at::Tensor* resid
     if (grad && codes) return py::none();
     c10::DeviceGuard guard(dev);
     if (grad) {
+        check_capture({x, weight, residual});
         const auto results = RmsNorm::apply(*x, *weight, residual ? std::optional<at::Tensor>(*residual) : std::nullopt, eps);
         return residual ? py::object(py::make_tuple(results[0], results[1])) : py::cast(results[0]);
     }
@@ -239,7 +264,7 @@ py::object matmul_fp8(py::handle ha, py::handle ha_scales, py::handle hb, py::ha
         b_scales->scalar_type() != at::kFloat)
         return py::none();
     for (const at::Tensor* t : {a, a_scales, b, b_scales})
-        if (t->device() != dev || !t->is_contiguous() || !t->has_storage()) return py::none();
+        if (t->device() != dev || !t->is_contiguous() || !t->has_storage() || t->is_neg()) return py::none();
     p.a = static_cast<const uint8_t*>(a->data_ptr());
     p.a_scales = static_cast<const float*>(a_scales->data_ptr());
     p.b = static_cast<const uint8_t*>(b->data_ptr());
@@ -259,6 +284,13 @@ py::object matmul_fp8(py::handle ha, py::handle ha_scales, py::handle hb, py::ha
     return py::cast(out);
 }
 
+// The same check for the Python path, of tensors or None.
+void capturable(py::handle x, py::handle weight, py::handle residual) {
+    const at::Tensor* t = tensor(x);
+    c10::DeviceGuard guard(t->device());
+    check_capture({t, tensor(weight), tensor(residual)});
+}
+
 void set_entry(uint64_t norm_address, uint64_t norm_fp8, uint64_t product, uint64_t grad_bytes, uint64_t grad,
                uint64_t error) {
     g_norm = reinterpret_cast<decltype(g_norm)>(norm_address);
@@ -276,5 +308,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("rms_norm_fp8", &rms_norm_fp8, "dsa_amd.rms_norm_fp8, or None");
     m.def("quantize_fp8", &quantize_fp8, "dsa_amd.quantize_fp8, or None");
     m.def("matmul_fp8", &matmul_fp8, "dsa_amd.matmul_fp8, or None");
+    m.def("capturable", &capturable, "raises where the gradient of these cannot be captured now");
     m.def("set_entry", &set_entry, "addresses of the library's entry points");
 }

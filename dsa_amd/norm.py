@@ -70,6 +70,11 @@ def _derivatives(*tensors):
     return torch.is_grad_enabled() and any(t.requires_grad for t in given), any(has_tangent(t) for t in given)
 
 
+def _plain(*tensors):
+    """Views whose sign is kept apart from their memory, as tensors that hold it."""
+    return [t if t is None else t.resolve_neg() for t in tensors]
+
+
 def _norm_args(x, weight, residual, eps, out, total):
     dim = x.shape[-1]
     args = _lib.DsaNormArgs()
@@ -118,7 +123,7 @@ class _RmsNorm(torch.autograd.Function):
         h, weight, inverse = ctx.saved_tensors
         dim, device = h.shape[-1], h.device
         needs_weight = ctx.needs_input_grad[1]
-        grad_y = grad_y.contiguous()
+        grad_y = grad_y.resolve_neg().contiguous()
         grad_h = torch.empty(h.shape, device=device, dtype=h.dtype)
         grad_weight = torch.empty_like(weight) if needs_weight else None
         grad_residual = grad_h if ctx.needs_input_grad[2] else None
@@ -128,7 +133,7 @@ class _RmsNorm(torch.autograd.Function):
         args.h, args.inverse, args.weight = h.data_ptr(), inverse.data_ptr(), weight.data_ptr()
         args.grad_out, args.grad_in = grad_y.data_ptr(), grad_h.data_ptr()
         if grad_total is not None:
-            grad_total = grad_total.contiguous()
+            grad_total = grad_total.resolve_neg().contiguous()
             args.grad_sum = grad_total.data_ptr()
         args.rows, args.h_stride, args.dim, args.dtype = h.numel() // dim, _row_stride(h), dim, DTYPES[h.dtype]
         args.weight_f32 = weight.dtype == torch.float32
@@ -155,7 +160,8 @@ def rms_norm(x, weight, residual=None, *, eps=1e-6):
 
     Gradients of ``x``, ``residual`` and ``weight`` are recorded where one of them
     requires it (once: there are none of the second order), sums over the rows in
-    a fixed order; forward-mode tangents are refused."""
+    a fixed order; forward-mode tangents are refused.  In a graph's capture so is a leaf
+    whose results of eager calls on the default stream are still kept with their graph."""
     fast = _fast_layer()
     if fast is not None:  # checked, allocated and launched in C++ (None: not taken)
         taken = fast.rms_norm(x, weight, residual, eps)
@@ -169,7 +175,10 @@ def rms_norm(x, weight, residual=None, *, eps=1e-6):
     grad, tangent = _derivatives(x, weight, residual)
     if tangent:
         raise ValueError("rms_norm has no forward-mode derivative")
+    x, weight, residual = _plain(x, weight, residual)
     if grad:
+        if fast is not None:
+            fast.capturable(x, weight, residual)
         return _RmsNorm.apply(x, weight, residual, eps)
     y, total, _ = _norm(x, weight, residual, eps, False)
     return y if residual is None else (y, total)
@@ -181,6 +190,7 @@ def _codes(x, weight, residual, eps, pow2_scales):
         raise ValueError(f"codes need a last dimension that is a multiple of 16 (got {dim})")
     if any(_derivatives(x, weight, residual)):
         raise ValueError("codes record no gradient and no forward-mode tangent: call it without them (torch.no_grad)")
+    x, weight, residual = _plain(x, weight, residual)
     codes = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
     scales = torch.empty((*x.shape[:-1], -(-dim // SCALE_BLOCK)), device=x.device, dtype=torch.float32)
     total = None if residual is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)

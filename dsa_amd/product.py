@@ -55,13 +55,14 @@ def matmul_fp8(a, a_scales, b, b_scales, *, dtype=torch.bfloat16):
         raise ValueError(f"expected a_scales[..., {blocks}] and b_scales[{-(-columns // SCALE_BLOCK)}, {blocks}]")
     device = a.device
     if device.type != "cuda" or torch.version.hip is None or any(
-            t.device != device or not t.is_contiguous() for t in (a, a_scales, b, b_scales)):
+            t.device != device or not t.is_contiguous() for t in (a, a_scales, b, b_scales)) or a.is_neg() or b.is_neg():
         raise ValueError("all inputs must be contiguous and on the same ROCm GPU")
     e4m3 = torch.float8_e4m3fn
     if a.dtype != e4m3 or b.dtype != e4m3 or a_scales.dtype != torch.float32 or b_scales.dtype != torch.float32:
         raise ValueError("a and b must be float8_e4m3fn, their scales float32")
     if dtype not in DTYPES:
         raise ValueError("dtype must be torch.bfloat16, torch.float16 or torch.float32")
+    a_scales, b_scales = a_scales.resolve_neg(), b_scales.resolve_neg()
     out = torch.empty((*a.shape[:-1], columns), device=device, dtype=dtype)
     if out.numel() == 0:
         return out

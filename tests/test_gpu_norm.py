@@ -380,6 +380,62 @@ def test_captured_gradients():
         torch.cuda.synchronize()
 
 
+def test_a_capture_beside_a_living_graph_is_refused():
+    """The leaves' sums of an eager graph on the default stream cannot be captured: the call says so, and nothing
+    is lost.  Without that graph, or without gradients, it is captured."""
+    x, w = make((40, 512), FULL).requires_grad_(), make(512, FULL, 1).requires_grad_()
+    kept = dsa_amd.rms_norm(x, w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: dsa_amd.rms_norm(x, w), lambda: dsa_amd.rms_norm(x.detach(), w),
+                     lambda: dsa_amd.rms_norm(x, w, eps=0)):  # eps as an int: checked in Python
+            with pytest.raises(ValueError, match="captured"):
+                call()
+        with torch.no_grad():
+            plain = dsa_amd.rms_norm(x, w)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(plain, kept)
+    del kept
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad(dsa_amd.rms_norm(x, w), w, x.detach())
+    graph.replay()
+    torch.cuda.synchronize()
+    (want,) = torch.autograd.grad(dsa_amd.rms_norm(x, w), w, x.detach())
+    assert torch.equal(got, want)
+
+
+def test_one_tensor_twice():
+    """x as its own residual: both summands' gradients arrive."""
+    x, w, g = make((33, 520), FULL).requires_grad_(), make(520, FULL, 1), make((33, 520), FULL, 2)
+    y, h = dsa_amd.rms_norm(x, w, x)
+    assert torch.equal(h, 2 * x)
+    (got,) = torch.autograd.grad((y, h), x, (g, g))
+    a, b = x.detach().clone().requires_grad_(), x.detach().clone().requires_grad_()
+    one, other = torch.autograd.grad(dsa_amd.rms_norm(a, w, b), (a, b), (g, g))
+    assert torch.equal(got, one + other)
+
+
+def test_views_of_the_other_sign():
+    """Views that keep their sign apart from their memory are taken by their values."""
+    x, w, r, g = make((9, 256), FULL), make(256, FULL, 1), make((9, 256), FULL, 2), make((9, 256), FULL, 3)
+    other = torch._neg_view
+    assert other(x).is_neg()
+    want = dsa_amd.rms_norm(-x, -w, -r)
+    for a, b in zip(want, dsa_amd.rms_norm(other(x), other(w), other(r))):
+        assert torch.equal(a, b)
+    for a, b in zip(dsa_amd.rms_norm_fp8(-x, w, -r) + dsa_amd.quantize_fp8(-x),
+                    dsa_amd.rms_norm_fp8(other(x), w, other(r)) + dsa_amd.quantize_fp8(other(x))):
+        assert torch.equal(a.float(), b.float())
+    for eps in (1e-6, 0):  # eps as an int: the Python path's backward
+        x1, r1 = x.clone().requires_grad_(), r.clone().requires_grad_()
+        want = torch.autograd.grad(dsa_amd.rms_norm(x1, w, r1, eps=eps), (x1, r1), (-g, -g))
+        got = torch.autograd.grad(dsa_amd.rms_norm(x1, w, r1, eps=eps), (x1, r1), (other(g), other(g)))
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
+
+
 def test_refusals():
     x, w = make((4, 512)), make(512)
     bad = [dict(x=x.double()), dict(x=x.cpu()), dict(x=x[:, ::2], weight=w[:256]), dict(x=None), dict(weight=None),

@@ -177,6 +177,16 @@ def test_repeats_streams_and_graphs(M, N, K):
         torch.cuda.synchronize()
 
 
+def test_views_of_the_other_sign():
+    a, sa, b, sb = make(4, 200, 256)
+    other = torch._neg_view
+    want = dsa_amd.matmul_fp8(a, -sa, b, -sb)
+    assert torch.equal(want, dsa_amd.matmul_fp8(a, other(sa), b, other(sb)))
+    for codes in (dict(a=other(a)), dict(b=other(b))):
+        with pytest.raises(ValueError):
+            dsa_amd.matmul_fp8(**{**dict(a=a, a_scales=sa, b=b, b_scales=sb), **codes})
+
+
 def test_refusals():
     a, sa, b, sb = make(4, 200, 256)
     good = dict(a=a, a_scales=sa, b=b, b_scales=sb)
