@@ -7,17 +7,21 @@
 // one block of weights, and have one scale.  The products of a block of 128 are
 // summed by the matrix cores from zero, and added to the result times that scale.
 //
-// The 8-bit matrix instructions do not keep all bits of their products: sums of 128
-// were off by 1.4e-5 (2^-16) of their size, far below the rounding of a 16-bit output
-// (2^-9 and 2^-12), far above that of a 32-bit one.  For 32-bit outputs the codes are
+// The 8-bit matrix instructions do not keep all bits of their products: of eight
+// neighbours each is cut, towards zero, to a multiple of 2^-13 of the power of two that
+// the largest one's exponents make (seen in sums of a large product, its opposite and
+// a third).  Sums of 128 were off by 1.4e-5 (2^-16) of their size, far below the
+// rounding of a 16-bit output (2^-9 and 2^-12), far above that of a 32-bit one.  For 32-bit outputs the codes are
 // widened to bf16, which holds them exactly, and go through the bf16 instructions,
 // whose sums were off by 1.3e-8, at half the rate (2.2 PFLOP/s for 4.6).
 //
 // One family of tiles, from 16 by 16 with K split over four waves to 256 by 256
 // (kVariants: which one, and what the others took).  Few rows are bound by the weights'
 // bytes and the latency of the steps (8 rows, 2112 columns, K 7168 6.0 us, 2.6 TB/s; 77,
-// 24576, 1536 11.3 us, 3.7 TB/s), many by the matrix cores beside the loads (8192, 7168,
-// 16384 838 us, 2.29 PFLOP/s; a library's product without these scales 699 us).  A step
+// 24576, 1536 10.5 us, 4.0 TB/s): from HBM a CU gets about 50 GB/s however much is under
+// way.  Middle ones (1000, 2112, 7168 26.1 us) by the steps of their smaller tiles, which
+// took as long on 17 workgroups alone.  Many by the matrix cores beside the loads (8192,
+// 7168, 16384 838 us, 2.29 PFLOP/s; a library's product without these scales 699 us).  A step
 // of a 256 by 256 tile takes 1.34 us on half the chip and 1.7 on all of it: 1.15 its
 // products and sums alone, 0.95 of that the products, and 1.1 its loads alone.
 #include <hip/hip_runtime.h>
@@ -88,7 +92,7 @@ __device__ __forceinline__ void store4(OUT* row, int n, int N, bool wide, const 
 // A workgroup computes TN columns by TM rows, a wave 16 NT by 16 MT of them, from a ring
 // of STAGES stages in LDS, which rows come into straight from memory.  A stage holds KS
 // blocks of 128 of K; KS groups of waves take one each, and join their sums at the end,
-// in their order.
+// in their order.  LW: waves of their own load, and the others do not.
 //
 // A row's 128 bytes lie in LDS as eight chunks of 16, chunk c of row r at c ^ swizzle(r):
 // a fragment read takes chunks g and 4 + g of 16 rows, and the 16 lanes of a
@@ -111,16 +115,17 @@ __device__ __forceinline__ void place(uint32_t t, int tiles_m, int tiles_n, int&
     n = (int)(in_band / high);
 }
 
-template <int NT, int MT, int WN, int WM, int KS, int STAGES>
+template <int NT, int MT, int WN, int WM, int KS, int STAGES, int LW = 0>
 struct Tile {
-    static constexpr int TN = 16 * NT * WN, TM = 16 * MT * WM, GROUP = WN * WM, WAVES = GROUP * KS, THREADS = 64 * WAVES;
-    static constexpr int B_LOADS = (TN + 8 * GROUP - 1) / (8 * GROUP), A_LOADS = (TM + 8 * GROUP - 1) / (8 * GROUP);  // a wave, of 8 rows each
+    static constexpr int TN = 16 * NT * WN, TM = 16 * MT * WM, GROUP = WN * WM, WAVES = GROUP * KS, THREADS = 64 * (WAVES + LW);
+    static constexpr int LOADING = LW ? LW : GROUP;  // waves that load a block
+    static constexpr int B_LOADS = (TN + 8 * LOADING - 1) / (8 * LOADING), A_LOADS = (TM + 8 * LOADING - 1) / (8 * LOADING);  // a wave, of 8 rows each
     static constexpr int LOADS = B_LOADS + A_LOADS;
-    static constexpr int A_OFF = B_LOADS * GROUP * 8 * kBlock, BLOCK = A_OFF + A_LOADS * GROUP * 8 * kBlock, STAGE = BLOCK * KS;
+    static constexpr int A_OFF = B_LOADS * LOADING * 8 * kBlock, BLOCK = A_OFF + A_LOADS * LOADING * 8 * kBlock, STAGE = BLOCK * KS;
     // Scales come 8 or 16 blocks of a row at a time, a row's 32 or 64 bytes, four or eight rows a load.
     static constexpr int S_BLOCKS = KS * (STAGES - 1) > 8 ? 16 : 8, S_STEPS = S_BLOCKS / KS, S_ROWS = 64 / S_BLOCKS;
-    static constexpr int S_LOADS = (TM + S_ROWS * WAVES - 1) / (S_ROWS * WAVES);
-    static constexpr int S_OFF = STAGES * STAGE, SB_OFF = S_LOADS * WAVES * 256, S_BYTES = SB_OFF + 256;
+    static constexpr int S_LOADS = (TM + S_ROWS * LOADING * KS - 1) / (S_ROWS * LOADING * KS);
+    static constexpr int S_OFF = STAGES * STAGE, SB_OFF = S_LOADS * LOADING * KS * 256, S_BYTES = SB_OFF + 256;
     static constexpr int JOIN_BYTES = KS > 1 ? WAVES * NT * MT * 1024 : 0;
     static constexpr int RING_BYTES = S_OFF + 2 * S_BYTES, LDS_BYTES = RING_BYTES > JOIN_BYTES ? RING_BYTES : JOIN_BYTES;
     // With two stages, the part of a stage that is read first -- the rows of a, and of
@@ -128,19 +133,21 @@ struct Tile {
     static constexpr bool HALVES = STAGES == 2 && NT % 2 == 0 && B_LOADS % 2 == 0 && TN % (8 * GROUP) == 0 && KS == 1;
     static constexpr int EARLY = A_LOADS + B_LOADS / 2;
     static constexpr int AHEAD = HALVES ? EARLY : (STAGES - 2) * LOADS;  // loads that may be in flight when a step begins
-    static_assert(S_BLOCKS % KS == 0 && S_STEPS >= STAGES - 1, "scales have landed by the step that needs them");
+    static_assert(LW == 0 || (KS == 1 && STAGES > 2), "operands a step ahead");
+    static_assert(S_BLOCKS % KS == 0 && S_STEPS >= STAGES - (LW ? 0 : 1), "scales have landed by the step that needs them");
     static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
-    static_assert((STAGES - 1) * LOADS < 64, "loads in flight are counted in six bits");
+    static_assert((STAGES - (LW ? 0 : 1)) * LOADS < 64, "loads in flight are counted in six bits");
     // a wave's columns lie in one block of weights
     static_assert(kBlock % (16 * NT) == 0, "one scale a wave");
 };
 
-template <typename OUT, int NT, int MT, int WN, int WM, int KS, int STAGES>
+template <typename OUT, int NT, int MT, int WN, int WM, int KS, int STAGES, int LW = 0>
 __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t lds, int m0, int n0) {
     constexpr bool EXACT = sizeof(OUT) == 4;
-    using T = Tile<NT, MT, WN, WM, KS, STAGES>;
+    using T = Tile<NT, MT, WN, WM, KS, STAGES, LW>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int group = KS > 1 ? wave / T::GROUP : 0, in_group = KS > 1 ? wave % T::GROUP : wave;
+    const bool loads = LW == 0 || wave >= T::WAVES;
+    const int group = KS > 1 ? wave / T::GROUP : 0, in_group = KS > 1 ? wave % T::GROUP : LW > 0 && loads ? wave - T::WAVES : wave;
     const int r = lane & 15, g = lane >> 4;
     const int K = p.K, blocks = (K + kBlock - 1) / kBlock, steps = (blocks + KS - 1) / KS;
     const int rows_m = min(T::TM, p.M - m0), rows_n = min(T::TN, p.N - n0);
@@ -182,11 +189,11 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
     auto issue_scales = [&](int c) __attribute__((always_inline)) {  // of blocks c * S_BLOCKS on
         const uint32_t to = lds + T::S_OFF + (uint32_t)(c & 1) * T::S_BYTES;
         const int k = c * T::S_BLOCKS + s_block;
-        if (wave == 0)  // the weights': those of 128 columns as those of a row
+        if (group == 0 && in_group == 0)  // the weights': those of 128 columns as those of a row
             gather_word(to + T::SB_OFF, rsb, k < blocks ? (uint32_t)(4 * (s_row * blocks + k)) : 0x80000000u);
 #pragma unroll
         for (int i = 0; i < T::S_LOADS; ++i) {
-            const int first = (wave * T::S_LOADS + i) * T::S_ROWS;
+            const int first = ((group * T::LOADING + in_group) * T::S_LOADS + i) * T::S_ROWS;
             gather_word(to + (uint32_t)first * (4 * T::S_BLOCKS), rs,
                         k < blocks ? (uint32_t)(4 * ((first + s_row) * blocks + k)) : 0x80000000u);
         }
@@ -202,73 +209,143 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    issue_scales(0);
+    auto read = [&](uint32_t lo, uint32_t hi, int tile) __attribute__((always_inline)) -> i32x8 {
+        const i32x4 l = lds_load<i32x4>(lo + tile * 16 * kBlock), h = lds_load<i32x4>(hi + tile * 16 * kBlock);
+        return __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    if constexpr (LW > 0) {
+        // Waves of their own load, whom a full queue stops alone, and the others read a
+        // step's operands in the step before, so that LDS and the matrix cores work beside
+        // each other.  Stage t is then free for loads in step t.
+        uint32_t at = 0;
+        if (loads) {
+            issue_scales(0);
 #pragma unroll
-    for (int t = 0; t < STAGES - 1; ++t) {
-        const Next n = next_at(t, (uint32_t)t * T::STAGE);
+            for (int t = 0; t < STAGES; ++t) {
+                const Next n = next_at(t, (uint32_t)t * T::STAGE);
 #pragma unroll
-        for (int i = 0; i < T::LOADS; ++i) issue(n, i);
-    }
-    if (T::HALVES) {
-        const Next n = next_at(1, T::STAGE);
-#pragma unroll
-        for (int i = 0; i < T::EARLY; ++i) issue(n, i);
-    }
-    uint32_t at = 0, ahead = (STAGES - 1) * T::STAGE;
-#pragma unroll 1
-    for (int t = 0; t < steps; ++t) {
-        wait_vmcnt<T::AHEAD>();
-        lds_barrier();  // stage t is there, and every wave is done with stage t - 1
-        const int k = t * KS + group;
-        const uint32_t stage = lds + at + (uint32_t)group * T::BLOCK;
-        const uint32_t b_lo = stage + b_frag, b_hi = b_lo ^ 64u, a_lo = stage + a_frag, a_hi = a_lo ^ 64u;
-        auto read = [&](uint32_t lo, uint32_t hi, int tile) __attribute__((always_inline)) -> i32x8 {
-            const i32x4 l = lds_load<i32x4>(lo + tile * 16 * kBlock), h = lds_load<i32x4>(hi + tile * 16 * kBlock);
-            return __builtin_shufflevector(l, h, 0, 1, 2, 3, 4, 5, 6, 7);
-        };
-        if (KS > 1 && k >= blocks) break;  // the last step, of a group that has no block: only the barriers of the end follow
-        i32x8 af[MT], bf[2];
-        float s[MT];
-        bf[0] = read(b_lo, b_hi, 0);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) af[i] = read(a_lo, a_hi, i);
-        const uint32_t chunk_at = (uint32_t)(k / T::S_BLOCKS & 1) * T::S_BYTES + 4u * (uint32_t)(k % T::S_BLOCKS);
-        const float sb = lds_load<float>(sb_frag + chunk_at);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) s[i] = lds_load<float>(s_frag + chunk_at + 64 * T::S_BLOCKS * i);
-        if (t % T::S_STEPS == 0) issue_scales(t / T::S_STEPS + 1);
-        const Next n = next_at(t + STAGES - 1, ahead);
-        const Next n2 = next_at(t + 2, at);
-        // products of tile j beside the sums of tile j - 1, and a few loads
-        f32x4 u[2][MT];
-#pragma unroll
-        for (int j = 0; j <= NT; ++j) {
-            if (j + 1 < NT) bf[(j + 1) & 1] = read(b_lo, b_hi, j + 1);
-            if constexpr (T::HALVES) {
-                // the last loads of stage t + 1, then, when all waves have read the first
-                // part of stage t (tiles up to NT / 2 - 1 are in registers), those of t + 2
-#pragma unroll
-                for (int i = T::EARLY; i < T::LOADS; ++i)
-                    if (i - T::EARLY == j) issue(n, i);
-                if (j == NT / 2 - 1) lds_barrier();
-#pragma unroll
-                for (int i = 0; i < T::EARLY; ++i)
-                    if (j >= NT / 2 - 1 && j < NT && i * (NT / 2 + 1) / T::EARLY == j - (NT / 2 - 1)) issue(n2, i);
-            } else {
-#pragma unroll
-                for (int i = 0; i < T::LOADS; ++i)
-                    if (i * NT / T::LOADS == j) issue(n, i);
+                for (int i = 0; i < T::LOADS; ++i) issue(n, i);
             }
+            wait_vmcnt<(STAGES - 1) * T::LOADS>();
+            lds_barrier();
+#pragma unroll 1
+            for (int t = 0; t < steps; ++t) {
+                wait_vmcnt<T::AHEAD>();
+                lds_barrier();
+                if (t % T::S_STEPS == 0) issue_scales(t / T::S_STEPS + 1);
+                const Next n = next_at(t + STAGES, at);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                if (j == 0) s[i] *= sb;
-                if (j < NT) u[j & 1][i] = dot128<EXACT>(bf[j & 1], af[i]);
-                if (j > 0) acc[j - 1][i] += u[(j - 1) & 1][i] * s[i];
+                for (int i = 0; i < T::LOADS; ++i) issue(n, i);
+                at = at + T::STAGE == T::S_OFF ? 0 : at + T::STAGE;
+            }
+            wait_vmcnt<0>();
+            return;
+        }
+        struct Operands {
+            i32x8 a[MT], b[NT];
+            float s[MT], sb;
+        };
+        auto fetch = [&](Operands& o, uint32_t stage, int t, int i) __attribute__((always_inline)) {
+            const uint32_t chunk_at = (uint32_t)(t / T::S_BLOCKS & 1) * T::S_BYTES + 4u * (uint32_t)(t % T::S_BLOCKS);
+            const uint32_t b_lo = lds + stage + b_frag, a_lo = lds + stage + a_frag;
+            if (i == 0) o.sb = lds_load<float>(sb_frag + chunk_at);
+            if (i < NT) {
+                o.b[i] = read(b_lo, b_lo ^ 64u, i);
+            } else {
+                o.a[i - NT] = read(a_lo, a_lo ^ 64u, i - NT);
+                o.s[i - NT] = lds_load<float>(s_frag + chunk_at + 64 * T::S_BLOCKS * (i - NT));
+            }
+        };
+        auto step = [&](const Operands& o, Operands& next, int t) __attribute__((always_inline)) {
+            lds_barrier();  // stage t + 1 is there, and every wave has read stage t
+            at = at + T::STAGE == T::S_OFF ? 0 : at + T::STAGE;
+            float s[MT];
+            f32x4 u[2];
+#pragma unroll
+            for (int i = 0; i <= NT * MT; ++i) {
+#pragma unroll
+                for (int k = 0; k < NT + MT; ++k)
+                    if (k * NT * MT / (NT + MT) == i) fetch(next, at, t + 1, k);
+                if (i < MT) s[i] = o.s[i] * o.sb;
+                if (i < NT * MT) u[i & 1] = dot128<EXACT>(o.b[i / MT], o.a[i % MT]);
+                if (i > 0) acc[(i - 1) / MT][(i - 1) % MT] += u[(i - 1) & 1] * s[(i - 1) % MT];
                 __builtin_amdgcn_sched_barrier(0);
             }
+        };
+        Operands even, odd;
+        lds_barrier();
+#pragma unroll
+        for (int k = 0; k < NT + MT; ++k) fetch(even, 0, 0, k);
+#pragma unroll 1
+        for (int t = 0; t < steps; t += 2) {
+            step(even, odd, t);
+            if (t + 1 < steps) step(odd, even, t + 1);
         }
-        at = at + T::STAGE == T::S_OFF ? 0 : at + T::STAGE;
-        ahead = ahead + T::STAGE == T::S_OFF ? 0 : ahead + T::STAGE;
+    } else {
+        issue_scales(0);
+#pragma unroll
+        for (int t = 0; t < STAGES - 1; ++t) {
+            const Next n = next_at(t, (uint32_t)t * T::STAGE);
+#pragma unroll
+            for (int i = 0; i < T::LOADS; ++i) issue(n, i);
+        }
+        if (T::HALVES) {
+            const Next n = next_at(1, T::STAGE);
+#pragma unroll
+            for (int i = 0; i < T::EARLY; ++i) issue(n, i);
+        }
+        uint32_t at = 0, ahead = (STAGES - 1) * T::STAGE;
+#pragma unroll 1
+        for (int t = 0; t < steps; ++t) {
+            wait_vmcnt<T::AHEAD>();
+            lds_barrier();  // stage t is there, and every wave is done with stage t - 1
+            const int k = t * KS + group;
+            const uint32_t stage = lds + at + (uint32_t)group * T::BLOCK;
+            const uint32_t b_lo = stage + b_frag, b_hi = b_lo ^ 64u, a_lo = stage + a_frag, a_hi = a_lo ^ 64u;
+            if (KS > 1 && k >= blocks) break;  // the last step, of a group that has no block: only the barriers of the end follow
+            i32x8 af[MT], bf[2];
+            float s[MT];
+            bf[0] = read(b_lo, b_hi, 0);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) af[i] = read(a_lo, a_hi, i);
+            const uint32_t chunk_at = (uint32_t)(k / T::S_BLOCKS & 1) * T::S_BYTES + 4u * (uint32_t)(k % T::S_BLOCKS);
+            const float sb = lds_load<float>(sb_frag + chunk_at);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) s[i] = lds_load<float>(s_frag + chunk_at + 64 * T::S_BLOCKS * i);
+            if (t % T::S_STEPS == 0) issue_scales(t / T::S_STEPS + 1);
+            const Next n = next_at(t + STAGES - 1, ahead);
+            const Next n2 = next_at(t + 2, at);
+            // products of tile j beside the sums of tile j - 1, and a few loads
+            f32x4 u[2][MT];
+#pragma unroll
+            for (int j = 0; j <= NT; ++j) {
+                if (j + 1 < NT) bf[(j + 1) & 1] = read(b_lo, b_hi, j + 1);
+                if constexpr (T::HALVES) {
+                    // the last loads of stage t + 1, then, when all waves have read the first
+                    // part of stage t (tiles up to NT / 2 - 1 are in registers), those of t + 2
+#pragma unroll
+                    for (int i = T::EARLY; i < T::LOADS; ++i)
+                        if (i - T::EARLY == j) issue(n, i);
+                    if (j == NT / 2 - 1) lds_barrier();
+#pragma unroll
+                    for (int i = 0; i < T::EARLY; ++i)
+                        if (j >= NT / 2 - 1 && j < NT && i * (NT / 2 + 1) / T::EARLY == j - (NT / 2 - 1)) issue(n2, i);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < T::LOADS; ++i)
+                        if (i * NT / T::LOADS == j) issue(n, i);
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    if (j == 0) s[i] *= sb;
+                    if (j < NT) u[j & 1][i] = dot128<EXACT>(bf[j & 1], af[i]);
+                    if (j > 0) acc[j - 1][i] += u[(j - 1) & 1][i] * s[i];
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            at = at + T::STAGE == T::S_OFF ? 0 : at + T::STAGE;
+            ahead = ahead + T::STAGE == T::S_OFF ? 0 : ahead + T::STAGE;
+        }
     }
     wait_vmcnt<0>();  // loads behind the last block write zeros into LDS
     const bool wide = (p.N & 3) == 0 && ((uintptr_t)p.out & (4 * sizeof(OUT) - 1)) == 0;
@@ -301,14 +378,14 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
     }
 }
 
-template <typename OUT, int NT, int MT, int WN, int WM, int KS, int STAGES>
-__global__ __launch_bounds__(64 * WN * WM * KS, 1) void product_tile_kernel(dsa_product_args p, int tiles_m, int tiles_n) {
-    using T = Tile<NT, MT, WN, WM, KS, STAGES>;
+template <typename OUT, int NT, int MT, int WN, int WM, int KS, int STAGES, int LW = 0>
+__global__ __launch_bounds__(64 * (WN * WM * KS + LW), 1) void product_tile_kernel(dsa_product_args p, int tiles_m, int tiles_n) {
+    using T = Tile<NT, MT, WN, WM, KS, STAGES, LW>;
     __shared__ __attribute__((aligned(1024))) char smem[T::LDS_BYTES];
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     int m, n;
     place(along_xcds(blockIdx.x, tiles_m * tiles_n), tiles_m, tiles_n, m, n);
-    product_tile<OUT, NT, MT, WN, WM, KS, STAGES>(p, lds, m * T::TM, n * T::TN);
+    product_tile<OUT, NT, MT, WN, WM, KS, STAGES, LW>(p, lds, m * T::TM, n * T::TN);
 }
 
 // Tiles of 256 by 256 for whole rounds of them, and those left over cut in two: a last
@@ -333,11 +410,11 @@ __global__ __launch_bounds__(Whole::THREADS, 1) void product_mixed_kernel(dsa_pr
     }
 }
 
-template <typename OUT, int NT, int MT, int WN, int WM, int KS, int STAGES>
+template <typename OUT, int NT, int MT, int WN, int WM, int KS, int STAGES, int LW = 0>
 void launch_tile(const dsa_product_args& p, hipStream_t stream) {
-    using T = Tile<NT, MT, WN, WM, KS, STAGES>;
+    using T = Tile<NT, MT, WN, WM, KS, STAGES, LW>;
     const int tiles_m = (p.M + T::TM - 1) / T::TM, tiles_n = (p.N + T::TN - 1) / T::TN;
-    hipLaunchKernelGGL((product_tile_kernel<OUT, NT, MT, WN, WM, KS, STAGES>), dim3(tiles_m * tiles_n), dim3(T::THREADS), 0, stream, p,
+    hipLaunchKernelGGL((product_tile_kernel<OUT, NT, MT, WN, WM, KS, STAGES, LW>), dim3(tiles_m * tiles_n), dim3(T::THREADS), 0, stream, p,
                        tiles_m, tiles_n);
 }
 
@@ -352,17 +429,21 @@ void launch_mixed(const dsa_product_args& p, int cus, hipStream_t stream) {
 // Tiles by the size of the call: a call takes as many rounds as its tiles fill CUs, and
 // a round its steps, and a start and end of about 2 us.  What a step takes was measured
 // on 17 to 256 workgroups with K from 1536 to 16384, and, where the stages of two
-// workgroups fit a CU's LDS, on 264 to 512.  Small tiles split K over their waves, so
-// that there are fewer steps.  Whole calls, us (rows, columns, K; columns x rows of a
-// tile, in `kVariants`' order):
-//   8, 2112, 7168      16x16 7.3, 32x16 10.4, 32x32 11.7, 64x32 14
-//   64, 2112, 7168     16x16 14.3, 32x32 11.5, 64x32 16.3, 64x64 20.5 and 21.4, 128x64 31.6
-//   16, 24576, 1536    16x16 13.4, 32x32 14.4, 64x32 12.4, 64x64 13.2 and 10.5, 128x32 10.0, 128x64 10.4
-//   512, 2112, 7168    32x32 45, 64x64 33.8 and 28.0, 128x32 46, 128x64 31.4, 128x128 37.3
-//   1000, 2112, 7168   64x64 49.0 and 45.5, 128x64 60.6, 128x80 34.4, 128x128 37.3, 128x256 63
-//   1024, 7168, 16384  64x64 239, 128x80 216, 128x128 168, 128x256 149, 256x256 189
-//   1024, 24576, 1536  128x128 76, 128x256 65, 256x256 63
-// Over 44 drawn calls of these ranges the chosen tile took 1.6 % longer than the best one.
+// workgroups fit a CU's LDS, on 264 to 512.  The smallest split K over their waves, so
+// that there are fewer steps; from 64 by 64 on waves of their own load: without them
+// (columns, rows, K) 128x64 took 31.6 us for 26.9 at (2112, 512, 7168), 128x96 32.6 for
+// 28.7 at (2112, 1000, 7168), 128x128 37.5 for 33.8.  The 32-bit outputs' widened codes
+// need more registers than a third wave a SIMD leaves, so that from 128x96 on they load
+// themselves.  Whole calls, us (rows, columns, K; columns x rows of a tile):
+//   8, 2112, 7168      16x16 7.0, 32x16 10.4, 32x32 9.7, 64x32 14, 64x64 15
+//   64, 2112, 7168     16x16 13.8, 32x32 11.4, 64x32 16.3, 64x64 20, 128x64 28.6
+//   16, 24576, 1536    64x32 12.3, 64x64 10.8, 128x32 9.7, 128x64 10.0, 128x96 10.4
+//   448, 2112, 7168    64x32 29.7, 64x64 19.5, 128x32 22.0, 128x64 26.9, 128x96 29.4
+//   512, 4096, 7168    64x64 33.1, 128x64 27.7, 128x96 28.0, 128x128 35.0
+//   1000, 2112, 7168   64x64 39.6, 128x64 43.7, 128x96 28.7, 128x128 33.8, 128x160 40.5
+//   2000, 2112, 7168   64x64 63.9, 128x96 56.0, 128x128 64.6, 128x160 46.3, 128x256 64
+//   1024, 7168, 16384  64x64 207, 128x96 181, 128x128 156, 128x160 172, 128x256 148, 256x256 189
+// Over 48 drawn calls of these ranges the chosen tile took 1.3 % longer than the best one.
 struct Variant {
     int columns, rows, blocks;  // of a tile, and blocks of K a step
     float step, both;           // us a step, alone on a CU and beside another; 0: does not fit beside another
@@ -372,14 +453,15 @@ struct Variant {
 const Variant kVariants[] = {
     {16, 16, 4, 0.31f, 0.58f, DSA_TILE(1, 1, 1, 1, 4, 4)},  {32, 16, 4, 0.53f, 0.70f, DSA_TILE(1, 1, 2, 1, 4, 3)},
     {32, 32, 4, 0.63f, 0.00f, DSA_TILE(1, 2, 2, 1, 4, 4)},  {64, 32, 2, 0.48f, 0.00f, DSA_TILE(1, 2, 4, 1, 2, 4)},
-    {64, 64, 2, 0.59f, 0.00f, DSA_TILE(2, 2, 2, 2, 2, 4)},  {64, 64, 1, 0.33f, 0.45f, DSA_TILE(2, 2, 2, 2, 1, 4)},
-    {128, 32, 1, 0.39f, 0.00f, DSA_TILE(1, 2, 8, 1, 1, 4)}, {128, 64, 1, 0.51f, 0.00f, DSA_TILE(1, 4, 8, 1, 1, 4)},
-    {128, 80, 1, 0.55f, 0.00f, DSA_TILE(1, 5, 8, 1, 1, 4)}, {128, 128, 1, 0.61f, 0.00f, DSA_TILE(2, 4, 4, 2, 1, 4)},
+    {64, 64, 1, 0.31f, 0.50f, DSA_TILE(2, 2, 2, 2, 1, 4, 4)},   {128, 32, 1, 0.36f, 0.00f, DSA_TILE(2, 2, 4, 1, 1, 4, 4)},
+    {128, 64, 1, 0.45f, 0.00f, DSA_TILE(2, 4, 4, 1, 1, 4, 4)},  {128, 96, 1, 0.48f, 0.00f, {launch_tile<__bf16, 2, 3, 4, 2, 1, 4, 4>, launch_tile<f16, 2, 3, 4, 2, 1, 4, 4>, launch_tile<float, 2, 3, 4, 2, 1, 4>}},
+    {128, 128, 1, 0.58f, 0.00f, {launch_tile<__bf16, 2, 4, 4, 2, 1, 4, 4>, launch_tile<f16, 2, 4, 4, 2, 1, 4, 4>, launch_tile<float, 2, 4, 4, 2, 1, 4>}},
+    {128, 160, 1, 0.68f, 0.00f, {launch_tile<__bf16, 4, 5, 2, 2, 1, 4, 4>, launch_tile<f16, 4, 5, 2, 2, 1, 4, 4>, nullptr}},
     {128, 256, 1, 1.07f, 0.00f, DSA_TILE(4, 4, 2, 4, 1, 2)},
 };
-// A grid's threads, 512 a tile, are counted in 32 bits.  The 128 by 256 tiles of the
+// A grid's threads, up to 768 a tile, are counted in 32 bits.  The 128 by 256 tiles of the
 // largest output, 2^37 with at most 2^24 rows and columns, always fit.
-constexpr int64_t kMaxTiles = (1 << 23) - 1;
+constexpr int64_t kMaxTiles = 5 << 20;
 static_assert(((int64_t)1 << 37) / (128 * 256) + (1 << 24) / 128 + (1 << 24) / 256 + 1 <= kMaxTiles, "one tile is left");
 constexpr float kWholeStep = 1.70f, kHalfStep = 1.07f;  // of the mixed kernel
 
@@ -391,7 +473,7 @@ int launch_product(const dsa_product_args& p, int cus, hipStream_t stream) {
     float least = 0.f;
     for (const Variant& v : kVariants) {
         const int64_t tiles = (int64_t)((p.M + v.rows - 1) / v.rows) * ((p.N + v.columns - 1) / v.columns);
-        if (tiles > kMaxTiles) continue;
+        if (tiles > kMaxTiles || !v.launch[p.dtype]) continue;
         const bool pairs = v.both > 0.f && tiles > cus;
         const int64_t fit = pairs ? 2 * cus : cus;
         const float time = (float)((tiles + fit - 1) / fit) *
