@@ -109,6 +109,14 @@ def test_short_products_of_every_large_tile(M, N, K, dtype):
     check(dsa_amd.matmul_fp8(*args, dtype=dtype), *args, cut=True)
 
 
+@pytest.mark.parametrize("dtype", [BF, FULL])
+@pytest.mark.parametrize("K", [16, 272, 400, 1040, 7184])
+@pytest.mark.parametrize("M, N", [(30, 2100), (9, 6001), (8, 2112), (61, 2111), (100, 2112), (9, 4500)])
+def test_short_products_of_every_small_tile(M, N, K, dtype):
+    args = make(M, N, K, seed=4)
+    check(dsa_amd.matmul_fp8(*args, dtype=dtype), *args, cut=True)
+
+
 def test_leading_dimensions_and_empty():
     a, sa, b, sb = make(24, 100, 256)
     want = dsa_amd.matmul_fp8(a, sa, b, sb)
