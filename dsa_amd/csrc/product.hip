@@ -20,10 +20,10 @@
 // bytes and the latency of the steps (8 rows, 2112 columns, K 7168 6.0 us, 2.6 TB/s; 77,
 // 24576, 1536 10.5 us, 4.0 TB/s): from HBM a CU gets about 50 GB/s however much is under
 // way.  Middle ones (1000, 2112, 7168 26.1 us) by the steps of their smaller tiles, which
-// took as long on 17 workgroups alone.  Many by the matrix cores beside the loads (8192,
-// 7168, 16384 838 us, 2.29 PFLOP/s; a library's product without these scales 699 us).  A step
-// of a 256 by 256 tile takes 1.34 us on half the chip and 1.7 on all of it: 1.15 its
-// products and sums alone, 0.95 of that the products, and 1.1 its loads alone.
+// took as long on 17 workgroups alone.  Many by the matrix cores, and the clock that is
+// left to them under load (8192, 7168, 16384 838 us, 2.29 PFLOP/s; a library's product
+// without these scales 699 us): a step of a 256 by 256 tile takes 1.34 us on half the chip
+// and 1.7 on all of it, its products and sums alone, of random codes, 0.97 and 1.20.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>
