@@ -124,6 +124,8 @@ struct Tile {
     static constexpr int A_OFF = B_LOADS * LOADING * 8 * kBlock, BLOCK = A_OFF + A_LOADS * LOADING * 8 * kBlock, STAGE = BLOCK * KS;
     // Scales come 8 or 16 blocks of a row at a time, a row's 32 or 64 bytes, four or eight rows a load.
     static constexpr int S_BLOCKS = KS * (STAGES - 1) > 8 ? 16 : 8, S_STEPS = S_BLOCKS / KS, S_ROWS = 64 / S_BLOCKS;
+    // Four rows (two, of 16 blocks) fill 32 banks: the next ones have their blocks in another order.
+    static __device__ constexpr int s_swizzle(int row) { return S_BLOCKS == 8 ? row >> 2 & 3 : row >> 1 & 7; }
     static constexpr int S_LOADS = (TM + S_ROWS * LOADING * KS - 1) / (S_ROWS * LOADING * KS);
     static constexpr int S_OFF = STAGES * STAGE, SB_OFF = S_LOADS * LOADING * KS * 256, S_BYTES = SB_OFF + 256;
     static constexpr int JOIN_BYTES = KS > 1 ? WAVES * NT * MT * 1024 : 0;
@@ -194,8 +196,9 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
 #pragma unroll
         for (int i = 0; i < T::S_LOADS; ++i) {
             const int first = ((group * T::LOADING + in_group) * T::S_LOADS + i) * T::S_ROWS;
+            const int of = c * T::S_BLOCKS + (s_block ^ T::s_swizzle(first + s_row));
             gather_word(to + (uint32_t)first * (4 * T::S_BLOCKS), rs,
-                        k < blocks ? (uint32_t)(4 * ((first + s_row) * blocks + k)) : 0x80000000u);
+                        of < blocks ? (uint32_t)(4 * ((first + s_row) * blocks + of)) : 0x80000000u);
         }
     };
     const int wn = in_group % WN, wm = in_group / WN;
@@ -203,6 +206,7 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
     const uint32_t frag = (uint32_t)r * kBlock + 16u * ((uint32_t)g ^ swizzle(r));
     const uint32_t b_frag = frag + (uint32_t)wn * NT * 16 * kBlock, a_frag = frag + T::A_OFF + (uint32_t)wm * MT * 16 * kBlock;
     const uint32_t s_frag = lds + T::S_OFF + 4u * T::S_BLOCKS * (uint32_t)(wm * MT * 16 + r);
+    const uint32_t s_order = 4u * (uint32_t)T::s_swizzle(r);
     const uint32_t sb_frag = lds + T::S_OFF + T::SB_OFF + 4u * T::S_BLOCKS * (uint32_t)((n0 % kBlock + 16 * NT * wn) / kBlock);
     f32x4 acc[NT][MT];
 #pragma unroll
@@ -247,13 +251,14 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
         };
         auto fetch = [&](Operands& o, uint32_t stage, int t, int i) __attribute__((always_inline)) {
             const uint32_t chunk_at = (uint32_t)(t / T::S_BLOCKS & 1) * T::S_BYTES + 4u * (uint32_t)(t % T::S_BLOCKS);
+            const uint32_t s_at = s_frag + (chunk_at ^ s_order);
             const uint32_t b_lo = lds + stage + b_frag, a_lo = lds + stage + a_frag;
             if (i == 0) o.sb = lds_load<float>(sb_frag + chunk_at);
             if (i < NT) {
                 o.b[i] = read(b_lo, b_lo ^ 64u, i);
             } else {
                 o.a[i - NT] = read(a_lo, a_lo ^ 64u, i - NT);
-                o.s[i - NT] = lds_load<float>(s_frag + chunk_at + 64 * T::S_BLOCKS * (i - NT));
+                o.s[i - NT] = lds_load<float>(s_at + 64 * T::S_BLOCKS * (i - NT));
             }
         };
         auto step = [&](const Operands& o, Operands& next, int t) __attribute__((always_inline)) {
@@ -311,7 +316,7 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
             const uint32_t chunk_at = (uint32_t)(k / T::S_BLOCKS & 1) * T::S_BYTES + 4u * (uint32_t)(k % T::S_BLOCKS);
             const float sb = lds_load<float>(sb_frag + chunk_at);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) s[i] = lds_load<float>(s_frag + chunk_at + 64 * T::S_BLOCKS * i);
+            for (int i = 0; i < MT; ++i) s[i] = lds_load<float>(s_frag + (chunk_at ^ s_order) + 64 * T::S_BLOCKS * i);
             if (t % T::S_STEPS == 0) issue_scales(t / T::S_STEPS + 1);
             const Next n = next_at(t + STAGES - 1, ahead);
             const Next n2 = next_at(t + 2, at);
