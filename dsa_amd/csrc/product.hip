@@ -134,8 +134,10 @@ struct Tile {
     // the weights half of each wave's -- is loaded again within the step that reads it.
     static constexpr bool HALVES = STAGES == 2 && NT % 2 == 0 && B_LOADS % 2 == 0 && TN % (8 * GROUP) == 0 && KS == 1;
     static constexpr int EARLY = A_LOADS + B_LOADS / 2;
-    static constexpr int AHEAD = HALVES ? EARLY : (STAGES - 2) * LOADS;  // loads that may be in flight when a step begins
+    static constexpr int EARLIEST = (NT / 2 * EARLY + NT / 2) / (NT / 2 + 1);  // of them, those issued before a step's last tile
+    static constexpr int AHEAD = HALVES ? EARLIEST : (STAGES - 2) * LOADS;  // loads that may be in flight when a step begins
     static_assert(LW == 0 || (KS == 1 && STAGES > 2), "operands a step ahead");
+    static_assert(STAGES > 2 || HALVES, "two stages by halves");
     static_assert(S_BLOCKS % KS == 0 && S_STEPS >= STAGES - (LW ? 0 : 1), "scales have landed by the step that needs them");
     static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
     static_assert((STAGES - (LW ? 0 : 1)) * LOADS < 64, "loads in flight are counted in six bits");
@@ -205,8 +207,11 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
     // fragment reads: chunk g (and 4 + g: ^ 64) of row r of a 16-row tile
     const uint32_t frag = (uint32_t)r * kBlock + 16u * ((uint32_t)g ^ swizzle(r));
     const uint32_t b_frag = frag + (uint32_t)wn * NT * 16 * kBlock, a_frag = frag + T::A_OFF + (uint32_t)wm * MT * 16 * kBlock;
-    const uint32_t s_frag = lds + T::S_OFF + 4u * T::S_BLOCKS * (uint32_t)(wm * MT * 16 + r);
-    const uint32_t s_order = 4u * (uint32_t)T::s_swizzle(r);
+    // a row's scale: of block k, its number ^ s_swizzle(row)
+    const uint32_t s_frag = lds + T::S_OFF + 4u * T::S_BLOCKS * (uint32_t)(wm * MT * 16 + r) + 4u * (uint32_t)T::s_swizzle(r);
+    auto scale_at = [&](int k) __attribute__((always_inline)) -> uint32_t {
+        return (s_frag ^ 4u * (uint32_t)(k % T::S_BLOCKS)) + (uint32_t)(k / T::S_BLOCKS & 1) * T::S_BYTES;
+    };
     const uint32_t sb_frag = lds + T::S_OFF + T::SB_OFF + 4u * T::S_BLOCKS * (uint32_t)((n0 % kBlock + 16 * NT * wn) / kBlock);
     f32x4 acc[NT][MT];
 #pragma unroll
@@ -251,7 +256,7 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
         };
         auto fetch = [&](Operands& o, uint32_t stage, int t, int i) __attribute__((always_inline)) {
             const uint32_t chunk_at = (uint32_t)(t / T::S_BLOCKS & 1) * T::S_BYTES + 4u * (uint32_t)(t % T::S_BLOCKS);
-            const uint32_t s_at = s_frag + (chunk_at ^ s_order);
+            const uint32_t s_at = scale_at(t);
             const uint32_t b_lo = lds + stage + b_frag, a_lo = lds + stage + a_frag;
             if (i == 0) o.sb = lds_load<float>(sb_frag + chunk_at);
             if (i < NT) {
@@ -286,6 +291,77 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
             step(even, odd, t);
             if (t + 1 < steps) step(odd, even, t + 1);
         }
+    } else if constexpr (T::HALVES) {
+        // Two stages.  A step's first operands are read beside the last products of the one
+        // before, in the place of those that it is done with, so that the matrix cores go
+        // on through the barrier: 8192 rows, 2112 columns, K 7168 168 -> 155 us.
+        issue_scales(0);
+        {
+            const Next n = next_at(0, 0), n1 = next_at(1, T::STAGE);
+#pragma unroll
+            for (int i = 0; i < T::LOADS; ++i) issue(n, i);
+#pragma unroll
+            for (int i = 0; i < T::EARLY; ++i) issue(n1, i);
+        }
+        uint32_t at = 0;  // stage t; t + 1: the other one
+        i32x8 af[MT], bf[2];
+        float next_s[MT], next_sb;
+        auto read_b = [&](uint32_t stage, int tile) __attribute__((always_inline)) -> i32x8 {
+            return read(lds + stage + b_frag, (lds + stage + b_frag) ^ 64u, tile);
+        };
+        auto read_a = [&](uint32_t stage, int tile) __attribute__((always_inline)) -> i32x8 {
+            return read(lds + stage + a_frag, (lds + stage + a_frag) ^ 64u, tile);
+        };
+        auto read_scales = [&](int k) __attribute__((always_inline)) {
+            const uint32_t chunk_at = (uint32_t)(k / T::S_BLOCKS & 1) * T::S_BYTES + 4u * (uint32_t)(k % T::S_BLOCKS);
+            next_sb = lds_load<float>(sb_frag + chunk_at);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) next_s[i] = lds_load<float>(scale_at(k) + 64 * T::S_BLOCKS * i);
+        };
+        wait_vmcnt<T::EARLY>();
+        lds_barrier();
+        bf[0] = read_b(0, 0);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) af[i] = read_a(0, i);
+        read_scales(0);
+#pragma unroll 1
+        for (int t = 0; t < steps; ++t) {
+            const uint32_t other = T::STAGE - at;
+            float s[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) s[i] = next_s[i] * next_sb;
+            if (t % T::S_STEPS == 0) issue_scales(t / T::S_STEPS + 1);
+            const Next n = next_at(t + 1, other), n2 = next_at(t + 2, at);
+            // products of tile j beside the sums of tile j - 1, and a few loads
+            f32x4 u[2][MT];
+#pragma unroll
+            for (int j = 0; j <= NT; ++j) {
+                if (j == NT - 1) {  // stage t + 1 is there, and every wave has read stage t: the next step's first operands
+                    wait_vmcnt<T::AHEAD>();
+                    lds_barrier();
+                    bf[0] = read_b(other, 0);
+                    read_scales(t + 1);
+                }
+                if (j + 1 < NT) bf[(j + 1) & 1] = read_b(at, j + 1);
+                // the last loads of stage t + 1, then, when all waves have read the first
+                // part of stage t (tiles up to NT / 2 - 1 are in registers), those of t + 2
+#pragma unroll
+                for (int i = T::EARLY; i < T::LOADS; ++i)
+                    if (i - T::EARLY == j) issue(n, i);
+                if (j == NT / 2 - 1) lds_barrier();
+#pragma unroll
+                for (int i = 0; i < T::EARLY; ++i)
+                    if (j >= NT / 2 - 1 && j < NT && i * (NT / 2 + 1) / T::EARLY == j - (NT / 2 - 1)) issue(n2, i);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    if (j < NT) u[j & 1][i] = dot128<EXACT>(bf[j & 1], af[i]);
+                    if (j > 0) acc[j - 1][i] += u[(j - 1) & 1][i] * s[i];
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (j == NT - 1) af[i] = read_a(other, i);
+                }
+            }
+            at = other;
+        }
     } else {
         issue_scales(0);
 #pragma unroll
@@ -293,11 +369,6 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
             const Next n = next_at(t, (uint32_t)t * T::STAGE);
 #pragma unroll
             for (int i = 0; i < T::LOADS; ++i) issue(n, i);
-        }
-        if (T::HALVES) {
-            const Next n = next_at(1, T::STAGE);
-#pragma unroll
-            for (int i = 0; i < T::EARLY; ++i) issue(n, i);
         }
         uint32_t at = 0, ahead = (STAGES - 1) * T::STAGE;
 #pragma unroll 1
@@ -316,30 +387,17 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
             const uint32_t chunk_at = (uint32_t)(k / T::S_BLOCKS & 1) * T::S_BYTES + 4u * (uint32_t)(k % T::S_BLOCKS);
             const float sb = lds_load<float>(sb_frag + chunk_at);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) s[i] = lds_load<float>(s_frag + (chunk_at ^ s_order) + 64 * T::S_BLOCKS * i);
+            for (int i = 0; i < MT; ++i) s[i] = lds_load<float>(scale_at(k) + 64 * T::S_BLOCKS * i);
             if (t % T::S_STEPS == 0) issue_scales(t / T::S_STEPS + 1);
             const Next n = next_at(t + STAGES - 1, ahead);
-            const Next n2 = next_at(t + 2, at);
             // products of tile j beside the sums of tile j - 1, and a few loads
             f32x4 u[2][MT];
 #pragma unroll
             for (int j = 0; j <= NT; ++j) {
                 if (j + 1 < NT) bf[(j + 1) & 1] = read(b_lo, b_hi, j + 1);
-                if constexpr (T::HALVES) {
-                    // the last loads of stage t + 1, then, when all waves have read the first
-                    // part of stage t (tiles up to NT / 2 - 1 are in registers), those of t + 2
 #pragma unroll
-                    for (int i = T::EARLY; i < T::LOADS; ++i)
-                        if (i - T::EARLY == j) issue(n, i);
-                    if (j == NT / 2 - 1) lds_barrier();
-#pragma unroll
-                    for (int i = 0; i < T::EARLY; ++i)
-                        if (j >= NT / 2 - 1 && j < NT && i * (NT / 2 + 1) / T::EARLY == j - (NT / 2 - 1)) issue(n2, i);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < T::LOADS; ++i)
-                        if (i * NT / T::LOADS == j) issue(n, i);
-                }
+                for (int i = 0; i < T::LOADS; ++i)
+                    if (i * NT / T::LOADS == j) issue(n, i);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
                     if (j == 0) s[i] *= sb;
@@ -448,8 +506,9 @@ void launch_mixed(const dsa_product_args& p, int cus, hipStream_t stream) {
 //   448, 2112, 7168    64x32 29.7, 64x64 19.5, 128x32 22.0, 128x64 26.9, 128x96 29.4
 //   512, 4096, 7168    64x64 33.1, 128x64 27.7, 128x96 28.0, 128x128 35.0
 //   1000, 2112, 7168   64x64 39.6, 128x64 43.7, 128x96 28.7, 128x128 33.8, 128x160 40.5
-//   2000, 2112, 7168   64x64 63.9, 128x96 56.0, 128x128 64.6, 128x160 46.3, 128x256 64
-//   1024, 7168, 16384  64x64 207, 128x96 181, 128x128 156, 128x160 172, 128x256 148, 256x256 189
+//   2000, 2112, 7168   64x64 63.9, 128x96 56.0, 128x128 62.0, 128x160 42.4, 128x256 58.9
+//   1000, 7168, 16384  64x64 207, 128x96 181, 128x128 156, 128x160 172, 128x256 135, 256x256 137
+//   8192, 2112, 7168   128x96 174, 128x128 172, 128x160 170, 128x256 175, 256x256 155
 // Over 48 drawn calls of these ranges the chosen tile took 2 % longer than the best one
 // (at most 21 %, where few rows meet 24576 by 16384).
 struct Variant {
@@ -466,13 +525,13 @@ const Variant kVariants[] = {
     {128, 64, 1, 0.45f, 0.00f, DSA_TILE(2, 4, 4, 1, 1, 4, 4)},  {128, 96, 1, 0.48f, 0.00f, {launch_tile<__bf16, 2, 3, 4, 2, 1, 4, 4>, launch_tile<f16, 2, 3, 4, 2, 1, 4, 4>, launch_tile<float, 2, 3, 4, 2, 1, 4>}},
     {128, 128, 1, 0.58f, 0.00f, {launch_tile<__bf16, 2, 4, 4, 2, 1, 4, 4>, launch_tile<f16, 2, 4, 4, 2, 1, 4, 4>, launch_tile<float, 2, 4, 4, 2, 1, 4>}},
     {128, 160, 1, 0.68f, 0.00f, {launch_tile<__bf16, 4, 5, 2, 2, 1, 4, 4>, launch_tile<f16, 4, 5, 2, 2, 1, 4, 4>, nullptr}},
-    {128, 256, 1, 1.07f, 0.00f, DSA_TILE(4, 4, 2, 4, 1, 2)},
+    {128, 256, 1, 1.02f, 0.00f, DSA_TILE(4, 4, 2, 4, 1, 2)},
 };
 // A grid's threads, up to 768 a tile, are counted in 32 bits.  The 128 by 256 tiles of the
 // largest output, 2^37 with at most 2^24 rows and columns, always fit.
 constexpr int64_t kMaxTiles = 5 << 20;
 static_assert(((int64_t)1 << 37) / (128 * 256) + (1 << 24) / 128 + (1 << 24) / 256 + 1 <= kMaxTiles, "one tile is left");
-constexpr float kWholeStep = 1.70f, kHalfStep = 1.07f;  // of the mixed kernel
+constexpr float kWholeStep = 1.70f, kHalfStep = 1.02f;  // of the mixed kernel
 
 }  // namespace
 
