@@ -136,6 +136,9 @@ struct Tile {
     static constexpr int EARLY = A_LOADS + B_LOADS / 2;
     static constexpr int EARLIEST = (NT / 2 * EARLY + NT / 2) / (NT / 2 + 1);  // of them, those issued before a step's last tile
     static constexpr int AHEAD = HALVES ? EARLIEST : (STAGES - 2) * LOADS;  // loads that may be in flight when a step begins
+    // Products that wait to be added (LW): what the registers hold beside the operands.
+    static constexpr int BEHIND = NT * MT <= 6 ? NT * MT : NT * MT <= 8 ? 4 : 2;
+    static_assert(NT * MT % BEHIND == 0 || LW == 0, "a product has one register");
     static_assert(LW == 0 || (KS == 1 && STAGES > 2), "operands a step ahead");
     static_assert(STAGES > 2 || HALVES, "two stages by halves");
     static_assert(S_BLOCKS % KS == 0 && S_STEPS >= STAGES - (LW ? 0 : 1), "scales have landed by the step that needs them");
@@ -266,23 +269,38 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
                 o.s[i - NT] = lds_load<float>(s_at + 64 * T::S_BLOCKS * (i - NT));
             }
         };
+        // A product is added D products later, so that none is waited for: those of a step's
+        // end beside the next step's first.
+        constexpr int P = NT * MT, D = T::BEHIND;
+        f32x4 u[D];
+        float last[MT];  // scales of the step before
+        auto add = [&](int i, const float (&s)[MT]) __attribute__((always_inline)) {  // what product i's register holds
+            const int of = i < D ? P + i - D : i - D;
+            acc[of / MT][of % MT] += u[i % D] * (i < D ? last : s)[of % MT];
+        };
         auto step = [&](const Operands& o, Operands& next, int t) __attribute__((always_inline)) {
             lds_barrier();  // stage t + 1 is there, and every wave has read stage t
             at = at + T::STAGE == T::S_OFF ? 0 : at + T::STAGE;
             float s[MT];
-            f32x4 u[2];
 #pragma unroll
-            for (int i = 0; i <= NT * MT; ++i) {
+            for (int i = 0; i < MT; ++i) s[i] = o.s[i] * o.sb;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
 #pragma unroll
                 for (int k = 0; k < NT + MT; ++k)
-                    if (k * NT * MT / (NT + MT) == i) fetch(next, at, t + 1, k);
-                if (i < MT) s[i] = o.s[i] * o.sb;
-                if (i < NT * MT) u[i & 1] = dot128<EXACT>(o.b[i / MT], o.a[i % MT]);
-                if (i > 0) acc[(i - 1) / MT][(i - 1) % MT] += u[(i - 1) & 1] * s[(i - 1) % MT];
+                    if (k * P / (NT + MT) == i) fetch(next, at, t + 1, k);
+                add(i, s);
+                u[i % D] = dot128<EXACT>(o.b[i / MT], o.a[i % MT]);
                 __builtin_amdgcn_sched_barrier(0);
             }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) last[i] = s[i];
         };
         Operands even, odd;
+#pragma unroll
+        for (int i = 0; i < D; ++i) u[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < MT; ++i) last[i] = 0.f;
         lds_barrier();
 #pragma unroll
         for (int k = 0; k < NT + MT; ++k) fetch(even, 0, 0, k);
@@ -291,6 +309,8 @@ __device__ __forceinline__ void product_tile(const dsa_product_args& p, uint32_t
             step(even, odd, t);
             if (t + 1 < steps) step(odd, even, t + 1);
         }
+#pragma unroll
+        for (int i = 0; i < D; ++i) add(i, last);
     } else if constexpr (T::HALVES) {
         // Two stages.  A step's first operands are read beside the last products of the one
         // before, in the place of those that it is done with, so that the matrix cores go
@@ -503,11 +523,11 @@ void launch_mixed(const dsa_product_args& p, int cus, hipStream_t stream) {
 //   32, 2112, 16384    16x16 17.9, 16x32 16.0, 32x16 16.9, 32x32 20.9, 64x32 28
 //   64, 2112, 7168     16x16 13.8, 32x32 11.4, 64x32 16.3, 64x64 20, 128x64 28.6
 //   16, 24576, 1536    64x32 12.3, 64x64 10.8, 128x32 9.7, 128x64 10.0, 128x96 10.4
-//   448, 2112, 7168    64x32 29.7, 64x64 19.5, 128x32 22.0, 128x64 26.9, 128x96 29.4
-//   512, 4096, 7168    64x64 33.1, 128x64 27.7, 128x96 28.0, 128x128 35.0
-//   1000, 2112, 7168   64x64 39.6, 128x64 43.7, 128x96 28.7, 128x128 33.8, 128x160 40.5
-//   2000, 2112, 7168   64x64 63.9, 128x96 56.0, 128x128 62.0, 128x160 42.4, 128x256 58.9
-//   1000, 7168, 16384  64x64 207, 128x96 181, 128x128 156, 128x160 172, 128x256 135, 256x256 137
+//   448, 2112, 7168    64x32 29.7, 64x64 19.5, 128x32 22.0, 128x64 26.2, 128x96 29.2
+//   512, 4096, 7168    64x64 33.7, 128x64 27.6, 128x96 27.6, 128x128 34.8
+//   1000, 2112, 7168   64x64 41, 128x64 41, 128x96 27.9, 128x128 33.4, 128x160 34.9
+//   2000, 2112, 7168   64x64 64, 128x96 52.4, 128x128 59, 128x160 41.3, 128x256 59
+//   1000, 7168, 16384  64x64 201, 128x96 170, 128x128 142, 128x160 156, 128x256 134, 256x256 134
 //   8192, 2112, 7168   128x96 174, 128x128 172, 128x160 170, 128x256 175, 256x256 155
 // Over 48 drawn calls of these ranges the chosen tile took 2 % longer than the best one
 // (at most 21 %, where few rows meet 24576 by 16384).
@@ -522,9 +542,9 @@ const Variant kVariants[] = {
     {16, 32, 4, 0.45f, 0.00f, DSA_TILE(1, 2, 1, 1, 4, 4)},  {32, 16, 4, 0.49f, 0.00f, DSA_TILE(1, 1, 2, 1, 4, 4)},
     {32, 16, 4, 0.53f, 0.70f, DSA_TILE(1, 1, 2, 1, 4, 3)},  {32, 32, 4, 0.60f, 0.00f, DSA_TILE(1, 2, 2, 1, 4, 4)},  {64, 32, 2, 0.48f, 0.00f, DSA_TILE(1, 2, 4, 1, 2, 4)},
     {64, 64, 1, 0.31f, 0.50f, DSA_TILE(2, 2, 2, 2, 1, 4, 4)},   {128, 32, 1, 0.36f, 0.00f, DSA_TILE(2, 2, 4, 1, 1, 4, 4)},
-    {128, 64, 1, 0.45f, 0.00f, DSA_TILE(2, 4, 4, 1, 1, 4, 4)},  {128, 96, 1, 0.48f, 0.00f, {launch_tile<__bf16, 2, 3, 4, 2, 1, 4, 4>, launch_tile<f16, 2, 3, 4, 2, 1, 4, 4>, launch_tile<float, 2, 3, 4, 2, 1, 4>}},
-    {128, 128, 1, 0.58f, 0.00f, {launch_tile<__bf16, 2, 4, 4, 2, 1, 4, 4>, launch_tile<f16, 2, 4, 4, 2, 1, 4, 4>, launch_tile<float, 2, 4, 4, 2, 1, 4>}},
-    {128, 160, 1, 0.68f, 0.00f, {launch_tile<__bf16, 4, 5, 2, 2, 1, 4, 4>, launch_tile<f16, 4, 5, 2, 2, 1, 4, 4>, nullptr}},
+    {128, 64, 1, 0.45f, 0.00f, DSA_TILE(2, 4, 4, 1, 1, 4, 4)},  {128, 96, 1, 0.47f, 0.00f, {launch_tile<__bf16, 2, 3, 4, 2, 1, 4, 4>, launch_tile<f16, 2, 3, 4, 2, 1, 4, 4>, launch_tile<float, 2, 3, 4, 2, 1, 4>}},
+    {128, 128, 1, 0.55f, 0.00f, {launch_tile<__bf16, 2, 4, 4, 2, 1, 4, 4>, launch_tile<f16, 2, 4, 4, 2, 1, 4, 4>, launch_tile<float, 2, 4, 4, 2, 1, 4>}},
+    {128, 160, 1, 0.61f, 0.00f, {launch_tile<__bf16, 4, 5, 2, 2, 1, 4, 4>, launch_tile<f16, 4, 5, 2, 2, 1, 4, 4>, nullptr}},
     {128, 256, 1, 1.02f, 0.00f, DSA_TILE(4, 4, 2, 4, 1, 2)},
 };
 // A grid's threads, up to 768 a tile, are counted in 32 bits.  The 128 by 256 tiles of the
