@@ -18,12 +18,12 @@
 // One family of tiles, from 16 by 16 with K split over four waves to 256 by 256
 // (kVariants: which one, and what the others took).  Few rows are bound by the weights'
 // bytes and the latency of the steps (8 rows, 2112 columns, K 7168 6.0 us, 2.6 TB/s; 77,
-// 24576, 1536 10.5 us, 4.0 TB/s): from HBM a CU gets about 50 GB/s however much is under
-// way.  Middle ones (1000, 2112, 7168 26.1 us) by the steps of their smaller tiles, which
-// took as long on 17 workgroups alone.  Many by the matrix cores, and the clock that is
-// left to them under load (8192, 7168, 16384 838 us, 2.29 PFLOP/s; a library's product
-// without these scales 699 us): a step of a 256 by 256 tile takes 1.34 us on half the chip
-// and 1.7 on all of it, its products and sums alone, of random codes, 0.97 and 1.20.
+// 24576, 1536 10.4 us, 4.0 TB/s): from HBM a CU gets about 50 GB/s however much is under
+// way.  Middle ones (1000, 2112, 7168 23.9 us) by the same and the steps of their smaller
+// tiles.  Many by the matrix cores, 57 % busy, and the clock that is left to them under
+// load (8192, 7168, 16384 811 us, 2.37 PFLOP/s; a library's product without these scales
+// 699 us): products and sums alone of a step of a 256 by 256 tile, of random codes, take
+// 0.97 us on half the chip and 1.20 on all of it.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>
@@ -514,8 +514,8 @@ void launch_mixed(const dsa_product_args& p, int cus, hipStream_t stream) {
 // on 17 to 256 workgroups with K from 1536 to 16384, and, where the stages of two
 // workgroups fit a CU's LDS, on 264 to 512.  The smallest split K over their waves, so
 // that there are fewer steps; from 64 by 64 on waves of their own load: without them
-// (columns, rows, K) 128x64 took 31.6 us for 26.9 at (2112, 512, 7168), 128x96 32.6 for
-// 28.7 at (2112, 1000, 7168), 128x128 37.5 for 33.8.  The 32-bit outputs' widened codes
+// (columns, rows, K) 128x64 took 31.6 us for 26.2 at (2112, 512, 7168), 128x96 32.6 for
+// 27.9 at (2112, 1000, 7168), 128x128 37.5 for 33.4.  The 32-bit outputs' widened codes
 // need more registers than a third wave a SIMD leaves, so that from 128x96 on they load
 // themselves.  Whole calls, us (rows, columns, K; columns x rows of a tile):
 //   8, 2112, 7168      16x16 6.7 (four stages 7.1), 16x32 8.1, 32x16 8.9, 32x32 9.9, 64x32 14
