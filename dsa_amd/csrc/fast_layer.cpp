@@ -60,6 +60,15 @@ void* stream_of(c10::Device dev) { return c10::hip::getCurrentHIPStream(dev.inde
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, ": ", g_error()); }
 
+// A tensor that was saved for the gradient.  Hooks of saved tensors may have put another
+// in its place: equal, says their contract, but laid out in any way.
+at::Tensor kept(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType type, at::ScalarType other, c10::Device dev) {
+    TORCH_CHECK(t.defined() && t.sizes() == sizes && (t.scalar_type() == type || t.scalar_type() == other) && t.device() == dev &&
+                    t.layout() == at::kStrided,
+                "rms_norm: a saved tensor came back with another shape, type or device");
+    return t.resolve_neg();
+}
+
 // The norm with its gradient, of arguments that norm() has checked: as the function of
 // the same name in dsa_amd/norm.py.
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
@@ -100,9 +109,13 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
         {
             at::NoGradGuard plain;
             const auto saved = ctx->get_saved_variables();
-            const at::Tensor &h = saved[0], &weight = saved[1], &inverse = saved[2];
-            const c10::Device dev = h.device();
+            const at::Tensor& like = grads[0].defined() ? grads[0] : grads[1];
+            const c10::Device dev = like.device();
             c10::DeviceGuard guard(dev);
+            const auto type = like.scalar_type();
+            at::Tensor h = kept(saved[0], like.sizes(), type, type, dev);
+            const at::Tensor weight = kept(saved[1], like.sizes().slice(like.dim() - 1), type, at::kFloat, dev).contiguous();
+            const at::Tensor inverse = kept(saved[2], like.sizes().slice(0, like.dim() - 1), at::kFloat, at::kFloat, dev).contiguous();
             const auto options = h.options().requires_grad(false).memory_format(std::nullopt);
             const at::Tensor grad_y = grads[0].defined() ? grads[0].resolve_neg().contiguous() : at::zeros(h.sizes(), options);
             at::Tensor grad_sum, workspace;
@@ -112,12 +125,15 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
                 grad_sum = grads[1].resolve_neg().contiguous();
                 a.grad_sum = grad_sum.data_ptr();
             }
+            if (!row_stride(h, a.h_stride)) {
+                h = h.contiguous();
+                row_stride(h, a.h_stride);
+            }
             a.h = h.data_ptr();
             a.inverse = static_cast<const float*>(inverse.data_ptr());
             a.weight = weight.data_ptr();
             a.grad_out = grad_y.data_ptr();
             a.grad_in = grad_h.data_ptr();
-            row_stride(h, a.h_stride);
             a.dim = (int32_t)h.size(-1);
             a.rows = h.numel() / a.dim;
             a.dtype = code_of(h.scalar_type());

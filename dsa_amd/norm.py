@@ -108,6 +108,14 @@ def _norm(x, weight, residual, eps, keep):
     return y, total, inverse
 
 
+def _kept(t, shape, dtypes, device):
+    """A tensor that was saved for the gradient.  Hooks of saved tensors may have put another
+    in its place: equal, says their contract, but laid out in any way."""
+    if t.shape != shape or t.dtype not in dtypes or t.device != device or t.layout != torch.strided:
+        raise RuntimeError("rms_norm: a saved tensor came back with another shape, type or device")
+    return t.resolve_neg()
+
+
 class _RmsNorm(torch.autograd.Function):
     """Keeps the stream behind the addition and a number a row; the gradient of both summands is the same."""
 
@@ -120,8 +128,14 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y, grad_total=None):
+        shape, dtype, device = grad_y.shape, grad_y.dtype, grad_y.device
         h, weight, inverse = ctx.saved_tensors
-        dim, device = h.shape[-1], h.device
+        h = _kept(h, shape, (dtype,), device)
+        if h.numel() > 0 and ((h.shape[-1] > 1 and h.stride(-1) != 1) or _row_stride(h) is None):
+            h = h.contiguous()
+        weight = _kept(weight, shape[-1:], (dtype, torch.float32), device).contiguous()
+        inverse = _kept(inverse, shape[:-1], (torch.float32,), device).contiguous()
+        dim = shape[-1]
         needs_weight = ctx.needs_input_grad[1]
         grad_y = grad_y.resolve_neg().contiguous()
         grad_h = torch.empty(h.shape, device=device, dtype=h.dtype)

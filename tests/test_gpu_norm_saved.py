@@ -1,0 +1,81 @@
+"""The norm's gradient beside hooks of saved tensors, which may give back an equal tensor
+that is laid out in another way."""
+import pytest
+import torch
+
+import dsa_amd
+
+pytestmark = pytest.mark.gpu
+
+BF, FULL = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no ROCm GPU")
+    torch.cuda.init()
+
+
+def make(shape, dtype, seed):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+def turned(t):
+    """Columns next to each other instead of rows; of a single dimension, every second element."""
+    if t.dim() > 1:
+        return t.transpose(0, -1).contiguous().transpose(0, -1)
+    return torch.stack([t, t], -1)[:, 0]
+
+
+def spaced(t):
+    return torch.cat([t, t], -1)[..., :t.shape[-1]]
+
+
+def uneven(t):
+    """Rows of a third dimension that follow each other at no even distance."""
+    return torch.cat([t, t[:, :1]], 1)[:, :-1] if t.dim() > 2 else t
+
+
+def away(t):
+    return t.cpu()
+
+
+def back(t):
+    return t.cuda()
+
+
+def negated(t):
+    return torch._neg_view(-t)
+
+
+@pytest.mark.parametrize("eps", [1e-6, 1])  # a whole number: the Python path
+@pytest.mark.parametrize("dtype", [BF, FULL])
+@pytest.mark.parametrize("pack, unpack", [(turned, lambda t: t), (spaced, lambda t: t), (uneven, lambda t: t), (away, back),
+                                          (negated, lambda t: t)])
+def test_saved_tensors_may_be_laid_out_otherwise(pack, unpack, dtype, eps):
+    base = [make((4, 3, 520), dtype, 0), make(520, dtype, 1), make((4, 3, 520), dtype, 2)]
+    given = [make((4, 3, 520), dtype, 3 + i) for i in range(2)]
+
+    def step(residual):
+        x, w, r = (t.clone().requires_grad_() for t in base)
+        if residual:
+            return torch.autograd.grad(dsa_amd.rms_norm(x, w, r, eps=eps), (x, w, r), given)
+        return torch.autograd.grad(dsa_amd.rms_norm(x, w, eps=eps), (x, w), given[0])
+
+    for residual in (False, True):
+        want = step(residual)
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            got = step(residual)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("eps", [1e-6, 1])
+@pytest.mark.parametrize("unpack", [lambda t: t.cpu(), lambda t: t.double(), lambda t: t[..., :-1], lambda t: t[None]])
+def test_another_tensor_is_refused(unpack, eps):
+    x, w = make((4, 520), FULL, 0).requires_grad_(), make(520, FULL, 1).requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = dsa_amd.rms_norm(x, w, eps=eps)
+        with pytest.raises(RuntimeError, match="came back"):
+            y.sum().backward()
