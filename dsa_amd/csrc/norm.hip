@@ -144,6 +144,50 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x121, 0xf, 0xf, true));
 }
 
+// Max over a team of values that are not negative; a NaN's bits exceed infinity's.
+template <int WAVES>
+__device__ __forceinline__ float team_max(float v, float (*parts)[WAVES], int turn) {
+    uint32_t m = row16_max(__float_as_uint(v));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) parts[turn & 1][threadIdx.x >> 6] = __uint_as_float(m);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) m = max(m, __float_as_uint(parts[turn & 1][w]));
+    }
+    return __uint_as_float(m);
+}
+
+// A row whose mean square and eps leave 32 bits' range, or come so near to its end that
+// squares lose bits, times a power of two: its largest value, or eps's root, is then 1/2
+// to 1.  `mean` becomes what its root is to be taken of; returns the power, and 0 for
+// a row that no power helps: of zeros, or with an infinity or a NaN.  From 2^-96 on the
+// squares that underflow, 2^-150 each, are 2^-40 of the mean at most.
+constexpr float kLeastMean = 0x1p-96f;
+template <int WAVES, int CH>
+__device__ __forceinline__ int scale_row(float (&h)[CH][8], float& mean, float eps, int dim, float (*parts)[WAVES], int& turn) {
+    float top = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(h[c][i]) & 0x7fffffffu));
+    top = team_max<WAVES>(top, parts, ++turn);
+    if (!(top > 0.f && top < INFINITY)) return 0;
+    int power = __builtin_amdgcn_frexp_expf(top);
+    if (eps > 0.f) power = max(power, (__builtin_amdgcn_frexp_expf(eps) + 1) >> 1);
+    float squares = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            h[c][i] = ldexpf(h[c][i], -power);
+            squares = fmaf(h[c][i], h[c][i], squares);
+        }
+    mean = team_sum<WAVES>(squares, parts, ++turn) / (float)dim + ldexpf(eps, -2 * power);
+    return power;
+}
+
 // e4m3 code of v clamped to +-448, NaN kept (0x7f with v's sign).
 __device__ __forceinline__ uint32_t code_special(float v) {
     if (v != v) return 0x7fu | (__float_as_uint(v) >> 31 << 7);
@@ -250,8 +294,12 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void norm_kernel(dsa
 #pragma unroll
                 for (int i = 0; i < 8; ++i) squares = fmaf(h[c][i], h[c][i], squares);
             squares = team_sum<WAVES>(squares, parts, turn);
-            const float inverse = 1.f / sqrtf(squares / (float)dim + p.eps);
-            if (!CODES && p.inverse && tid == 0) p.inverse[r] = inverse;
+            float mean = squares / (float)dim + p.eps;
+            int power = 0;
+            if (__builtin_expect(!(mean >= kLeastMean && mean < INFINITY), 0))  // the same in all of the team
+                power = scale_row<WAVES, CH>(h, mean, p.eps, dim, parts, turn);
+            const float inverse = 1.f / sqrtf(mean);
+            if (!CODES && p.inverse && tid == 0) p.inverse[r] = ldexpf(inverse, -power);
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll

@@ -165,8 +165,9 @@ def rms_norm(x, weight, residual=None, *, eps=1e-6):
     ``residual`` the stream ``x + residual``, rounded to its type.
 
     Returns ``y``, or with a residual ``(y, h)``: new contiguous tensors of ``x``'s
-    type.  Sums and products are 32-bit (a row whose squares pass 3.4e38 comes out 0),
-    ``y`` rounded once.
+    type.  Sums and products are 32-bit, ``y`` rounded once; a row whose squares leave
+    their range, at either end, is multiplied by a power of two first.  A row of zeros
+    with ``eps=0``, and one with an infinity or a NaN, are what the formula says.
 
     ``x`` and ``residual``: bf16, fp16 or fp32, dim up to 16384, evenly spaced rows
     any distance apart (a slice of a projection's output goes in as it is);

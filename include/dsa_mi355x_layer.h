@@ -36,8 +36,10 @@ extern "C" {
  *   unused without residual, where it must be given
  *   scales [rows, ceil(dim / 128)]; inverse [rows] 32-bit, or NULL
  * Outputs are contiguous and lie apart from the inputs.  dim at most
- * DSA_NORM_MAX_DIM; codes: a multiple of 16, out 16-byte aligned.  Sums are 32-bit: a
- * row whose squares pass 3.4e38 comes out 0.
+ * DSA_NORM_MAX_DIM; codes: a multiple of 16, out 16-byte aligned.  Sums are 32-bit; a
+ * row whose squares leave their range, at either end, is multiplied by a power of two
+ * first.  The inverse itself is held in 32 bits: infinite where it would pass 3.4e38,
+ * of rows below 2.9e-39 with eps 0, whose gradients then are not finite.
  */
 #define DSA_NORM_MAX_DIM 16384
 typedef struct dsa_norm_args {
