@@ -280,7 +280,7 @@ py::object matmul_fp8(py::handle ha, py::handle ha_scales, py::handle hb, py::ha
         b_scales->scalar_type() != at::kFloat)
         return py::none();
     for (const at::Tensor* t : {a, a_scales, b, b_scales})
-        if (t->device() != dev || !t->is_contiguous() || !t->has_storage() || t->is_neg()) return py::none();
+        if (t->device() != dev || !t->is_contiguous() || !plain(*t) || wants_grad(t)) return py::none();
     p.a = static_cast<const uint8_t*>(a->data_ptr());
     p.a_scales = static_cast<const float*>(a_scales->data_ptr());
     p.b = static_cast<const uint8_t*>(b->data_ptr());

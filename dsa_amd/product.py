@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from .api import _fast_layer, _on_device
-from .norm import SCALE_BLOCK
+from .norm import SCALE_BLOCK, _derivatives
 from .rotary import DTYPES
 
 
@@ -33,8 +33,9 @@ def matmul_fp8(a, a_scales, b, b_scales, *, dtype=torch.bfloat16):
     eight neighbours (an error of 1.5e-5 of a sum's size was measured); for float32
     they are whole, at half the rate.  The same inputs give the same
     bits.  K is a multiple of 16 below 2^20.  All inputs are contiguous, the codes
-    16-byte aligned.  The output is a fresh tensor, which records no gradient and no
-    forward-mode tangent, and nothing synchronises."""
+    16-byte aligned.  The output is a fresh tensor, and nothing synchronises.  No gradient
+    is recorded, and as with :func:`dsa_amd.rms_norm_fp8` no input may require one while
+    gradients are enabled, or carry a forward-mode tangent."""
     fast = _fast_layer()
     if fast is not None:  # checked, allocated and launched in C++ (None: not taken)
         taken = fast.matmul_fp8(a, a_scales, b, b_scales, dtype)
@@ -63,6 +64,8 @@ def matmul_fp8(a, a_scales, b, b_scales, *, dtype=torch.bfloat16):
         raise ValueError("a and b must be float8_e4m3fn, their scales float32")
     if dtype not in DTYPES:
         raise ValueError("dtype must be torch.bfloat16, torch.float16 or torch.float32")
+    if any(_derivatives(a, a_scales, b, b_scales)):
+        raise ValueError("matmul_fp8 records no gradient and no forward-mode tangent: call it without them (torch.no_grad)")
     a_scales, b_scales = a_scales.resolve_neg(), b_scales.resolve_neg()
     out = torch.empty((*a.shape[:-1], columns), device=device, dtype=dtype)
     if out.numel() == 0:
