@@ -201,6 +201,8 @@ PRIVATE_SIGNATURES = {
     "dsa_kv_quantize_rows": (_i32, [_vp, _vp, _vp, _i64, _i32, _vp]),
     "dsa_kv_expand_rows": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _vp]),
     "dsa_bucket_indices_paged": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32, _i32, _i32, _vp]),
+    "dsa_product_tile": (_i32, [_i32] * 5),
+    "dsa_product_tiles": (ctypes.c_uint32, [_i32]),
 }
 
 _lock = threading.Lock()

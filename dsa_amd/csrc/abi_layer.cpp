@@ -8,6 +8,7 @@
 #include <cstdio>
 
 #include "../../include/dsa_mi355x_layer.h"
+#include "host_entry.h"
 #include "kernels.h"
 
 namespace {
@@ -127,5 +128,19 @@ int dsa_matmul_fp8(const dsa_product_args* a, void* stream) {
     if (rc) return fail(rc, "device query: %s", hipGetErrorString((hipError_t)rc));
     return finish(dsa::launch_product(*a, cus, static_cast<hipStream_t>(stream)), "product launch");
 }
+
+int dsa_product_tile(int M, int N, int K, int dtype, int cus) {
+    dsa_product_args a{};
+    a.M = M;
+    a.N = N;
+    a.K = K;
+    a.dtype = dtype;
+    if (const int rc = check_product(&a)) return rc;
+    if (cus <= 0 || cus > 1 << 16) return fail(-1, "cus must be in [1, 2^16] (got %d)", cus);
+    dsa::set_error(0, "%s", "");
+    return dsa::product_tile(a, cus);
+}
+
+unsigned dsa_product_tiles(int dtype) { return known(dtype) ? dsa::product_tiles(dtype) : 0; }
 
 }  // extern "C"

@@ -33,6 +33,12 @@ int dsa_bucket_indices_paged(const int32_t* idx, int32_t* out, int B, int SQ, in
                              const int32_t* block_table, int max_blocks, int block_size, int num_blocks,
                              void* stream);
 
+// Which of its tiles dsa_matmul_fp8 takes for a call of these sizes, of type dtype, on a
+// device of `cus` compute units: their number, or < 0.  And the numbers that there are
+// for a type, as bits (0: no such type).  Neither touches a device.
+int dsa_product_tile(int M, int N, int K, int dtype, int cus);
+unsigned dsa_product_tiles(int dtype);
+
 #ifdef __cplusplus
 }
 #endif

@@ -234,6 +234,8 @@ int launch_norm_grad(const dsa_norm_grad_args& p, bool vector, hipStream_t strea
 int64_t norm_grad_teams(int64_t rows, int dim);  // rows of 32-bit sums in the workspace
 
 // 8-bit products (product.hip).
+int product_tile(const dsa_product_args& p, int cus);  // number of the tiles that launch_product takes
+unsigned product_tiles(int dtype);                     // the numbers that there are for a type, as bits
 int launch_product(const dsa_product_args& p, int cus, hipStream_t stream);  // cus: compute units to plan for
 
 }  // namespace dsa

@@ -553,32 +553,45 @@ constexpr int64_t kMaxTiles = 5 << 20;
 static_assert(((int64_t)1 << 37) / (128 * 256) + (1 << 24) / 128 + (1 << 24) / 256 + 1 <= kMaxTiles, "one tile is left");
 constexpr float kWholeStep = 1.70f, kHalfStep = 1.02f;  // of the mixed kernel
 
+constexpr int kTiles = sizeof kVariants / sizeof kVariants[0];  // and the mixed kernel's number
+
 }  // namespace
 
-int launch_product(const dsa_product_args& p, int cus, hipStream_t stream) {
+// The number of the tiles that a call takes: kVariants', or kTiles.
+int product_tile(const dsa_product_args& p, int cus) {
     const int blocks = (p.K + kBlock - 1) / kBlock;
-    const Variant* best = nullptr;
+    int best = -1;
     float least = 0.f;
-    for (const Variant& v : kVariants) {
+    for (int i = 0; i < kTiles; ++i) {
+        const Variant& v = kVariants[i];
         const int64_t tiles = (int64_t)((p.M + v.rows - 1) / v.rows) * ((p.N + v.columns - 1) / v.columns);
         if (tiles > kMaxTiles || !v.launch[p.dtype]) continue;
         const bool pairs = v.both > 0.f && tiles > cus;
         const int64_t fit = pairs ? 2 * cus : cus;
         const float time = (float)((tiles + fit - 1) / fit) *
                            (2.f + (pairs ? v.both : v.step) * (float)((blocks + v.blocks - 1) / v.blocks));
-        if (!best || time < least) best = &v, least = time;
+        if (best < 0 || time < least) best = i, least = time;
     }
     if (p.dtype != DSA_F32) {  // the widened codes of 32-bit outputs would need more registers
         const int64_t tiles = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256), rest = tiles % cus;
         const float time = (float)(tiles / cus) * (2.f + kWholeStep * (float)blocks) +
                            (float)((2 * rest + cus - 1) / cus) * (2.f + kHalfStep * (float)blocks);
-        if (time < least) {
-            if (p.dtype == DSA_BF16) launch_mixed<__bf16>(p, cus, stream);
-            else launch_mixed<f16>(p, cus, stream);
-            return (int)hipGetLastError();
-        }
+        if (time < least) best = kTiles;
     }
-    best->launch[p.dtype](p, stream);
+    return best;
+}
+
+unsigned product_tiles(int dtype) {
+    unsigned set = dtype == DSA_F32 ? 0u : 1u << kTiles;
+    for (int i = 0; i < kTiles; ++i) set |= kVariants[i].launch[dtype] ? 1u << i : 0u;
+    return set;
+}
+
+int launch_product(const dsa_product_args& p, int cus, hipStream_t stream) {
+    const int tile = product_tile(p, cus);
+    if (tile < kTiles) kVariants[tile].launch[p.dtype](p, stream);
+    else if (p.dtype == DSA_BF16) launch_mixed<__bf16>(p, cus, stream);
+    else launch_mixed<f16>(p, cus, stream);
     return (int)hipGetLastError();
 }
 
