@@ -204,7 +204,7 @@ __device__ __forceinline__ uint2 encode8(const float (&f)[8], bool pow2, float& 
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
     m = row16_max(m);
-    const float top = __uint_as_float(m);
+    const float top = __uint_as_float(m);  // of a block with a NaN a NaN: scale 1, as in an fp8 cache row
     scale = top > 0.f ? top * (1.f / 448.f) : 1.f;
     if (!(scale > 0.f)) scale = __uint_as_float(1);  // the product of the least numbers underflows
     float x[8];

@@ -223,8 +223,10 @@ def rms_norm_fp8(x, weight, residual=None, *, eps=1e-6, pow2_scales=True):
 
     Returns ``(codes, scales)``, or with a residual ``(codes, scales, h)``.  A scale is
     the least power of two that is not below the largest of its 128 values over 448
-    (``pow2_scales=False``: that quotient itself); 1 where all are zero.  NaN keeps
-    to its own code; an infinity makes its block's scale one, and its own code NaN.
+    (``pow2_scales=False``: that quotient itself); 1 where all are zero.  A block with a
+    NaN has a scale of 1 too: a NaN has its own code, and the other values there are coded
+    as they are, past 448 as 448 and below 2^-10 as 0.  Without one an infinity makes its
+    block's scale infinite: its code is NaN, the others' 0.
 
     dim: a multiple of 16 up to 16384.  No gradient is recorded, and no input may
     require one while gradients are enabled, or carry a forward-mode tangent."""

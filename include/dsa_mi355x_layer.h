@@ -27,8 +27,9 @@ extern "C" {
  * block may be shorter):
  *   scale = max|y| / 448, pow2_scales: the least power of two not below that; 1 for
  *   a block of zeros;  code = e4m3(y / scale), to nearest even
- * and without weight the codes of h itself.  A NaN keeps to its own code; an
- * infinity makes its block's scale one.
+ * and without weight the codes of h itself.  A block with a NaN has scale 1 (the NaN
+ * its own code, the others e4m3(y), past 448 as 448); without one an infinity makes its
+ * block's scale infinite, its own code NaN and the others 0.
  *
  *   x, residual [rows, dim], x_stride and residual_stride elements apart (at
  *   least 0, last stride 1); weight [dim] of x's type, or 32-bit (weight_f32)
