@@ -109,7 +109,8 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
         {
             at::NoGradGuard plain;
             const auto saved = ctx->get_saved_variables();
-            const at::Tensor& like = grads[0].defined() ? grads[0] : grads[1];
+            // the node is called without any gradient too, where a function behind it gives none: of zeros then
+            const at::Tensor& like = grads[0].defined() ? grads[0] : grads.size() > 1 && grads[1].defined() ? grads[1] : saved[0];
             const c10::Device dev = like.device();
             c10::DeviceGuard guard(dev);
             const auto type = like.scalar_type();

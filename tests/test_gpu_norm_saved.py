@@ -79,3 +79,41 @@ def test_another_tensor_is_refused(unpack, eps):
         y = dsa_amd.rms_norm(x, w, eps=eps)
         with pytest.raises(RuntimeError, match="came back"):
             y.sum().backward()
+
+
+class _Nothing(torch.autograd.Function):
+    """A function that gives its inputs no gradient."""
+
+    @staticmethod
+    def forward(ctx, *tensors):
+        return tensors[0].sum()
+
+    @staticmethod
+    def backward(ctx, grad):
+        return (None,) * len(ctx.needs_input_grad)
+
+
+@pytest.mark.parametrize("eps", [1e-6, 1])
+@pytest.mark.parametrize("outputs", [(0,), (1,), (0, 1)])
+def test_without_any_gradient(outputs, eps):
+    """Behind a function that gives none the gradients are zeros."""
+    x, w, r = make((4, 520), FULL, 0).requires_grad_(), make(520, FULL, 1).requires_grad_(), make((4, 520), FULL, 2).requires_grad_()
+    out = dsa_amd.rms_norm(x, w, r, eps=eps)
+    _Nothing.apply(*(out[i] for i in outputs)).backward()
+    assert not x.grad.any() and not w.grad.any() and not r.grad.any()
+    if outputs == (0,):
+        w.grad = None
+        _Nothing.apply(dsa_amd.rms_norm(x.detach(), w, eps=eps)).backward()
+        assert w.grad.shape == (520,) and not w.grad.any()
+
+
+@pytest.mark.parametrize("eps", [1e-6, 1])
+def test_a_row_without_leading_dimensions(eps):
+    x, w, g = make((1, 520), FULL, 0), make(520, FULL, 1), make((1, 520), FULL, 2)
+    leaves = [x[0].clone().requires_grad_(), w.clone().requires_grad_(), x[0].clone().requires_grad_()]
+    y, h = dsa_amd.rms_norm(*leaves, eps=eps)
+    got = torch.autograd.grad((y, h), leaves, (g[0], g[0]))
+    leaves = [x.clone().requires_grad_(), w.clone().requires_grad_(), x.clone().requires_grad_()]
+    want = torch.autograd.grad(dsa_amd.rms_norm(*leaves, eps=eps), leaves, (g, g))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b.view(a.shape))
