@@ -4,10 +4,11 @@
 //
 // A row is held in registers by a team of one to sixteen waves, eight values a thread
 // (sixteen above 8192), so that it is read once: the sum of squares needs all of it
-// before the first output.  Bound by HBM (4095 rows of 4096 with a residual 26.9 us, 5.0
-// TB/s; their gradients 25.6, 5.2 TB/s, and 4.0 for the weight's; codes of 4095 rows of
-// 16384 33.2 us, 6.1 TB/s), and in a decode step by the launch and a trip to memory (8
-// rows of 7168 3.7 us, 192 with codes 5.0).
+// before the first output.  Bound by HBM (4095 rows of 4096 with a residual 25.8 to 26.9
+// us, 5.0 to 5.2 TB/s; their gradients 25.0, and 3.9 for the weight's; codes of 4095 rows
+// of 16384 34.3 us, 5.9 TB/s, of 4096 of 7168 with a norm and a residual 43.6 us, 4.7),
+// and in a decode step by the launch and a trip to memory (8 rows of 7168 3.8 us, 192 with
+// codes 4.8).
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>

@@ -16,14 +16,17 @@
 // whose sums were off by 1.3e-8, at half the rate (2.2 PFLOP/s for 4.6).
 //
 // One family of tiles, from 16 by 16 with K split over four waves to 256 by 256
-// (kVariants: which one, and what the others took).  Few rows are bound by the weights'
-// bytes and the latency of the steps (8 rows, 2112 columns, K 7168 6.0 us, 2.6 TB/s; 77,
-// 24576, 1536 10.4 us, 4.0 TB/s): from HBM a CU gets about 50 GB/s however much is under
-// way.  Middle ones (1000, 2112, 7168 23.9 us) by the same and the steps of their smaller
-// tiles.  Many by the matrix cores, 57 % busy, and the clock that is left to them under
-// load (8192, 7168, 16384 811 us, 2.37 PFLOP/s; a library's product without these scales
-// 699 us): products and sums alone of a step of a 256 by 256 tile, of random codes, take
-// 0.97 us on half the chip and 1.20 on all of it.
+// (kVariants: which one, and what the others took).  Times below: weights out of 1 GiB of
+// them in turn, so that they come from HBM, and in brackets those of a few in turn, which
+// stay in the last cache.  Few rows are bound by the weights' bytes and the latency of the
+// steps (8 rows, 2112 columns, K 7168 7.0 to 8.1 us (6.1); 77, 24576, 1536 12.7 (10.4, 4.0
+// TB/s); 8, 7168, 16384 24.6, 4.8 TB/s): from HBM a CU gets about 50 GB/s however much is
+// under way.  Middle ones (1000, 2112, 7168 27.8 (23.9 to 25.3)) by the same and the steps
+// of their smaller tiles.  Many by the matrix cores, 57 % busy, and the clock that is left
+// to them under load (8192, 7168, 16384 803 to 846 us, 2.27 to 2.4 PFLOP/s; a library's
+// product without these scales 699): products and sums alone of a step of a 256 by 256
+// tile, of random codes, take 0.97 us on half the chip and 1.20 on all of it.  32-bit
+// outputs: 8, 77, 1000 and 8192 rows 7.2 to 8.1, 16, 54 and 1608 to 1680 us, 1.2 PFLOP/s.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>
@@ -517,20 +520,25 @@ void launch_mixed(const dsa_product_args& p, int cus, hipStream_t stream) {
 // (columns, rows, K) 128x64 took 31.6 us for 26.2 at (2112, 512, 7168), 128x96 32.6 for
 // 27.9 at (2112, 1000, 7168), 128x128 37.5 for 33.4.  The 32-bit outputs' widened codes
 // need more registers than a third wave a SIMD leaves, so that from 128x96 on they load
-// themselves.  Whole calls, us (rows, columns, K; columns x rows of a tile):
-//   8, 2112, 7168      16x16 6.7 (four stages 7.1), 16x32 8.1, 32x16 8.9, 32x32 9.9, 64x32 14
-//   5, 4300, 7168      16x16 9.9, 32x16 9.4 (three stages 11.1), 32x32 10.3, 64x32 14
-//   32, 2112, 16384    16x16 17.9, 16x32 16.0, 32x16 16.9, 32x32 20.9, 64x32 28
-//   64, 2112, 7168     16x16 13.8, 32x32 11.4, 64x32 16.3, 64x64 20, 128x64 28.6
-//   16, 24576, 1536    64x32 12.3, 64x64 10.8, 128x32 9.7, 128x64 10.0, 128x96 10.4
-//   448, 2112, 7168    64x32 29.7, 64x64 19.5, 128x32 22.0, 128x64 26.2, 128x96 29.2
-//   512, 4096, 7168    64x64 33.7, 128x64 27.6, 128x96 27.6, 128x128 34.8
-//   1000, 2112, 7168   64x64 41, 128x64 41, 128x96 27.9, 128x128 33.4, 128x160 34.9
-//   2000, 2112, 7168   64x64 64, 128x96 52.4, 128x128 59, 128x160 41.3, 128x256 59
-//   1000, 7168, 16384  64x64 201, 128x96 170, 128x128 142, 128x160 156, 128x256 134, 256x256 134
-//   8192, 2112, 7168   128x96 174, 128x128 172, 128x160 170, 128x256 175, 256x256 155
-// Over 48 drawn calls of these ranges the chosen tile took 2 % longer than the best one
-// (at most 21 %, where few rows meet 24576 by 16384).
+// themselves.  Whole calls, us (rows, columns, K; columns x rows of a tile; weights from
+// HBM; two runs differ by up to 10 % below 10 us):
+//   8, 2112, 7168      16x16 7.8 (four stages 7.8), 16x32 8.5, 32x16 9.1, 32x32 9.7, 64x32 15
+//   5, 4300, 7168      16x16 12.2 (9.9), 32x16 9.3 (three stages 10.7), 32x32 10.1, 64x32 15
+//   32, 2112, 16384    16x16 21.1 (17.5), 16x32 16.0, 32x16 16.9, 32x32 21.0, 64x32 32
+//   64, 2112, 7168     16x16 17.1 (14.1), 32x32 11.3, 64x32 15.9, 64x64 20, 128x64 28
+//   204, 623, 5648     16x16 10.6 (8.3), 16x32 13.0, 32x16 13.6 (10.9), 32x32 8.8, 64x32 13.2
+//   16, 24576, 1536    64x32 12.3, 64x64 10.8, 128x32 9.7, 128x64 9.9, 128x96 10.3
+//   448, 2112, 7168    64x32 29.5, 64x64 19.5, 128x32 22.1, 128x64 26.2, 128x96 29.3
+//   512, 4096, 7168    64x64 33.2, 128x64 26.9, 128x96 27.3, 128x128 34.7
+//   1000, 2112, 7168   64x64 39, 128x64 41, 128x96 27.8, 128x128 33.7, 128x160 35.1
+//   2000, 2112, 7168   64x64 63, 128x96 51.5, 128x128 59, 128x160 39.2, 128x256 59
+//   1000, 7168, 16384  64x64 203, 128x96 167, 128x128 140, 128x160 155, 128x256 135, 256x256 136
+//   8192, 2112, 7168   128x96 159, 128x128 163, 128x160 154, 128x256 172, 256x256 151
+// Over 170 calls, most of them drawn from these ranges, the chosen tile took 1.5 % longer
+// than the best one (at most 22 %, where few rows meet 24576 by 14240 or 16384).  32-bit
+// outputs go by the same step times, though theirs are longer, up to 1.9 times in the
+// larger tiles: over 270 calls that choice took 1.3 % longer than the best (at most 20 %,
+// the same ones), and 1.2 % with their own medians in place of these.
 struct Variant {
     int columns, rows, blocks;  // of a tile, and blocks of K a step
     float step, both;           // us a step, alone on a CU and beside another; 0: does not fit beside another

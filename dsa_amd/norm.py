@@ -176,7 +176,9 @@ def rms_norm(x, weight, residual=None, *, eps=1e-6):
     Gradients of ``x``, ``residual`` and ``weight`` are recorded where one of them
     requires it (once: there are none of the second order), sums over the rows in
     a fixed order; forward-mode tangents are refused.  In a graph's capture so is a leaf
-    whose results of eager calls on the default stream are still kept with their graph."""
+    whose results of eager calls on the default stream are still kept with their graph:
+    its gradient there would end the process, so the call itself says so, whether or not
+    a gradient would follow (``torch.no_grad`` captures the norm alone)."""
     fast = _fast_layer()
     if fast is not None:  # checked, allocated and launched in C++ (None: not taken)
         taken = fast.rms_norm(x, weight, residual, eps)

@@ -87,7 +87,9 @@ def forward_shared(q, kv, q_rope, k_rope, lengths, prefix=0, *, scale=None, bloc
     its block table row) for every sequence.  The caller vouches that they are
     the same; it need not be a multiple of the block size.  0: nothing shared.
 
-    The output is finite for max|kv| < 2^38.  Caches hold fewer than 2^25 rows.
+    Scores, sums and statistics are 32-bit; the weights are rounded to bf16, by half a
+    step (2^-8 of each) at most, before their product with the values.  The output is
+    finite for max|kv| < 2^38.  Caches hold fewer than 2^25 rows.
     Outputs are fresh tensors, which record no gradient and no forward-mode tangent
     (as :func:`dsa_amd.forward`'s), the workspace is the caching allocator's, and
     nothing synchronises."""
@@ -114,8 +116,9 @@ def forward_tree(q, kv, q_rope, k_rope, lengths, tree, prefix=0, *, scale=None, 
     (:func:`dsa_amd.write_kv_rows`), rotated by its own position.  A query with no row
     gives output 0, max -inf and sum 0.
 
-    All else, and the three results, as :func:`forward_shared`'s; rows below ``prefix``
-    are sequence 0's."""
+    All else, and the three results, as :func:`forward_shared`'s, its weights in bf16
+    among it; rows below ``prefix`` are sequence 0's.  A padding token of
+    :func:`dsa_amd.draft_tree` has no bits, and sees its sequence's rows all the same."""
     fast = _fast_cache()
     if fast is not None:  # checked, allocated and launched in C++ (None: not taken)
         taken = fast.forward_tree(q, kv, q_rope, k_rope, lengths, tree, prefix, scale, block_table)

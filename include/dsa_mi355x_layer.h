@@ -66,7 +66,8 @@ int dsa_rms_norm_fp8(const dsa_norm_args* args, void* stream);
  *   grad_in = (b - u * mean(b * u)) * inverse + grad_sum     (of x and the residual)
  *   grad_weight = sum over the rows of grad_out * u
  * h [rows, dim] h_stride apart; grad_out, grad_sum (or NULL), grad_in [rows, dim]
- * contiguous, of h's type; grad_weight [dim] of the weight's type, or NULL.
+ * contiguous, of h's type; grad_weight [dim] of the weight's type, or NULL.  Outputs lie
+ * apart from the inputs.
  * workspace: at least dsa_rms_norm_grad_ws_bytes(rows, dim) bytes, 16-byte aligned,
  * any contents; unused without grad_weight.  The order of the sums is fixed.
  */
@@ -94,7 +95,8 @@ int dsa_rms_norm_grad(const dsa_norm_grad_args* args, void* stream);
  *   a [M, K], b [N, K] e4m3 codes, 16-byte aligned, K a multiple of 16 below 2^20,
  *   M * N at most 2^37
  *   a_scales [M, ceil(K / 128)], b_scales [ceil(N / 128), ceil(K / 128)] 32-bit
- *   out [M, N] of type dtype, rounded once; sums are 32-bit.  For 16-bit outputs the
+ *   out [M, N] of type dtype, rounded once; sums are 32-bit, and so is the product of
+ *   two scales, which has to be in their range.  For 16-bit outputs the
  *   matrix cores cut each product to 2^-13 of the largest of eight neighbours (an error
  *   of 1.5e-5 of a sum's size was measured), for DSA_F32 they are whole.
  */
