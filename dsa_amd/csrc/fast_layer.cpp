@@ -66,7 +66,7 @@ at::Tensor kept(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType type,
     TORCH_CHECK(t.defined() && t.sizes() == sizes && (t.scalar_type() == type || t.scalar_type() == other) && t.device() == dev &&
                     t.layout() == at::kStrided,
                 "rms_norm: a saved tensor came back with another shape, type or device");
-    return t.resolve_neg();
+    return t.is_neg() ? t.resolve_neg() : t;
 }
 
 // The norm with its gradient, of arguments that norm() has checked: as the function of
